@@ -44,6 +44,27 @@ int hb_qkv_post(const void* qkv, int dtype, const float* inv_freq, int rot_pairs
                 void* v_pages, int page_size, int write_kv, int n_tokens, int nh, int nkv, int hd,
                 cudaStream_t stream);
 
+// The cache in four bits (four_bit.cuh, four_bit_cache.cu): pages [pages][nkv][page_size / 16] blocks of 16 rows, keys and values,
+// 20 hd bytes each; hd 64 or 128, page sizes 16, 32 and multiples of 64. hb_qkv_post into such a cache:
+int hb_qkv_post_4bit(const void* qkv, const float* inv_freq, int rot_pairs, int interleaved, int qk_norm, float qk_eps,
+                     int temp_on, float floor_scale, float attn_scale, const float* q_norm_w, const float* k_norm_w,
+                     int norm_first, int norm_dim, float rot_mul, int v_is_k, const int* positions,
+                     const int* seq_of_token, const int* block_table, int table_stride, void* q_out, void* pages,
+                     int page_size, int write_kv, int n_tokens, int nh, int nkv, int hd, cudaStream_t stream);
+// the pages that the requests' new tokens may read, as bfloat16 pages [total, nkv, page_size, hd], and the table of them
+int hb_expand_pages_4bit(const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
+                         const int* positions, int n_seqs, int total, int page_size, int chunk, int window, int keep,
+                         int skip_single, int nkv, int hd, void* k, void* v, int* table, cudaStream_t stream);
+// attention of single tokens over it; splits of split_tiles x 64 positions; splits > 1: partial rows for hb_attention_merge_rows
+int hb_attention_decode_4bit(const void* q, const void* pages, const int* block_table, int table_stride,
+                             const int* seq_of_token, const int* positions, void* out, int n_tokens, int nh, int nkv, int hd,
+                             int page_size, int chunk, int window, int keep, float scale, int sink,
+                             const float* sink_values, int split_tiles, int splits, float* part_acc, float* part_ml,
+                             int* status, const long long* rows, int step_tokens, cudaStream_t stream);
+// x [tokens, K] (rows x_ld elements apart) times a weight of four bits in blocks of 16 rows x 128 k (four_bit_linear.cu)
+int hb_four_bit_linear(const void* x, long long x_ld, const void* w, const void* bias, void* out, int out_dtype, int tokens,
+                       int n_out, int K, int group, cudaStream_t stream);
+
 // sink != 0 (every attention entry point): the softmax's denominator has one more term of score 0,
 // p_j = e^{s_j} / (1 + sum e^{s_j}); the term has no value. The general kernel and the merge also take
 // sink_values (float32 [nh] or null): the term's score is the head's own number instead of 0. The general

@@ -1,0 +1,387 @@
+// Attention of single decoded tokens over the cache in four bits (four_bit.cuh has its blocks): with the key k_jd = s_jg c_jd + l_jg
+// and the value v_jd = t_jg e_jd + m_jg of group g (32 dims),
+//   score_ij = sum_g s_jg (sum_d q_d c_jd) + sum_g l_jg (sum_d q_d)            d over the group
+//   o_d      = sum_j (p_j t_jg) e_jd + sum_j p_j m_jg                          p_j = exp(score - max), then over sum_j p_j
+// so the codes enter the tensor cores as they are (whole numbers, exact), a key's scale multiplies the sum of its group, and a value's scale
+// the weight it meets. Rounded to bfloat16 are the weights alone, once times the scale and once bare for the lows and for the sum.
+//
+// Both products are taken transposed, keys (then dims) as the 16 rows of mma.sync and the query heads of a kv head as its 8 columns, half
+// the columns that heads as rows would leave empty; the weights change over with movmatrix. The lows' part is one more product a
+// block of 16 keys: l times the queries' sums in three pieces of bfloat16, and for the values a matrix whose rows are the groups' lows and
+// a row of ones, which sums the weights.
+//
+// Grid (split, kv head x tiles of 8 heads, token). A warp has steps of 32 keys of its own: 2 blocks, which lie side by side in a
+// page of 32 and more, come as one bulk copy that the warp's own barrier counts, a few steps ahead; the warps meet at the end only,
+// where their sums are joined, and the splits' by attention_merge. A step's copies leave out blocks behind the token's own.
+// Rows of a block that the token may not read (not written yet, out of its window) hold anything, NaN as well: their scores, scales
+// and lows are replaced. Every wait is bounded; on a time-out the kernel says so in `status` and its output is invalid.
+#include "api.h"
+#include "common.cuh"
+#include "four_bit.cuh"
+#include "tc.cuh"
+
+namespace {
+
+constexpr int STEP = 32;         // keys a warp takes at a time
+constexpr int TILE = 64;         // splits are cut in these
+constexpr int WARPS = 4;
+constexpr int STAGES = 2;        // steps in flight a warp
+constexpr int HEADS = 8;         // query heads of a block
+
+struct Args {
+  const __nv_bfloat16* q;
+  const uint8_t* pages;
+  const int* block_table;
+  const int* seq_of_token;
+  const int* positions;
+  __nv_bfloat16* out;
+  float* part_acc;
+  float* part_ml;
+  int* status;
+  const long long* rows;         // the tokens of the launch among the step's, or null
+  const float* sink_values;
+  int step_tokens, table_stride, nh, nkv, page_size, chunk, window, keep, split_tiles, splits, sink;
+  float scale;
+};
+
+__device__ __forceinline__ unsigned transpose8(unsigned v) {      // an 8 x 8 matrix of 16 bits over the warp
+  unsigned r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+template <int G> struct Words;
+template <> struct Words<4> {
+  unsigned w[4];
+  __device__ __forceinline__ explicit Words(const uint8_t* p) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  }
+};
+template <> struct Words<2> {
+  unsigned w[2];
+  __device__ __forceinline__ explicit Words(const uint8_t* p) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  }
+};
+// two bfloat16 of a word as floats
+__device__ __forceinline__ float low_half(unsigned w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_half(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
+
+template <int G>
+__global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const Args a) {
+  using B = fb::Block<G>;
+  constexpr int HD = 32 * G, MT = STEP / 16;
+  constexpr float RAISE = 64.f;                                   // weights carry 2^64 (four_bit.cuh)
+  extern __shared__ __align__(128) uint8_t ring_all[];            // [WARPS][STAGES][MT][B::BYTES]
+  __shared__ uint64_t full[WARPS][STAGES];
+  __shared__ float ml_s[WARPS][HEADS][2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q4 = lane & 3;
+  const int split = blockIdx.x, per = a.nh / a.nkv, head_tiles = (per + HEADS - 1) / HEADS;
+  const int kvh = blockIdx.y / head_tiles, h0 = blockIdx.y % head_tiles * HEADS, heads = min(HEADS, per - h0);
+  const int t = blockIdx.z;
+  const long long chosen = a.rows ? a.rows[t] : t;
+  if (chosen < 0 || chosen >= a.step_tokens) {
+    if (threadIdx.x == 0) atomicExch(a.status, 32);
+    return;
+  }
+  const int token = (int)chosen, pos = a.positions[token];
+  const int* table = a.block_table + (size_t)a.seq_of_token[token] * a.table_stride;
+  int lo = 0;
+  if (a.chunk > 0) lo = pos / a.chunk * a.chunk;
+  if (a.window > 0) lo = max(lo, pos - a.window + 1);
+  // tiles of 64 positions: those of the first tokens that the window keeps, then lo's to the token's own
+  const int t0 = lo / TILE, kept = min((a.keep + TILE - 1) / TILE, t0);
+  const int n_tiles = pos < 0 ? 0 : kept + pos / TILE - t0 + 1;
+  const int first = split * a.split_tiles, mine = min(a.split_tiles, n_tiles - first);
+  const size_t part0 = (size_t)t * a.nh + (size_t)kvh * per + h0, row0 = (size_t)token * a.nh + (size_t)kvh * per + h0;
+  if (mine <= 0) {                                                // the token has fewer splits
+    if (a.splits > 1) {
+      if (threadIdx.x < heads) {
+        float* ml = a.part_ml + ((part0 + threadIdx.x) * a.splits + split) * 2;
+        ml[0] = -INFINITY;
+        ml[1] = 0.f;
+      }
+    } else {
+      for (int i = threadIdx.x; i < heads * HD; i += WARPS * 32) a.out[row0 * HD + i] = __float2bfloat16_rn(0.f);
+    }
+    return;
+  }
+
+  uint8_t* ring = ring_all + warp * (STAGES * MT * B::BYTES);
+  const uint32_t ring_at = tc::smem_u32(ring), full_at = tc::smem_u32(&full[warp][0]);
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) tc::mbar_init(&full[warp][s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  // steps of the split, dealt out in turn; step i covers the keys from key_of(i) on
+  const int steps_all = mine * (TILE / STEP), steps = (steps_all - warp + WARPS - 1) / WARPS;
+  auto key_of = [&](int i) {
+    const int s = warp + i * WARPS, tile = first + s / (TILE / STEP);
+    return (tile < kept ? tile : t0 + tile - kept) * TILE + s % (TILE / STEP) * STEP;
+  };
+  auto bring = [&](int i) {                                       // lane b: block b of the step (lane 0 all of it from one page)
+    const int key = key_of(i), blocks = min(MT, (pos - key) / fb::BLOCK_ROWS + 1);      // <= 0: nothing of the step is the token's
+    const bool together = a.page_size >= STEP;
+    const int n = together ? 1 : MT, each = together ? blocks : 1, at = key + lane * 16;
+    const bool copies = lane < n && lane < blocks;
+    int page = -1;
+    if (copies) page = table[at / a.page_size];
+    const uint32_t bytes = each * B::BYTES;
+    const unsigned who = __ballot_sync(0xffffffffu, copies && page >= 0);
+    if (lane == 0) tc::mbar_expect_tx(&full[warp][i % STAGES], __popc(who) * bytes);
+    __syncwarp();
+    if (copies && page >= 0)
+      bulk_load(ring_at + (i % STAGES * MT + lane) * B::BYTES,
+                a.pages + (((size_t)page * a.nkv + kvh) * (a.page_size / 16) + at % a.page_size / 16) * B::BYTES, bytes,
+                full_at + i % STAGES * 8);
+  };
+  for (int i = 0; i < min(STAGES, steps); ++i) bring(i);
+
+  // the heads' queries as columns, raised; their sums over a group in three pieces
+  uint4 qf[G];
+  uint2 q_sums;
+  {
+    float sums[G];
+#pragma unroll
+    for (int c = 0; c < G; ++c) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (g < heads) v = *reinterpret_cast<const uint4*>(a.q + (row0 + g) * HD + c * 32 + q4 * 8);
+      const unsigned w[4] = {v.x, v.y, v.z, v.w};
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += low_half(w[i]) + high_half(w[i]);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sums[c] = sum / fb::UNSCALE;
+      qf[c] = fb::raised(v);
+    }
+    unsigned p[3];
+    if constexpr (G == 4) {
+      const bool second = q4 & 1;
+      hb::split3(second ? sums[2] : sums[0], second ? sums[3] : sums[1], p);
+      q_sums = make_uint2(q4 < 2 ? p[0] : p[1], q4 < 2 ? p[2] : 0u);
+    } else {
+      hb::split3(sums[0], sums[1], p);
+      q_sums = make_uint2(q4 == 0 ? p[0] : q4 == 1 ? p[1] : q4 == 2 ? p[2] : 0u, 0u);
+    }
+  }
+  const float to_log2 = a.scale * 1.4426950408889634f * fb::UNSCALE;
+
+  float m_run[2] = {-INFINITY, -INFINITY};
+  float o[2 * G][4], low[4] = {0.f, 0.f, 0.f, 0.f};               // dims 4 g + (0, 1) and (2, 3) of every group; lows' sums and the weights'
+#pragma unroll
+  for (int c = 0; c < 2 * G; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[c][e] = 0.f;
+  bool ok = true;
+  int asked = min(STAGES, steps);
+
+  for (int i = 0; i < steps; ++i) {
+    if (!tc::mbar_wait_warp(&full[warp][i % STAGES], (i / STAGES) & 1)) {
+      if (lane == 0) atomicExch(a.status, 31);
+      ok = false;
+      break;
+    }
+    const int key = key_of(i);
+    const uint8_t* blocks = ring + i % STAGES * MT * B::BYTES;
+    const bool whole = key + STEP - 1 <= pos && (key >= lo || key + STEP - 1 < a.keep);
+    auto seen = [&](int row) { return key + row <= pos && (key + row >= lo || key + row < a.keep); };
+    float s[MT][4];
+    float m_step[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const uint8_t* b = blocks + mt * B::BYTES;
+      const Words<G> ka(b + B::key_word(g, q4, 0)), kb(b + B::key_word(g + 8, q4, 0));
+      const int pair = G == 4 ? 2 * (q4 & 1) : 0;
+      const unsigned la = *reinterpret_cast<const unsigned*>(b + B::key_low(g, pair)),
+                     lb = *reinterpret_cast<const unsigned*>(b + B::key_low(g + 8, pair));
+      const unsigned lows[4] = {la, lb, G == 4 ? la : 0u, G == 4 ? lb : 0u};
+      float total[4] = {0.f, 0.f, 0.f, 0.f};
+      hb::mma_bf16(total, lows, q_sums.x, q_sums.y);
+#pragma unroll
+      for (int c = 0; c < G; ++c) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        fb::mma_codes(acc, ka.w[c], kb.w[c], qf[c]);
+        const unsigned sa = *reinterpret_cast<const unsigned*>(b + B::scale(g, 0, c & ~1)),
+                       sb = *reinterpret_cast<const unsigned*>(b + B::scale(g + 8, 0, c & ~1));
+        const float fa = c & 1 ? high_half(sa) : low_half(sa), fb_ = c & 1 ? high_half(sb) : low_half(sb);
+        total[0] = fmaf(acc[0], fa, total[0]);
+        total[1] = fmaf(acc[1], fa, total[1]);
+        total[2] = fmaf(acc[2], fb_, total[2]);
+        total[3] = fmaf(acc[3], fb_, total[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = total[e] * to_log2;
+        if (!whole && !seen(mt * 16 + g + 8 * (e >> 1))) v = -INFINITY;
+        s[mt][e] = v;
+        m_step[e & 1] = fmaxf(m_step[e & 1], v);
+      }
+    }
+    bool grows = false;
+    float correct[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float m = m_step[h];
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+      m = fmaxf(m, m_run[h]);
+      correct[h] = m == m_run[h] ? 1.f : exp2_fast(m_run[h] - m);       // (the first maximum: exp2(-inf) = 0)
+      grows = grows || m != m_run[h];
+      m_run[h] = m;
+    }
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int c = 0; c < 2 * G; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[c][e] *= correct[e & 1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) low[e] *= correct[e & 1];
+    }
+    // a step that is not the token's at all leaves a maximum of -inf; its weights are zeros
+    const float base[2] = {m_run[0] == -INFINITY ? 0.f : RAISE - m_run[0], m_run[1] == -INFINITY ? 0.f : RAISE - m_run[1]};
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const uint8_t* b = blocks + mt * B::BYTES;
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = exp2_fast(s[mt][e] + base[e & 1]);
+      unsigned la = 0u, lb = 0u;                                  // rows of the lows' product: a group's lows, or ones
+      if (g < G) {
+        la = *reinterpret_cast<const unsigned*>(b + B::value_low(2 * q4, g));
+        lb = *reinterpret_cast<const unsigned*>(b + B::value_low(2 * q4 + 8, g));
+        if (!whole) {
+          const int r = mt * 16 + 2 * q4;
+          la &= (seen(r) ? 0xffffu : 0u) | (seen(r + 1) ? 0xffff0000u : 0u);
+          lb &= (seen(r + 8) ? 0xffffu : 0u) | (seen(r + 9) ? 0xffff0000u : 0u);
+        }
+      } else if (g == G) {
+        la = lb = 0x3f803f80u;
+      }
+      const unsigned lows[4] = {la, 0u, lb, 0u};
+      hb::mma_bf16(low, lows, transpose8(hb::pack_bf16(p[0], p[1])), transpose8(hb::pack_bf16(p[2], p[3])));
+      const Words<G> va(b + B::value_word(2 * q4, g, 0)), vb(b + B::value_word(2 * q4 + 8, g, 0));
+      const bool see_a = whole || seen(mt * 16 + g), see_b = whole || seen(mt * 16 + g + 8);
+#pragma unroll
+      for (int c = 0; c < G; ++c) {
+        const unsigned sa = *reinterpret_cast<const unsigned*>(b + B::scale(g, 1, c & ~1)),
+                       sb = *reinterpret_cast<const unsigned*>(b + B::scale(g + 8, 1, c & ~1));
+        const float fa = see_a ? (c & 1 ? high_half(sa) : low_half(sa)) : 0.f, fb_ = see_b ? (c & 1 ? high_half(sb) : low_half(sb)) : 0.f;
+        const unsigned x = transpose8(hb::pack_bf16(p[0] * fa, p[1] * fa)), y = transpose8(hb::pack_bf16(p[2] * fb_, p[3] * fb_));
+        unsigned wa = va.w[c], wb = vb.w[c];
+        const unsigned a0[4] = {wa & fb::LOW, wa & fb::HIGH, wb & fb::LOW, wb & fb::HIGH};
+        hb::mma_bf16(o[2 * c], a0, x, y);
+        wa >>= 8;
+        wb >>= 8;
+        const unsigned a1[4] = {wa & fb::LOW, wa & fb::HIGH, wb & fb::LOW, wb & fb::HIGH};
+        hb::mma_bf16(o[2 * c + 1], a1, x, y);
+      }
+    }
+    __syncwarp();                                                 // all lanes are through with the stage
+    if (asked < steps) bring(asked++);
+  }
+  if (!ok) {                                                      // no copy is under way when the block ends
+    for (int i = max(0, asked - STAGES); i < asked; ++i) tc::mbar_wait_warp(&full[warp][i % STAGES], (i / STAGES) & 1);
+  }
+
+  // this warp's sums in their size, over 2^64 still: o, and per head the sum of weights
+  constexpr float DOWN = 1.f / 18446744073709551616.f;            // 2^-64
+  float l_run[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) l_run[h] = __shfl_sync(0xffffffffu, low[h], 4 * G + q4) * DOWN;
+#pragma unroll
+  for (int c = 0; c < G; ++c) {
+    const float mean[2] = {__shfl_sync(0xffffffffu, low[0], 4 * c + q4) * DOWN, __shfl_sync(0xffffffffu, low[1], 4 * c + q4) * DOWN};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[2 * c + i][e] = fmaf(o[2 * c + i][e], e < 2 ? fb::UNSCALE : fb::UNSCALE / 16.f, mean[e & 1]);
+  }
+  __syncthreads();                                                // every warp is through with its ring
+  float* o_s = reinterpret_cast<float*>(ring_all);                // [WARPS][HEADS][HD]
+  if (g == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      ml_s[warp][2 * q4 + h][0] = m_run[h];
+      ml_s[warp][2 * q4 + h][1] = l_run[h];
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < G; ++c)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *reinterpret_cast<float4*>(o_s + (warp * HEADS + 2 * q4 + h) * HD + c * 32 + g * 4) =
+          make_float4(o[2 * c][h], o[2 * c][2 + h], o[2 * c + 1][h], o[2 * c + 1][2 + h]);
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * (HD / 4); i += WARPS * 32) {
+    const int h = i / (HD / 4), d = i % (HD / 4) * 4;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, ml_s[w][h][0]);
+    float l = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (ml_s[w][h][1] == 0.f) continue;                         // no key of its steps is the token's
+      const float f = exp2_fast(ml_s[w][h][0] - m);
+      const float4 v = *reinterpret_cast<const float4*>(o_s + (w * HEADS + h) * HD + d);
+      l = fmaf(ml_s[w][h][1], f, l);
+      sum.x = fmaf(v.x, f, sum.x);
+      sum.y = fmaf(v.y, f, sum.y);
+      sum.z = fmaf(v.z, f, sum.z);
+      sum.w = fmaf(v.w, f, sum.w);
+    }
+    // of scores, not of their base-2 form; a row with a NaN says so in both numbers
+    const float m_nat = l != l ? l : m * 0.6931471805599453f;
+    if (a.splits > 1) {
+      const size_t at = (part0 + h) * a.splits + split;
+      *reinterpret_cast<float4*>(a.part_acc + at * HD + d) = sum;
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_nat, l);
+    } else {
+      if (a.sink && l > 0.f) l += expf((a.sink_values ? a.sink_values[kvh * per + h0 + h] : 0.f) - m_nat);
+      const float inv = l > 0.f ? 1.f / l : l;                    // (a NaN stays one)
+      *reinterpret_cast<uint2*>(a.out + (row0 + h) * HD + d) =
+          make_uint2(hb::pack_bf16(sum.x * inv, sum.y * inv), hb::pack_bf16(sum.z * inv, sum.w * inv));
+    }
+  }
+}
+
+}  // namespace
+
+extern "C" int hb_attention_decode_4bit(const void* q, const void* pages, const int* block_table, int table_stride,
+                                        const int* seq_of_token, const int* positions, void* out, int n_tokens, int nh, int nkv, int hd,
+                                        int page_size, int chunk, int window, int keep, float scale, int sink,
+                                        const float* sink_values, int split_tiles, int splits, float* part_acc, float* part_ml,
+                                        int* status, const long long* rows, int step_tokens, cudaStream_t stream) {
+  if (!q || !pages || !block_table || !seq_of_token || !positions || !out || !status || n_tokens < 0 || nh <= 0 || nkv <= 0 ||
+      nh % nkv || table_stride <= 0 || chunk < 0 || window < 0 || keep < 0 || split_tiles < 1 || splits < 1 ||
+      (splits > 1 && (!part_acc || !part_ml)))
+    return HB_ERR_BAD_ARG;
+  if ((hd != 64 && hd != 128) || !(page_size == 16 || page_size == 32 || (page_size > 0 && page_size % 64 == 0))) return HB_ERR_UNSUPPORTED;
+  const int tiles = (nh / nkv + HEADS - 1) / HEADS;
+  if (n_tokens > 65535 || (long long)nkv * tiles > 65535) return HB_ERR_UNSUPPORTED;
+  if (n_tokens == 0) return HB_OK;
+  const Args a{(const __nv_bfloat16*)q, (const uint8_t*)pages, block_table, seq_of_token, positions, (__nv_bfloat16*)out, part_acc,
+               part_ml, status, rows, sink_values, rows ? step_tokens : n_tokens, table_stride, nh, nkv, page_size, chunk, window, keep,
+               split_tiles, splits, sink, scale};
+  const dim3 grid(splits, nkv * tiles, n_tokens);
+  const int smem = WARPS * STAGES * (STEP / 16) * 20 * hd;        // blocks of 20 hd bytes; the sums at the end take less
+  auto* kernel = hd == 128 ? attn_decode_4bit_kernel<4> : attn_decode_4bit_kernel<2>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return (int)e;
+  kernel<<<grid, WARPS * 32, smem, stream>>>(a);
+  HB_LAUNCH_CHECK();
+  return HB_OK;
+}

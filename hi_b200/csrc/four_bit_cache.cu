@@ -1,0 +1,308 @@
+// The cache in four bits: the append of a step's keys and values, and the expansion of pages for the kernels that read bfloat16.
+//
+// A row of a head is cut into groups of 32 dims. With y the row's values in bfloat16, as the bfloat16 cache would hold them:
+//   low = min y, scale = bfloat16((max y - low) / 15), code = round((y - low) / scale) held to 0 .. 15;  y ~ scale * code + low
+// (float32 division; a group of one value has scale 0 and codes 0). The scale is rounded to bfloat16 because it is kept so, 32 bits a
+// group beside 128 of codes, and the codes are taken with the rounded one. A group that holds a value that is not finite is kept as
+// scale = low = NaN, so that it shows wherever it is read, as it would from a bfloat16 cache.
+//
+// Both kernels are bound by memory, and in decode steps by their launch. The append's stores are 2 and 4 bytes each, as the attention
+// kernel's order of the codes has it (four_bit.cuh); they meet in L2.
+#include "api.h"
+#include "common.cuh"
+#include "four_bit.cuh"
+
+namespace {
+
+struct Post {
+  const __nv_bfloat16* qkv;
+  const float* inv_freq;
+  const float* q_w;
+  const float* k_w;
+  const int* positions;
+  const int* seq_of_token;
+  const int* block_table;
+  __nv_bfloat16* q_out;
+  uint8_t* pages;
+  int rot_pairs, interleaved, qk_norm, temp_on, norm_first, norm_dim, v_is_k;
+  float qk_eps, floor_scale, attn_scale, rot_mul;
+  int table_stride, page_size, write_kv, n_tokens, nh, nkv;
+};
+
+__device__ __forceinline__ float group_min(float v) {      // over 8 neighbouring lanes
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Four dims of a row a lane, eight lanes a group: codes, scale and low. Every lane of the warp calls it.
+struct Quantised { unsigned codes; __nv_bfloat16 scale, low; };
+__device__ __forceinline__ Quantised quantise(const float (&y)[4]) {
+  const float low = group_min(fminf(fminf(y[0], y[1]), fminf(y[2], y[3])));
+  const float high = -group_min(-fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) finite = finite && fabsf(y[i]) <= 3.4028234663852886e38f;
+  const unsigned all = __ballot_sync(0xffffffffu, finite);
+  const bool whole = (all >> (threadIdx.x & 24) & 0xffu) == 0xffu;
+  Quantised r;
+  r.scale = __float2bfloat16_rn((high - low) / 15.f);
+  r.low = __float2bfloat16_rn(low);                        // exact
+  const float step = __bfloat162float(r.scale);
+  r.codes = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float c = step > 0.f ? fminf(fmaxf(rintf((y[i] - low) / step), 0.f), 15.f) : 0.f;
+    r.codes |= (unsigned)c << (4 * i);
+  }
+  if (!whole) {
+    r.codes = 0;
+    r.scale = r.low = __ushort_as_bfloat16(0x7fffu);
+  }
+  return r;
+}
+
+// A block is one token; a head is taken by hd / 4 lanes, four neighbouring dims each. The rotation's partners meet in shared memory.
+template <int G>
+__global__ void __launch_bounds__(256) qkv_post_4bit_kernel(const Post a) {
+  constexpr int HD = 32 * G, LPH = HD / 4, HPW = 32 / LPH;
+  using B = fb::Block<G>;
+  __shared__ float cs[HD / 2], sn[HD / 2];
+  __shared__ float rows[8][HPW * HD];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int li = lane % LPH, t = blockIdx.x, pos = a.positions[t];
+  for (int j = threadIdx.x; j < a.rot_pairs; j += blockDim.x) {
+    float s, c;
+    sincosf((float)pos * a.inv_freq[j], &s, &c);
+    sn[j] = s * a.rot_mul;
+    cs[j] = c * a.rot_mul;
+  }
+  __syncthreads();
+  const int heads = a.nh + (a.v_is_k ? 1 : 2) * a.nkv, todo = a.write_kv ? heads : a.nh;
+  int page = -1;
+  if (a.write_kv && pos >= 0) page = a.block_table[(size_t)a.seq_of_token[t] * a.table_stride + pos / a.page_size];
+  float* row = rows[warp] + lane / LPH * HD;
+  const int d0 = 4 * li, group = d0 / 32, rot = 2 * a.rot_pairs;
+  for (int h0 = (blockIdx.y * warps + warp) * HPW; h0 < todo; h0 += gridDim.y * warps * HPW) {
+    const int head = h0 + lane / LPH;
+    const bool active = head < todo;
+    const int kind = head < a.nh ? 0 : head < a.nh + a.nkv ? 1 : 2;
+    float y[4], raw[4];
+    {
+      uint2 v = make_uint2(0u, 0u);
+      if (active) v = *reinterpret_cast<const uint2*>(a.qkv + ((size_t)t * heads + head) * HD + d0);
+      raw[0] = y[0] = __uint_as_float(v.x << 16);
+      raw[1] = y[1] = __uint_as_float(v.x & 0xffff0000u);
+      raw[2] = y[2] = __uint_as_float(v.y << 16);
+      raw[3] = y[3] = __uint_as_float(v.y & 0xffff0000u);
+    }
+    if (a.norm_first && a.qk_norm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ss += d0 + i < a.norm_dim ? y[i] * y[i] : 0.f;
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float inv = rsqrtf(ss / (float)a.norm_dim + a.qk_eps);
+      const float* w = kind == 0 ? a.q_w : a.k_w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] *= kind == 2 ? 1.f : inv * (w ? w[d0 + i] : 1.f);
+    }
+    __syncwarp();
+    if (rot > 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) row[d0 + i] = y[i];
+      __syncwarp();
+      if (kind != 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = d0 + i;
+          if (d >= rot) continue;
+          const int j = a.interleaved ? d >> 1 : d < a.rot_pairs ? d : d - a.rot_pairs;
+          const bool second = a.interleaved ? d & 1 : d >= a.rot_pairs;
+          const float other = row[a.interleaved ? d ^ 1 : second ? d - a.rot_pairs : d + a.rot_pairs];
+          y[i] = second ? y[i] * cs[j] + other * sn[j] : y[i] * cs[j] - other * sn[j];
+        }
+      __syncwarp();
+    }
+    if (!a.norm_first && a.qk_norm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ss += d0 + i < a.norm_dim ? y[i] * y[i] : 0.f;
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float inv = rsqrtf(ss / (float)a.norm_dim + a.qk_eps);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] *= kind == 2 ? 1.f : inv;
+    }
+    if (kind == 0 && a.temp_on) {
+      const float mul = logf(floorf(((float)pos + 1.f) / a.floor_scale) + 1.f) * a.attn_scale + 1.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] *= mul;
+    }
+    const uint2 packed = make_uint2(hb::pack_bf16(y[0], y[1]), hb::pack_bf16(y[2], y[3]));
+    if (kind == 0 && active) *reinterpret_cast<uint2*>(a.q_out + ((size_t)t * a.nh + head) * HD + d0) = packed;
+    if (!a.write_kv || __all_sync(0xffffffffu, kind == 0)) continue;
+    y[0] = __uint_as_float(packed.x << 16);
+    y[1] = __uint_as_float(packed.x & 0xffff0000u);
+    y[2] = __uint_as_float(packed.y << 16);
+    y[3] = __uint_as_float(packed.y & 0xffff0000u);
+    const int kvh = kind == 0 ? 0 : kind == 1 ? head - a.nh : head - a.nh - a.nkv;
+    const bool writes = active && kind != 0 && page >= 0;      // the host reserves pages before the step
+    const int at = pos >= 0 ? pos % a.page_size : 0, r = at % fb::BLOCK_ROWS;
+    uint8_t* block = a.pages + (((size_t)(writes ? page : 0) * a.nkv + kvh) * (a.page_size / fb::BLOCK_ROWS) + at / fb::BLOCK_ROWS) * B::BYTES;
+    const Quantised z = quantise(y);
+    // a key's word: even dims in the lower half; two lanes share it
+    unsigned word = (z.codes & 0xfu) | (z.codes & 0xf0u) << 12 | (z.codes & 0xf00u) >> 4 | (z.codes & 0xf000u) << 8;
+    if (li & 1) word <<= 8;
+    word |= __shfl_xor_sync(0xffffffffu, word, 1);
+    if (writes && kind == 1) {
+      if (!(li & 1)) *reinterpret_cast<unsigned*>(block + B::key_word(r, (li % 8) / 2, group)) = word;
+      if (li % 8 == 0) {
+        *reinterpret_cast<__nv_bfloat16*>(block + B::scale(r, 0, group)) = z.scale;
+        *reinterpret_cast<__nv_bfloat16*>(block + B::key_low(r, group)) = z.low;
+      }
+    }
+    Quantised v = z;
+    if (a.v_is_k) v = quantise(raw);                         // the key as projected is the value
+    if (writes && (kind == 2 || a.v_is_k)) {
+      *reinterpret_cast<uint16_t*>(block + B::value_word(r, li % 8, group) + (r & 1) * 2) = (uint16_t)v.codes;
+      if (li % 8 == 0) {
+        *reinterpret_cast<__nv_bfloat16*>(block + B::scale(r, 1, group)) = v.scale;
+        *reinterpret_cast<__nv_bfloat16*>(block + B::value_low(r, group)) = v.low;
+      }
+    }
+  }
+}
+
+// ---- pages of the step's portions as bfloat16. Request s needs its pages first_s .. last_s: from the oldest position that its first
+// new token may read to its last one; they lie side by side in the result, request after request, and `table` [n_seqs, table_stride]
+// says where (entries outside first_s .. last_s are left at 0: no kernel that is told of the same mask reads them).
+struct Expand {
+  const uint8_t* pages;
+  const int* block_table;
+  const int* cu_seqlens;
+  const int* positions;
+  __nv_bfloat16* k;
+  __nv_bfloat16* v;
+  int* table;
+  int n_seqs, table_stride, page_size, chunk, window, keep, skip_single, nkv, total;
+};
+
+__device__ __forceinline__ void span(const Expand& a, int s, int& first, int& count) {
+  const int begin = a.cu_seqlens[s], n = a.cu_seqlens[s + 1] - begin;
+  first = count = 0;
+  if (n <= 0 || (n == 1 && a.skip_single)) return;
+  const int start = a.positions[begin];
+  int lo = 0;
+  if (a.chunk > 0) lo = start / a.chunk * a.chunk;
+  else if (a.window > 0 && a.keep == 0) lo = max(0, start - a.window + 1);
+  first = lo / a.page_size;
+  count = (start + n - 1) / a.page_size - first + 1;
+}
+
+template <int G>
+__global__ void __launch_bounds__(128) expand_4bit_kernel(const Expand a) {
+  constexpr int HD = 32 * G;
+  using B = fb::Block<G>;
+  __shared__ int found[2];
+  const int out_page = blockIdx.x, kvh = blockIdx.y, lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {          // whose page is this? the requests' counts are summed 32 at a time
+    int before = 0, seq = -1, index = 0;
+    for (int s0 = 0; s0 < a.n_seqs && seq < 0; s0 += 32) {
+      int first = 0, count = 0;
+      if (s0 + lane < a.n_seqs) span(a, s0 + lane, first, count);
+      int upto = count;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + upto > out_page);
+      const int who = hit ? __ffs(hit) - 1 : 0;
+      const int start = __shfl_sync(0xffffffffu, before + upto - count, who), from = __shfl_sync(0xffffffffu, first, who);
+      if (hit) { seq = s0 + who; index = from + out_page - start; }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) { found[0] = seq; found[1] = index; }
+  }
+  __syncthreads();
+  const int seq = found[0], index = found[1];
+  if (seq < 0 || index >= a.table_stride) return;
+  const int page = a.block_table[(size_t)seq * a.table_stride + index];
+  if (kvh == 0 && threadIdx.x == 0) a.table[(size_t)seq * a.table_stride + index] = page < 0 ? -1 : out_page;
+  const size_t out = ((size_t)out_page * a.nkv + kvh) * a.page_size * HD;
+  if (page < 0) return;
+  const uint8_t* from = a.pages + ((size_t)page * a.nkv + kvh) * (a.page_size / fb::BLOCK_ROWS) * B::BYTES;
+  auto number = [](const uint8_t* p) { return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p)); };
+  for (int i = threadIdx.x; i < a.page_size * 4 * G; i += blockDim.x) {      // eight dims of a key
+    const int row = i / (4 * G), r = row % fb::BLOCK_ROWS, group = i % (4 * G) / 4, q = i % 4;
+    const uint8_t* block = from + row / fb::BLOCK_ROWS * B::BYTES;
+    const unsigned w = *reinterpret_cast<const unsigned*>(block + B::key_word(r, q, group));
+    const float scale = number(block + B::scale(r, 0, group)), low = number(block + B::key_low(r, group));
+    unsigned o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o[e] = hb::pack_bf16(fmaf(scale, (float)(w >> (4 * e) & 15), low), fmaf(scale, (float)(w >> (16 + 4 * e) & 15), low));
+    *reinterpret_cast<uint4*>(a.k + out + (size_t)row * HD + group * 32 + q * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+  for (int i = threadIdx.x; i < a.page_size / 2 * 8 * G; i += blockDim.x) {  // four dims of the values of two tokens
+    const int row = i / (8 * G) * 2, r = row % fb::BLOCK_ROWS, group = i % (8 * G) / 8, g = i % 8;
+    const uint8_t* block = from + row / fb::BLOCK_ROWS * B::BYTES;
+    const unsigned w = *reinterpret_cast<const unsigned*>(block + B::value_word(r, g, group));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float scale = number(block + B::scale(r + e, 1, group)), low = number(block + B::value_low(r + e, group));
+      const unsigned c = w >> (16 * e);
+      *reinterpret_cast<uint2*>(a.v + out + (size_t)(row + e) * HD + group * 32 + g * 4) = make_uint2(
+          hb::pack_bf16(fmaf(scale, (float)(c & 15), low), fmaf(scale, (float)(c >> 4 & 15), low)),
+          hb::pack_bf16(fmaf(scale, (float)(c >> 8 & 15), low), fmaf(scale, (float)(c >> 12 & 15), low)));
+    }
+  }
+}
+
+bool good_page(int page_size) { return page_size == 16 || page_size == 32 || (page_size > 0 && page_size % 64 == 0); }
+
+}  // namespace
+
+extern "C" int hb_qkv_post_4bit(const void* qkv, const float* inv_freq, int rot_pairs, int interleaved, int qk_norm, float qk_eps,
+                                int temp_on, float floor_scale, float attn_scale, const float* q_norm_w, const float* k_norm_w,
+                                int norm_first, int norm_dim, float rot_mul, int v_is_k, const int* positions,
+                                const int* seq_of_token, const int* block_table, int table_stride, void* q_out, void* pages,
+                                int page_size, int write_kv, int n_tokens, int nh, int nkv, int hd, cudaStream_t stream) {
+  if (!qkv || !positions || !q_out || n_tokens < 0 || nh <= 0 || nkv <= 0) return HB_ERR_BAD_ARG;
+  if (write_kv && (!pages || !block_table || !seq_of_token || table_stride <= 0)) return HB_ERR_BAD_ARG;
+  if (!inv_freq) rot_pairs = 0;
+  if (norm_dim <= 0) norm_dim = hd;
+  if (rot_pairs < 0 || norm_dim > hd || 2 * rot_pairs > norm_dim || (temp_on && !(floor_scale > 0.f))) return HB_ERR_BAD_ARG;
+  // a weightless norm after a rotation keeps its sum of squares only where the rotation keeps lengths
+  if ((hd != 64 && hd != 128) || !good_page(page_size) || (qk_norm && !norm_first && (rot_mul != 1.f || q_norm_w || k_norm_w)))
+    return HB_ERR_UNSUPPORTED;
+  if (n_tokens == 0) return HB_OK;
+  const Post a{(const __nv_bfloat16*)qkv, inv_freq, q_norm_w, k_norm_w, positions, seq_of_token, block_table, (__nv_bfloat16*)q_out,
+               (uint8_t*)pages, rot_pairs, interleaved, qk_norm, temp_on, norm_first, norm_dim, v_is_k, qk_eps, floor_scale, attn_scale,
+               rot_mul, table_stride, page_size, write_kv, n_tokens, nh, nkv};
+  const int heads = nh + (v_is_k ? 1 : 2) * nkv, per_warp = hd == 64 ? 2 : 1;
+  const int all = (heads + per_warp - 1) / per_warp;
+  const dim3 grid(n_tokens, n_tokens < 148 ? (all + 7) / 8 : 1);      // few tokens: a warp a head, many: the sines are worth sharing
+  if (hd == 128) qkv_post_4bit_kernel<4><<<grid, 256, 0, stream>>>(a);
+  else qkv_post_4bit_kernel<2><<<grid, 256, 0, stream>>>(a);
+  HB_LAUNCH_CHECK();
+  return HB_OK;
+}
+
+extern "C" int hb_expand_pages_4bit(const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
+                                    const int* positions, int n_seqs, int total, int page_size, int chunk, int window, int keep,
+                                    int skip_single, int nkv, int hd, void* k, void* v, int* table, cudaStream_t stream) {
+  if (!pages || !block_table || !cu_seqlens || !positions || !table || n_seqs < 0 || total < 0 || nkv <= 0 || table_stride <= 0 ||
+      chunk < 0 || window < 0 || keep < 0 || (total > 0 && (!k || !v)))
+    return HB_ERR_BAD_ARG;
+  if ((hd != 64 && hd != 128) || !good_page(page_size) || nkv > 65535) return HB_ERR_UNSUPPORTED;
+  if (n_seqs == 0 || total == 0) return HB_OK;
+  const Expand a{(const uint8_t*)pages, block_table, cu_seqlens, positions, (__nv_bfloat16*)k, (__nv_bfloat16*)v, table, n_seqs,
+                 table_stride, page_size, chunk, window, keep, skip_single, nkv, total};
+  const dim3 grid(total, nkv);
+  if (hd == 128) expand_4bit_kernel<4><<<grid, 128, 0, stream>>>(a);
+  else expand_4bit_kernel<2><<<grid, 128, 0, stream>>>(a);
+  HB_LAUNCH_CHECK();
+  return HB_OK;
+}

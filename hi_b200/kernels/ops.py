@@ -36,6 +36,10 @@ _SIGNATURES = {
     "hb_convert": [P, I, P, I, c_longlong, P],
     "hb_moe_combine": [P, P, P, P, I, P, I, I, I, P],
     "hb_qkv_post": [P, I, P, I, I, I, F, I, F, F, P, P, I, I, F, P, I, I, I, P, P, P, I, P, P, P, I, I, I, I, I, I, P],
+    "hb_qkv_post_4bit": [P, P, I, I, I, F, I, F, F, P, P, I, I, F, I, P, P, P, I, P, P, I, I, I, I, I, I, P],
+    "hb_expand_pages_4bit": [P, P, I, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P],
+    "hb_attention_decode_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, P, I, I, P, P, P, P, I, P],
+    "hb_four_bit_linear": [P, c_longlong, P, P, P, I, I, I, I, I, P],
     "hb_paged_attention": [P, I, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, F, P, P, I, I, P, P, P],
     "hb_attention_portions": [P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, F, I, F, P, P, I, P, P, P],
     "hb_attention_merge": [P, P, P, I, I, I, I, I, I, P, P],
@@ -2467,3 +2471,277 @@ def ranked_rows(logits: torch.Tensor, temperatures: torch.Tensor, top_ps: torch.
             raise KernelError(f"{nm} needs one entry per row")
     _check(lib().hb_ranked_rows(_ptr(logits), rows, logits.shape[1], _ptr(temperatures), _ptr(top_ps), _ptr(top_ks),
                                 _ptr(uniforms), _ptr(out), _stream()), "ranked_rows")
+
+
+# --------------------------------------------------------------------------- four bits
+FOUR_BIT_GROUPS = (32, 64, 128)      # inputs of a weight's row that share a scale
+FOUR_BIT_ROW_LENGTHS = (64, 128)     # head sizes of the 4-bit cache
+
+
+def _on_current_device(*tensors) -> None:
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != device:
+            raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{device}")
+
+
+class FourBitWeight:
+    """A weight [M, K] held in four bits: w[m, k] = scale[m, k // group] * (code[m, k] - 8). ``blocks`` is its bytes as the kernels
+    read them (csrc/four_bit_linear.cu): uint8 [ceil(M / 16), ceil(K / 128), 1024 + 32 * (128 / group)]. ``ops.pack_weight`` and
+    ``ops.quantize_weight`` make one; ``parts.linear.linear`` takes it in a weight's place."""
+
+    dtype = torch.bfloat16           # of what it is multiplied with
+
+    def __init__(self, blocks: torch.Tensor, shape, group: int):
+        self.blocks, self.shape, self.group = blocks, tuple(shape), int(group)
+
+    @property
+    def device(self):
+        return self.blocks.device
+
+
+def pack_weight(codes: torch.Tensor, scales: torch.Tensor) -> FourBitWeight:
+    """``codes`` uint8 [M, K] of 0 .. 15 and ``scales`` bfloat16 [M, K / group] (group 32, 64 or 128) as a :class:`FourBitWeight`.
+    Once, when a model is loaded; works on any device."""
+    if codes.dim() != 2 or codes.dtype != torch.uint8 or scales.dim() != 2 or scales.dtype != torch.bfloat16 or \
+            scales.shape[0] != codes.shape[0] or codes.device != scales.device:
+        raise KernelError("a 4-bit weight is uint8 codes [M, K] and bfloat16 scales [M, K / group] on one device")
+    (m, k), groups = codes.shape, scales.shape[1]
+    group = k // groups if groups and k % groups == 0 else 0
+    if m == 0 or group not in FOUR_BIT_GROUPS:
+        raise KernelError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)}: groups of {FOUR_BIT_GROUPS} are taken")
+    tiles, chunks, per = -(-m // 16), -(-k // 128), 128 // group
+    c = torch.full((tiles * 16, chunks * 128), 8, dtype=torch.uint8, device=codes.device)
+    c[:m, :k] = codes & 15
+    c = c.view(tiles, 16, chunks, 4, 4, 8).permute(0, 2, 1, 4, 3, 5)          # [tile, chunk, row, lane, word, eight k]
+    c = c[..., [0, 4, 1, 5]] | c[..., [2, 6, 3, 7]] << 4
+    s = torch.zeros((tiles * 16, chunks * per), dtype=torch.bfloat16, device=codes.device)
+    s[:m, : groups] = scales
+    s = s.view(tiles, 16, chunks, per).transpose(1, 2).contiguous().view(torch.uint8)
+    blocks = torch.cat([c.reshape(tiles, chunks, 1024), s.view(tiles, chunks, 32 * per)], dim=2).contiguous()
+    return FourBitWeight(blocks, (m, k), group)
+
+
+def quantize_weight(weight: torch.Tensor, group: int = 64) -> FourBitWeight:
+    """A floating weight [M, K] in four bits: a group's scale is a seventh of its largest magnitude, rounded to bfloat16, and
+    the codes are taken with the rounded scale. A group with a value that is not finite becomes NaN."""
+    if weight.dim() != 2 or not weight.dtype.is_floating_point or group not in FOUR_BIT_GROUPS or weight.shape[1] % group:
+        raise KernelError(f"a weight [M, K] with K a multiple of the group ({FOUR_BIT_GROUPS}) is quantised, "
+                          f"not {tuple(weight.shape)} in groups of {group}")
+    codes, scales = [], []
+    for rows in weight.split(max(1, (1 << 27) // max(weight.shape[1], 1))):          # a part at a time: float32 copies are large
+        w = rows.to(torch.float32).unflatten(1, (-1, group))
+        scale = (w.abs().amax(-1) / 7.0).to(torch.bfloat16)
+        scale = torch.where(torch.isfinite(w).all(-1), scale, torch.full_like(scale, float("nan")))
+        step = scale.to(torch.float32).unsqueeze(-1)
+        code = torch.where(step > 0, (w / step).round().clamp(-8, 7), torch.zeros_like(w))
+        codes.append((code + 8).to(torch.uint8).flatten(1))
+        scales.append(scale)
+    return pack_weight(torch.cat(codes), torch.cat(scales))
+
+
+def four_bit_linear(x: torch.Tensor, weight: FourBitWeight, out_dtype: torch.dtype = torch.bfloat16,
+                    bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x @ weight.T (+ bias)`` for bfloat16 ``x`` [N, K] (its rows may be a column slice of a wider matrix) and a weight held in
+    four bits, with float32 sums, in ``out_dtype`` (bfloat16 or float32); ``bias`` bfloat16 [M]."""
+    if not x.is_cuda:
+        raise KernelError("x must be a CUDA tensor; this engine has no CPU path")
+    m, k = weight.shape
+    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != k or out_dtype not in (torch.bfloat16, torch.float32):
+        raise KernelError(f"a 4-bit weight {weight.shape} multiplies bfloat16 [N, {k}] into bfloat16 or float32, "
+                          f"not {x.dtype} {tuple(x.shape)} into {out_dtype}")
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        raise KernelError("products with 4-bit weights have no gradients")
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) % 8) or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    if bias is not None:
+        _need(bias, "bias", torch.bfloat16)
+        if bias.numel() != m:
+            raise KernelError(f"bias has {bias.numel()} elements for {m} outputs")
+    _need(weight.blocks, "weight", torch.uint8)
+    _on_current_device(x, weight.blocks, bias)
+    n = x.shape[0]
+    out = torch.empty((n, m), dtype=out_dtype, device=x.device)
+    if n == 0:
+        return out
+    _check(lib().hb_four_bit_linear(_ptr(x), x.stride(0) if n > 1 else k, _ptr(weight.blocks), _ptr(bias), _ptr(out), _dt(out), n, m,
+                                    k, weight.group, _stream()), "four_bit_linear")
+    return out
+
+
+def four_bit_page_bytes(page_size: int, hd: int) -> int:
+    """Bytes of one head's page in the 4-bit cache: keys and values, codes, scales and lows (a row of ``hd`` dims takes 10/8 hd)."""
+    if hd not in FOUR_BIT_ROW_LENGTHS or not (page_size in (16, 32) or (page_size > 0 and page_size % 64 == 0)):
+        raise KernelError(f"a 4-bit cache has heads of {FOUR_BIT_ROW_LENGTHS} and pages of 16, 32 or a multiple of 64 positions, "
+                          f"not heads of {hd} and pages of {page_size}")
+    return page_size * hd * 5 // 4
+
+
+def _four_bit_pages(kv_pages: torch.Tensor, hd: int) -> Tuple[int, int, int]:
+    """(pages, kv heads, page size) of a 4-bit pool."""
+    _need(kv_pages, "kv_pages", torch.uint8)
+    if kv_pages.dim() != 3 or hd not in FOUR_BIT_ROW_LENGTHS or kv_pages.shape[2] % (hd * 5 // 4) or kv_pages.data_ptr() % 16:
+        raise KernelError(f"4-bit cache pages are uint8 [pages, kv_heads, four_bit_page_bytes(page_size, {hd})] on 16 bytes")
+    page_size = kv_pages.shape[2] // (hd * 5 // 4)
+    four_bit_page_bytes(page_size, hd)
+    return kv_pages.shape[0], kv_pages.shape[1], page_size
+
+
+def _step_tables(n: int, block_table, seq_of_token, positions) -> None:
+    for t, nm in ((block_table, "block_table"), (seq_of_token, "seq_of_token"), (positions, "positions")):
+        _need(t, nm, torch.int32)
+    if seq_of_token.numel() < n or positions.numel() < n or block_table.dim() != 2:
+        raise KernelError("seq_of_token and positions hold a number for every token, block_table is [requests, width]")
+
+
+def qkv_post_4bit(qkv: torch.Tensor, nh: int, nkv: int, hd: int, positions: torch.Tensor, inv_freq: Optional[torch.Tensor],
+                  interleaved: bool, qk_norm: bool, qk_eps: float, temperature: Optional[Tuple[float, float]],
+                  seq_of_token: torch.Tensor, block_table: torch.Tensor, kv_pages: torch.Tensor, write_kv: bool = True,
+                  q_norm_weight: Optional[torch.Tensor] = None, k_norm_weight: Optional[torch.Tensor] = None,
+                  norm_first: bool = False, norm_dim: int = 0, rot_mul: float = 1.0, values_are_keys: bool = False) -> torch.Tensor:
+    """:func:`qkv_post` for a cache held in four bits: the same encoding of q, k and v from bfloat16 ``qkv``, after which the rows of
+    k and v are quantised in groups of 32 dims (a bfloat16 scale and a bfloat16 least value each) and appended to ``kv_pages``
+    (uint8 [pages, nkv, :func:`four_bit_page_bytes`]). Returns q [N, nh, hd]."""
+    _need(qkv, "qkv", torch.bfloat16)
+    _, nkv2, page_size = _four_bit_pages(kv_pages, hd)
+    n, columns = qkv.shape[0], (nh + (1 if values_are_keys else 2) * nkv) * hd
+    _step_tables(n, block_table, seq_of_token, positions)
+    if qkv.dim() != 2 or qkv.shape[1] != columns or nkv2 != nkv or qkv.data_ptr() % 8:
+        raise KernelError(f"qkv is [N, {columns}] on 8 bytes beside pages of {nkv} kv heads, not {tuple(qkv.shape)} beside {nkv2}")
+    rot_pairs = 0
+    if inv_freq is not None:
+        _need(inv_freq, "inv_freq", torch.float32)
+        rot_pairs = inv_freq.numel()
+    if 2 * rot_pairs > (norm_dim or hd) or norm_dim > hd:
+        raise KernelError("more rotating or normed dims than a head has")
+    for wt, nm in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
+        if wt is not None:
+            _need(wt, nm, torch.float32)
+            if wt.numel() != hd:
+                raise KernelError(f"{nm} needs one weight per dim of a head ({hd})")
+    if temperature is not None and not temperature[0] > 0:
+        raise KernelError("the temperature's scale of positions is above zero")
+    _on_current_device(qkv, positions, seq_of_token, block_table, kv_pages, inv_freq, q_norm_weight, k_norm_weight)
+    q = torch.empty((n, nh, hd), dtype=qkv.dtype, device=qkv.device)
+    if n == 0:
+        return q
+    fs, asc = temperature if temperature is not None else (1.0, 0.0)
+    _check(lib().hb_qkv_post_4bit(_ptr(qkv), _ptr(inv_freq), rot_pairs, int(interleaved), int(qk_norm), float(qk_eps),
+                                  int(temperature is not None), float(fs), float(asc), _ptr(q_norm_weight), _ptr(k_norm_weight),
+                                  int(norm_first), int(norm_dim), float(rot_mul), int(values_are_keys), _ptr(positions),
+                                  _ptr(seq_of_token), _ptr(block_table), block_table.shape[1], _ptr(q), _ptr(kv_pages), page_size,
+                                  int(write_kv), n, nh, nkv, hd, _stream()), "qkv_post_4bit")
+    return q
+
+
+def expand_pages_4bit(kv_pages: torch.Tensor, hd: int, block_table: torch.Tensor, cu_seqlens: torch.Tensor, positions: torch.Tensor,
+                      start_pos, n_new, chunk: int = 0, window: int = 0, keep: int = 0, skip_single: bool = False):
+    """The pages that the step's new tokens may read, in bfloat16: ``(k_pages, v_pages, table)`` with pages [P, nkv, page_size, hd],
+    request after request from the page of the oldest position that its first new token reads (``chunk``, ``window``, ``keep``
+    as in :func:`paged_attention`; with ``keep`` from the request's first page on) to its last token's, and the block table
+    that names them. Rows behind a request's last token hold whatever the pool holds there. ``start_pos`` and ``n_new`` are the host's
+    copies of what ``positions`` and ``cu_seqlens`` say on the device. ``skip_single``: requests of one new token are left out."""
+    _, nkv, page_size = _four_bit_pages(kv_pages, hd)
+    for t, nm in ((block_table, "block_table"), (cu_seqlens, "cu_seqlens"), (positions, "positions")):
+        _need(t, nm, torch.int32)
+    start_pos, n_new = list(start_pos), list(n_new)
+    n_seqs = len(n_new)
+    if len(start_pos) != n_seqs or cu_seqlens.numel() != n_seqs + 1 or block_table.dim() != 2 or block_table.shape[0] < n_seqs or \
+            positions.numel() < sum(n_new):
+        raise KernelError("start_pos, n_new, cu_seqlens and block_table do not speak of the same requests")
+    _on_current_device(kv_pages, block_table, cu_seqlens, positions)
+    total = 0
+    for start, n in zip(start_pos, n_new):
+        if n <= 0 or (n == 1 and skip_single):
+            continue
+        last = (start + n - 1) // page_size
+        if start < 0 or last >= block_table.shape[1]:
+            raise KernelError(f"positions {start} .. {start + n - 1} lie outside the block table's {block_table.shape[1]} pages")
+        low = start // chunk * chunk if chunk > 0 else max(0, start - window + 1) if window > 0 and not keep else 0
+        total += last - low // page_size + 1
+    k = torch.empty((total, nkv, page_size, hd), dtype=torch.bfloat16, device=kv_pages.device)
+    v = torch.empty_like(k)
+    table = torch.zeros_like(block_table)
+    if total == 0:
+        return k, v, table
+    _check(lib().hb_expand_pages_4bit(_ptr(kv_pages), _ptr(block_table), block_table.shape[1], _ptr(cu_seqlens), _ptr(positions), n_seqs,
+                                      total, page_size, int(chunk), int(window), int(keep), int(skip_single), nkv, hd, _ptr(k), _ptr(v),
+                                      _ptr(table), _stream()), "expand_pages_4bit")
+    return k, v, table
+
+
+@functools.lru_cache(maxsize=4096)
+def _four_bit_splits(tiles: int, groups: int) -> Tuple[int, int]:
+    """The cut of ``tiles`` tiles of 64 keys for the 4-bit decode kernel: (tiles of a split, splits)."""
+    best = (None, tiles, 1)
+    for s in range(1, max(1, min(tiles // 2, 64)) + 1):
+        size = -(-tiles // s)
+        real = -(-tiles // size)
+        waves = -(-(real * groups) // (148 * 4))
+        cost = waves * (4.0 + 0.35 * size) + (3.4 + 0.000215 * real * groups if real > 1 else 0.0)
+        if best[0] is None or cost < best[0]:
+            best = (cost, size, real)
+    return best[1], best[2]
+
+
+def decode_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table: torch.Tensor, seq_of_token: torch.Tensor,
+                          positions: torch.Tensor, chunk: int, window: int, scale: float, max_context: int, sink: bool = False,
+                          sink_values: Optional[torch.Tensor] = None, keep: int = 0, rows: Optional[torch.Tensor] = None,
+                          out: Optional[torch.Tensor] = None, most_keys: int = 0) -> torch.Tensor:
+    """:func:`decode_attention` over a cache held in four bits: every row of bfloat16 ``q`` [N, nh, hd] (or with ``rows``, int64 and distinct,
+    those tokens, into ``out``) is one request's token. ``chunk``, ``window``, ``keep``, ``sink``, ``sink_values``, ``max_context``,
+    ``most_keys`` as there."""
+    _need(q, "q", torch.bfloat16)
+    if q.dim() != 3:
+        raise KernelError("q is [tokens, heads, head_dim]")
+    n, nh, hd = q.shape
+    step_tokens = n
+    _, nkv, page_size = _four_bit_pages(kv_pages, hd)
+    if nh % nkv:
+        raise KernelError(f"{nh} query heads are not a multiple of {nkv} kv heads")
+    seq_of_token, positions = seq_of_token.contiguous(), positions.contiguous()
+    _step_tables(n, block_table, seq_of_token, positions)
+    if rows is not None:
+        rows = rows.contiguous()
+        _need(rows, "rows", torch.int64)
+        if out is None or out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            raise KernelError("tokens decoded in place need an output of the queries' shape and type")
+        n = rows.numel()
+    elif out is not None:
+        raise KernelError("an output is given with the rows that are decoded into it")
+    if sink_values is not None:
+        _need(sink_values, "sink_values", torch.float32)
+        if sink_values.numel() != nh:
+            raise KernelError("sink_values needs one number per query head")
+    _on_current_device(q, kv_pages, block_table, seq_of_token, positions, rows, out, sink_values)
+    longest = max(int(max_context), 1)
+    tiles = -(-longest // 64)
+    if chunk > 0:
+        tiles = min(tiles, -(-(chunk + 63) // 64))       # (a chunk that does not start on a tile straddles one more)
+    if window > 0:
+        tiles = min(tiles, -(-(window + 63) // 64) + -(-keep // 64))
+    split_tiles, splits = _four_bit_splits(tiles, n * nkv * -(-(nh // nkv) // 8))
+    if 0 < most_keys < 64 * split_tiles:
+        split_tiles = max(1, most_keys // 64)
+        splits = -(-tiles // split_tiles)
+    if rows is None:
+        out = torch.empty_like(q)
+    if n == 0:
+        return out
+    part_acc = part_ml = None
+    if splits > 1:
+        part_acc = torch.empty((n, nh, splits, hd), dtype=torch.float32, device=q.device)
+        part_ml = torch.empty((n, nh, splits, 2), dtype=torch.float32, device=q.device)
+    sink = bool(sink) or sink_values is not None
+    TC_USED[0] = True
+    _check(lib().hb_attention_decode_4bit(_ptr(q), _ptr(kv_pages), _ptr(block_table), block_table.shape[1], _ptr(seq_of_token),
+                                          _ptr(positions), _ptr(out), n, nh, nkv, hd, page_size, int(chunk), int(window), int(keep),
+                                          float(scale), int(sink), _ptr(sink_values), split_tiles, splits, _ptr(part_acc),
+                                          _ptr(part_ml), _ptr(_tc_status(q.device)), _ptr(rows), step_tokens, _stream()),
+           "attention_decode_4bit")
+    if splits > 1:
+        _check(lib().hb_attention_merge_rows(_ptr(part_acc), _ptr(part_ml), _ptr(out), _dt(out), n * nh, hd, splits, int(sink), nh,
+                                             _ptr(sink_values), _ptr(rows), step_tokens, _stream()), "attention_merge")
+    return out

@@ -59,7 +59,8 @@ def _key_splits(portions, rows: int, nh: int, nkv: int, hd: int, chunk: int, sli
 
 
 def attend_over_pages(q, k_pages, v_pages, block_table, ctx, nh: int, nkv: int, hd: int, chunk: int, sliding: int,
-                      scale: float, sink: bool = False, softcap: float = 0.0, slopes=None, sink_values=None, keep: int = 0):
+                      scale: float, sink: bool = False, softcap: float = 0.0, slopes=None, sink_values=None, keep: int = 0,
+                      decode=None):
     """softmax(q k^T scale + mask) v for the step's tokens over the paged keys and values that are in
     the cache already, by the kernel that fits the step: single decoded tokens, portions of prompts
     (with single tokens of other requests beside them), or the general kernel for what those refuse
@@ -68,15 +69,17 @@ def attend_over_pages(q, k_pages, v_pages, block_table, ctx, nh: int, nkv: int, 
     ``sink``: the softmax's denominator has one more term of score 0 (it has no value); ``sink_values``
     (float32 [nh]): of the head's own score instead. ``softcap`` > 0: scores become softcap tanh(score / softcap);
     ``slopes`` (float32 [nh]): slopes[head] * (distance to the key) is taken off after the cap.
-    ``keep``: first tokens of a request that a sliding window keeps."""
+    ``keep``: first tokens of a request that a sliding window keeps. ``decode(longest, rows, out, most_keys)``: how single
+    tokens are decoded, where their keys lie elsewhere than in ``k_pages`` and ``v_pages``."""
     positions = ctx.positions
     decode_ok = ops.decode_attention_supported(q.dtype, nh, nkv, hd)
 
-    def decode(longest, rows=None, out=None, most_keys=0):
+    def decode_pages(longest, rows=None, out=None, most_keys=0):
         return ops.decode_attention(q, k_pages, v_pages, block_table, ctx.seq_of_token, positions, chunk, sliding, scale, longest,
                                     sink=sink, softcap=softcap, slopes=slopes, sink_values=sink_values, keep=keep, rows=rows,
                                     out=out, most_keys=most_keys)
 
+    decode = decode or decode_pages
     if ctx.max_new == 1 and decode_ok:
         # every token of the step is one request's decoded token: the tensor-core kernel
         return decode(ctx.max_context)
@@ -128,6 +131,26 @@ def attend_over_pages(q, k_pages, v_pages, block_table, ctx, nh: int, nkv: int, 
     return ops.paged_attention(q, k_pages, v_pages, block_table, ctx.seq_of_token, positions,
                                chunk, sliding, scale, ctx.max_context, sink=sink, softcap=softcap, slopes=slopes,
                                sink_values=sink_values, keep=keep)
+
+
+def attend_over_four_bit_pages(q, kv_pages, block_table, ctx, nh: int, nkv: int, hd: int, chunk: int, sliding: int, scale: float,
+                               sink: bool = False, sink_values=None, keep: int = 0):
+    """:func:`attend_over_pages` over a cache held in four bits (``ops.qkv_post_4bit`` fills it). Single tokens read it as it is; for
+    portions of prompts the pages that they may read are expanded to bfloat16 once and go through the tensor-core kernels, which
+    read every key once a query tile."""
+    if q.shape != (ctx.n_tokens, nh, hd) or kv_pages.shape[1] != nkv:
+        raise ValueError(f"queries {tuple(q.shape)} and pages of {kv_pages.shape[1]} kv heads for {ctx.n_tokens} tokens, {nh} heads on {nkv}")
+
+    def decode(longest, rows=None, out=None, most_keys=0):
+        return ops.decode_attention_4bit(q, kv_pages, block_table, ctx.seq_of_token, ctx.positions, chunk, sliding, scale, longest,
+                                         sink=sink, sink_values=sink_values, keep=keep, rows=rows, out=out, most_keys=most_keys)
+
+    if ctx.max_new <= 1:
+        return decode(ctx.max_context)
+    k, v, table = ops.expand_pages_4bit(kv_pages, hd, block_table, ctx.cu_seqlens, ctx.positions, ctx.start_pos, ctx.n_new, chunk, sliding,
+                                        keep, skip_single=ctx.decode_rows is not None)
+    return attend_over_pages(q, k, v, table, ctx, nh, nkv, hd, chunk, sliding, scale, sink=sink, sink_values=sink_values, keep=keep,
+                             decode=decode)
 
 
 def differential_attend_over_pages(q, k_pages, v_pages, block_table, ctx, chunk: int, sliding: int, keep: int, scale: float,
