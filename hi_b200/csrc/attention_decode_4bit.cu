@@ -1,14 +1,16 @@
 // Attention of single decoded tokens over the cache in four bits (four_bit.cuh has its blocks): with the key k_jd = s_jg c_jd + l_jg
 // and the value v_jd = t_jg e_jd + m_jg of group g (32 dims),
 //   score_ij = sum_g s_jg (sum_d q_d c_jd) + sum_g l_jg (sum_d q_d)            d over the group
-//   o_d      = sum_j (p_j t_jg) e_jd + sum_j p_j m_jg                          p_j = exp(score - max), then over sum_j p_j
+//   o_d      = sum_j (p_j t_jg) (e_jd - 8) + sum_j p_j (m_jg + 8 t_jg)         p_j = exp(score - max), then over sum_j p_j
 // so the codes enter the tensor cores as they are (whole numbers, exact), a key's scale multiplies the sum of its group, and a value's scale
-// the weight it meets. Rounded to bfloat16 are the weights alone, once times the scale and once bare for the lows and for the sum.
+// the weight it meets. Rounded to bfloat16 are the weights alone, once times the scale and once bare, beside the group's middle and in their
+// sum: what they are off by is then relative to values of their own size. (With e_jd and m_jg as they are it was relative to the group's
+// range: 0.0036 of the result's size over a long context instead of the 0.0024 that the bfloat16 cache's kernels have.)
 //
 // Both products are taken transposed, keys (then dims) as the 16 rows of mma.sync and the query heads of a kv head as its 8 columns, half
-// the columns that heads as rows would leave empty; the weights change over with movmatrix. The lows' part is one more product a
-// block of 16 keys: l times the queries' sums in three pieces of bfloat16, and for the values a matrix whose rows are the groups' lows and
-// a row of ones, which sums the weights.
+// the columns that heads as rows would leave empty; the weights change over with movmatrix. The rest is a few more products a
+// block of 16 keys: l times the queries' sums in three pieces of bfloat16; for the values a matrix whose rows are the groups' lows, the
+// groups' scales and ones, times the bare weights; and the eights, a row a group, times the scaled ones.
 //
 // Grid (split, kv head x tiles of 8 heads, token). A warp has steps of 32 keys of its own: 2 blocks, which lie side by side in a
 // page of 32 and more, come as one bulk copy that the warp's own barrier counts, a few steps ahead; the warps meet at the end only,
@@ -81,7 +83,7 @@ template <int G>
 __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const Args a) {
   using B = fb::Block<G>;
   constexpr int HD = 32 * G, MT = STEP / 16;
-  constexpr float RAISE = 64.f;                                   // weights carry 2^64 (four_bit.cuh)
+  constexpr float RAISE = 18446744073709551616.f;                 // 2^64, of weights that meet codes (four_bit.cuh)
   extern __shared__ __align__(128) uint8_t ring_all[];            // [WARPS][STAGES][MT][B::BYTES]
   __shared__ uint64_t full[WARPS][STAGES];
   __shared__ float ml_s[WARPS][HEADS][2];
@@ -179,7 +181,9 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
   const float to_log2 = a.scale * 1.4426950408889634f * fb::UNSCALE;
 
   float m_run[2] = {-INFINITY, -INFINITY};
-  float o[2 * G][4], low[4] = {0.f, 0.f, 0.f, 0.f};               // dims 4 g + (0, 1) and (2, 3) of every group; lows' sums and the weights'
+  float o[2 * G][4];                                              // dims 4 g + (0, 1) and (2, 3) of every group
+  float low[4] = {0.f, 0.f, 0.f, 0.f};                            // rows g < G: lows' sums, G .. 2 G - 1: scales'; row 8: the weights'
+  float eight[4] = {0.f, 0.f, 0.f, 0.f};                          // rows g < G: the eights'
 #pragma unroll
   for (int c = 0; c < 2 * G; ++c)
 #pragma unroll
@@ -248,31 +252,43 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[c][e] *= correct[e & 1];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) low[e] *= correct[e & 1];
+      for (int e = 0; e < 4; ++e) {
+        low[e] *= correct[e & 1];
+        eight[e] *= correct[e & 1];
+      }
     }
     // a step that is not the token's at all leaves a maximum of -inf; its weights are zeros
-    const float base[2] = {m_run[0] == -INFINITY ? 0.f : RAISE - m_run[0], m_run[1] == -INFINITY ? 0.f : RAISE - m_run[1]};
+    const float base[2] = {m_run[0] == -INFINITY ? 0.f : -m_run[0], m_run[1] == -INFINITY ? 0.f : -m_run[1]};
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const uint8_t* b = blocks + mt * B::BYTES;
       float p[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) p[e] = exp2_fast(s[mt][e] + base[e & 1]);
-      unsigned la = 0u, lb = 0u;                                  // rows of the lows' product: a group's lows, or ones
-      if (g < G) {
-        la = *reinterpret_cast<const unsigned*>(b + B::value_low(2 * q4, g));
-        lb = *reinterpret_cast<const unsigned*>(b + B::value_low(2 * q4 + 8, g));
+      // rows of the bare weights' product: a group's lows, a group's scales (columns of the records of 8 keys), at 8 ones
+      unsigned la, lb;
+      {
+        const bool has = q4 < G;
+        const unsigned ra = has ? *reinterpret_cast<const unsigned*>(b + B::scale(g, 0, 2 * q4)) : 0u,
+                       rb = has ? *reinterpret_cast<const unsigned*>(b + B::scale(g + 8, 0, 2 * q4)) : 0u;
+        la = transpose8(ra);
+        lb = transpose8(rb);
+        if (g < G) {
+          la = *reinterpret_cast<const unsigned*>(b + B::value_low(2 * q4, g));
+          lb = *reinterpret_cast<const unsigned*>(b + B::value_low(2 * q4 + 8, g));
+        }
         if (!whole) {
           const int r = mt * 16 + 2 * q4;
           la &= (seen(r) ? 0xffffu : 0u) | (seen(r + 1) ? 0xffff0000u : 0u);
           lb &= (seen(r + 8) ? 0xffffu : 0u) | (seen(r + 9) ? 0xffff0000u : 0u);
         }
-      } else if (g == G) {
-        la = lb = 0x3f803f80u;
       }
-      const unsigned lows[4] = {la, 0u, lb, 0u};
-      hb::mma_bf16(low, lows, transpose8(hb::pack_bf16(p[0], p[1])), transpose8(hb::pack_bf16(p[2], p[3])));
+      const unsigned ones = g == 0 ? 0x3f803f80u : 0u;
+      const unsigned rest[4] = {la, ones, lb, ones};
+      hb::mma_bf16(low, rest, transpose8(hb::pack_bf16(p[0], p[1])), transpose8(hb::pack_bf16(p[2], p[3])));
       const Words<G> va(b + B::value_word(2 * q4, g, 0)), vb(b + B::value_word(2 * q4 + 8, g, 0));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] *= RAISE;
       const bool see_a = whole || seen(mt * 16 + g), see_b = whole || seen(mt * 16 + g + 8);
 #pragma unroll
       for (int c = 0; c < G; ++c) {
@@ -287,6 +303,9 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
         wb >>= 8;
         const unsigned a1[4] = {wa & fb::LOW, wa & fb::HIGH, wb & fb::LOW, wb & fb::HIGH};
         hb::mma_bf16(o[2 * c + 1], a1, x, y);
+        const unsigned eights = g == c ? 0x00080008u : 0u;
+        const unsigned a2[4] = {eights, 0u, eights, 0u};
+        hb::mma_bf16(eight, a2, x, y);
       }
     }
     __syncwarp();                                                 // all lanes are through with the stage
@@ -296,18 +315,24 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
     for (int i = max(0, asked - STAGES); i < asked; ++i) tc::mbar_wait_warp(&full[warp][i % STAGES], (i / STAGES) & 1);
   }
 
-  // this warp's sums in their size, over 2^64 still: o, and per head the sum of weights
-  constexpr float DOWN = 1.f / 18446744073709551616.f;            // 2^-64
+  // this warp's sums in their size: o, and per head the sum of weights
   float l_run[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) l_run[h] = __shfl_sync(0xffffffffu, low[h], 4 * G + q4) * DOWN;
+  for (int h = 0; h < 2; ++h) l_run[h] = __shfl_sync(0xffffffffu, low[2 + h], q4);
 #pragma unroll
   for (int c = 0; c < G; ++c) {
-    const float mean[2] = {__shfl_sync(0xffffffffu, low[0], 4 * c + q4) * DOWN, __shfl_sync(0xffffffffu, low[1], 4 * c + q4) * DOWN};
+    float rest[2], eights[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float m = __shfl_sync(0xffffffffu, low[h], 4 * c + q4), t = __shfl_sync(0xffffffffu, low[h], 4 * (c + G) + q4);
+      rest[h] = fmaf(8.f, t, m);
+      eights[h] = __shfl_sync(0xffffffffu, eight[h], 4 * c + q4);
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[2 * c + i][e] = fmaf(o[2 * c + i][e], e < 2 ? fb::UNSCALE : fb::UNSCALE / 16.f, mean[e & 1]);
+      for (int e = 0; e < 4; ++e)
+        o[2 * c + i][e] = fmaf(e < 2 ? o[2 * c + i][e] - eights[e & 1] : fmaf(o[2 * c + i][e], 1.f / 16.f, -eights[e & 1]), fb::UNSCALE, rest[e & 1]);
   }
   __syncthreads();                                                // every warp is through with its ring
   float* o_s = reinterpret_cast<float*>(ring_all);                // [WARPS][HEADS][HD]

@@ -129,7 +129,8 @@ __device__ __forceinline__ bool work_of(const PrefillPairArgs& a, int bx, int by
   return true;
 }
 
-template <int HD>
+// HALF: operands and P in float16, values scaled by a.v_factor
+template <int HD, bool HALF>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const PrefillPairArgs a) {
@@ -308,8 +309,8 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (!ok && queries > 0) tc::mbar_wait_warp(q_full, (queries - 1) & 1);
       for (int i = max(0, n - STAGES); i < n; ++i) tc::mbar_wait_warp(ok ? &empty[i % STAGES] : &full[i % STAGES], (i / STAGES) & 1);
     } else if (warp == 9) {                     // ---- the products: the whole warp walks, one lane issues
-      constexpr uint32_t idesc_qk = tc::idesc_bf16(BQ, BK, false);
-      constexpr uint32_t idesc_pv = tc::idesc_bf16(BQ, HD, true);
+      constexpr uint32_t idesc_qk = HALF ? tc::idesc_f16(BQ, BK, false) : tc::idesc_bf16(BQ, BK, false);
+      constexpr uint32_t idesc_pv = HALF ? tc::idesc_f16(BQ, HD, true) : tc::idesc_bf16(BQ, HD, true);
       const uint32_t q_addr = tc::smem_u32(q_s), ring_addr = tc::smem_u32(ring);
       bool ok = true;
       int stage = 0, turn = 0, loads = 0, phase[2] = {0, 0};    // the ring's; Q tiles taken; P tiles taken of either item
@@ -490,8 +491,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const float2 y = __ffma2_rn(make_float2(sv[at], sv[at + 1]), scale2, base2);
             const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));
             part[c & 1] = __fadd2_rn(part[c & 1], p);
-            __nv_bfloat162 hh = __floats2bfloat162_rn(p.x, p.y);
-            packed[c] = *reinterpret_cast<uint32_t*>(&hh);
+            packed[c] = tc::pack16<HALF>(p.x, p.y);
           }
           tc::st16_nowait(s_addr + 16 * h, packed);
           if (32 * (h + 1) == EARLY || 32 * (h + 1) == BK) {
@@ -518,6 +518,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         break;
       }
       tc::fence_after();
+      const float factor = HALF ? a.v_factor[x.head / (a.nh / a.nkv)] : 1.f;
       if (a.key_splits > 1) {
         // this share of the keys only: the row as it is, with its maximum and sum, for the merge
         const size_t at = ((size_t)(x.tok0 + r) * a.nh + x.head) * a.key_splits + piece;
@@ -530,6 +531,9 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           uint32_t o[32];
           tc::ld32_nowait(o_addr + c, o);
           tc::wait_ld();
+          if constexpr (HALF)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
 #pragma unroll
           for (int h = 0; h < 32; h += 16) {
             uint4 v[4];
@@ -547,7 +551,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
       } else {
         if (a.sink && l > 0.f) l += exp2f((a.sink_values ? a.sink_values[x.head] * 1.4426950408889634f : 0.f) - m);
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = (l > 0.f ? 1.f / l : 0.f) * factor;
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           uint32_t o[32];
@@ -583,7 +587,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   }
 }
 
-template <int HD>
+template <int HD, bool HALF>
 int launch(const void* q, const void* k_pages, const void* v_pages, const PrefillPairArgs& a, int n_tokens, long long pool_rows,
            int n_seqs, int max_new, cudaStream_t stream) {
   CUtensorMap mq, mk, mv;
@@ -592,11 +596,11 @@ int launch(const void* q, const void* k_pages, const void* v_pages, const Prefil
       !tc::make_map_bf16(&mv, v_pages, (uint64_t)pool_rows, HD, a.box_rows))
     return HB_ERR_UNSUPPORTED;
   const size_t smem = Layout<HD>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute(attn_prefill_pair_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(attn_prefill_pair_kernel<HD, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   const long long pairs = ((long long)((max_new + BQ - 1) / BQ) * (a.nh / a.nkv) + 1) / 2;
   if (pairs > 65535 || n_seqs > 65535 || (long long)a.nkv * a.key_splits > 0x7fffffffLL) return HB_ERR_UNSUPPORTED;
-  attn_prefill_pair_kernel<HD><<<dim3(a.nkv * a.key_splits, n_seqs, (unsigned)pairs), THREADS, smem, stream>>>(mq, mk, mv, a);
+  attn_prefill_pair_kernel<HD, HALF><<<dim3(a.nkv * a.key_splits, n_seqs, (unsigned)pairs), THREADS, smem, stream>>>(mq, mk, mv, a);
   HB_LAUNCH_CHECK();
   return HB_OK;
 }
@@ -605,7 +609,9 @@ int launch(const void* q, const void* k_pages, const void* v_pages, const Prefil
 
 int hb_prefill_pair_launch(const void* q, const void* k_pages, const void* v_pages, const PrefillPairArgs& a, int n_tokens,
                            long long pool_rows, int n_seqs, int max_new, int hd, cudaStream_t stream) {
-  if (hd == 128) return launch<128>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
-  if (hd == 64) return launch<64>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
+  if (hd == 128 && a.v_factor) return launch<128, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
+  if (hd == 64 && a.v_factor) return launch<64, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
+  if (hd == 128) return launch<128, false>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
+  if (hd == 64) return launch<64, false>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
   return HB_ERR_UNSUPPORTED;
 }

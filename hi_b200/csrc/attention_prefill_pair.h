@@ -18,6 +18,8 @@ struct PrefillPairArgs {
   float* part_ml;
   int sink;                  // 1: the denominator has one more term, e^0, or e^sink_values[head]
   const float* sink_values;
+  // not null: q, k and v are float16 (four_bit_cache.cu), and the values of kv head h have been divided by v_factor[h]
+  const float* v_factor;
 };
 
 // head_dim 64 or 128; HB_ERR_UNSUPPORTED for others

@@ -105,9 +105,11 @@ struct Args {
   int newest_first;
   int keep;                  // a sliding window's kept first tokens
   Pair pair;                 // kPair only
+  const float* v_factor;     // HALF only: the values of kv head h have been divided by v_factor[h]
 };
 
-template <int HD, bool kPair>
+// HALF: operands and P in float16
+template <int HD, bool kPair, bool HALF>
 __global__ void __launch_bounds__(THREADS, 2)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const Args a) {
@@ -259,8 +261,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     }
   } else if (warp == 1) {
     // ---- MMA issuer: S_j = Q K_j^T, then O += P_{j-1} V_{j-1}; the whole warp walks, one lane issues
-    constexpr uint32_t idesc_qk = tc::idesc_bf16(BQ, BKEYS, false);
-    constexpr uint32_t idesc_pv = tc::idesc_bf16(BQ, HD, true);
+    constexpr uint32_t idesc_qk = HALF ? tc::idesc_f16(BQ, BKEYS, false) : tc::idesc_bf16(BQ, BKEYS, false);
+    constexpr uint32_t idesc_pv = HALF ? tc::idesc_f16(BQ, HD, true) : tc::idesc_bf16(BQ, HD, true);
     bool ok = true;
     auto wait = [&](uint64_t* bar, int parity, int code) {
       if (ok && !tc::mbar_wait_warp(bar, parity)) {
@@ -465,8 +467,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         uint32_t packed[BKEYS / 2];
 #pragma unroll
         for (int i = 0; i < BKEYS / 2; ++i) {
-          __nv_bfloat162 hh = __floats2bfloat162_rn(sv[2 * i], sv[2 * i + 1]);
-          packed[i] = *reinterpret_cast<uint32_t*>(&hh);
+          packed[i] = tc::pack16<HALF>(sv[2 * i], sv[2 * i + 1]);
         }
         tc::st32_nowait(tmem + lane_addr + sb * S_COLS, packed);
         tc::wait_st();
@@ -511,7 +512,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           float* ex_ss = ex + 2 * TOKENS * EXS;                // [2][64]
           static_assert((2 * TOKENS * EXS + 2 * TOKENS) * 4 <= KST * KBYTES, "the exchange fits the K tiles");
           const int mp = r / TOKENS;
-          const float inv = l > 0.f ? 1.f / l : 0.f;
+          const float inv = (l > 0.f ? 1.f / l : 0.f) * (HALF ? a.v_factor[h / (a.nh / a.nkv)] : 1.f);
 #pragma unroll 1
           for (int c = 0; c < HALF; c += 32) {
             float o[32];
@@ -651,6 +652,9 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             uint32_t o[32];
             tc::ld32_nowait(tmem_o + lane_addr + c, o);
             tc::wait_ld();
+            if constexpr (HALF)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a.v_factor[h / (a.nh / a.nkv)]);
 #pragma unroll
             for (int i = 0; i < 32; i += 16) {
               uint4 v[4];
@@ -668,7 +672,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           }
         } else {
         if (a.sink && l > 0.f) l += exp2f((a.sink_values ? a.sink_values[h] * 1.4426950408889634f : 0.f) - m);   // m is in units of log 2
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = (l > 0.f ? 1.f / l : 0.f) * (HALF ? a.v_factor[h / (a.nh / a.nkv)] : 1.f);
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           float o[32];
@@ -703,7 +707,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   }
 }
 
-template <int HD, bool kPair = false>
+template <int HD, bool kPair = false, bool HALF = false>
 int launch(const void* q, const void* k_pages, const void* v_pages, const Args& a, int n_tokens, long long pool_rows,
            int n_seqs, int max_new, cudaStream_t stream) {
   CUtensorMap mq, mk, mv;
@@ -712,14 +716,14 @@ int launch(const void* q, const void* k_pages, const void* v_pages, const Args& 
       !tc::make_map_bf16(&mv, v_pages, (uint64_t)pool_rows, HD, a.box_rows))
     return HB_ERR_UNSUPPORTED;
   const size_t smem = (size_t)BQ * HD * 2 + (KST + 2) * (size_t)BKEYS * HD * 2 + 256;
-  cudaError_t e = cudaFuncSetAttribute(attn_prefill_tc_kernel<HD, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(attn_prefill_tc_kernel<HD, kPair, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   const int tokens = kPair ? BQ / 2 : BQ;
   const int q_tiles = (max_new + tokens - 1) / tokens;
   if (q_tiles > 65535 || n_seqs > 65535) return HB_ERR_UNSUPPORTED;
   if ((long long)a.nh * a.key_splits > 0x7fffffffLL) return HB_ERR_UNSUPPORTED;
   dim3 grid((kPair ? a.nh / 2 : a.nh) * a.key_splits, q_tiles, n_seqs);
-  attn_prefill_tc_kernel<HD, kPair><<<grid, THREADS, smem, stream>>>(mq, mk, mv, a);
+  attn_prefill_tc_kernel<HD, kPair, HALF><<<grid, THREADS, smem, stream>>>(mq, mk, mv, a);
   HB_LAUNCH_CHECK();
   return HB_OK;
 }
@@ -738,7 +742,7 @@ int prefill_tc(const void* q, const void* k_pages, const void* v_pages, const in
                int nh, int nkv, int hd, int page_size, int chunk, int window, float scale, int skip_single, int sink,
                const float* head_bias, int key_splits, float* part_acc, float* part_ml, int* status, int turn_inside,
                const float* v_inv_freq, int v_pairs, int v_interleaved, float softcap, const float* slopes,
-               const float* sink_values, int keep, const Pair* pair, int one_tile, cudaStream_t stream);
+               const float* sink_values, int keep, const Pair* pair, int one_tile, const float* v_factor, cudaStream_t stream);
 }  // namespace
 
 // one_tile: plain softmax rows of 64 and 128 too go one query tile a block (ops.prefill_one_tile says where that is faster)
@@ -750,7 +754,7 @@ extern "C" int hb_attention_prefill_tc(const void* q, const void* k_pages, const
                                        float* part_ml, int one_tile, int* status, cudaStream_t stream) {
   return prefill_tc(q, k_pages, v_pages, block_table, table_stride, cu_seqlens, positions, out, n_tokens, n_pages, n_seqs,
                     max_new, nh, nkv, hd, page_size, chunk, window, scale, skip_single, sink, head_bias, key_splits,
-                    part_acc, part_ml, status, 0, nullptr, 0, 0, 0.f, nullptr, nullptr, 0, nullptr, one_tile, stream);
+                    part_acc, part_ml, status, 0, nullptr, 0, 0, 0.f, nullptr, nullptr, 0, nullptr, one_tile, nullptr, stream);
 }
 
 // The same with reshaped scores (see Args): a cap, a distance bias per head, a sink with a score per head.
@@ -763,7 +767,20 @@ extern "C" int hb_attention_prefill_tc_reshaped(const void* q, const void* k_pag
                                                 float* part_acc, float* part_ml, int one_tile, int* status, cudaStream_t stream) {
   return prefill_tc(q, k_pages, v_pages, block_table, table_stride, cu_seqlens, positions, out, n_tokens, n_pages, n_seqs,
                     max_new, nh, nkv, hd, page_size, chunk, window, scale, skip_single, sink, nullptr, key_splits,
-                    part_acc, part_ml, status, 0, nullptr, 0, 0, softcap, slopes, sink_values, keep, nullptr, one_tile, stream);
+                    part_acc, part_ml, status, 0, nullptr, 0, 0, softcap, slopes, sink_values, keep, nullptr, one_tile, nullptr, stream);
+}
+
+// q, k and v in float16, the values of kv head h divided by v_factor[h] (hb_expand_half_4bit makes them); hd 64 or 128.
+extern "C" int hb_attention_prefill_tc_half(const void* q, const void* k_pages, const void* v_pages, const float* v_factor,
+                                            const int* block_table, int table_stride, const int* cu_seqlens, const int* positions,
+                                            void* out, int n_tokens, int n_pages, int n_seqs, int max_new, int nh, int nkv, int hd,
+                                            int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
+                                            const float* sink_values, int key_splits, float* part_acc, float* part_ml,
+                                            int one_tile, int* status, cudaStream_t stream) {
+  if (!v_factor || sink < 0 || sink > 1) return HB_ERR_BAD_ARG;
+  return prefill_tc(q, k_pages, v_pages, block_table, table_stride, cu_seqlens, positions, out, n_tokens, n_pages, n_seqs,
+                    max_new, nh, nkv, hd, page_size, chunk, window, scale, skip_single, sink, nullptr, key_splits,
+                    part_acc, part_ml, status, 0, nullptr, 0, 0, 0.f, nullptr, sink_values, keep, nullptr, one_tile, v_factor, stream);
 }
 
 // Sigmoid weights with the result written by the kernel itself: `out` [n_tokens, nh, hd] bfloat16 takes every
@@ -780,7 +797,7 @@ extern "C" int hb_sigmoid_prefill_tc(const void* q, const void* k_pages, const v
   if (v_pairs > 0 && !v_interleaved && 2 * v_pairs != hd) return HB_ERR_UNSUPPORTED;
   return prefill_tc(q, k_pages, v_pages, block_table, table_stride, cu_seqlens, positions, out, n_tokens, n_pages, n_seqs,
                     max_new, nh, nkv, hd, page_size, chunk, window, scale, skip_single, 2, head_bias, 1, nullptr, nullptr,
-                    status, 1, v_inv_freq, v_pairs, v_interleaved, 0.f, nullptr, nullptr, 0, nullptr, 1, stream);
+                    status, 1, v_inv_freq, v_pairs, v_interleaved, 0.f, nullptr, nullptr, 0, nullptr, 1, nullptr, stream);
 }
 
 // Differential attention: q [n_tokens, nh, hd] holds the two maps of head a as heads 2a and 2a + 1, both over the same
@@ -799,7 +816,7 @@ extern "C" int hb_diff_prefill_tc(const void* q, const void* k_pages, const void
   const Pair pair{lambda, eps, mul, vdim, vec ? 1 : 0, (const __nv_bfloat16*)gate, gate_stride};
   return prefill_tc(q, k_pages, v_pages, block_table, table_stride, cu_seqlens, positions, out, n_tokens, n_pages, n_seqs,
                     max_new, nh, nkv, hd, page_size, chunk, window, scale, skip_single, 0, nullptr, 1, nullptr, nullptr,
-                    status, 0, nullptr, 0, 0, 0.f, nullptr, nullptr, keep, &pair, 1, stream);
+                    status, 0, nullptr, 0, 0, 0.f, nullptr, nullptr, keep, &pair, 1, nullptr, stream);
 }
 
 namespace {
@@ -808,7 +825,7 @@ int prefill_tc(const void* q, const void* k_pages, const void* v_pages, const in
                int nh, int nkv, int hd, int page_size, int chunk, int window, float scale, int skip_single, int sink,
                const float* head_bias, int key_splits, float* part_acc, float* part_ml, int* status, int turn_inside,
                const float* v_inv_freq, int v_pairs, int v_interleaved, float softcap, const float* slopes,
-               const float* sink_values, int keep, const Pair* pair, int one_tile, cudaStream_t stream) {
+               const float* sink_values, int keep, const Pair* pair, int one_tile, const float* v_factor, cudaStream_t stream) {
   if (sink == 2 && (softcap > 0.f || slopes || sink_values)) return HB_ERR_UNSUPPORTED;
   if (!q || !k_pages || !v_pages || !block_table || !cu_seqlens || !positions || !out || !status) return HB_ERR_BAD_ARG;
   if (n_tokens < 0 || n_pages <= 0 || n_seqs < 0 || max_new < 0 || nh <= 0 || nkv <= 0 || nh % nkv != 0 ||
@@ -822,19 +839,24 @@ int prefill_tc(const void* q, const void* k_pages, const void* v_pages, const in
   if (n_seqs == 0 || max_new == 0 || n_tokens == 0) return HB_OK;
   Args a{block_table, cu_seqlens, positions, (__nv_bfloat16*)out, status, table_stride, nh, nkv, page_size, chunk,
          window, skip_single, page_size < BKEYS ? page_size : BKEYS, scale * 1.4426950408889634f, key_splits, part_acc, part_ml, sink, head_bias,
-         turn_inside, v_pairs, v_interleaved, v_inv_freq, softcap, slopes, sink_values, slopes ? 1 : 0, keep, pair ? *pair : Pair{}};
+         turn_inside, v_pairs, v_interleaved, v_inv_freq, softcap, slopes, sink_values, slopes ? 1 : 0, keep, pair ? *pair : Pair{}, v_factor};
   const long long pool_rows = (long long)n_pages * nkv * page_size;
   // (a launch of more pairs than a grid holds goes one tile a block)
   const long long pairs = ((max_new + 127LL) / 128 * (nh / nkv) + 1) / 2;
   if (!one_tile && !pair && !turn_inside && sink != 2 && softcap <= 0.f && !slopes && keep == 0 && hd <= 128 && pairs <= 65535) {
     const PrefillPairArgs b{block_table, cu_seqlens, positions, (__nv_bfloat16*)out, status, table_stride, nh, nkv, page_size, chunk, window,
-                            skip_single, a.box_rows, a.scale_log2, key_splits, part_acc, part_ml, sink, sink_values};
+                            skip_single, a.box_rows, a.scale_log2, key_splits, part_acc, part_ml, sink, sink_values, v_factor};
     return hb_prefill_pair_launch(q, k_pages, v_pages, b, n_tokens, pool_rows, n_seqs, max_new, hd, stream);
   }
   if (pair) {
     if (hd == 192) return launch<192, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
     if (hd == 128) return launch<128, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
     if (hd == 64) return launch<64, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
+    return HB_ERR_UNSUPPORTED;
+  }
+  if (v_factor) {
+    if (hd == 128) return launch<128, false, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
+    if (hd == 64) return launch<64, false, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
     return HB_ERR_UNSUPPORTED;
   }
   if (hd == 192) return launch<192>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);

@@ -4,13 +4,15 @@
 //   low = min y, scale = bfloat16((max y - low) / 15), code = round((y - low) / scale) held to 0 .. 15;  y ~ scale * code + low
 // (float32 division; a group of one value has scale 0 and codes 0). The scale is rounded to bfloat16 because it is kept so, 32 bits a
 // group beside 128 of codes, and the codes are taken with the rounded one. A group that holds a value that is not finite is kept as
-// scale = low = NaN, so that it shows wherever it is read, as it would from a bfloat16 cache.
+// low = NaN, so that it shows wherever it is read, as it would from a bfloat16 cache; its scale is 0, which keeps it out of the sums of
+// other groups (attention_decode_4bit.cu).
 //
 // Both kernels are bound by memory, and in decode steps by their launch. The append's stores are 2 and 4 bytes each, as the attention
 // kernel's order of the codes has it (four_bit.cuh); they meet in L2.
 #include "api.h"
 #include "common.cuh"
 #include "four_bit.cuh"
+#include "tc.cuh"
 
 namespace {
 
@@ -57,7 +59,8 @@ __device__ __forceinline__ Quantised quantise(const float (&y)[4]) {
   }
   if (!whole) {
     r.codes = 0;
-    r.scale = r.low = __ushort_as_bfloat16(0x7fffu);
+    r.scale = __ushort_as_bfloat16(0u);
+    r.low = __ushort_as_bfloat16(0x7fffu);
   }
   return r;
 }
@@ -182,10 +185,16 @@ struct Expand {
   const int* block_table;
   const int* cu_seqlens;
   const int* positions;
-  __nv_bfloat16* k;
-  __nv_bfloat16* v;
+  uint16_t* k;                     // bfloat16, or float16
+  uint16_t* v;
   int* table;
   int n_seqs, table_stride, page_size, chunk, window, keep, skip_single, nkv, total;
+  // float16 only
+  const __nv_bfloat16* q;
+  int n_tokens, nh;
+  int* most;                       // [nkv][keys, values]
+  uint16_t* q_half;
+  float* v_factor;
 };
 
 __device__ __forceinline__ void span(const Expand& a, int s, int& first, int& count) {
@@ -200,15 +209,13 @@ __device__ __forceinline__ void span(const Expand& a, int s, int& first, int& co
   count = (start + n - 1) / a.page_size - first + 1;
 }
 
-template <int G>
-__global__ void __launch_bounds__(128) expand_4bit_kernel(const Expand a) {
-  constexpr int HD = 32 * G;
-  using B = fb::Block<G>;
+// The request and its page that page `out_page` of the result is; false: none (or the table has no such page). A whole block asks.
+__device__ __forceinline__ bool find_page(const Expand& a, int out_page, int& seq, int& index) {
   __shared__ int found[2];
-  const int out_page = blockIdx.x, kvh = blockIdx.y, lane = threadIdx.x & 31;
-  if (threadIdx.x < 32) {          // whose page is this? the requests' counts are summed 32 at a time
-    int before = 0, seq = -1, index = 0;
-    for (int s0 = 0; s0 < a.n_seqs && seq < 0; s0 += 32) {
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {          // the requests' counts are summed 32 at a time
+    int before = 0, who_seq = -1, at = 0;
+    for (int s0 = 0; s0 < a.n_seqs && who_seq < 0; s0 += 32) {
       int first = 0, count = 0;
       if (s0 + lane < a.n_seqs) span(a, s0 + lane, first, count);
       int upto = count;
@@ -220,29 +227,100 @@ __global__ void __launch_bounds__(128) expand_4bit_kernel(const Expand a) {
       const unsigned hit = __ballot_sync(0xffffffffu, before + upto > out_page);
       const int who = hit ? __ffs(hit) - 1 : 0;
       const int start = __shfl_sync(0xffffffffu, before + upto - count, who), from = __shfl_sync(0xffffffffu, first, who);
-      if (hit) { seq = s0 + who; index = from + out_page - start; }
+      if (hit) { who_seq = s0 + who; at = from + out_page - start; }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    if (lane == 0) { found[0] = seq; found[1] = index; }
+    if (lane == 0) { found[0] = who_seq; found[1] = at; }
   }
   __syncthreads();
-  const int seq = found[0], index = found[1];
-  if (seq < 0 || index >= a.table_stride) return;
+  seq = found[0];
+  index = found[1];
+  return seq >= 0 && index < a.table_stride;
+}
+__device__ __forceinline__ float number(const uint8_t* p) { return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p)); }
+
+// The largest magnitudes of a kv head's keys and values on the pages (of rows that are there; a group's ends: its low and fifteen steps
+// above it), as the bits of floats, whose order is theirs: the least power of two above one divides the head's numbers, so that float16 holds
+// them to 2^-12 of their size, or 2^-25 of the largest one's where they are small.
+template <int G>
+__global__ void __launch_bounds__(128) most_4bit_kernel(const Expand a) {
+  using B = fb::Block<G>;
+  const int kvh = blockIdx.y;
+  int seq, index;
+  if (!find_page(a, blockIdx.x, seq, index)) return;
+  const int page = a.block_table[(size_t)seq * a.table_stride + index];
+  if (page < 0) return;
+  const int begin = a.cu_seqlens[seq], last = a.positions[begin] + a.cu_seqlens[seq + 1] - begin - 1;
+  const int rows = min(a.page_size, last - index * a.page_size + 1);
+  const uint8_t* from = a.pages + ((size_t)page * a.nkv + kvh) * (a.page_size / fb::BLOCK_ROWS) * B::BYTES;
+  float k_most = 0.f, v_most = 0.f;
+  for (int i = threadIdx.x; i < rows * G; i += blockDim.x) {
+    const int row = i / G, r = row % fb::BLOCK_ROWS, group = i % G;
+    const uint8_t* block = from + row / fb::BLOCK_ROWS * B::BYTES;
+    const float k = number(block + B::key_low(r, group)), v = number(block + B::value_low(r, group));
+    k_most = fmaxf(k_most, fmaxf(fabsf(k), fabsf(fmaf(number(block + B::scale(r, 0, group)), 15.f, k))));
+    v_most = fmaxf(v_most, fmaxf(fabsf(v), fabsf(fmaf(number(block + B::scale(r, 1, group)), 15.f, v))));
+  }
+  k_most = hb::warp_max(k_most);
+  v_most = hb::warp_max(v_most);
+  if (threadIdx.x % 32 == 0) {
+    atomicMax(a.most + 2 * kvh, __float_as_int(k_most));
+    atomicMax(a.most + 2 * kvh + 1, __float_as_int(v_most));
+  }
+}
+// two to the power that is the least above a magnitude of these bits, within what a float can be divided by
+__device__ __forceinline__ int power_above(int bits) {
+  const int e = (bits >> 23) - 126;
+  return bits == 0 ? 0 : max(-100, min(e, 120));
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+// a float as float16, a finite one too large for it as its largest
+__device__ __forceinline__ float held(float x) { return fabsf(x) > 65504.f && fabsf(x) < INFINITY ? copysignf(65504.f, x) : x; }
+
+constexpr int Q_TOKENS = 8;        // of a block that converts queries
+
+template <int G, bool HALF>
+__global__ void __launch_bounds__(128) expand_4bit_kernel(const Expand a) {
+  constexpr int HD = 32 * G;
+  using B = fb::Block<G>;
+  const int out_page = blockIdx.x, kvh = blockIdx.y;
+  float k_down = 1.f, v_down = 1.f;
+  if constexpr (HALF) {
+    const int ek = power_above(a.most[2 * kvh]), ev = power_above(a.most[2 * kvh + 1]);
+    k_down = power_of_two(-ek);
+    v_down = power_of_two(-ev);
+    if (out_page == 0 && threadIdx.x == 0) a.v_factor[kvh] = power_of_two(ev);
+    if (out_page >= a.total) {     // queries of this kv head
+      const float up = power_of_two(ek - 8);
+      const int per = a.nh / a.nkv, t0 = (out_page - a.total) * Q_TOKENS, words = per * HD / 8;
+      for (int i = threadIdx.x; i < min(Q_TOKENS, a.n_tokens - t0) * words; i += blockDim.x) {
+        const size_t at = ((size_t)(t0 + i / words) * a.nh + kvh * per) * HD + i % words * 8;
+        float x[8];
+        hb::load8(a.q + at, x);
+        unsigned o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = tc::pack16<true>(held(x[2 * e] * up), held(x[2 * e + 1] * up));
+        *reinterpret_cast<uint4*>(a.q_half + at) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      return;
+    }
+  }
+  int seq, index;
+  if (!find_page(a, out_page, seq, index)) return;
   const int page = a.block_table[(size_t)seq * a.table_stride + index];
   if (kvh == 0 && threadIdx.x == 0) a.table[(size_t)seq * a.table_stride + index] = page < 0 ? -1 : out_page;
   const size_t out = ((size_t)out_page * a.nkv + kvh) * a.page_size * HD;
   if (page < 0) return;
   const uint8_t* from = a.pages + ((size_t)page * a.nkv + kvh) * (a.page_size / fb::BLOCK_ROWS) * B::BYTES;
-  auto number = [](const uint8_t* p) { return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p)); };
   for (int i = threadIdx.x; i < a.page_size * 4 * G; i += blockDim.x) {      // eight dims of a key
     const int row = i / (4 * G), r = row % fb::BLOCK_ROWS, group = i % (4 * G) / 4, q = i % 4;
     const uint8_t* block = from + row / fb::BLOCK_ROWS * B::BYTES;
     const unsigned w = *reinterpret_cast<const unsigned*>(block + B::key_word(r, q, group));
-    const float scale = number(block + B::scale(r, 0, group)), low = number(block + B::key_low(r, group));
+    const float scale = number(block + B::scale(r, 0, group)) * k_down, low = number(block + B::key_low(r, group)) * k_down;
     unsigned o[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      o[e] = hb::pack_bf16(fmaf(scale, (float)(w >> (4 * e) & 15), low), fmaf(scale, (float)(w >> (16 + 4 * e) & 15), low));
+      o[e] = tc::pack16<HALF>(fmaf(scale, (float)(w >> (4 * e) & 15), low), fmaf(scale, (float)(w >> (16 + 4 * e) & 15), low));
     *reinterpret_cast<uint4*>(a.k + out + (size_t)row * HD + group * 32 + q * 8) = make_uint4(o[0], o[1], o[2], o[3]);
   }
   for (int i = threadIdx.x; i < a.page_size / 2 * 8 * G; i += blockDim.x) {  // four dims of the values of two tokens
@@ -251,11 +329,11 @@ __global__ void __launch_bounds__(128) expand_4bit_kernel(const Expand a) {
     const unsigned w = *reinterpret_cast<const unsigned*>(block + B::value_word(r, g, group));
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float scale = number(block + B::scale(r + e, 1, group)), low = number(block + B::value_low(r + e, group));
+      const float scale = number(block + B::scale(r + e, 1, group)) * v_down, low = number(block + B::value_low(r + e, group)) * v_down;
       const unsigned c = w >> (16 * e);
       *reinterpret_cast<uint2*>(a.v + out + (size_t)(row + e) * HD + group * 32 + g * 4) = make_uint2(
-          hb::pack_bf16(fmaf(scale, (float)(c & 15), low), fmaf(scale, (float)(c >> 4 & 15), low)),
-          hb::pack_bf16(fmaf(scale, (float)(c >> 8 & 15), low), fmaf(scale, (float)(c >> 12 & 15), low)));
+          tc::pack16<HALF>(fmaf(scale, (float)(c & 15), low), fmaf(scale, (float)(c >> 4 & 15), low)),
+          tc::pack16<HALF>(fmaf(scale, (float)(c >> 8 & 15), low), fmaf(scale, (float)(c >> 12 & 15), low)));
     }
   }
 }
@@ -290,19 +368,48 @@ extern "C" int hb_qkv_post_4bit(const void* qkv, const float* inv_freq, int rot_
   return HB_OK;
 }
 
+namespace {
+int expand(const Expand& a, int hd, bool half, cudaStream_t stream) {
+  if (!a.pages || !a.block_table || !a.cu_seqlens || !a.positions || !a.table || a.n_seqs < 0 || a.total < 0 || a.nkv <= 0 || a.table_stride <= 0 ||
+      a.chunk < 0 || a.window < 0 || a.keep < 0 || (a.total > 0 && (!a.k || !a.v)))
+    return HB_ERR_BAD_ARG;
+  if ((hd != 64 && hd != 128) || !good_page(a.page_size) || a.nkv > 65535) return HB_ERR_UNSUPPORTED;
+  if (a.n_seqs == 0 || a.total == 0) return HB_OK;
+  const dim3 grid(a.total, a.nkv);
+  if (half) {
+    const dim3 more(a.total + (a.n_tokens + Q_TOKENS - 1) / Q_TOKENS, a.nkv);
+    if (hd == 128) most_4bit_kernel<4><<<grid, 128, 0, stream>>>(a);
+    else most_4bit_kernel<2><<<grid, 128, 0, stream>>>(a);
+    HB_LAUNCH_CHECK();
+    if (hd == 128) expand_4bit_kernel<4, true><<<more, 128, 0, stream>>>(a);
+    else expand_4bit_kernel<2, true><<<more, 128, 0, stream>>>(a);
+  } else if (hd == 128) {
+    expand_4bit_kernel<4, false><<<grid, 128, 0, stream>>>(a);
+  } else {
+    expand_4bit_kernel<2, false><<<grid, 128, 0, stream>>>(a);
+  }
+  HB_LAUNCH_CHECK();
+  return HB_OK;
+}
+}  // namespace
+
 extern "C" int hb_expand_pages_4bit(const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
                                     const int* positions, int n_seqs, int total, int page_size, int chunk, int window, int keep,
                                     int skip_single, int nkv, int hd, void* k, void* v, int* table, cudaStream_t stream) {
-  if (!pages || !block_table || !cu_seqlens || !positions || !table || n_seqs < 0 || total < 0 || nkv <= 0 || table_stride <= 0 ||
-      chunk < 0 || window < 0 || keep < 0 || (total > 0 && (!k || !v)))
+  return expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)k, (uint16_t*)v, table, n_seqs,
+                       table_stride, page_size, chunk, window, keep, skip_single, nkv, total, nullptr, 0, 0, nullptr, nullptr, nullptr},
+                hd, false, stream);
+}
+
+// The scores of q_half and k are those of q and the keys over 256.
+extern "C" int hb_expand_half_4bit(const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
+                                   const int* positions, int n_seqs, int total, int page_size, int chunk, int window, int keep,
+                                   int skip_single, const void* q, int n_tokens, int nh, int nkv, int hd, void* k, void* v, int* table,
+                                   int* most, void* q_half, float* v_factor, cudaStream_t stream) {
+  if (!q || !most || !q_half || !v_factor || n_tokens < 0 || nh <= 0 || nkv <= 0 || nh % nkv || (reinterpret_cast<uintptr_t>(q) & 15))
     return HB_ERR_BAD_ARG;
-  if ((hd != 64 && hd != 128) || !good_page(page_size) || nkv > 65535) return HB_ERR_UNSUPPORTED;
-  if (n_seqs == 0 || total == 0) return HB_OK;
-  const Expand a{(const uint8_t*)pages, block_table, cu_seqlens, positions, (__nv_bfloat16*)k, (__nv_bfloat16*)v, table, n_seqs,
-                 table_stride, page_size, chunk, window, keep, skip_single, nkv, total};
-  const dim3 grid(total, nkv);
-  if (hd == 128) expand_4bit_kernel<4><<<grid, 128, 0, stream>>>(a);
-  else expand_4bit_kernel<2><<<grid, 128, 0, stream>>>(a);
-  HB_LAUNCH_CHECK();
-  return HB_OK;
+  return expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)k, (uint16_t*)v, table, n_seqs,
+                       table_stride, page_size, chunk, window, keep, skip_single, nkv, total, (const __nv_bfloat16*)q, n_tokens, nh, most,
+                       (uint16_t*)q_half, v_factor},
+                hd, true, stream);
 }

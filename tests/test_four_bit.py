@@ -247,18 +247,31 @@ DECODE = [
 ]
 
 
+def _check_rows(step, s, got, mask, scale, sink, decoded):
+    q, k, v, seen = step.expected(s, **mask)
+    want, size = attention(q, k, v, seen, scale, sink)
+    if decoded:
+        # weights are rounded to bfloat16 (2^-8) times the scale, before codes less eight, and bare, before the group's middle and in the
+        # sum of weights; scores are off by float32 sums only (2^-13 of the weights covers |score| up to 500); the result is rounded
+        codes, t, low = quantise(step.v[s])
+        t, low = t.double().unsqueeze(-1), low.double().unsqueeze(-1)
+        grown = (t * (codes.double().unflatten(-1, (-1, 32)) - 8).abs() + (low + 8 * t).abs()).flatten(-2)
+        _, size = attention(q, k, grown, seen, scale, sink)
+        tol = 2.0 ** -8 * (size + 2 * want.abs()) + 2.0 ** -13 * size
+    else:
+        # keys, values and weights in float16 (2^-11 each; the queries are exact in it but for parts 2^-25 of a key's and a query's largest):
+        # a score is off by up to 2^-11 scale sum |q| |k|, and twice that moves a weight against its sum; the result is rounded
+        per = q.shape[1] // k.shape[1]
+        off = 2.0 ** -10.5 * scale * torch.einsum("nhd,thd->nht", q.double().abs(), k.abs().repeat_interleave(per, 1))
+        off = off.masked_fill(~seen.unsqueeze(1), 0).amax(-1, keepdim=True)
+        tol = (2 * off * (1 + off) + 3 * 2.0 ** -11) * size + 2.0 ** -11 * want.abs() + 2.0 ** -8 * want.abs() + 2.0 ** -20 * size.amax()
+    diff = (got[step.cu[s]: step.cu[s + 1]].double() - want).abs()
+    assert (diff <= tol).all(), (s, float((diff / tol).max()))
+
+
 def _check_decode(step, got, mask, scale, sink=None):
     for s in range(len(step.portions)):
-        q, k, v, seen = step.expected(s, **mask)
-        want, _ = attention(q, k, v, seen, scale, sink)
-        codes, t, low = quantise(step.v[s])
-        grown = (t.double().unsqueeze(-1) * codes.double().unflatten(-1, (-1, 32)) + low.double().abs().unsqueeze(-1)).flatten(-2)
-        _, size = attention(q, k, grown, seen, scale, sink)
-        a, b = step.cu[s], step.cu[s + 1]
-        # weights rounded to bfloat16 (2^-8): bare in the sum of weights and before the lows, times the scale before the codes; scores are
-        # off by float32 sums only (2^-13 of the weights covers |score| up to 500); the result is rounded
-        tol = 2.0 ** -8 * (size + 2 * want.abs()) + 2.0 ** -13 * size
-        assert ((got[a:b].double() - want).abs() <= tol).all(), (s, float(((got[a:b].double() - want).abs() / tol).max()))
+        _check_rows(step, s, got, mask, scale, sink, True)
 
 
 @pytest.mark.parametrize("case", DECODE, ids=lambda c: f"{c[0]}on{c[1]}x{c[2]}p{c[3]}n{len(c[4])}" + "".join(f"_{k}{v}" for k, v in c[5].items()))
@@ -342,28 +355,50 @@ PORTIONS = [
 
 @pytest.mark.parametrize("case", PORTIONS, ids=lambda c: f"{c[0]}on{c[1]}x{c[2]}p{c[3]}" + "".join(f"_{k}{v}" for k, v in c[5].items()))
 def test_portions(case):
-    """Portions beside single tokens: the former over the expanded pages, so keys and values in bfloat16."""
+    """Portions beside single tokens: the former over the expanded pages, the latter, and steps of a few tokens a request, as they are."""
     from hi_b200.kernels import ops
-    from hi_b200.parts.attention import attend_over_four_bit_pages
+    from hi_b200.parts.attention import FOUR_BIT_DECODED, attend_over_four_bit_pages
 
     nh, nkv, hd, page, portions, mask = case
     step = Step(portions, nh, nkv, hd, page, seed=nh + page).fill()
     scale = hd ** -0.5
-    sinks = torch.randn(nh, device=DEV, generator=_gen(3))
-    for sink in (None, sinks):
+    few = max(n for n, _c in portions) <= FOUR_BIT_DECODED
+    for sink in (None, torch.randn(nh, device=DEV, generator=_gen(3))):
         got = attend_over_four_bit_pages(step.q, step.pages, step.table, step.ctx, nh, nkv, hd, mask.get("chunk", 0), mask.get("window", 0),
                                          scale, sink_values=sink, keep=mask.get("keep", 0))
         ops.check_tc_status()
         for s, (n, _c) in enumerate(portions):
-            q, k, v, seen = step.expected(s, **mask)
-            if n > 1:
-                k, v = k.to(BF16).double(), v.to(BF16).double()
-            want, size = attention(q, k, v, seen, scale, sink)
-            a, b = step.cu[s], step.cu[s + 1]
-            # weights rounded to bfloat16 against their float32 sum, and the result; single tokens: as test_decode, where scale * code +
-            # |low| is at most |value| + 2 |low|, and no group's low is under -8 here
-            tol = 2.0 ** -8 * (size + 2 * want.abs() + (0 if n > 1 else 16)) + 2.0 ** -13 * size
-            assert ((got[a:b].double() - want).abs() <= tol).all(), (s, float(((got[a:b].double() - want).abs() / tol).max()))
+            _check_rows(step, s, got, mask, scale, sink, few or n == 1)
+
+
+@pytest.mark.parametrize("k_size,v_size,q_size", [(2.0 ** 30, 2.0 ** -40, 2.0 ** -30), (2.0 ** -20, 2.0 ** 60, 2.0 ** 18), (1.0, 2.0 ** -20, 1.0)])
+def test_portions_of_any_size(k_size, v_size, q_size):
+    """Keys and values that float16 does not hold as they are."""
+    from hi_b200.kernels import ops
+    from hi_b200.parts.attention import attend_over_four_bit_pages
+
+    step = Step([(40, 100), (150, 0), (1, 70)], 8, 2, 128, 64, seed=12)
+    step.k, step.v, step.q = [k * k_size for k in step.k], [v * v_size for v in step.v], step.q * q_size
+    step.v[0][:, 1] *= 2.0 ** -10                # one head's values much smaller than the other's
+    step.fill()
+    got = attend_over_four_bit_pages(step.q, step.pages, step.table, step.ctx, 8, 2, 128, 0, 0, 0.09)
+    ops.check_tc_status()
+    for s in range(3):
+        _check_rows(step, s, got, {}, 0.09, None, s == 2)
+
+
+def test_reshaped_scores_go_over_bfloat16_pages():
+    from hi_b200.kernels import ops
+    from hi_b200.parts.attention import attend_over_four_bit_pages, attend_over_pages
+
+    step = Step([(40, 100), (1, 70), (1, 900)], 8, 2, 64, 64, seed=13).fill()
+    slopes = torch.rand(8, device=DEV, generator=_gen(1)) * 0.01
+    ctx = step.ctx
+    k, v, table = ops.expand_pages_4bit(step.pages, 64, step.table, ctx.cu_seqlens, step.positions, ctx.start_pos, ctx.n_new)
+    want = attend_over_pages(step.q, k, v, table, ctx, 8, 2, 64, 0, 0, 0.125, softcap=20.0, slopes=slopes)
+    got = attend_over_four_bit_pages(step.q, step.pages, step.table, ctx, 8, 2, 64, 0, 0, 0.125, softcap=20.0, slopes=slopes)
+    ops.check_tc_status()
+    assert torch.equal(got, want) and not got.isnan().any()
 
 
 def test_cache_refusals():
