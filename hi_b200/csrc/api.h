@@ -74,9 +74,12 @@ int hb_attention_decode_4bit(const void* q, const void* pages, const int* block_
                              int page_size, int chunk, int window, int keep, float scale, int sink,
                              const float* sink_values, int split_tiles, int splits, float* part_acc, float* part_ml,
                              int* status, const long long* rows, int step_tokens, cudaStream_t stream);
-// x [tokens, K] (rows x_ld elements apart) times a weight of four bits in blocks of 16 rows x 128 k (four_bit_linear.cu)
+// x [tokens, K] (rows x_ld elements apart) times a weight of four bits in blocks of 16 rows x 128 k: up to 16 tokens
+// (four_bit_linear.cu), many (four_bit_gemm_tc.cu)
 int hb_four_bit_linear(const void* x, long long x_ld, const void* w, const void* bias, void* out, int out_dtype, int tokens,
                        int n_out, int K, int group, cudaStream_t stream);
+int hb_four_bit_linear_tc(const void* x, long long x_ld, const void* w, const void* bias, void* out, int out_dtype, int tokens,
+                          int n_out, int K, int group, int* status, cudaStream_t stream);
 
 // sink != 0 (every attention entry point): the softmax's denominator has one more term of score 0,
 // p_j = e^{s_j} / (1 + sum e^{s_j}); the term has no value. The general kernel and the merge also take

@@ -1,0 +1,417 @@
+// Products of many tokens with weights of four bits on the 5th-generation tensor cores (tcgen05): out[t, n] = sum_k x[t, k] w[n, k]
+// (+ bias[n]), w in the blocks of four_bit_linear.cu, x bfloat16, float32 sums in tensor memory.
+//
+// The product is taken transposed as in grouped_gemm_tc.cu: 128 weight rows are the MMA's M, up to 256 tokens its N. The operand in shared
+// memory has to be bfloat16, so here, unlike for a few tokens, scale * (code - 8) is rounded to it (2^-9 of a weight at most, as a bfloat16
+// checkpoint's weights are; the group's scale cannot wait for the sum, which runs over all groups in tensor memory). A stage is 128 k, one
+// block of weights a row tile of 16:
+//   warp 0        brings the tokens' tile by TMA (two boxes of 64 k, 128-byte swizzle)
+//   warps 2 .. 9  each takes one of the 8 row tiles: its block comes four stages ahead into registers (two 16-byte loads a lane),
+//                 each word of eight codes becomes eight bfloat16 (code in the mantissa of 128, minus 136, times the scale: 15
+//                 instructions) and one 16-byte store into the swizzled tile; odd rows store their words in another order, so that
+//                 eight lanes meet eight banks of 16 bytes
+//   warp 1        issues the products, eight of 16 k a stage, and the commits
+//   warps 10 .. 13 read the sums back, add the bias and store: the next tile accumulates into the other half of tensor memory
+// Every row tile is unpacked once per tile of tokens: some 150 instructions a warp against 256 to 1,024 cycles of products (64 to 256 tokens).
+// PAIR: two blocks of a cluster on 256 rows x up to 256 tokens (cta_group::2), each with its 128 rows and half of the tokens, for
+// many tokens, where the tokens' way from L2 would bound single blocks. SPLIT: few tiles: the blocks of a cluster share out K, one tile a cluster; each
+// sends its sums to the block that finishes those tokens, which adds them in the order of the blocks.
+// Every wait is bounded; a block that gave up says where in `status` and leaves by the common exit.
+#include <cuda.h>
+
+#include "api.h"
+#include "common.cuh"
+#include "tc.cuh"
+
+namespace {
+
+constexpr int BF = 128, KB = 128;                 // weight rows of a block, k of a stage
+constexpr int A_BYTES = BF * KB * 2;
+constexpr int UNPACK = 8, EPILOGUE = 4, THREADS = 32 * (2 + UNPACK + EPILOGUE);
+constexpr int AHEAD = 4;
+
+struct Params {
+  const uint8_t* w;
+  const __nv_bfloat16* bias;
+  void* out;
+  int* status;
+  int out_f32, tokens, n_out, chunks, most;       // most: tokens of a tile, a multiple of 16
+};
+
+// a wait for arrivals from the other block of a pair as well
+__device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(tc::smem_u32(bar)), "r"(parity) : "memory");
+  return __all_sync(0xffffffffu, ok != 0) || (tc::mbar_wait_warp(bar, parity) && wait_pair(bar, parity));
+}
+template <int GPC> __device__ __forceinline__ uint2 load_scales(const uint8_t* p) {
+  if constexpr (GPC == 1) return make_uint2(__ldg(reinterpret_cast<const unsigned short*>(p)), 0u);
+  else if constexpr (GPC == 2) return make_uint2(__ldg(reinterpret_cast<const unsigned*>(p)), 0u);
+  else return __ldg(reinterpret_cast<const uint2*>(p));
+}
+// both halves of a word: scale i of four
+__device__ __forceinline__ unsigned scale_pair(uint2 v, int i) {
+  return __byte_perm(i < 2 ? v.x : v.y, 0u, i & 1 ? 0x3232 : 0x1010);
+}
+// eight codes as bfloat16 scale * (code - 8)
+__device__ __forceinline__ uint4 unpack(unsigned w, unsigned scale) {
+  unsigned r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    unsigned x = (w >> (4 * i) & 0x000f000fu) | 0x43004300u;          // 128 + code
+    asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0x43084308u));    // exact
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(x), "r"(scale));
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <bool PAIR, bool SPLIT, int BT, int STAGES, int GPC>
+__global__ void __launch_bounds__(THREADS, 1)
+four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) {
+  constexpr int XR = PAIR ? BT / 2 : BT;          // token rows of a stage
+  constexpr int X_BYTES = XR * KB * 2, STAGE_BYTES = A_BYTES + X_BYTES;
+  constexpr int BLOCK_BYTES = 1024 + 32 * GPC;
+  constexpr int SLOTS = SPLIT ? 1 : 2;
+  constexpr int TMEM_COLS = SPLIT ? 128 : SLOTS * BT;      // (a run of 32 columns of a share may start at the 48th of 64)
+  static_assert(!(PAIR && SPLIT) && TMEM_COLS <= 512, "a form at a time, sums within tensor memory");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full_x = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  uint64_t* full_a = full_x + STAGES;
+  uint64_t* empty = full_a + STAGES;
+  uint64_t* acc_full = empty + STAGES;            // [2]
+  uint64_t* acc_empty = acc_full + 2;             // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+
+  const int warp = tc::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rank = PAIR || SPLIT ? (int)tc::cluster_rank() : 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      tc::mbar_init(&full_x[s], 1);
+      tc::mbar_init(&full_a[s], PAIR ? 2 * UNPACK : UNPACK);
+      tc::mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], PAIR ? 2 * EPILOGUE : EPILOGUE); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) tc::alloc_pair(tmem_slot, TMEM_COLS);
+    else tc::alloc(tmem_slot, TMEM_COLS);
+  }
+  tc::fence_before();
+  if constexpr (PAIR) tc::cluster_meet();         // (the other block's barriers are ready too)
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  constexpr int FEATURES = PAIR ? 2 * BF : BF;
+  const int f_tiles = (p.n_out + FEATURES - 1) / FEATURES, t_tiles = (p.tokens + p.most - 1) / p.most, all = f_tiles * t_tiles;
+  int splits = 1;
+  if constexpr (SPLIT) asm("mov.u32 %0, %cluster_nctaid.x;" : "=r"(splits));
+  const int group = PAIR ? 2 : splits, units = gridDim.x / group, unit = blockIdx.x / group;
+  const int share = (p.chunks + splits - 1) / splits;
+  const int c0 = SPLIT ? rank * share : 0, c1 = SPLIT ? min(p.chunks, c0 + share) : p.chunks;
+  // tiles in order of weights: neighbours share their tokens
+  auto tile_at = [&](int i, int& f0, int& t0, int& n) {
+    const int t = unit + i * units;
+    if (t >= all) return false;
+    f0 = t % f_tiles * FEATURES;
+    t0 = t / f_tiles * p.most;
+    n = min(p.most, p.tokens - t0);
+    return true;
+  };
+
+  if (warp == 0) {                                // ---- tokens
+    int s = 0, turn = 1, issued = 0, f0, t0, n;
+    bool ok = true;
+    const uint32_t mine = tc::elect_one(), ring = tc::smem_u32(smem), bars = PAIR ? tc::even_block(full_x) : tc::smem_u32(full_x);
+    for (int i = 0; ok && tile_at(i, f0, t0, n); ++i) {
+      const int row = tc::uniform(t0 + (PAIR ? rank * ((n + 15) / 16 * 8) : 0));      // a pair's tokens are half in one block, half in the other
+      for (int c = tc::uniform(c0); c < c1; ++c) {
+        if (!tc::mbar_wait_warp(&empty[s], turn)) {
+          if (lane == 0) atomicExch(p.status, 51);
+          ok = false;
+          break;
+        }
+        const uint32_t to = ring + s * STAGE_BYTES + A_BYTES, bar = bars + s * 8;
+        if (mine && rank == 0 | !PAIR) tc::mbar_expect_tx(&full_x[s], (PAIR ? 2 : 1) * X_BYTES);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if constexpr (PAIR) tc::tma_load_2d_pair_if(mine, to + h * (X_BYTES / 2), &map_x, c * KB + h * 64, row, bar);
+          else tc::tma_load_2d_if(mine, to + h * (X_BYTES / 2), &map_x, c * KB + h * 64, row, bar);
+        }
+        if (++s == STAGES) { s = 0; turn ^= 1; }
+        ++issued;
+      }
+    }
+    // nothing reaches for the block's memory when it ends: the last commits have arrived, which come behind the products and those behind
+    // the copies; where a wait ran out they may never, and the copies on their way are waited for
+    if (ok) {
+      for (int i = 0; i < STAGES && tc::mbar_wait_warp(&empty[s], turn); ++i)
+        if (++s == STAGES) { s = 0; turn ^= 1; }
+    } else if (rank == 0 || !PAIR) {
+      for (int i = max(0, issued - STAGES); i < issued; ++i) tc::mbar_wait_warp(&full_x[i % STAGES], (i / STAGES) & 1);
+    }
+  } else if (warp == 1) {                         // ---- products
+    const uint32_t mine = tc::elect_one();
+    const uint64_t ring = tc::desc_kmajor(tc::smem_u32(smem));
+    int s = 0, turn = 0, f0, t0, n;
+    bool ok = true;
+    for (int i = 0; (rank == 0 || !PAIR) && ok && tile_at(i, f0, t0, n); ++i) {
+      const int b = i % SLOTS;
+      if (i >= SLOTS && !tc::mbar_wait_warp(&acc_empty[b], (i / SLOTS - 1) & 1)) {
+        if (lane == 0) atomicExch(p.status, 54);
+        break;
+      }
+      tc::fence_after();
+      const uint32_t idesc = tc::idesc_bf16(FEATURES, tc::uniform((n + 15) & ~15), false), acc = tmem + b * BT;
+      for (int c = c0; c < c1; ++c) {
+        if (!tc::mbar_wait_warp(&full_x[s], turn) || !(PAIR ? wait_pair(&full_a[s], turn) : tc::mbar_wait_warp(&full_a[s], turn))) {
+          if (lane == 0) atomicExch(p.status, 52);
+          ok = false;
+          break;
+        }
+        tc::fence_after();
+        const uint64_t a = ring + s * (STAGE_BYTES >> 4), x = a + (A_BYTES >> 4);
+#pragma unroll
+        for (int k = 0; k < KB / 16; ++k) {
+          const uint64_t ka = a + ((k / 4 * (A_BYTES / 2) + k % 4 * 32) >> 4), kx = x + ((k / 4 * (X_BYTES / 2) + k % 4 * 32) >> 4);
+          if constexpr (PAIR) tc::mma_pair_if(mine, acc, ka, kx, idesc, (c - c0) | k);
+          else tc::mma_if(mine, acc, ka, kx, idesc, (c - c0) | k);
+        }
+        if constexpr (PAIR) tc::commit_pair_if(mine, &empty[s]);
+        else tc::commit_if(mine, &empty[s]);
+        if (++s == STAGES) { s = 0; turn ^= 1; }
+      }
+      if constexpr (PAIR) tc::commit_pair_if(mine, &acc_full[b]);
+      else tc::commit_if(mine, &acc_full[b]);
+    }
+  } else if (warp < 2 + UNPACK) {                 // ---- weights
+    const int part = warp - 2, g = lane >> 2, q4 = lane & 3, odd = g & 1;
+    const int row_tiles = (p.n_out + 15) / 16;
+    int s = 0, turn = 1, f0, t0, n;
+    uint4 lo[AHEAD], hi[AHEAD];
+    uint2 s_lo[AHEAD], s_hi[AHEAD];
+    int l_i = 0, l_c = c0;                        // what is loaded next: its tile and stage
+    bool l_more = tile_at(0, f0, t0, n) && c0 < c1;
+    int l_row = l_more ? f0 / 16 + rank * (PAIR ? 8 : 0) + part : 0;
+    auto load = [&](int u) {
+      if (!l_more) return;
+      if (l_row < row_tiles) {
+        const uint8_t* b = p.w + ((size_t)l_row * p.chunks + l_c) * BLOCK_BYTES;
+        lo[u] = __ldg(reinterpret_cast<const uint4*>(b) + lane);
+        hi[u] = __ldg(reinterpret_cast<const uint4*>(b) + 32 + lane);
+        s_lo[u] = load_scales<GPC>(b + 1024 + g * 2 * GPC);
+        s_hi[u] = load_scales<GPC>(b + 1024 + (g + 8) * 2 * GPC);
+      }
+      if (++l_c == c1) {
+        l_c = c0;
+        int f = 0, t, m;
+        l_more = tile_at(++l_i, f, t, m);
+        l_row = f / 16 + rank * (PAIR ? 8 : 0) + part;
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) load(u);
+    const uint32_t bars = PAIR ? tc::even_block(full_a) : 0;
+    // of this lane's rows g and g + 8 in the tile: the 16-byte places of its words of even and odd turns
+    uint8_t* const row = smem + (part * 16 + g) * 128;
+    int i = 0, c = c0;
+    bool more = tile_at(0, f0, t0, n) && c0 < c1;
+    while (more) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (!more) break;
+        if (!tc::mbar_wait_warp(&empty[s], turn)) {
+          if (lane == 0) atomicExch(p.status, 53);
+          more = false;
+          break;
+        }
+        const bool there = f0 / 16 + rank * (PAIR ? 8 : 0) + part < row_tiles;      // (rows past the weight's are not stored: anything may be there)
+        if (there) {
+          const unsigned wl[4] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w}, wh[4] = {hi[u].x, hi[u].y, hi[u].z, hi[u].w};
+          uint8_t* const to = row + s * STAGE_BYTES;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {           // words j and j ^ 1 change places in odd rows
+            const unsigned a = odd ? wl[j ^ 1] : wl[j], b = odd ? wh[j ^ 1] : wh[j];
+            const unsigned sa = GPC == 4 ? (odd ? scale_pair(s_lo[u], j ^ 1) : scale_pair(s_lo[u], j)) : scale_pair(s_lo[u], j * GPC / 4);
+            const unsigned sb = GPC == 4 ? (odd ? scale_pair(s_hi[u], j ^ 1) : scale_pair(s_hi[u], j)) : scale_pair(s_hi[u], j * GPC / 4);
+            uint8_t* at = to + (j >> 1) * (A_BYTES / 2) + (((((j & 1) ^ odd) << 2 | q4) ^ g) << 4);
+            *reinterpret_cast<uint4*>(at) = unpack(a, sa);
+            *reinterpret_cast<uint4*>(at + 8 * 128) = unpack(b, sb);
+          }
+        }
+        load(u);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) tc::arrive_even(bars + s * 8);
+          else tc::mbar_arrive(&full_a[s]);
+        }
+        if (++s == STAGES) { s = 0; turn ^= 1; }
+        if (++c == c1) {
+          c = c0;
+          more = tile_at(++i, f0, t0, n);
+        }
+      }
+    }
+  } else if constexpr (!SPLIT) {                  // ---- results
+    const int quarter = warp & 3;
+    int f0, t0, n;
+    for (int i = 0; tile_at(i, f0, t0, n); ++i) {
+      const int b = i % SLOTS, f = f0 + rank * BF + quarter * 32 + lane;
+      const bool f_ok = f < p.n_out;
+      const float bias = p.bias && f_ok ? __bfloat162float(p.bias[f]) : 0.f;
+      if (!tc::mbar_wait_warp(&acc_full[b], (i / SLOTS) & 1)) {
+        if (lane == 0) atomicExch(p.status, 55);
+        break;
+      }
+      tc::fence_after();
+#pragma unroll 1
+      for (int c = 0; c < n; c += 32) {
+        float v[32];
+        tc::ld32(tmem + b * BT + ((uint32_t)(quarter * 32) << 16) + c, v);
+        if (!f_ok) continue;
+        const size_t at = (size_t)(t0 + c) * p.n_out + f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          if (c + j >= n) break;
+          if (p.out_f32) reinterpret_cast<float*>(p.out)[at + (size_t)j * p.n_out] = v[j] + bias;
+          else reinterpret_cast<__nv_bfloat16*>(p.out)[at + (size_t)j * p.n_out] = __float2bfloat16_rn(v[j] + bias);
+        }
+      }
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) tc::arrive_even(tc::even_block(&acc_empty[b]));
+        else tc::mbar_arrive(&acc_empty[b]);
+      }
+    }
+  }
+  if constexpr (SPLIT) {
+    // the cluster's one tile: every block sends its sums of a run of tokens to the block that finishes it
+    int f0, t0, n;
+    const bool there = tile_at(0, f0, t0, n);
+    bool ok = true;
+    if (there && c0 < c1 && warp >= 2 + UNPACK) {
+      ok = tc::mbar_wait_warp(&acc_full[0], 0);
+      if (!ok && lane == 0) atomicExch(p.status, 55);
+    }
+    tc::fence_after();
+    __syncwarp();
+    tc::cluster_meet();                           // every block's ring is free
+    const int run = (n + splits - 1) / splits;
+    if (there && c0 < c1 && warp >= 2 + UNPACK) {
+      const int quarter = warp & 3;
+#pragma unroll 1
+      for (int r = 0; r < splits; ++r) {
+        uint32_t at;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at)
+            : "r"(tc::smem_u32(smem) + (uint32_t)((rank * run * BF + quarter * 32 + lane) * 4)), "r"(r));
+        const int end = min(n, (r + 1) * run);
+#pragma unroll 1
+        for (int c = r * run; c < end; c += 32) {
+          float v[32];
+          tc::ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < end) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + (c - r * run + j) * BF * 4), "f"(v[j]) : "memory");
+        }
+      }
+    }
+    __syncwarp();
+    tc::cluster_meet();
+    const int mine = there ? min(run, n - rank * run) : 0;
+    const float* sums = reinterpret_cast<const float*>(smem);
+    for (int i = threadIdx.x; i < mine * BF; i += THREADS) {
+      const int f = f0 + i % BF;
+      if (f >= p.n_out) continue;
+      float v = 0.f;
+      for (int r = 0; r * share < p.chunks; ++r) v += sums[r * run * BF + i];      // (of the blocks that had a part of K)
+      if (p.bias) v += __bfloat162float(p.bias[f]);
+      const size_t at = (size_t)(t0 + rank * run + i / BF) * p.n_out + f;
+      if (p.out_f32) reinterpret_cast<float*>(p.out)[at] = v;
+      else reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+    }
+  }
+  tc::fence_before();
+  __syncwarp();
+  if constexpr (PAIR) tc::cluster_meet();         // no product of the pair reads this block any more
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after();
+    if constexpr (PAIR) tc::dealloc_pair(tmem, TMEM_COLS);
+    else tc::dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// [rows, cols] bfloat16, rows ld elements apart
+bool make_map_rows(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
+  tc::EncodeTiledFn fn = tc::encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld * 2};
+  const cuuint32_t box[2] = {64, box_rows}, elem[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool PAIR, bool SPLIT, int BT, int STAGES, int GPC>
+int launch(const void* x, long long x_ld, int K, const Params& p, int blocks, int cluster, cudaStream_t stream) {
+  CUtensorMap map;
+  if (!make_map_rows(&map, x, p.tokens, K, x_ld, PAIR ? BT / 2 : BT)) return HB_ERR_UNSUPPORTED;
+  const size_t smem = STAGES * (size_t)(A_BYTES + (PAIR ? BT / 2 : BT) * KB * 2) + 1024 + 256;
+  auto* kernel = four_bit_gemm_kernel<PAIR, SPLIT, BT, STAGES, GPC>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(blocks);
+  config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = cluster > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&config, kernel, map, p);
+  return e == cudaSuccess ? HB_OK : (int)e;
+}
+
+template <int GPC>
+int gemm(const void* x, long long x_ld, int K, Params p, cudaStream_t stream) {
+  const int f_tiles = (p.n_out + BF - 1) / BF;
+  if (p.tokens > 128) {
+    const int t_tiles = (p.tokens + 255) / 256, pairs = (f_tiles + 1) / 2 * t_tiles;
+    p.most = (((p.tokens + t_tiles - 1) / t_tiles) + 15) / 16 * 16;
+    return launch<true, false, 256, 3, GPC>(x, x_ld, K, p, 2 * (pairs < 74 ? pairs : 74), 2, stream);
+  }
+  p.most = p.tokens;
+  int splits = f_tiles > 74 ? 1 : f_tiles > 37 ? 2 : 4;
+  while (splits > 1 && p.chunks < 4 * splits) splits /= 2;
+  if (splits == 1) {
+    const int blocks = f_tiles < 148 ? f_tiles : 148;
+    return p.tokens <= 64 ? launch<false, false, 64, 4, GPC>(x, x_ld, K, p, blocks, 1, stream)
+                          : launch<false, false, 128, 3, GPC>(x, x_ld, K, p, blocks, 1, stream);
+  }
+  return p.tokens <= 64 ? launch<false, true, 64, 4, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream)
+                        : launch<false, true, 128, 3, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream);
+}
+
+}  // namespace
+
+// Arguments as hb_four_bit_linear; x_ld at least K (a tensor map's rows); status: one int on the device, nonzero after a wait that ran out.
+extern "C" int hb_four_bit_linear_tc(const void* x, long long x_ld, const void* w, const void* bias, void* out, int out_dtype,
+                                     int tokens, int n_out, int K, int group, int* status, cudaStream_t stream) {
+  if (!x || !w || !out || !status || tokens < 0 || n_out < 0 || K < 0 || (out_dtype != HB_DTYPE_F32 && out_dtype != HB_DTYPE_BF16))
+    return HB_ERR_BAD_ARG;
+  if ((group != 32 && group != 64 && group != 128) || K % group || K == 0 || x_ld % 8 || x_ld < K ||
+      ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15))
+    return HB_ERR_UNSUPPORTED;
+  if (tokens == 0 || n_out == 0) return HB_OK;
+  const Params p{(const uint8_t*)w, (const __nv_bfloat16*)bias, out, status, out_dtype == HB_DTYPE_F32, tokens, n_out, (K + KB - 1) / KB, 0};
+  return group == 128 ? gemm<1>(x, x_ld, K, p, stream) : group == 64 ? gemm<2>(x, x_ld, K, p, stream) : gemm<4>(x, x_ld, K, p, stream);
+}

@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) four_bit_few_kernel(const 
   float2* start = reinterpret_cast<float2*>(xs + (size_t)a.panel * NT * 128);     // [panel][GPC][NT][4]: what the eights come to, negative
   float* red = reinterpret_cast<float*>(start + (size_t)a.panel * GPC * NT * 4);  // [2][warps][TILE]
   float* kept = red + 2 * warps * TILE;                                           // [tiles][TILE], of earlier panels
-  const int t0 = blockIdx.y * 8 * NT, tokens = min(8 * NT, a.tokens - t0);
+  const int tokens = a.tokens;
   const int row_tiles = (a.n_out + ROWS - 1) / ROWS;
   const int tiles = (row_tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;
   int turn = 0;
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) four_bit_few_kernel(const 
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int token = n * 8 + g;
-        const __nv_bfloat16* from = a.x + (size_t)(t0 + min(token, tokens - 1)) * a.x_ld;
+        const __nv_bfloat16* from = a.x + (size_t)min(token, tokens - 1) * a.x_ld;
         float eights[GPC][4];
 #pragma unroll
         for (int k = 0; k < GPC; ++k)
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) four_bit_few_kernel(const 
         if (t >= tokens || row >= a.n_out) continue;
         sum *= fb::UNSCALE;
         if (a.bias) sum += __bfloat162float(a.bias[row]);
-        const size_t at = (size_t)(t0 + t) * a.n_out + row;
+        const size_t at = (size_t)t * a.n_out + row;
         if (a.out_f32) reinterpret_cast<float*>(a.out)[at] = sum;
         else reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(sum);
       }
@@ -184,19 +184,19 @@ int launch_few(Few a, cudaStream_t stream) {
   auto* kernel = four_bit_few_kernel<NT, GPC>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return (int)e;
-  kernel<<<dim3(blocks, (a.tokens + 8 * NT - 1) / (8 * NT)), warps * 32, smem, stream>>>(a);
+  kernel<<<blocks, warps * 32, smem, stream>>>(a);
   HB_LAUNCH_CHECK();
   return HB_OK;
 }
 
 }  // namespace
 
-// x [tokens, K] with rows x_ld elements apart, w blocks as above, bias [n_out] bfloat16 or null, out [tokens, n_out] contiguous.
+// x [tokens, K] with rows x_ld elements apart, up to 16 of them, w blocks as above, bias [n_out] bfloat16 or null, out [tokens, n_out] contiguous.
 extern "C" int hb_four_bit_linear(const void* x, long long x_ld, const void* w, const void* bias, void* out, int out_dtype, int tokens,
                                   int n_out, int K, int group, cudaStream_t stream) {
   if (!x || !w || !out || tokens < 0 || n_out < 0 || K < 0 || (out_dtype != HB_DTYPE_F32 && out_dtype != HB_DTYPE_BF16))
     return HB_ERR_BAD_ARG;
-  if ((group != 32 && group != 64 && group != 128) || K % group || K == 0 || x_ld % 8 ||
+  if (tokens > 16 || (group != 32 && group != 64 && group != 128) || K % group || K == 0 || x_ld % 8 ||
       ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15))
     return HB_ERR_UNSUPPORTED;
   if (tokens == 0 || n_out == 0) return HB_OK;

@@ -42,6 +42,7 @@ _SIGNATURES = {
     "hb_attention_prefill_tc_half": [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, I, I, P, I, P, P, I, P, P],
     "hb_attention_decode_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, P, I, I, P, P, P, P, I, P],
     "hb_four_bit_linear": [P, c_longlong, P, P, P, I, I, I, I, I, P],
+    "hb_four_bit_linear_tc": [P, c_longlong, P, P, P, I, I, I, I, I, P, P],
     "hb_paged_attention": [P, I, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, F, P, P, I, I, P, P, P],
     "hb_attention_portions": [P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, F, I, F, P, P, I, P, P, P],
     "hb_attention_merge": [P, P, P, I, I, I, I, I, I, P, P],
@@ -2289,7 +2290,7 @@ def _tc_status(device: torch.device) -> torch.Tensor:
 
 def check_tc_status(device=None) -> None:
     """Raise if a kernel with bounded mbarrier waits (the tcgen05 products and attention, the TMA
-    decode attention, the recurrences by chunks) timed out on one of its barriers since the last check, or the decode
+    and the 4-bit decode attention, the recurrences by chunks) timed out on one of its barriers since the last check, or the decode
     attention was given a row that its step does not have
     (synchronises; skipped while a stream is being captured)."""
     TC_USED[0] = False
@@ -2309,7 +2310,12 @@ def check_tc_status(device=None) -> None:
                      3: "grouped product: the epilogue waiting for the accumulator",
                      4: "grouped product: the MMA issuer waiting for a free accumulator",
                      31: "decode attention: the warps waiting for a tile's TMA loads",
-                     41: "recurrence by chunks: the warps waiting for a chunk's copies"}.get(
+                     41: "recurrence by chunks: the warps waiting for a chunk's copies",
+                     51: "4-bit product: the TMA producer waiting for a free stage",
+                     52: "4-bit product: the MMA issuer waiting for a stage",
+                     53: "4-bit product: the warps that unpack weights waiting for a free stage",
+                     54: "4-bit product: the MMA issuer waiting for a free accumulator",
+                     55: "4-bit product: the epilogue waiting for the accumulator"}.get(
                 code, f"prefill attention, wait {code}" if code >= 11 else f"code {code}")
             raise KernelError(f"a kernel gave up a bounded wait ({where}); its output is invalid")
 
@@ -2500,6 +2506,7 @@ def ranked_rows(logits: torch.Tensor, temperatures: torch.Tensor, top_ps: torch.
 # --------------------------------------------------------------------------- four bits
 FOUR_BIT_GROUPS = (32, 64, 128)      # inputs of a weight's row that share a scale
 FOUR_BIT_ROW_LENGTHS = (64, 128)     # head sizes of the 4-bit cache
+FOUR_BIT_FEW = 16                    # tokens up to which a product streams the weights through mma.sync; more go through tcgen05
 
 
 def _on_current_device(*tensors) -> None:
@@ -2567,7 +2574,8 @@ def quantize_weight(weight: torch.Tensor, group: int = 64) -> FourBitWeight:
 def four_bit_linear(x: torch.Tensor, weight: FourBitWeight, out_dtype: torch.dtype = torch.bfloat16,
                     bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ weight.T (+ bias)`` for bfloat16 ``x`` [N, K] (its rows may be a column slice of a wider matrix) and a weight held in
-    four bits, with float32 sums, in ``out_dtype`` (bfloat16 or float32); ``bias`` bfloat16 [M]."""
+    four bits, with float32 sums, in ``out_dtype`` (bfloat16 or float32); ``bias`` bfloat16 [M]. Up to 16 rows of ``x`` the products are
+    those of the weight's exact values; more rows take each value rounded to bfloat16, as a bfloat16 weight would hold it."""
     if not x.is_cuda:
         raise KernelError("x must be a CUDA tensor; this engine has no CPU path")
     m, k = weight.shape
@@ -2576,7 +2584,7 @@ def four_bit_linear(x: torch.Tensor, weight: FourBitWeight, out_dtype: torch.dty
                           f"not {x.dtype} {tuple(x.shape)} into {out_dtype}")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise KernelError("products with 4-bit weights have no gradients")
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) % 8) or x.data_ptr() % 16:
+    if x.stride(1) != 1 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < k)) or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
@@ -2590,8 +2598,13 @@ def four_bit_linear(x: torch.Tensor, weight: FourBitWeight, out_dtype: torch.dty
     out = torch.empty((n, m), dtype=out_dtype, device=x.device)
     if n == 0:
         return out
-    _check(lib().hb_four_bit_linear(_ptr(x), x.stride(0) if n > 1 else k, _ptr(weight.blocks), _ptr(bias), _ptr(out), _dt(out), n, m,
-                                    k, weight.group, _stream()), "four_bit_linear")
+    if n <= FOUR_BIT_FEW:
+        _check(lib().hb_four_bit_linear(_ptr(x), x.stride(0) if n > 1 else k, _ptr(weight.blocks), _ptr(bias), _ptr(out), _dt(out), n, m,
+                                        k, weight.group, _stream()), "four_bit_linear")
+    else:
+        TC_USED[0] = True
+        _check(lib().hb_four_bit_linear_tc(_ptr(x), x.stride(0), _ptr(weight.blocks), _ptr(bias), _ptr(out), _dt(out), n, m, k,
+                                           weight.group, _ptr(_tc_status(x.device)), _stream()), "four_bit_linear_tc")
     return out
 
 

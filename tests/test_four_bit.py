@@ -22,14 +22,16 @@ def _weight(m, k, group, g):
 
 
 def _check_linear(got, x, codes, scales, bias=None):
-    """Products of whole numbers with x are exact; what is rounded: float32 sums (the tensor cores drop what lies 2^-23 under the
+    """Up to 16 tokens: products of whole numbers with x are exact; what is rounded: float32 sums (the tensor cores drop what lies 2^-23 under the
     largest term, up to 9 times a group, then a few dozen additions: 2^-18 of the sum of all magnitudes, the eights' among them) and
-    the result."""
+    the result. More tokens: each weight is rounded to bfloat16, 2^-8 of every product, and the float32 sums as before."""
     want = x.double() @ weight_values(codes, scales).t()
     size = x.double().abs() @ ((codes.double() + 8) * scales.double().repeat_interleave(codes.shape[1] // scales.shape[1], 1)).t()
     if bias is not None:
         want = want + bias.double()
     tol = 2.0 ** -18 * size
+    if x.shape[0] > 16:
+        tol = tol + 2.0 ** -8 * (x.double().abs() @ weight_values(codes, scales).abs().t())
     if got.dtype == BF16:
         tol = tol + 2.0 ** -8 * want.abs()
     else:
@@ -49,9 +51,34 @@ def test_linear(m, k, group, tokens, out_dtype):
     wide = torch.randn(tokens, k + 24, device=DEV, generator=g).to(BF16)
     x = wide[:, 8: 8 + k]
     bias = torch.randn(m, device=DEV, generator=g).to(BF16)
-    if tokens <= 16 or out_dtype == BF16:
-        _check_linear(linear(x, w, out_dtype=out_dtype), x, codes, scales)
-        _check_linear(linear(x, w, out_dtype=out_dtype, bias=bias), x, codes, scales, bias)
+    from hi_b200.kernels import ops
+
+    _check_linear(linear(x, w, out_dtype=out_dtype), x, codes, scales)
+    _check_linear(linear(x, w, out_dtype=out_dtype, bias=bias), x, codes, scales, bias)
+    ops.check_tc_status()
+
+
+@pytest.mark.parametrize("m,k,group", [(16, 32, 32), (129, 640, 128), (300, 2112, 64), (5000, 1056, 32), (9700, 256, 128), (19200, 128, 64)])
+@pytest.mark.parametrize("tokens", [17, 64, 65, 128, 129, 200, 256, 257, 600])
+def test_linear_of_many_tokens(m, k, group, tokens):
+    """Row tiles of 128 and of a pair's 256 that are not full, one block a tile and clusters that share K, tiles of 64, 128 and up to 256
+    tokens, more tiles than blocks; against the product with the rounded weights too, which leaves float32 sums."""
+    from hi_b200.kernels import ops
+    from hi_b200.parts.linear import linear
+
+    g = _gen(m + k + tokens)
+    w, codes, scales = _weight(m, k, group, g)
+    wide = torch.randn(tokens, k + 8, device=DEV, generator=g).to(BF16)
+    x = wide[:, :k]
+    bias = torch.randn(m, device=DEV, generator=g).to(BF16)
+    got = linear(x, w, out_dtype=torch.float32, bias=bias)
+    ops.check_tc_status()
+    rounded = weight_values(codes, scales).to(BF16).double()
+    want, size = x.double() @ rounded.t() + bias.double(), x.double().abs() @ rounded.abs().t()
+    assert ((got.double() - want).abs() <= 2.0 ** -18 * size + 2.0 ** -24 * want.abs()).all()
+    got16 = linear(x, w, bias=bias)
+    assert torch.equal(got16, got.to(BF16)) and torch.equal(linear(x.contiguous(), w, bias=bias), got16)
+    ops.check_tc_status()
 
 
 def test_linear_edges():
