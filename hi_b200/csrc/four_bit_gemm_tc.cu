@@ -6,13 +6,14 @@
 // checkpoint's weights are; the group's scale cannot wait for the sum, which runs over all groups in tensor memory). A stage is 128 k, one
 // block of weights a row tile of 16:
 //   warp 0        brings the tokens' tile by TMA (two boxes of 64 k, 128-byte swizzle)
-//   warps 2 .. 9  each takes one of the 8 row tiles: its block comes four stages ahead into registers (two 16-byte loads a lane),
-//                 each word of eight codes becomes eight bfloat16 (code in the mantissa of 128, minus 136, times the scale: 15
-//                 instructions) and one 16-byte store into the swizzled tile; odd rows store their words in another order, so that
-//                 eight lanes meet eight banks of 16 bytes
+//   warp 2        brings the 8 row tiles' blocks of codes as one bulk copy each, stages ahead, into a ring of their own
+//   warps 3 .. 18 unpack: eight of them take a stage, the others the next, each a row tile; a word of eight codes becomes eight bfloat16
+//                 (code in the mantissa of 128, minus 136, times the scale: 15 instructions) and one 16-byte store into the swizzled
+//                 tile; odd rows store their words in another order, so that eight lanes meet eight banks of 16 bytes
 //   warp 1        issues the products, eight of 16 k a stage, and the commits
-//   warps 10 .. 13 read the sums back, add the bias and store: the next tile accumulates into the other half of tensor memory
-// Every row tile is unpacked once per tile of tokens: some 150 instructions a warp against 256 to 1,024 cycles of products (64 to 256 tokens).
+//   warps 19 .. 22 read the sums back, add the bias and store: the next tile accumulates into the other half of tensor memory
+// Every row tile is unpacked once per tile of tokens. Eight unpacking warps with their loads in registers took 2,100 cycles a stage, most of
+// it waiting for the fence that shows their stores to the tensor cores and for loads, against 256 to 1,024 of products.
 // PAIR: two blocks of a cluster on 256 rows x up to 256 tokens (cta_group::2), each with its 128 rows and half of the tokens, for
 // many tokens, where the tokens' way from L2 would bound single blocks. SPLIT: few tiles: the blocks of a cluster share out K, one tile a cluster; each
 // sends its sums to the block that finishes those tokens, which adds them in the order of the blocks.
@@ -27,8 +28,9 @@ namespace {
 
 constexpr int BF = 128, KB = 128;                 // weight rows of a block, k of a stage
 constexpr int A_BYTES = BF * KB * 2;
-constexpr int UNPACK = 8, EPILOGUE = 4, THREADS = 32 * (2 + UNPACK + EPILOGUE);
-constexpr int AHEAD = 4;
+constexpr int UNPACK = 8, EPILOGUE = 4;           // warps: to unpack a stage (two stages at a time), to write results
+constexpr int FIRST_UNPACK = 3, FIRST_EPILOGUE = FIRST_UNPACK + 2 * UNPACK, THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE);
+constexpr int RAW_BLOCK = 1152;                   // room for a block of codes and scales, the largest
 
 struct Params {
   const uint8_t* w;
@@ -47,10 +49,10 @@ __device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity) {
       "selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(tc::smem_u32(bar)), "r"(parity) : "memory");
   return __all_sync(0xffffffffu, ok != 0) || (tc::mbar_wait_warp(bar, parity) && wait_pair(bar, parity));
 }
-template <int GPC> __device__ __forceinline__ uint2 load_scales(const uint8_t* p) {
-  if constexpr (GPC == 1) return make_uint2(__ldg(reinterpret_cast<const unsigned short*>(p)), 0u);
-  else if constexpr (GPC == 2) return make_uint2(__ldg(reinterpret_cast<const unsigned*>(p)), 0u);
-  else return __ldg(reinterpret_cast<const uint2*>(p));
+template <int GPC> __device__ __forceinline__ uint2 row_scales(const uint8_t* p) {
+  if constexpr (GPC == 1) return make_uint2(*reinterpret_cast<const unsigned short*>(p), 0u);
+  else if constexpr (GPC == 2) return make_uint2(*reinterpret_cast<const unsigned*>(p), 0u);
+  else return *reinterpret_cast<const uint2*>(p);
 }
 // both halves of a word: scale i of four
 __device__ __forceinline__ unsigned scale_pair(uint2 v, int i) {
@@ -68,7 +70,7 @@ __device__ __forceinline__ uint4 unpack(unsigned w, unsigned scale) {
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-template <bool PAIR, bool SPLIT, int BT, int STAGES, int GPC>
+template <bool PAIR, bool SPLIT, int BT, int STAGES, int RAW, int GPC>
 __global__ void __launch_bounds__(THREADS, 1)
 four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) {
   constexpr int XR = PAIR ? BT / 2 : BT;          // token rows of a stage
@@ -79,12 +81,15 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
   static_assert(!(PAIR && SPLIT) && TMEM_COLS <= 512, "a form at a time, sums within tensor memory");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full_x = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  uint8_t* raw = smem + STAGES * STAGE_BYTES;     // [RAW][UNPACK][RAW_BLOCK]
+  uint64_t* full_x = reinterpret_cast<uint64_t*>(raw + RAW * UNPACK * RAW_BLOCK);
   uint64_t* full_a = full_x + STAGES;
   uint64_t* empty = full_a + STAGES;
   uint64_t* acc_full = empty + STAGES;            // [2]
   uint64_t* acc_empty = acc_full + 2;             // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* raw_full = acc_empty + 2;             // [RAW]
+  uint64_t* raw_empty = raw_full + RAW;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + RAW);
 
   const int warp = tc::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int rank = PAIR || SPLIT ? (int)tc::cluster_rank() : 0;
@@ -94,6 +99,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
       tc::mbar_init(&full_a[s], PAIR ? 2 * UNPACK : UNPACK);
       tc::mbar_init(&empty[s], 1);
     }
+    for (int r = 0; r < RAW; ++r) { tc::mbar_init(&raw_full[r], 1); tc::mbar_init(&raw_empty[r], UNPACK); }
     for (int b = 0; b < 2; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], PAIR ? 2 * EPILOGUE : EPILOGUE); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -189,74 +195,76 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
       if constexpr (PAIR) tc::commit_pair_if(mine, &acc_full[b]);
       else tc::commit_if(mine, &acc_full[b]);
     }
-  } else if (warp < 2 + UNPACK) {                 // ---- weights
-    const int part = warp - 2, g = lane >> 2, q4 = lane & 3, odd = g & 1;
+  } else if (warp == 2) {                         // ---- codes
     const int row_tiles = (p.n_out + 15) / 16;
-    int s = 0, turn = 1, f0, t0, n;
-    uint4 lo[AHEAD], hi[AHEAD];
-    uint2 s_lo[AHEAD], s_hi[AHEAD];
-    int l_i = 0, l_c = c0;                        // what is loaded next: its tile and stage
-    bool l_more = tile_at(0, f0, t0, n) && c0 < c1;
-    int l_row = l_more ? f0 / 16 + rank * (PAIR ? 8 : 0) + part : 0;
-    auto load = [&](int u) {
-      if (!l_more) return;
-      if (l_row < row_tiles) {
-        const uint8_t* b = p.w + ((size_t)l_row * p.chunks + l_c) * BLOCK_BYTES;
-        lo[u] = __ldg(reinterpret_cast<const uint4*>(b) + lane);
-        hi[u] = __ldg(reinterpret_cast<const uint4*>(b) + 32 + lane);
-        s_lo[u] = load_scales<GPC>(b + 1024 + g * 2 * GPC);
-        s_hi[u] = load_scales<GPC>(b + 1024 + (g + 8) * 2 * GPC);
-      }
-      if (++l_c == c1) {
-        l_c = c0;
-        int f = 0, t, m;
-        l_more = tile_at(++l_i, f, t, m);
-        l_row = f / 16 + rank * (PAIR ? 8 : 0) + part;
-      }
-    };
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) load(u);
-    const uint32_t bars = PAIR ? tc::even_block(full_a) : 0;
-    // of this lane's rows g and g + 8 in the tile: the 16-byte places of its words of even and odd turns
-    uint8_t* const row = smem + (part * 16 + g) * 128;
-    int i = 0, c = c0;
-    bool more = tile_at(0, f0, t0, n) && c0 < c1;
-    while (more) {
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        if (!more) break;
-        if (!tc::mbar_wait_warp(&empty[s], turn)) {
-          if (lane == 0) atomicExch(p.status, 53);
-          more = false;
+    int r = 0, turn = 1, issued = 0, f0, t0, n;
+    bool ok = true;
+    for (int i = 0; ok && tile_at(i, f0, t0, n); ++i) {
+      const int tile = f0 / 16 + rank * (PAIR ? UNPACK : 0), tiles = max(0, min(UNPACK, row_tiles - tile));
+      const uint8_t* from = p.w + ((size_t)(tile + lane) * p.chunks + c0) * BLOCK_BYTES;
+      for (int c = c0; c < c1; ++c, from += BLOCK_BYTES) {
+        if (!tc::mbar_wait_warp(&raw_empty[r], turn)) {
+          if (lane == 0) atomicExch(p.status, 56);
+          ok = false;
           break;
         }
-        const bool there = f0 / 16 + rank * (PAIR ? 8 : 0) + part < row_tiles;      // (rows past the weight's are not stored: anything may be there)
-        if (there) {
-          const unsigned wl[4] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w}, wh[4] = {hi[u].x, hi[u].y, hi[u].z, hi[u].w};
-          uint8_t* const to = row + s * STAGE_BYTES;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {           // words j and j ^ 1 change places in odd rows
-            const unsigned a = odd ? wl[j ^ 1] : wl[j], b = odd ? wh[j ^ 1] : wh[j];
-            const unsigned sa = GPC == 4 ? (odd ? scale_pair(s_lo[u], j ^ 1) : scale_pair(s_lo[u], j)) : scale_pair(s_lo[u], j * GPC / 4);
-            const unsigned sb = GPC == 4 ? (odd ? scale_pair(s_hi[u], j ^ 1) : scale_pair(s_hi[u], j)) : scale_pair(s_hi[u], j * GPC / 4);
-            uint8_t* at = to + (j >> 1) * (A_BYTES / 2) + (((((j & 1) ^ odd) << 2 | q4) ^ g) << 4);
-            *reinterpret_cast<uint4*>(at) = unpack(a, sa);
-            *reinterpret_cast<uint4*>(at + 8 * 128) = unpack(b, sb);
-          }
-        }
-        load(u);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (lane == 0) tc::mbar_expect_tx(&raw_full[r], tiles * BLOCK_BYTES);
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR) tc::arrive_even(bars + s * 8);
-          else tc::mbar_arrive(&full_a[s]);
-        }
-        if (++s == STAGES) { s = 0; turn ^= 1; }
-        if (++c == c1) {
-          c = c0;
-          more = tile_at(++i, f0, t0, n);
-        }
+        if (lane < tiles)
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                       ::"r"(tc::smem_u32(raw + (r * UNPACK + lane) * RAW_BLOCK)), "l"(from), "r"(BLOCK_BYTES), "r"(tc::smem_u32(&raw_full[r]))
+                       : "memory");
+        if (++r == RAW) { r = 0; turn ^= 1; }
+        ++issued;
       }
+    }
+    for (int i = max(0, issued - RAW); i < issued; ++i) tc::mbar_wait_warp(&raw_full[i % RAW], (i / RAW) & 1);      // no copy is under way at the end
+  } else if (warp < FIRST_EPILOGUE) {             // ---- weights
+    const int part = (warp - FIRST_UNPACK) % UNPACK, first = (warp - FIRST_UNPACK) / UNPACK, g = lane >> 2, q4 = lane & 3, odd = g & 1;
+    int f0, t0, n;
+    const uint32_t bars = PAIR ? tc::even_block(full_a) : tc::smem_u32(full_a);
+    uint8_t* const row = smem + (part * 16 + g) * 128;
+    int tiles = 0;
+    while (tile_at(tiles, f0, t0, n)) ++tiles;
+    const int stages = c1 > c0 ? tiles * (c1 - c0) : 0;
+    int s = first % STAGES, turn = 1 ^ (first / STAGES & 1), r = first % RAW, r_turn = first / RAW & 1;
+    for (int i = first; i < stages; i += 2) {
+      if (!tc::mbar_wait_warp(&raw_full[r], r_turn)) {
+        if (lane == 0) atomicExch(p.status, 57);
+        break;
+      }
+      const uint8_t* block = raw + (r * UNPACK + part) * RAW_BLOCK;        // (rows past the weight's: whatever is there; they are not written out)
+      const uint4 lo = *reinterpret_cast<const uint4*>(block + lane * 16), hi = *reinterpret_cast<const uint4*>(block + 512 + lane * 16);
+      const uint2 s_lo = row_scales<GPC>(block + 1024 + g * 2 * GPC), s_hi = row_scales<GPC>(block + 1024 + (g + 8) * 2 * GPC);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&raw_empty[r]);
+      const unsigned wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+      uint4 a[4], b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {               // words j and j ^ 1 change places in odd rows
+        const unsigned sa = GPC == 4 ? (odd ? scale_pair(s_lo, j ^ 1) : scale_pair(s_lo, j)) : scale_pair(s_lo, j * GPC / 4);
+        const unsigned sb = GPC == 4 ? (odd ? scale_pair(s_hi, j ^ 1) : scale_pair(s_hi, j)) : scale_pair(s_hi, j * GPC / 4);
+        a[j] = unpack(odd ? wl[j ^ 1] : wl[j], sa);
+        b[j] = unpack(odd ? wh[j ^ 1] : wh[j], sb);
+      }
+      if (!tc::mbar_wait_warp(&empty[s], turn)) {
+        if (lane == 0) atomicExch(p.status, 53);
+        break;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint8_t* at = row + s * STAGE_BYTES + (j >> 1) * (A_BYTES / 2) + (((((j & 1) ^ odd) << 2 | q4) ^ g) << 4);
+        *reinterpret_cast<uint4*>(at) = a[j];
+        *reinterpret_cast<uint4*>(at + 8 * 128) = b[j];
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) tc::arrive_even(bars + s * 8);
+        else tc::mbar_arrive(&full_a[s]);
+      }
+      if ((s += 2) >= STAGES) { s -= STAGES; turn ^= 1; }
+      if ((r += 2) >= RAW) { r -= RAW; r_turn ^= 1; }
     }
   } else if constexpr (!SPLIT) {                  // ---- results
     const int quarter = warp & 3;
@@ -296,7 +304,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
     int f0, t0, n;
     const bool there = tile_at(0, f0, t0, n);
     bool ok = true;
-    if (there && c0 < c1 && warp >= 2 + UNPACK) {
+    if (there && c0 < c1 && warp >= FIRST_EPILOGUE) {
       ok = tc::mbar_wait_warp(&acc_full[0], 0);
       if (!ok && lane == 0) atomicExch(p.status, 55);
     }
@@ -304,7 +312,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
     __syncwarp();
     tc::cluster_meet();                           // every block's ring is free
     const int run = (n + splits - 1) / splits;
-    if (there && c0 < c1 && warp >= 2 + UNPACK) {
+    if (there && c0 < c1 && warp >= FIRST_EPILOGUE) {
       const int quarter = warp & 3;
 #pragma unroll 1
       for (int r = 0; r < splits; ++r) {
@@ -358,12 +366,13 @@ bool make_map_rows(CUtensorMap* map, const void* base, uint64_t rows, uint64_t c
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool PAIR, bool SPLIT, int BT, int STAGES, int GPC>
+template <bool PAIR, bool SPLIT, int BT, int STAGES, int RAW, int GPC>
 int launch(const void* x, long long x_ld, int K, const Params& p, int blocks, int cluster, cudaStream_t stream) {
   CUtensorMap map;
   if (!make_map_rows(&map, x, p.tokens, K, x_ld, PAIR ? BT / 2 : BT)) return HB_ERR_UNSUPPORTED;
-  const size_t smem = STAGES * (size_t)(A_BYTES + (PAIR ? BT / 2 : BT) * KB * 2) + 1024 + 256;
-  auto* kernel = four_bit_gemm_kernel<PAIR, SPLIT, BT, STAGES, GPC>;
+  const size_t smem = STAGES * (size_t)(A_BYTES + (PAIR ? BT / 2 : BT) * KB * 2) + RAW * UNPACK * RAW_BLOCK + 1024 + 512;
+  static_assert(STAGES >= 2 && RAW >= 2, "the unpacking warps take every other stage");
+  auto* kernel = four_bit_gemm_kernel<PAIR, SPLIT, BT, STAGES, RAW, GPC>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t config = {};
@@ -387,18 +396,18 @@ int gemm(const void* x, long long x_ld, int K, Params p, cudaStream_t stream) {
   if (p.tokens > 128) {
     const int t_tiles = (p.tokens + 255) / 256, pairs = (f_tiles + 1) / 2 * t_tiles;
     p.most = (((p.tokens + t_tiles - 1) / t_tiles) + 15) / 16 * 16;
-    return launch<true, false, 256, 3, GPC>(x, x_ld, K, p, 2 * (pairs < 74 ? pairs : 74), 2, stream);
+    return launch<true, false, 256, 3, 3, GPC>(x, x_ld, K, p, 2 * (pairs < 74 ? pairs : 74), 2, stream);
   }
   p.most = p.tokens;
   int splits = f_tiles > 74 ? 1 : f_tiles > 37 ? 2 : 4;
   while (splits > 1 && p.chunks < 4 * splits) splits /= 2;
   if (splits == 1) {
     const int blocks = f_tiles < 148 ? f_tiles : 148;
-    return p.tokens <= 64 ? launch<false, false, 64, 4, GPC>(x, x_ld, K, p, blocks, 1, stream)
-                          : launch<false, false, 128, 3, GPC>(x, x_ld, K, p, blocks, 1, stream);
+    return p.tokens <= 64 ? launch<false, false, 64, 3, 8, GPC>(x, x_ld, K, p, blocks, 1, stream)
+                          : launch<false, false, 128, 3, 3, GPC>(x, x_ld, K, p, blocks, 1, stream);
   }
-  return p.tokens <= 64 ? launch<false, true, 64, 4, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream)
-                        : launch<false, true, 128, 3, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream);
+  return p.tokens <= 64 ? launch<false, true, 64, 3, 8, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream)
+                        : launch<false, true, 128, 3, 3, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream);
 }
 
 }  // namespace

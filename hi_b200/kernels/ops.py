@@ -2315,7 +2315,9 @@ def check_tc_status(device=None) -> None:
                      52: "4-bit product: the MMA issuer waiting for a stage",
                      53: "4-bit product: the warps that unpack weights waiting for a free stage",
                      54: "4-bit product: the MMA issuer waiting for a free accumulator",
-                     55: "4-bit product: the epilogue waiting for the accumulator"}.get(
+                     55: "4-bit product: the epilogue waiting for the accumulator",
+                     56: "4-bit product: the warp that brings codes waiting for a free place",
+                     57: "4-bit product: the warps that unpack weights waiting for their codes"}.get(
                 code, f"prefill attention, wait {code}" if code >= 11 else f"code {code}")
             raise KernelError(f"a kernel gave up a bounded wait ({where}); its output is invalid")
 
