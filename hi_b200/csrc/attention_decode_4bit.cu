@@ -44,6 +44,7 @@ struct Args {
   const float* sink_values;
   int step_tokens, table_stride, nh, nkv, page_size, chunk, window, keep, split_tiles, splits, sink;
   float scale;
+  unsigned zero;                 // 0, unknown to the compiler
 };
 
 __device__ __forceinline__ unsigned transpose8(unsigned v) {      // an 8 x 8 matrix of 16 bits over the warp
@@ -132,7 +133,9 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
     const int s = warp + i * WARPS, tile = first + s / (TILE / STEP);
     return (tile < kept ? tile : t0 + tile - kept) * TILE + s % (TILE / STEP) * STEP;
   };
-  auto bring = [&](int i) {                                       // lane b: block b of the step (lane 0 all of it from one page)
+  // lane b: block b of the step (lane 0 all of it from one page). `after` is 0 and comes from what was read out of the stage last: the
+  // copy into it is not asked for before those loads have come.
+  auto bring = [&](int i, unsigned after) {
     const int key = key_of(i), blocks = min(MT, (pos - key) / fb::BLOCK_ROWS + 1);      // <= 0: nothing of the step is the token's
     const bool together = a.page_size >= STEP;
     const int n = together ? 1 : MT, each = together ? blocks : 1, at = key + lane * 16;
@@ -144,11 +147,11 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
     if (lane == 0) tc::mbar_expect_tx(&full[warp][i % STAGES], __popc(who) * bytes);
     __syncwarp();
     if (copies && page >= 0)
-      bulk_load(ring_at + (i % STAGES * MT + lane) * B::BYTES,
+      bulk_load(ring_at + (i % STAGES * MT + lane) * B::BYTES + after,
                 a.pages + (((size_t)page * a.nkv + kvh) * (a.page_size / 16) + at % a.page_size / 16) * B::BYTES, bytes,
                 full_at + i % STAGES * 8);
   };
-  for (int i = 0; i < min(STAGES, steps); ++i) bring(i);
+  for (int i = 0; i < min(STAGES, steps); ++i) bring(i, 0u);
 
   // the heads' queries as columns, raised; their sums over a group in three pieces
   uint4 qf[G];
@@ -201,6 +204,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
     const uint8_t* blocks = ring + i % STAGES * MT * B::BYTES;
     const bool whole = key + STEP - 1 <= pos && (key >= lo || key + STEP - 1 < a.keep);
     auto seen = [&](int row) { return key + row <= pos && (key + row >= lo || key + row < a.keep); };
+    unsigned spent = 0u;
     float s[MT][4];
     float m_step[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -297,6 +301,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
         const float fa = see_a ? (c & 1 ? high_half(sa) : low_half(sa)) : 0.f, fb_ = see_b ? (c & 1 ? high_half(sb) : low_half(sb)) : 0.f;
         const unsigned x = transpose8(hb::pack_bf16(p[0] * fa, p[1] * fa)), y = transpose8(hb::pack_bf16(p[2] * fb_, p[3] * fb_));
         unsigned wa = va.w[c], wb = vb.w[c];
+        if (mt == MT - 1) spent ^= wa ^ wb ^ x ^ y;
         const unsigned a0[4] = {wa & fb::LOW, wa & fb::HIGH, wb & fb::LOW, wb & fb::HIGH};
         hb::mma_bf16(o[2 * c], a0, x, y);
         wa >>= 8;
@@ -309,7 +314,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
       }
     }
     __syncwarp();                                                 // all lanes are through with the stage
-    if (asked < steps) bring(asked++);
+    if (asked < steps) bring(asked++, spent & a.zero);
   }
   if (!ok) {                                                      // no copy is under way when the block ends
     for (int i = max(0, asked - STAGES); i < asked; ++i) tc::mbar_wait_warp(&full[warp][i % STAGES], (i / STAGES) & 1);
@@ -400,7 +405,7 @@ extern "C" int hb_attention_decode_4bit(const void* q, const void* pages, const 
   if (n_tokens == 0) return HB_OK;
   const Args a{(const __nv_bfloat16*)q, (const uint8_t*)pages, block_table, seq_of_token, positions, (__nv_bfloat16*)out, part_acc,
                part_ml, status, rows, sink_values, rows ? step_tokens : n_tokens, table_stride, nh, nkv, page_size, chunk, window, keep,
-               split_tiles, splits, sink, scale};
+               split_tiles, splits, sink, scale, 0u};
   const dim3 grid(splits, nkv * tiles, n_tokens);
   const int smem = WARPS * STAGES * (STEP / 16) * 20 * hd;        // blocks of 20 hd bytes; the sums at the end take less
   auto* kernel = hd == 128 ? attn_decode_4bit_kernel<4> : attn_decode_4bit_kernel<2>;

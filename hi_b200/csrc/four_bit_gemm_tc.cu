@@ -7,11 +7,13 @@
 // block of weights a row tile of 16:
 //   warp 0        brings the tokens' tile by TMA (two boxes of 64 k, 128-byte swizzle)
 //   warp 2        brings the 8 row tiles' blocks of codes as one bulk copy each, stages ahead, into a ring of their own
-//   warps 3 .. 18 unpack: eight of them take a stage, the others the next, each a row tile; a word of eight codes becomes eight bfloat16
-//                 (code in the mantissa of 128, minus 136, times the scale: 15 instructions) and one 16-byte store into the swizzled
-//                 tile; odd rows store their words in another order, so that eight lanes meet eight banks of 16 bytes
+//   warps 3 .. 18 unpack: eight of them the stage's first 64 k, the others the rest, each a row tile; a word of eight codes becomes eight bfloat16
+//                 and one 16-byte store into the swizzled tile; eight lanes take rows i and i + 4, which meet eight banks of 16 bytes
 //   warp 1        issues the products, eight of 16 k a stage, and the commits
 //   warps 19 .. 22 read the sums back, add the bias and store: the next tile accumulates into the other half of tensor memory
+// A pair of codes is a pair of denormals after an AND (four_bit.cuh), and code * 2^-133 times scale * 2^73 minus 8 scale * 2^-60 is one
+// instruction with one rounding: the tile holds 2^-60 of the weights, the results are multiplied by 2^60. 9 instructions a word (code in
+// the mantissa of 128, minus 136, times the scale: 15, and the tile of 64 tokens waited for them: 16,384 x 5,120 28 us -> XX).
 // Every row tile is unpacked once per tile of tokens. Eight unpacking warps with their loads in registers took 2,100 cycles a stage, most of
 // it waiting for the fence that shows their stores to the tensor cores and for loads, against 256 to 1,024 of products.
 // PAIR: two blocks of a cluster on 256 rows x up to 256 tokens (cta_group::2), each with its 128 rows and half of the tokens, for
@@ -22,13 +24,14 @@
 
 #include "api.h"
 #include "common.cuh"
+#include "four_bit.cuh"
 #include "tc.cuh"
 
 namespace {
 
 constexpr int BF = 128, KB = 128;                 // weight rows of a block, k of a stage
 constexpr int A_BYTES = BF * KB * 2;
-constexpr int UNPACK = 8, EPILOGUE = 4;           // warps: to unpack a stage (two stages at a time), to write results
+constexpr int UNPACK = 8, EPILOGUE = 4;           // warps: to unpack half a stage, to write results
 constexpr int FIRST_UNPACK = 3, FIRST_EPILOGUE = FIRST_UNPACK + 2 * UNPACK, THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE);
 constexpr int RAW_BLOCK = 1152;                   // room for a block of codes and scales, the largest
 
@@ -38,34 +41,42 @@ struct Params {
   void* out;
   int* status;
   int out_f32, tokens, n_out, chunks, most;       // most: tokens of a tile, a multiple of 16
+  unsigned zero;                                  // 0, unknown to the compiler
 };
 
-// a wait for arrivals from the other block of a pair as well
-__device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n.reg .pred p;\n"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-      "selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(tc::smem_u32(bar)), "r"(parity) : "memory");
-  return __all_sync(0xffffffffu, ok != 0) || (tc::mbar_wait_warp(bar, parity) && wait_pair(bar, parity));
+// An arrival on the even block's barrier of what this block's own tensor cores read from its own shared memory: ordered within the block (a
+// release towards the cluster took 1,500 cycles a stage).
+__device__ __forceinline__ void arrive_pair(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint2 load8(const uint8_t* p) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(tc::smem_u32(p)) : "memory");
+  return v;
 }
 template <int GPC> __device__ __forceinline__ uint2 row_scales(const uint8_t* p) {
   if constexpr (GPC == 1) return make_uint2(*reinterpret_cast<const unsigned short*>(p), 0u);
   else if constexpr (GPC == 2) return make_uint2(*reinterpret_cast<const unsigned*>(p), 0u);
   else return *reinterpret_cast<const uint2*>(p);
 }
-// both halves of a word: scale i of four
-__device__ __forceinline__ unsigned scale_pair(uint2 v, int i) {
-  return __byte_perm(i < 2 ? v.x : v.y, 0u, i & 1 ? 0x3232 : 0x1010);
+// Scale i of four, what it multiplies codes by in each place of a word, and what eight of it comes to; in both halves.
+struct Factors { unsigned low, high, minus_eight; };
+__device__ __forceinline__ Factors factors(uint2 v, int i) {
+  const unsigned s = __byte_perm(i < 2 ? v.x : v.y, 0u, i & 1 ? 0x3232 : 0x1010);
+  Factors f;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(f.low) : "r"(s), "r"(0x64006400u));             // 2^73
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(f.high) : "r"(s), "r"(0x62006200u));            // 2^69
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(f.minus_eight) : "r"(s), "r"(0xa300a300u));     // -2^-57
+  return f;
 }
-// eight codes as bfloat16 scale * (code - 8)
-__device__ __forceinline__ uint4 unpack(unsigned w, unsigned scale) {
+constexpr float GROW = 1152921504606846976.f;     // 2^60, of the results
+// eight codes as bfloat16 scale * (code - 8) * 2^-60
+__device__ __forceinline__ uint4 unpack(unsigned w, const Factors& f) {
   unsigned r[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    unsigned x = (w >> (4 * i) & 0x000f000fu) | 0x43004300u;          // 128 + code
-    asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0x43084308u));    // exact
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(x), "r"(scale));
+  for (int i = 0; i < 2; ++i, w >>= 8) {
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r[2 * i]) : "r"(w & fb::LOW), "r"(f.low), "r"(f.minus_eight));
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r[2 * i + 1]) : "r"(w & fb::HIGH), "r"(f.high), "r"(f.minus_eight));
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
@@ -96,10 +107,10 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       tc::mbar_init(&full_x[s], 1);
-      tc::mbar_init(&full_a[s], PAIR ? 2 * UNPACK : UNPACK);
+      tc::mbar_init(&full_a[s], (PAIR ? 4 : 2) * UNPACK);
       tc::mbar_init(&empty[s], 1);
     }
-    for (int r = 0; r < RAW; ++r) { tc::mbar_init(&raw_full[r], 1); tc::mbar_init(&raw_empty[r], UNPACK); }
+    for (int r = 0; r < RAW; ++r) { tc::mbar_init(&raw_full[r], 1); tc::mbar_init(&raw_empty[r], 2 * UNPACK); }
     for (int b = 0; b < 2; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], PAIR ? 2 * EPILOGUE : EPILOGUE); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -175,7 +186,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
       tc::fence_after();
       const uint32_t idesc = tc::idesc_bf16(FEATURES, tc::uniform((n + 15) & ~15), false), acc = tmem + b * BT;
       for (int c = c0; c < c1; ++c) {
-        if (!tc::mbar_wait_warp(&full_x[s], turn) || !(PAIR ? wait_pair(&full_a[s], turn) : tc::mbar_wait_warp(&full_a[s], turn))) {
+        if (!tc::mbar_wait_warp(&full_x[s], turn) || !tc::mbar_wait_warp(&full_a[s], turn)) {
           if (lane == 0) atomicExch(p.status, 52);
           ok = false;
           break;
@@ -220,51 +231,57 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
     }
     for (int i = max(0, issued - RAW); i < issued; ++i) tc::mbar_wait_warp(&raw_full[i % RAW], (i / RAW) & 1);      // no copy is under way at the end
   } else if (warp < FIRST_EPILOGUE) {             // ---- weights
-    const int part = (warp - FIRST_UNPACK) % UNPACK, first = (warp - FIRST_UNPACK) / UNPACK, g = lane >> 2, q4 = lane & 3, odd = g & 1;
+    const int part = (warp - FIRST_UNPACK) % UNPACK, half = (warp - FIRST_UNPACK) / UNPACK, g = lane >> 3 | (lane & 4), q4 = lane & 3;
     int f0, t0, n;
     const uint32_t bars = PAIR ? tc::even_block(full_a) : tc::smem_u32(full_a);
-    uint8_t* const row = smem + (part * 16 + g) * 128;
+    uint8_t* const row = smem + half * (A_BYTES / 2) + (part * 16 + g) * 128;
     int tiles = 0;
     while (tile_at(tiles, f0, t0, n)) ++tiles;
     const int stages = c1 > c0 ? tiles * (c1 - c0) : 0;
-    int s = first % STAGES, turn = 1 ^ (first / STAGES & 1), r = first % RAW, r_turn = first / RAW & 1;
-    for (int i = first; i < stages; i += 2) {
+    int s = 0, turn = 1, r = 0, r_turn = 0;
+    uint4 a0, a1, b0, b1;                         // what goes into the next stage: rows g and g + 8, two words of 32 k each
+    auto next = [&]() {                           // false: the codes did not come
       if (!tc::mbar_wait_warp(&raw_full[r], r_turn)) {
         if (lane == 0) atomicExch(p.status, 57);
-        break;
+        return false;
       }
       const uint8_t* block = raw + (r * UNPACK + part) * RAW_BLOCK;        // (rows past the weight's: whatever is there; they are not written out)
-      const uint4 lo = *reinterpret_cast<const uint4*>(block + lane * 16), hi = *reinterpret_cast<const uint4*>(block + 512 + lane * 16);
+      const uint8_t* words = block + (g * 4 + q4) * 16 + half * 8;
+      const uint2 lo = load8(words), hi = load8(words + 512);
       const uint2 s_lo = row_scales<GPC>(block + 1024 + g * 2 * GPC), s_hi = row_scales<GPC>(block + 1024 + (g + 8) * 2 * GPC);
+      const int k0 = GPC == 1 ? 0 : GPC == 2 ? half : 2 * half, k1 = GPC == 4 ? k0 + 1 : k0;
+      const Factors lo0 = factors(s_lo, k0), hi0 = factors(s_hi, k0);
+      const Factors lo1 = GPC == 4 ? factors(s_lo, k1) : lo0, hi1 = GPC == 4 ? factors(s_hi, k1) : hi0;
+      a0 = unpack(lo.x, lo0);
+      a1 = unpack(lo.y, lo1);
+      b0 = unpack(hi.x, hi0);
+      b1 = unpack(hi.y, hi1);
+      // The place is given back when the loads have come: the barrier's address waits for them. (An arrival right behind the loads, and one behind
+      // their use as the source has it, overtook them at times, and the next codes were read.)
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&raw_empty[r]);
-      const unsigned wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-      uint4 a[4], b[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {               // words j and j ^ 1 change places in odd rows
-        const unsigned sa = GPC == 4 ? (odd ? scale_pair(s_lo, j ^ 1) : scale_pair(s_lo, j)) : scale_pair(s_lo, j * GPC / 4);
-        const unsigned sb = GPC == 4 ? (odd ? scale_pair(s_hi, j ^ 1) : scale_pair(s_hi, j)) : scale_pair(s_hi, j * GPC / 4);
-        a[j] = unpack(odd ? wl[j ^ 1] : wl[j], sa);
-        b[j] = unpack(odd ? wh[j ^ 1] : wh[j], sb);
-      }
+      if (lane == 0) tc::mbar_arrive(&raw_empty[r] + ((lo.x ^ lo.y ^ hi.x ^ hi.y ^ s_lo.x ^ s_lo.y ^ s_hi.x ^ s_hi.y) & p.zero));
+      if (++r == RAW) { r = 0; r_turn ^= 1; }
+      return true;
+    };
+    bool ok = stages > 0 && next();
+    for (int i = 0; ok && i < stages; ++i) {
       if (!tc::mbar_wait_warp(&empty[s], turn)) {
         if (lane == 0) atomicExch(p.status, 53);
         break;
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint8_t* at = row + s * STAGE_BYTES + (j >> 1) * (A_BYTES / 2) + (((((j & 1) ^ odd) << 2 | q4) ^ g) << 4);
-        *reinterpret_cast<uint4*>(at) = a[j];
-        *reinterpret_cast<uint4*>(at + 8 * 128) = b[j];
-      }
+      uint8_t *at0 = row + s * STAGE_BYTES + ((q4 ^ g) << 4), *at1 = row + s * STAGE_BYTES + (((4 | q4) ^ g) << 4);
+      *reinterpret_cast<uint4*>(at0) = a0;
+      *reinterpret_cast<uint4*>(at1) = a1;
+      *reinterpret_cast<uint4*>(at0 + 8 * 128) = b0;
+      *reinterpret_cast<uint4*>(at1 + 8 * 128) = b1;
+      if (i + 1 < stages) ok = next();            // while the stores are on their way: the fence waits for them
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
-        if constexpr (PAIR) tc::arrive_even(bars + s * 8);
+        if constexpr (PAIR) arrive_pair(bars + s * 8);
         else tc::mbar_arrive(&full_a[s]);
       }
-      if ((s += 2) >= STAGES) { s -= STAGES; turn ^= 1; }
-      if ((r += 2) >= RAW) { r -= RAW; r_turn ^= 1; }
+      if (++s == STAGES) { s = 0; turn ^= 1; }
     }
   } else if constexpr (!SPLIT) {                  // ---- results
     const int quarter = warp & 3;
@@ -287,8 +304,8 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
           if (c + j >= n) break;
-          if (p.out_f32) reinterpret_cast<float*>(p.out)[at + (size_t)j * p.n_out] = v[j] + bias;
-          else reinterpret_cast<__nv_bfloat16*>(p.out)[at + (size_t)j * p.n_out] = __float2bfloat16_rn(v[j] + bias);
+          if (p.out_f32) reinterpret_cast<float*>(p.out)[at + (size_t)j * p.n_out] = fmaf(v[j], GROW, bias);
+          else reinterpret_cast<__nv_bfloat16*>(p.out)[at + (size_t)j * p.n_out] = __float2bfloat16_rn(fmaf(v[j], GROW, bias));
         }
       }
       tc::fence_before();
@@ -339,7 +356,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
       if (f >= p.n_out) continue;
       float v = 0.f;
       for (int r = 0; r * share < p.chunks; ++r) v += sums[r * run * BF + i];      // (of the blocks that had a part of K)
-      if (p.bias) v += __bfloat162float(p.bias[f]);
+      v = fmaf(v, GROW, p.bias ? __bfloat162float(p.bias[f]) : 0.f);
       const size_t at = (size_t)(t0 + rank * run + i / BF) * p.n_out + f;
       if (p.out_f32) reinterpret_cast<float*>(p.out)[at] = v;
       else reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
@@ -371,7 +388,6 @@ int launch(const void* x, long long x_ld, int K, const Params& p, int blocks, in
   CUtensorMap map;
   if (!make_map_rows(&map, x, p.tokens, K, x_ld, PAIR ? BT / 2 : BT)) return HB_ERR_UNSUPPORTED;
   const size_t smem = STAGES * (size_t)(A_BYTES + (PAIR ? BT / 2 : BT) * KB * 2) + RAW * UNPACK * RAW_BLOCK + 1024 + 512;
-  static_assert(STAGES >= 2 && RAW >= 2, "the unpacking warps take every other stage");
   auto* kernel = four_bit_gemm_kernel<PAIR, SPLIT, BT, STAGES, RAW, GPC>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
@@ -421,6 +437,6 @@ extern "C" int hb_four_bit_linear_tc(const void* x, long long x_ld, const void* 
       ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15))
     return HB_ERR_UNSUPPORTED;
   if (tokens == 0 || n_out == 0) return HB_OK;
-  const Params p{(const uint8_t*)w, (const __nv_bfloat16*)bias, out, status, out_dtype == HB_DTYPE_F32, tokens, n_out, (K + KB - 1) / KB, 0};
+  const Params p{(const uint8_t*)w, (const __nv_bfloat16*)bias, out, status, out_dtype == HB_DTYPE_F32, tokens, n_out, (K + KB - 1) / KB, 0, 0u};
   return group == 128 ? gemm<1>(x, x_ld, K, p, stream) : group == 64 ? gemm<2>(x, x_ld, K, p, stream) : gemm<4>(x, x_ld, K, p, stream);
 }
