@@ -41,6 +41,7 @@ struct Params {
   void* out;
   int* status;
   int out_f32, tokens, n_out, chunks, most;       // most: tokens of a tile, a multiple of 16
+  int box;                                        // rows of a tokens' box: as many as a tile needs
   unsigned zero;                                  // 0, unknown to the compiler
 };
 
@@ -154,7 +155,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
           break;
         }
         const uint32_t to = ring + s * STAGE_BYTES + A_BYTES, bar = bars + s * 8;
-        if (mine && rank == 0 | !PAIR) tc::mbar_expect_tx(&full_x[s], (PAIR ? 2 : 1) * X_BYTES);
+        if (mine && rank == 0 | !PAIR) tc::mbar_expect_tx(&full_x[s], (PAIR ? 2 : 1) * p.box * KB * 2);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if constexpr (PAIR) tc::tma_load_2d_pair_if(mine, to + h * (X_BYTES / 2), &map_x, c * KB + h * 64, row, bar);
@@ -384,9 +385,10 @@ bool make_map_rows(CUtensorMap* map, const void* base, uint64_t rows, uint64_t c
 }
 
 template <bool PAIR, bool SPLIT, int BT, int STAGES, int RAW, int GPC>
-int launch(const void* x, long long x_ld, int K, const Params& p, int blocks, int cluster, cudaStream_t stream) {
+int launch(const void* x, long long x_ld, int K, Params p, int blocks, int cluster, cudaStream_t stream) {
   CUtensorMap map;
-  if (!make_map_rows(&map, x, p.tokens, K, x_ld, PAIR ? BT / 2 : BT)) return HB_ERR_UNSUPPORTED;
+  p.box = (p.most + 15) / 16 * (PAIR ? 8 : 16);
+  if (!make_map_rows(&map, x, p.tokens, K, x_ld, p.box)) return HB_ERR_UNSUPPORTED;
   const size_t smem = STAGES * (size_t)(A_BYTES + (PAIR ? BT / 2 : BT) * KB * 2) + RAW * UNPACK * RAW_BLOCK + 1024 + 512;
   auto* kernel = four_bit_gemm_kernel<PAIR, SPLIT, BT, STAGES, RAW, GPC>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -437,6 +439,6 @@ extern "C" int hb_four_bit_linear_tc(const void* x, long long x_ld, const void* 
       ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15))
     return HB_ERR_UNSUPPORTED;
   if (tokens == 0 || n_out == 0) return HB_OK;
-  const Params p{(const uint8_t*)w, (const __nv_bfloat16*)bias, out, status, out_dtype == HB_DTYPE_F32, tokens, n_out, (K + KB - 1) / KB, 0, 0u};
+  const Params p{(const uint8_t*)w, (const __nv_bfloat16*)bias, out, status, out_dtype == HB_DTYPE_F32, tokens, n_out, (K + KB - 1) / KB, 0, 0, 0u};
   return group == 128 ? gemm<1>(x, x_ld, K, p, stream) : group == 64 ? gemm<2>(x, x_ld, K, p, stream) : gemm<4>(x, x_ld, K, p, stream);
 }
