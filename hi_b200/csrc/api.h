@@ -55,20 +55,25 @@ int hb_qkv_post_4bit(const void* qkv, const float* inv_freq, int rot_pairs, int 
 int hb_expand_pages_4bit(const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
                          const int* positions, int n_seqs, int total, int page_size, int chunk, int window, int keep,
                          int skip_single, int nkv, int hd, void* k, void* v, int* table, cudaStream_t stream);
-// the same for the kernels that take float16 (hb_attention_prefill_tc_half): keys and values divided by a power of two per kv head, so
-// that none is above 1, q [n_tokens, nh, hd] (bfloat16) times the keys' power over 256 in q_half; v_factor [nkv] takes the values' powers.
-// `most` [2 * nkv] ints, zero before the call
-int hb_expand_half_4bit(const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
-                        const int* positions, int n_seqs, int total, int page_size, int chunk, int window, int keep,
-                        int skip_single, const void* q, int n_tokens, int nh, int nkv, int hd, void* k, void* v, int* table,
-                        int* most, void* q_half, float* v_factor, cudaStream_t stream);
+// how many pages that is (from the host's copies of the requests' positions), or -1
+long long hb_expand_total(const int* start_pos, const int* n_new, int n_seqs, int width, int page_size, int chunk, int window,
+                          int keep, int skip_single);
+// attention of portions over it: pages expanded to float16 in the workspace (so many bytes of it), then the tcgen05 prefill kernels on them
+long long hb_prefill_attention_4bit_bytes(int total, int n_tokens, int n_seqs, int table_stride, int nh, int nkv, int hd,
+                                          int page_size, int key_splits);
+int hb_prefill_attention_4bit(const void* q, const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
+                              const int* positions, void* out, int n_tokens, int n_seqs, int max_new, int nh, int nkv, int hd,
+                              int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
+                              const float* sink_values, int key_splits, int one_tile, int total, void* workspace,
+                              long long workspace_bytes, int* status, cudaStream_t stream);
+// q, k and v in float16, values of kv head h divided by v_factor[h] (attention_prefill_tc.cu)
 int hb_attention_prefill_tc_half(const void* q, const void* k_pages, const void* v_pages, const float* v_factor,
                                  const int* block_table, int table_stride, const int* cu_seqlens, const int* positions,
                                  void* out, int n_tokens, int n_pages, int n_seqs, int max_new, int nh, int nkv, int hd,
                                  int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
                                  const float* sink_values, int key_splits, float* part_acc, float* part_ml,
                                  int one_tile, int* status, cudaStream_t stream);
-// attention of single tokens over it; splits of split_tiles x 64 positions; splits > 1: partial rows for hb_attention_merge_rows
+// attention of single tokens over it; splits of split_tiles x 64 positions, brought together in part_acc and part_ml where there are several
 int hb_attention_decode_4bit(const void* q, const void* pages, const int* block_table, int table_stride,
                              const int* seq_of_token, const int* positions, void* out, int n_tokens, int nh, int nkv, int hd,
                              int page_size, int chunk, int window, int keep, float scale, int sink,

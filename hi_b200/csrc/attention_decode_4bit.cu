@@ -409,9 +409,13 @@ extern "C" int hb_attention_decode_4bit(const void* q, const void* pages, const 
   const dim3 grid(splits, nkv * tiles, n_tokens);
   const int smem = WARPS * STAGES * (STEP / 16) * 20 * hd;        // blocks of 20 hd bytes; the sums at the end take less
   auto* kernel = hd == 128 ? attn_decode_4bit_kernel<4> : attn_decode_4bit_kernel<2>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned long long> allowed[2]{};
+  const cudaError_t e = hb::allow_smem(kernel, smem, allowed[hd == 128]);
   if (e != cudaSuccess) return (int)e;
   kernel<<<grid, WARPS * 32, smem, stream>>>(a);
   HB_LAUNCH_CHECK();
+  if (splits > 1)
+    return hb_attention_merge_rows(part_acc, part_ml, out, HB_DTYPE_BF16, n_tokens * nh, hd, splits, sink, nh, sink_values, rows, step_tokens,
+                                   stream);
   return HB_OK;
 }

@@ -770,7 +770,7 @@ extern "C" int hb_attention_prefill_tc_reshaped(const void* q, const void* k_pag
                     part_acc, part_ml, status, 0, nullptr, 0, 0, softcap, slopes, sink_values, keep, nullptr, one_tile, nullptr, stream);
 }
 
-// q, k and v in float16, the values of kv head h divided by v_factor[h] (hb_expand_half_4bit makes them); hd 64 or 128.
+// q, k and v in float16, the values of kv head h divided by v_factor[h] (hb_prefill_attention_4bit makes them); hd 64 or 128.
 extern "C" int hb_attention_prefill_tc_half(const void* q, const void* k_pages, const void* v_pages, const float* v_factor,
                                             const int* block_table, int table_stride, const int* cu_seqlens, const int* positions,
                                             void* out, int n_tokens, int n_pages, int n_seqs, int max_new, int nh, int nkv, int hd,

@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #define HB_OK 0
 #define HB_ERR_BAD_ARG 1001      // a size, pointer or dtype the kernel refuses
 #define HB_ERR_UNSUPPORTED 1002  // a shape outside what this kernel was written for
@@ -18,6 +20,18 @@
   } while (0)
 
 namespace hb {
+
+// A kernel's limit of dynamic shared memory, asked for once a device (`done` is the caller's static, one per kernel).
+template <typename Kernel> inline cudaError_t allow_smem(Kernel* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (device & 63);
+  if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }

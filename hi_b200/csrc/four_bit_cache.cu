@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256) qkv_post_4bit_kernel(const Post a) {
 
 // ---- pages of the step's portions as bfloat16. Request s needs its pages first_s .. last_s: from the oldest position that its first
 // new token may read to its last one; they lie side by side in the result, request after request, and `table` [n_seqs, table_stride]
-// says where (entries outside first_s .. last_s are left at 0: no kernel that is told of the same mask reads them).
+// says where (entries outside first_s .. last_s are 0: no kernel that is told of the same mask reads them).
 struct Expand {
   const uint8_t* pages;
   const int* block_table;
@@ -306,6 +306,12 @@ __global__ void __launch_bounds__(128) expand_4bit_kernel(const Expand a) {
     }
   }
   int seq, index;
+  if (kvh == 0)                    // the entries that no page of the result is for
+    for (int i = out_page * blockDim.x + threadIdx.x; i < a.n_seqs * a.table_stride; i += a.total * blockDim.x) {
+      int first, count;
+      span(a, i / a.table_stride, first, count);
+      if (i % a.table_stride < first || i % a.table_stride >= first + count) a.table[i] = 0;
+    }
   if (!find_page(a, out_page, seq, index)) return;
   const int page = a.block_table[(size_t)seq * a.table_stride + index];
   if (kvh == 0 && threadIdx.x == 0) a.table[(size_t)seq * a.table_stride + index] = page < 0 ? -1 : out_page;
@@ -401,15 +407,76 @@ extern "C" int hb_expand_pages_4bit(const void* pages, const int* block_table, i
                 hd, false, stream);
 }
 
-// The scores of q_half and k are those of q and the keys over 256.
-extern "C" int hb_expand_half_4bit(const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
-                                   const int* positions, int n_seqs, int total, int page_size, int chunk, int window, int keep,
-                                   int skip_single, const void* q, int n_tokens, int nh, int nkv, int hd, void* k, void* v, int* table,
-                                   int* most, void* q_half, float* v_factor, cudaStream_t stream) {
-  if (!q || !most || !q_half || !v_factor || n_tokens < 0 || nh <= 0 || nkv <= 0 || nh % nkv || (reinterpret_cast<uintptr_t>(q) & 15))
+// What hb_prefill_attention_4bit needs of its workspace, in order, each part on 1,024 bytes.
+namespace {
+struct Room {
+  size_t k, v, q_half, table, most, v_factor, part_acc, part_ml, all;
+  Room(int total, int n_tokens, int n_seqs, int table_stride, int nh, int nkv, int hd, int page_size, int key_splits) {
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 1023) / 1024 * 1024; return here; };
+    k = take((size_t)total * nkv * page_size * hd * 2);
+    v = take((size_t)total * nkv * page_size * hd * 2);
+    q_half = take((size_t)n_tokens * nh * hd * 2);
+    table = take((size_t)n_seqs * table_stride * 4);
+    most = take((size_t)nkv * 8);
+    v_factor = take((size_t)nkv * 4);
+    part_acc = take(key_splits > 1 ? (size_t)n_tokens * nh * key_splits * hd * 4 : 0);
+    part_ml = take(key_splits > 1 ? (size_t)n_tokens * nh * key_splits * 8 : 0);
+    all = at;
+  }
+};
+}  // namespace
+
+// How many pages the requests' new tokens may read, by what the host knows of them (cu_seqlens and positions on the device say the same);
+// -1: a position lies outside a block table of `width` pages a request.
+extern "C" long long hb_expand_total(const int* start_pos, const int* n_new, int n_seqs, int width, int page_size, int chunk, int window,
+                                     int keep, int skip_single) {
+  long long total = 0;
+  if (!start_pos || !n_new || n_seqs < 0 || page_size <= 0) return -1;
+  for (int s = 0; s < n_seqs; ++s) {
+    const long long start = start_pos[s], n = n_new[s];
+    if (n <= 0 || (n == 1 && skip_single)) continue;
+    const long long last = (start + n - 1) / page_size;
+    if (start < 0 || last >= width) return -1;
+    const long long low = chunk > 0 ? start / chunk * chunk : window > 0 && keep == 0 ? (start - window + 1 > 0 ? start - window + 1 : 0) : 0;
+    total += last - low / page_size + 1;
+  }
+  return total;
+}
+extern "C" long long hb_prefill_attention_4bit_bytes(int total, int n_tokens, int n_seqs, int table_stride, int nh, int nkv, int hd,
+                                                     int page_size, int key_splits) {
+  return (long long)Room(total, n_tokens, n_seqs, table_stride, nh, nkv, hd, page_size, key_splits).all;
+}
+
+// The pages in float16 (a 4-bit cache's values have up to 13 bits, of which bfloat16 keeps 8 and float16 11), keys and values divided by a
+// power of two per kv head that brings the largest of them under 1, q times the keys' over 256; then the tcgen05 prefill attention on them,
+// whose scores are a 256th of q k^T, and the merge of shared keys.
+extern "C" int hb_prefill_attention_4bit(const void* q, const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
+                                         const int* positions, void* out, int n_tokens, int n_seqs, int max_new, int nh, int nkv, int hd,
+                                         int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
+                                         const float* sink_values, int key_splits, int one_tile, int total, void* workspace,
+                                         long long workspace_bytes, int* status, cudaStream_t stream) {
+  if (!q || !workspace || n_tokens < 0 || nh <= 0 || nkv <= 0 || nh % nkv || total < 1 || key_splits < 1 ||
+      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(workspace)) & 15))
     return HB_ERR_BAD_ARG;
-  return expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)k, (uint16_t*)v, table, n_seqs,
-                       table_stride, page_size, chunk, window, keep, skip_single, nkv, total, (const __nv_bfloat16*)q, n_tokens, nh, most,
-                       (uint16_t*)q_half, v_factor},
-                hd, true, stream);
+  const Room room(total, n_tokens, n_seqs, table_stride, nh, nkv, hd, page_size, key_splits);
+  if ((long long)room.all > workspace_bytes) return HB_ERR_BAD_ARG;
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  int* most = reinterpret_cast<int*>(w + room.most);
+  float* v_factor = reinterpret_cast<float*>(w + room.v_factor);
+  const cudaError_t e = cudaMemsetAsync(most, 0, (size_t)nkv * 8, stream);
+  if (e != cudaSuccess) return (int)e;
+  int* table = reinterpret_cast<int*>(w + room.table);
+  int code = expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)(w + room.k), (uint16_t*)(w + room.v), table,
+                           n_seqs, table_stride, page_size, chunk, window, keep, skip_single, nkv, total, (const __nv_bfloat16*)q, n_tokens, nh,
+                           most, (uint16_t*)(w + room.q_half), v_factor},
+                    hd, true, stream);
+  if (code != HB_OK) return code;
+  float* part_acc = key_splits > 1 ? reinterpret_cast<float*>(w + room.part_acc) : nullptr;
+  float* part_ml = key_splits > 1 ? reinterpret_cast<float*>(w + room.part_ml) : nullptr;
+  code = hb_attention_prefill_tc_half(w + room.q_half, w + room.k, w + room.v, v_factor, table, table_stride, cu_seqlens, positions, out,
+                                      n_tokens, total, n_seqs, max_new, nh, nkv, hd, page_size, chunk, window, keep, 256.f * scale, skip_single,
+                                      sink, sink_values, key_splits, part_acc, part_ml, one_tile, status, stream);
+  if (code != HB_OK || key_splits == 1) return code;
+  return hb_attention_merge(part_acc, part_ml, out, HB_DTYPE_BF16, n_tokens * nh, hd, key_splits, sink, nh, sink_values, stream);
 }

@@ -391,7 +391,8 @@ int launch(const void* x, long long x_ld, int K, Params p, int blocks, int clust
   if (!make_map_rows(&map, x, p.tokens, K, x_ld, p.box)) return HB_ERR_UNSUPPORTED;
   const size_t smem = STAGES * (size_t)(A_BYTES + (PAIR ? BT / 2 : BT) * KB * 2) + RAW * UNPACK * RAW_BLOCK + 1024 + 512;
   auto* kernel = four_bit_gemm_kernel<PAIR, SPLIT, BT, STAGES, RAW, GPC>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<unsigned long long> allowed{0};
+  cudaError_t e = hb::allow_smem(kernel, (int)smem, allowed);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(blocks);

@@ -182,7 +182,8 @@ int launch_few(Few a, cudaStream_t stream) {
   }
   const int smem = fixed + kept + a.panel * each;
   auto* kernel = four_bit_few_kernel<NT, GPC>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = hb::allow_smem(kernel, MOST_SMEM + 16 * 1024, allowed);
   if (e != cudaSuccess) return (int)e;
   kernel<<<blocks, warps * 32, smem, stream>>>(a);
   HB_LAUNCH_CHECK();

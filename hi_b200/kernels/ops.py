@@ -38,8 +38,7 @@ _SIGNATURES = {
     "hb_qkv_post": [P, I, P, I, I, I, F, I, F, F, P, P, I, I, F, P, I, I, I, P, P, P, I, P, P, P, I, I, I, I, I, I, P],
     "hb_qkv_post_4bit": [P, P, I, I, I, F, I, F, F, P, P, I, I, F, I, P, P, P, I, P, P, I, I, I, I, I, I, P],
     "hb_expand_pages_4bit": [P, P, I, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P],
-    "hb_expand_half_4bit": [P, P, I, P, P, I, I, I, I, I, I, I, P, I, I, I, I, P, P, P, P, P, P, P],
-    "hb_attention_prefill_tc_half": [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, I, I, P, I, P, P, I, P, P],
+    "hb_prefill_attention_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, I, F, I, I, P, I, I, I, P, c_longlong, P, P],
     "hb_attention_decode_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, P, I, I, P, P, P, P, I, P],
     "hb_four_bit_linear": [P, c_longlong, P, P, P, I, I, I, I, I, P],
     "hb_four_bit_linear_tc": [P, c_longlong, P, P, P, I, I, I, I, I, P, P],
@@ -126,6 +125,10 @@ def lib():
         handle.hb_recurrence_chunked_scratch_floats.restype = c_longlong
         handle.hb_prefill_pair_idle_us.argtypes = [P, I, I, I, I, I, I, I, ctypes.c_double]
         handle.hb_prefill_pair_idle_us.restype = ctypes.c_double
+        handle.hb_expand_total.argtypes = [P, P, I, I, I, I, I, I, I]
+        handle.hb_expand_total.restype = c_longlong
+        handle.hb_prefill_attention_4bit_bytes.argtypes = [I, I, I, I, I, I, I, I, I]
+        handle.hb_prefill_attention_4bit_bytes.restype = c_longlong
         handle.hb_moe_down_tc_scratch_floats.argtypes = [I]
         handle.hb_moe_down_tc_scratch_floats.restype = c_longlong
         _lib = handle
@@ -1362,11 +1365,7 @@ def sigmoid_prefill_attention_tc(q: torch.Tensor, k_pages: torch.Tensor, v_pages
     n_pages, nkv, page_size, hd2 = k_pages.shape
     if hd2 != hd or k_pages.shape != v_pages.shape or head_bias.numel() != nh:
         raise KernelError("cache pages or head_bias do not match the query's heads")
-    if half:
-        _need(v_factor, "v_factor", torch.float32)
-        if softcap or slopes is not None or hd > 128 or v_factor.numel() != nkv:
-            raise KernelError("float16 operands are taken for plain scores of rows of 64 and 128, with a factor per kv head")
-    if not prefill_attention_tc_supported(torch.bfloat16, nh, nkv, hd, page_size):
+    if not prefill_attention_tc_supported(q.dtype, nh, nkv, hd, page_size):
         raise KernelError(f"tcgen05 prefill attention does not take nh={nh} nkv={nkv} head_dim={hd} page={page_size}")
     if cu_seqlens.numel() != n_seqs + 1 or block_table.shape[0] < n_seqs:
         raise KernelError("cu_seqlens / block_table do not match the number of requests")
@@ -1758,32 +1757,24 @@ def prefill_attention_tc(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
                          window: int, scale: float, skip_single: bool = False,
                          out: Optional[torch.Tensor] = None, key_splits: int = 1, sink: bool = False,
                          softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
-                         sink_values: Optional[torch.Tensor] = None, keep: int = 0, one_tile: bool = False,
-                         v_factor: Optional[torch.Tensor] = None) -> torch.Tensor:
+                         sink_values: Optional[torch.Tensor] = None, keep: int = 0, one_tile: bool = False) -> torch.Tensor:
     """As :func:`prefill_attention`, on tcgen05 (S, P V and O in tensor memory, TMA page loads).
     ``key_splits`` > 1: that many blocks share the key tiles of every (query tile, head) and a
     merge kernel combines their rows (see :func:`prefill_key_splits`). ``softcap``, ``slopes``, ``sink_values``, ``keep``:
-    as :func:`paged_attention`. ``one_tile``: one query tile a block also where two are the rule (:func:`prefill_pairs`).
-    ``v_factor`` (float32 [nkv]): q, k and v are float16 as :func:`expand_half_4bit` makes them (plain scores, rows of 64 and 128); the
-    result is bfloat16."""
-    half = v_factor is not None
-    _need(q, "q", torch.float16 if half else torch.bfloat16); _need(k_pages, "k_pages", q.dtype); _need(v_pages, "v_pages", q.dtype)
+    as :func:`paged_attention`. ``one_tile``: one query tile a block also where two are the rule (:func:`prefill_pairs`)."""
+    _need(q, "q", torch.bfloat16); _need(k_pages, "k_pages", q.dtype); _need(v_pages, "v_pages", q.dtype)
     for t, nm in ((block_table, "block_table"), (cu_seqlens, "cu_seqlens"), (positions, "positions")):
         _need(t, nm, torch.int32)
     n, nh, hd = q.shape
     n_pages, nkv, page_size, hd2 = k_pages.shape
     if hd2 != hd or k_pages.shape != v_pages.shape:
         raise KernelError("cache pages do not match the query's head_dim")
-    if half:
-        _need(v_factor, "v_factor", torch.float32)
-        if softcap or slopes is not None or hd > 128 or v_factor.numel() != nkv:
-            raise KernelError("float16 operands are taken for plain scores of rows of 64 and 128, with a factor per kv head")
-    if not prefill_attention_tc_supported(torch.bfloat16, nh, nkv, hd, page_size):
+    if not prefill_attention_tc_supported(q.dtype, nh, nkv, hd, page_size):
         raise KernelError(f"tcgen05 prefill attention does not take nh={nh} nkv={nkv} head_dim={hd} page={page_size}")
     if cu_seqlens.numel() != n_seqs + 1 or block_table.shape[0] < n_seqs:
         raise KernelError("cu_seqlens / block_table do not match the number of requests")
     if out is None:
-        out = torch.empty_like(q, dtype=torch.bfloat16)
+        out = torch.empty_like(q)
     key_splits = int(key_splits)
     part_acc = part_ml = None
     if key_splits > 1:
@@ -1795,13 +1786,7 @@ def prefill_attention_tc(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
             if t.numel() != nh:
                 raise KernelError(f"{nm} needs one number per query head")
     sink = bool(sink) or sink_values is not None
-    if half:
-        _check(lib().hb_attention_prefill_tc_half(
-            _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(v_factor), _ptr(block_table), block_table.shape[1], _ptr(cu_seqlens),
-            _ptr(positions), _ptr(out), n, n_pages, n_seqs, int(max_new), nh, nkv, hd, page_size, int(chunk), int(window), int(keep),
-            float(scale), int(skip_single), int(sink), _ptr(sink_values), key_splits, _ptr(part_acc), _ptr(part_ml), int(one_tile),
-            _ptr(_tc_status(q.device)), _stream()), "attention_prefill_tc_half")
-    elif softcap or slopes is not None or sink_values is not None or keep > 0:
+    if softcap or slopes is not None or sink_values is not None or keep > 0:
         _check(lib().hb_attention_prefill_tc_reshaped(
             _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(block_table), block_table.shape[1], _ptr(cu_seqlens),
             _ptr(positions), _ptr(out), n, n_pages, n_seqs, int(max_new), nh, nkv, hd, page_size, int(chunk), int(window),
@@ -1847,11 +1832,7 @@ def diff_prefill_attention_tc(q: torch.Tensor, k_pages: torch.Tensor, v_pages: t
     n_pages, nkv, page_size, hd2 = k_pages.shape
     if hd2 != hd or k_pages.shape != v_pages.shape or nh % 2:
         raise KernelError("cache pages do not match the query's pairs of heads")
-    if half:
-        _need(v_factor, "v_factor", torch.float32)
-        if softcap or slopes is not None or hd > 128 or v_factor.numel() != nkv:
-            raise KernelError("float16 operands are taken for plain scores of rows of 64 and 128, with a factor per kv head")
-    if not prefill_attention_tc_supported(torch.bfloat16, nh, nkv, hd, page_size):
+    if not prefill_attention_tc_supported(q.dtype, nh, nkv, hd, page_size):
         raise KernelError(f"tcgen05 prefill attention does not take nh={nh} nkv={nkv} head_dim={hd} page={page_size}")
     if cu_seqlens.numel() != n_seqs + 1 or block_table.shape[0] < n_seqs:
         raise KernelError("cu_seqlens / block_table do not match the number of requests")
@@ -2512,9 +2493,9 @@ FOUR_BIT_FEW = 16                    # tokens up to which a product streams the 
 
 
 def _on_current_device(*tensors) -> None:
-    device = torch.cuda.current_device()
+    device = torch._C._cuda_getDevice()
     for t in tensors:
-        if t is not None and t.device.index != device:
+        if t is not None and t.get_device() != device:
             raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{device}")
 
 
@@ -2685,15 +2666,11 @@ def _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos,
             positions.numel() < sum(n_new):
         raise KernelError("start_pos, n_new, cu_seqlens and block_table do not speak of the same requests")
     _on_current_device(kv_pages, block_table, cu_seqlens, positions)
-    total, width = 0, block_table.shape[1]
-    for start, n in zip(start_pos, n_new):
-        if n <= 0 or (n == 1 and skip_single):
-            continue
-        last = (start + n - 1) // page_size
-        if start < 0 or last >= width:
-            raise KernelError(f"positions {start} .. {start + n - 1} lie outside the block table's {width} pages")
-        low = start // chunk * chunk if chunk > 0 else max(0, start - window + 1) if window > 0 and not keep else 0
-        total += last - low // page_size + 1
+    numbers = I * n_seqs
+    total = lib().hb_expand_total(numbers(*start_pos), numbers(*n_new), n_seqs, block_table.shape[1], page_size, chunk, window, keep, skip_single)
+    if total < 0 or total >= 1 << 31:
+        raise KernelError(f"positions of {list(zip(start_pos, n_new))[:4]}... (first, count) lie outside the block table's "
+                          f"{block_table.shape[1]} pages a request")
     return nkv, page_size, total
 
 
@@ -2706,36 +2683,44 @@ def expand_pages_4bit(kv_pages: torch.Tensor, hd: int, block_table: torch.Tensor
     copies of what ``positions`` and ``cu_seqlens`` say on the device. ``skip_single``: requests of one new token are left out."""
     nkv, page_size, total = _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos, n_new, chunk, window, keep, skip_single)
     k, v = torch.empty((2, total, nkv, page_size, hd), dtype=torch.bfloat16, device=kv_pages.device).unbind(0)
-    table = torch.zeros_like(block_table)
-    if total:
-        _check(lib().hb_expand_pages_4bit(_ptr(kv_pages), _ptr(block_table), block_table.shape[1], _ptr(cu_seqlens), _ptr(positions),
-                                          len(n_new), total, page_size, int(chunk), int(window), int(keep), int(skip_single), nkv, hd,
-                                          _ptr(k), _ptr(v), _ptr(table), _stream()), "expand_pages_4bit")
+    if not total:
+        return k, v, torch.zeros_like(block_table)
+    table = torch.empty_like(block_table)
+    _check(lib().hb_expand_pages_4bit(_ptr(kv_pages), _ptr(block_table), block_table.shape[1], _ptr(cu_seqlens), _ptr(positions),
+                                      len(n_new), total, page_size, chunk, window, keep, skip_single, nkv, hd, _ptr(k), _ptr(v), _ptr(table),
+                                      _stream()), "expand_pages_4bit")
     return k, v, table
 
 
-def expand_half_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor, positions: torch.Tensor,
-                     start_pos, n_new, chunk: int = 0, window: int = 0, keep: int = 0, skip_single: bool = False):
-    """:func:`expand_pages_4bit` for :func:`prefill_attention_tc` on float16: a 4-bit cache's values have up to 13 bits, of which bfloat16
-    keeps 8 and float16 11. Returns ``(q_half, k_pages, v_pages, table, v_factor)``; keys and values of a kv head are divided by
-    a power of two that brings the largest of them under 1, q [N, nh, hd] (bfloat16) is multiplied by the keys' over 256: the scores are
-    a 256th of q k^T."""
+def prefill_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                           positions: torch.Tensor, start_pos, n_new, chunk: int, window: int, scale: float, skip_single: bool = False,
+                           key_splits: int = 1, sink: bool = False, sink_values: Optional[torch.Tensor] = None, keep: int = 0,
+                           one_tile: bool = False) -> torch.Tensor:
+    """:func:`prefill_attention_tc` over a cache held in four bits: the pages that the step's new tokens may read (``start_pos`` and
+    ``n_new`` as in :func:`expand_pages_4bit`) are expanded to float16 first, keys and values of a kv head divided by a power of two, and
+    the tcgen05 kernels run on those. Rows of requests that ``skip_single`` leaves out are not written."""
     _need(q, "q", torch.bfloat16)
     n, nh, hd = q.shape
     nkv, page_size, total = _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos, n_new, chunk, window, keep, skip_single)
-    if nh % nkv or not total or q.data_ptr() % 16:
-        raise KernelError(f"{nh} query heads on {nkv} kv heads (a multiple), q on 16 bytes and at least one portion are expanded for")
-    _on_current_device(q)
-    k, v = torch.empty((2, total, nkv, page_size, hd), dtype=torch.float16, device=q.device).unbind(0)
-    q_half = torch.empty_like(q, dtype=torch.float16)
-    seqs, width = block_table.shape
-    zeros = torch.zeros(seqs * width + 2 * nkv, dtype=torch.int32, device=q.device)
-    table, most = zeros[: seqs * width].view(seqs, width), zeros[seqs * width:]
-    v_factor = torch.empty(nkv, dtype=torch.float32, device=q.device)
-    _check(lib().hb_expand_half_4bit(_ptr(kv_pages), _ptr(block_table), width, _ptr(cu_seqlens), _ptr(positions), len(n_new), total, page_size,
-                                     int(chunk), int(window), int(keep), int(skip_single), _ptr(q), n, nh, nkv, hd, _ptr(k), _ptr(v),
-                                     _ptr(table), _ptr(most), _ptr(q_half), _ptr(v_factor), _stream()), "expand_half_4bit")
-    return q_half, k, v, table, v_factor
+    if nh % nkv or q.data_ptr() % 16 or not scale > 0:
+        raise KernelError(f"{nh} query heads on {nkv} kv heads (a multiple), q on 16 bytes and a scale above zero are taken")
+    if sink_values is not None:
+        _need(sink_values, "sink_values", torch.float32)
+        if sink_values.numel() != nh:
+            raise KernelError("sink_values needs one number per query head")
+    _on_current_device(q, sink_values)
+    out = torch.empty_like(q)
+    if not total:
+        return out
+    n_seqs, width = len(n_new), block_table.shape[1]
+    room = lib().hb_prefill_attention_4bit_bytes(total, n, n_seqs, width, nh, nkv, hd, page_size, key_splits)
+    workspace = torch.empty(room, dtype=torch.uint8, device=q.device)
+    TC_USED[0] = True
+    _check(lib().hb_prefill_attention_4bit(_ptr(q), _ptr(kv_pages), _ptr(block_table), width, _ptr(cu_seqlens), _ptr(positions), _ptr(out), n,
+                                           n_seqs, max(n_new), nh, nkv, hd, page_size, chunk, window, keep, scale, skip_single,
+                                           bool(sink) or sink_values is not None, _ptr(sink_values), key_splits, one_tile, total,
+                                           _ptr(workspace), room, _ptr(_tc_status(q.device)), _stream()), "prefill_attention_4bit")
+    return out
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2798,16 +2783,14 @@ def decode_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table: 
         return out
     part_acc = part_ml = None
     if splits > 1:
-        part_acc = torch.empty((n, nh, splits, hd), dtype=torch.float32, device=q.device)
-        part_ml = torch.empty((n, nh, splits, 2), dtype=torch.float32, device=q.device)
-    sink = bool(sink) or sink_values is not None
+        rows_of = n * nh * splits
+        scratch = torch.empty(rows_of * (hd + 2), dtype=torch.float32, device=q.device)
+        part_acc = scratch.data_ptr()
+        part_ml = part_acc + 4 * rows_of * hd
     TC_USED[0] = True
     _check(lib().hb_attention_decode_4bit(_ptr(q), _ptr(kv_pages), _ptr(block_table), block_table.shape[1], _ptr(seq_of_token),
-                                          _ptr(positions), _ptr(out), n, nh, nkv, hd, page_size, int(chunk), int(window), int(keep),
-                                          float(scale), int(sink), _ptr(sink_values), split_tiles, splits, _ptr(part_acc),
-                                          _ptr(part_ml), _ptr(_tc_status(q.device)), _ptr(rows), step_tokens, _stream()),
+                                          _ptr(positions), _ptr(out), n, nh, nkv, hd, page_size, chunk, window, keep, scale,
+                                          bool(sink) or sink_values is not None, _ptr(sink_values), split_tiles, splits, part_acc,
+                                          part_ml, _ptr(_tc_status(q.device)), _ptr(rows), step_tokens, _stream()),
            "attention_decode_4bit")
-    if splits > 1:
-        _check(lib().hb_attention_merge_rows(_ptr(part_acc), _ptr(part_ml), _ptr(out), _dt(out), n * nh, hd, splits, int(sink), nh,
-                                             _ptr(sink_values), _ptr(rows), step_tokens, _stream()), "attention_merge")
     return out

@@ -60,7 +60,7 @@ def _key_splits(portions, rows: int, nh: int, nkv: int, hd: int, chunk: int, sli
 
 def attend_over_pages(q, k_pages, v_pages, block_table, ctx, nh: int, nkv: int, hd: int, chunk: int, sliding: int,
                       scale: float, sink: bool = False, softcap: float = 0.0, slopes=None, sink_values=None, keep: int = 0,
-                      decode=None, half=None):
+                      decode=None, prefill=None):
     """softmax(q k^T scale + mask) v for the step's tokens over the paged keys and values that are in
     the cache already, by the kernel that fits the step: single decoded tokens, portions of prompts
     (with single tokens of other requests beside them), or the general kernel for what those refuse
@@ -70,8 +70,8 @@ def attend_over_pages(q, k_pages, v_pages, block_table, ctx, nh: int, nkv: int, 
     (float32 [nh]): of the head's own score instead. ``softcap`` > 0: scores become softcap tanh(score / softcap);
     ``slopes`` (float32 [nh]): slopes[head] * (distance to the key) is taken off after the cap.
     ``keep``: first tokens of a request that a sliding window keeps. ``decode(longest, rows, out, most_keys)``: how single
-    tokens are decoded, where their keys lie elsewhere than in ``k_pages`` and ``v_pages``. ``half``: (q in float16, ``v_factor``) for
-    pages in float16 (``ops.expand_half_4bit``), which the tcgen05 kernels take at any number of tokens."""
+    tokens are decoded, where their keys lie elsewhere than in ``k_pages`` and ``v_pages``. ``prefill(skip_single, key_splits, one_tile)``: the same of
+    portions, which all go to the tcgen05 kernels then."""
     positions = ctx.positions
     decode_ok = ops.decode_attention_supported(q.dtype, nh, nkv, hd)
 
@@ -85,9 +85,8 @@ def attend_over_pages(q, k_pages, v_pages, block_table, ctx, nh: int, nkv: int, 
         # every token of the step is one request's decoded token: the tensor-core kernel
         return decode(ctx.max_context)
     # at least a tile of new tokens somewhere: the tcgen05 kernel; short portions: mma.sync
-    tc = half is not None or \
+    tc = prefill is not None or \
         (ctx.max_new >= ops.PREFILL_TC_MIN_TOKENS and ops.prefill_attention_tc_supported(q.dtype, nh, nkv, hd, ctx.page_size))
-    q_tc, v_factor = half if half is not None else (q, None)
     if ctx.max_new > 1 and ops.prefill_attention_supported(q.dtype, nh, nkv, hd):
         # portions of prompts (single tokens of other requests ride along as one-row tiles)
         single = ctx.decode_rows is not None and decode_ok
@@ -103,10 +102,12 @@ def attend_over_pages(q, k_pages, v_pages, block_table, ctx, nh: int, nkv: int, 
                 current = torch.cuda.current_stream()
                 stream, before, after = _decode_aside(q.device)
                 before.record(current)
-            o = ops.prefill_attention_tc(q_tc, k_pages, v_pages, block_table, ctx.cu_seqlens, positions,
-                                         ctx.n_seqs, ctx.max_new, chunk, sliding, scale if half is None else 256.0 * scale,
-                                         skip_single=single, key_splits=shares, sink=sink, softcap=softcap, slopes=slopes,
-                                         sink_values=sink_values, keep=keep, one_tile=one_tile, v_factor=v_factor)
+            if prefill is not None:
+                o = prefill(single, shares, one_tile)
+            else:
+                o = ops.prefill_attention_tc(q, k_pages, v_pages, block_table, ctx.cu_seqlens, positions,
+                                             ctx.n_seqs, ctx.max_new, chunk, sliding, scale, skip_single=single, key_splits=shares, sink=sink,
+                                             softcap=softcap, slopes=slopes, sink_values=sink_values, keep=keep, one_tile=one_tile)
             if aside:
                 # other rows of the same output; nothing of the call's is freed before the streams have met again
                 stream.wait_event(before)
@@ -147,9 +148,9 @@ def attend_over_four_bit_pages(q, kv_pages, block_table, ctx, nh: int, nkv: int,
     kernels. Reshaped scores (``softcap``, ``slopes``) are taken by the kernels of the bfloat16 cache, over pages expanded to that."""
     if q.shape != (ctx.n_tokens, nh, hd) or kv_pages.shape[1] != nkv:
         raise ValueError(f"queries {tuple(q.shape)} and pages of {kv_pages.shape[1]} kv heads for {ctx.n_tokens} tokens, {nh} heads on {nkv}")
-    spans = (block_table, ctx.cu_seqlens, ctx.positions, ctx.start_pos, ctx.n_new, chunk, sliding, keep)
+    spans = (block_table, ctx.cu_seqlens, ctx.positions, ctx.start_pos, ctx.n_new)
     if softcap or slopes is not None:
-        k, v, table = ops.expand_pages_4bit(kv_pages, hd, *spans)
+        k, v, table = ops.expand_pages_4bit(kv_pages, hd, *spans, chunk, sliding, keep)
         return attend_over_pages(q, k, v, table, ctx, nh, nkv, hd, chunk, sliding, scale, sink=sink, softcap=softcap, slopes=slopes,
                                  sink_values=sink_values, keep=keep)
 
@@ -157,11 +158,14 @@ def attend_over_four_bit_pages(q, kv_pages, block_table, ctx, nh: int, nkv: int,
         return ops.decode_attention_4bit(q, kv_pages, block_table, ctx.seq_of_token, ctx.positions, chunk, sliding, scale, longest,
                                          sink=sink, sink_values=sink_values, keep=keep, rows=rows, out=out, most_keys=most_keys)
 
+    def prefill(skip_single, key_splits, one_tile):
+        return ops.prefill_attention_4bit(q, kv_pages, *spans, chunk, sliding, scale, skip_single, key_splits, sink, sink_values, keep,
+                                          one_tile)
+
     if ctx.max_new <= FOUR_BIT_DECODED:
         return decode(ctx.max_context)
-    q_half, k, v, table, v_factor = ops.expand_half_4bit(q, kv_pages, *spans, skip_single=ctx.decode_rows is not None)
-    return attend_over_pages(q, k, v, table, ctx, nh, nkv, hd, chunk, sliding, scale, sink=sink, sink_values=sink_values, keep=keep,
-                             decode=decode, half=(q_half, v_factor))
+    return attend_over_pages(q, None, None, block_table, ctx, nh, nkv, hd, chunk, sliding, scale, sink=sink, sink_values=sink_values,
+                             keep=keep, decode=decode, prefill=prefill)
 
 
 def differential_attend_over_pages(q, k_pages, v_pages, block_table, ctx, chunk: int, sliding: int, keep: int, scale: float,
