@@ -73,11 +73,12 @@ int hb_attention_prefill_tc_half(const void* q, const void* k_pages, const void*
                                  int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
                                  const float* sink_values, int key_splits, float* part_acc, float* part_ml,
                                  int one_tile, int* status, cudaStream_t stream);
-// attention of single tokens over it; splits of split_tiles x 64 positions, brought together in part_acc and part_ml where there are several
+// attention of single tokens over it; splits of split_tiles x 64 positions, brought together in a cluster (2 to 8)
+// or in part_acc and part_ml
 int hb_attention_decode_4bit(const void* q, const void* pages, const int* block_table, int table_stride,
                              const int* seq_of_token, const int* positions, void* out, int n_tokens, int nh, int nkv, int hd,
                              int page_size, int chunk, int window, int keep, float scale, int sink,
-                             const float* sink_values, int split_tiles, int splits, float* part_acc, float* part_ml,
+                             const float* sink_values, int split_tiles, int splits, int cluster, float* part_acc, float* part_ml,
                              int* status, const long long* rows, int step_tokens, cudaStream_t stream);
 // x [tokens, K] (rows x_ld elements apart) times a weight of four bits in blocks of 16 rows x 128 k: up to 16 tokens
 // (four_bit_linear.cu), many (four_bit_gemm_tc.cu)

@@ -14,9 +14,11 @@
 //
 // Grid (split, kv head x tiles of 8 heads, token). A warp has steps of 32 keys of its own: 2 blocks, which lie side by side in a
 // page of 32 and more, come as one bulk copy that the warp's own barrier counts, a few steps ahead; the warps meet at the end only,
-// where their sums are joined, and the splits' by attention_merge. A step's copies leave out blocks behind the token's own.
+// where their sums are joined. The splits of a token are a cluster, which reads one another's shared memory, or leave their rows to
+// attention_merge. A step's copies leave out blocks behind the token's own.
 // Rows of a block that the token may not read (not written yet, out of its window) hold anything, NaN as well: their scores, scales
-// and lows are replaced. Every wait is bounded; on a time-out the kernel says so in `status` and its output is invalid.
+// and lows are replaced, in a form of the step for those that have such rows. Every wait is bounded; on a time-out the kernel says so in
+// `status` and its output is invalid.
 #include "api.h"
 #include "common.cuh"
 #include "four_bit.cuh"
@@ -29,6 +31,7 @@ constexpr int TILE = 64;         // splits are cut in these
 constexpr int WARPS = 4;
 constexpr int STAGES = 2;        // steps in flight a warp
 constexpr int HEADS = 8;         // query heads of a block
+constexpr int MOST_CLUSTER = 8;
 
 struct Args {
   const __nv_bfloat16* q;
@@ -42,7 +45,7 @@ struct Args {
   int* status;
   const long long* rows;         // the tokens of the launch among the step's, or null
   const float* sink_values;
-  int step_tokens, table_stride, nh, nkv, page_size, chunk, window, keep, split_tiles, splits, sink;
+  int step_tokens, table_stride, nh, nkv, page_size, page_shift, chunk, window, keep, split_tiles, splits, sink;      // page_shift: of a power of two, or -1
   float scale;
   unsigned zero;                 // 0, unknown to the compiler
 };
@@ -69,6 +72,10 @@ template <> struct Words<4> {
     w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   }
 };
+template <> struct Words<1> {
+  unsigned w[1];
+  __device__ __forceinline__ explicit Words(const uint8_t* p) { w[0] = *reinterpret_cast<const unsigned*>(p); }
+};
 template <> struct Words<2> {
   unsigned w[2];
   __device__ __forceinline__ explicit Words(const uint8_t* p) {
@@ -80,7 +87,15 @@ template <> struct Words<2> {
 __device__ __forceinline__ float low_half(unsigned w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_half(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
 
-template <int G>
+__device__ __forceinline__ uint32_t in_block(const void* smem, int rank) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(tc::smem_u32(smem)), "r"(rank));
+  return at;
+}
+template <bool B> struct Const { static constexpr bool value = B; };
+
+// CLUSTER: the splits of a token's heads are a cluster
+template <int G, bool CLUSTER>
 __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const Args a) {
   using B = fb::Block<G>;
   constexpr int HD = 32 * G, MT = STEP / 16;
@@ -107,7 +122,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
   const int n_tiles = pos < 0 ? 0 : kept + pos / TILE - t0 + 1;
   const int first = split * a.split_tiles, mine = min(a.split_tiles, n_tiles - first);
   const size_t part0 = (size_t)t * a.nh + (size_t)kvh * per + h0, row0 = (size_t)token * a.nh + (size_t)kvh * per + h0;
-  if (mine <= 0) {                                                // the token has fewer splits
+  if (mine <= 0 && !CLUSTER) {                                    // the token has fewer splits
     if (a.splits > 1) {
       if (threadIdx.x < heads) {
         float* ml = a.part_ml + ((part0 + threadIdx.x) * a.splits + split) * 2;
@@ -128,29 +143,36 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
   }
   __syncwarp();
   // steps of the split, dealt out in turn; step i covers the keys from key_of(i) on
-  const int steps_all = mine * (TILE / STEP), steps = (steps_all - warp + WARPS - 1) / WARPS;
+  const int steps_all = max(mine, 0) * (TILE / STEP), steps = (steps_all - warp + WARPS - 1) / WARPS;
   auto key_of = [&](int i) {
     const int s = warp + i * WARPS, tile = first + s / (TILE / STEP);
     return (tile < kept ? tile : t0 + tile - kept) * TILE + s % (TILE / STEP) * STEP;
   };
-  // lane b: block b of the step (lane 0 all of it from one page). `after` is 0 and comes from what was read out of the stage last: the
-  // copy into it is not asked for before those loads have come.
+  // Lane b brings block b of a step (lane 0 all of it from one page). Its page is looked up a step before the copy is asked for.
+  const bool together = a.page_size >= STEP;
+  const int n_copies = together ? 1 : MT;
+  int next_page = -1, next_key = 0;
+  auto look = [&](int i) {
+    if (i >= steps) return;
+    next_key = key_of(i);
+    const int at = next_key + lane * 16;
+    next_page = lane < n_copies && at <= pos ? table[a.page_shift >= 0 ? at >> a.page_shift : at / a.page_size] : -1;
+  };
+  // `after` is 0 and comes from what was read out of the stage last: the copy into it is not asked for before those loads have come.
   auto bring = [&](int i, unsigned after) {
-    const int key = key_of(i), blocks = min(MT, (pos - key) / fb::BLOCK_ROWS + 1);      // <= 0: nothing of the step is the token's
-    const bool together = a.page_size >= STEP;
-    const int n = together ? 1 : MT, each = together ? blocks : 1, at = key + lane * 16;
-    const bool copies = lane < n && lane < blocks;
-    int page = -1;
-    if (copies) page = table[at / a.page_size];
-    const uint32_t bytes = each * B::BYTES;
-    const unsigned who = __ballot_sync(0xffffffffu, copies && page >= 0);
+    const int at = next_key + lane * 16, in_page = a.page_shift >= 0 ? at & (a.page_size - 1) : at % a.page_size;
+    const int blocks = together ? min(MT, (pos - next_key) / fb::BLOCK_ROWS + 1) : 1;
+    const uint32_t bytes = blocks * B::BYTES;
+    const bool copies = next_page >= 0;
+    const unsigned who = __ballot_sync(0xffffffffu, copies);
     if (lane == 0) tc::mbar_expect_tx(&full[warp][i % STAGES], __popc(who) * bytes);
     __syncwarp();
-    if (copies && page >= 0)
+    if (copies)
       bulk_load(ring_at + (i % STAGES * MT + lane) * B::BYTES + after,
-                a.pages + (((size_t)page * a.nkv + kvh) * (a.page_size / 16) + at % a.page_size / 16) * B::BYTES, bytes,
-                full_at + i % STAGES * 8);
+                a.pages + (((size_t)next_page * a.nkv + kvh) * (a.page_size / 16) + in_page / 16) * B::BYTES, bytes, full_at + i % STAGES * 8);
+    look(i + 1);
   };
+  look(0);
   for (int i = 0; i < min(STAGES, steps); ++i) bring(i, 0u);
 
   // the heads' queries as columns, raised; their sums over a group in three pieces
@@ -202,9 +224,10 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
     }
     const int key = key_of(i);
     const uint8_t* blocks = ring + i % STAGES * MT * B::BYTES;
-    const bool whole = key + STEP - 1 <= pos && (key >= lo || key + STEP - 1 < a.keep);
-    auto seen = [&](int row) { return key + row <= pos && (key + row >= lo || key + row < a.keep); };
     unsigned spent = 0u;
+    auto seen = [&](int row) { return key + row <= pos && (key + row >= lo || key + row < a.keep); };
+    auto step = [&](auto all_seen) {
+    constexpr bool whole = decltype(all_seen)::value;
     float s[MT][4];
     float m_step[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -215,60 +238,58 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
       const unsigned la = *reinterpret_cast<const unsigned*>(b + B::key_low(g, pair)),
                      lb = *reinterpret_cast<const unsigned*>(b + B::key_low(g + 8, pair));
       const unsigned lows[4] = {la, lb, G == 4 ? la : 0u, G == 4 ? lb : 0u};
-      float total[4] = {0.f, 0.f, 0.f, 0.f};
-      hb::mma_bf16(total, lows, q_sums.x, q_sums.y);
+      const Words<G / 2> sa(b + B::scale(g, 0, 0)), sb(b + B::scale(g + 8, 0, 0));
+      fb::mma_first(s[mt], lows, q_sums.x, q_sums.y);
 #pragma unroll
       for (int c = 0; c < G; ++c) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        fb::mma_codes(acc, ka.w[c], kb.w[c], qf[c]);
-        const unsigned sa = *reinterpret_cast<const unsigned*>(b + B::scale(g, 0, c & ~1)),
-                       sb = *reinterpret_cast<const unsigned*>(b + B::scale(g + 8, 0, c & ~1));
-        const float fa = c & 1 ? high_half(sa) : low_half(sa), fb_ = c & 1 ? high_half(sb) : low_half(sb);
-        total[0] = fmaf(acc[0], fa, total[0]);
-        total[1] = fmaf(acc[1], fa, total[1]);
-        total[2] = fmaf(acc[2], fb_, total[2]);
-        total[3] = fmaf(acc[3], fb_, total[3]);
+        float acc[4];
+        fb::mma_codes_first(acc, ka.w[c], kb.w[c], qf[c]);
+        const float fa = c & 1 ? high_half(sa.w[c / 2]) : low_half(sa.w[c / 2]), fb_ = c & 1 ? high_half(sb.w[c / 2]) : low_half(sb.w[c / 2]);
+        s[mt][0] = fmaf(acc[0], fa, s[mt][0]);
+        s[mt][1] = fmaf(acc[1], fa, s[mt][1]);
+        s[mt][2] = fmaf(acc[2], fb_, s[mt][2]);
+        s[mt][3] = fmaf(acc[3], fb_, s[mt][3]);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float v = total[e] * to_log2;
-        if (!whole && !seen(mt * 16 + g + 8 * (e >> 1))) v = -INFINITY;
-        s[mt][e] = v;
-        m_step[e & 1] = fmaxf(m_step[e & 1], v);
+        if (!whole && !seen(mt * 16 + g + 8 * (e >> 1))) s[mt][e] = -INFINITY;
+        m_step[e & 1] = fmaxf(m_step[e & 1], s[mt][e]);
       }
     }
+    // The weights are taken against `m_run`, which follows the maximum only when a head's has grown by more than 2^8 (a power of 2 of scores
+    // in units of log 2): they stay below 256 and most steps leave the sums as they are.
     bool grows = false;
-    float correct[2];
+    float m_new[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float m = m_step[h];
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-      m = fmaxf(m, m_run[h]);
-      correct[h] = m == m_run[h] ? 1.f : exp2_fast(m_run[h] - m);       // (the first maximum: exp2(-inf) = 0)
-      grows = grows || m != m_run[h];
-      m_run[h] = m;
+      m_new[h] = m * to_log2;                                     // (the scale is positive)
+      grows = grows || m_new[h] > m_run[h] + 8.f;                 // (of a head that has seen nothing yet: any)
     }
     if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-      for (int c = 0; c < 2 * G; ++c)
+      for (int h = 0; h < 2; ++h) {
+        const float m = fmaxf(m_new[h], m_run[h]), correct = m == m_run[h] ? 1.f : exp2_fast(m_run[h] - m);     // (the first: exp2(-inf) = 0)
+        m_run[h] = m;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[c][e] *= correct[e & 1];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        low[e] *= correct[e & 1];
-        eight[e] *= correct[e & 1];
+        for (int c = 0; c < 2 * G; ++c) { o[c][h] *= correct; o[c][2 + h] *= correct; }
+        low[h] *= correct;
+        low[2 + h] *= correct;
+        eight[h] *= correct;
+        eight[2 + h] *= correct;
       }
     }
-    // a step that is not the token's at all leaves a maximum of -inf; its weights are zeros
+    // a head that has seen nothing yet has a maximum of -inf; its weights are zeros
     const float base[2] = {m_run[0] == -INFINITY ? 0.f : -m_run[0], m_run[1] == -INFINITY ? 0.f : -m_run[1]};
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const uint8_t* b = blocks + mt * B::BYTES;
       float p[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = exp2_fast(s[mt][e] + base[e & 1]);
+      for (int e = 0; e < 4; ++e) p[e] = exp2_fast(fmaf(s[mt][e], to_log2, base[e & 1]));
       // rows of the bare weights' product: a group's lows, a group's scales (columns of the records of 8 keys), at 8 ones
       unsigned la, lb;
       {
@@ -293,12 +314,12 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
       const Words<G> va(b + B::value_word(2 * q4, g, 0)), vb(b + B::value_word(2 * q4 + 8, g, 0));
 #pragma unroll
       for (int e = 0; e < 4; ++e) p[e] *= RAISE;
+      const Words<G / 2> sa(b + B::scale(g, 1, 0)), sb(b + B::scale(g + 8, 1, 0));
       const bool see_a = whole || seen(mt * 16 + g), see_b = whole || seen(mt * 16 + g + 8);
 #pragma unroll
       for (int c = 0; c < G; ++c) {
-        const unsigned sa = *reinterpret_cast<const unsigned*>(b + B::scale(g, 1, c & ~1)),
-                       sb = *reinterpret_cast<const unsigned*>(b + B::scale(g + 8, 1, c & ~1));
-        const float fa = see_a ? (c & 1 ? high_half(sa) : low_half(sa)) : 0.f, fb_ = see_b ? (c & 1 ? high_half(sb) : low_half(sb)) : 0.f;
+        const float ta = c & 1 ? high_half(sa.w[c / 2]) : low_half(sa.w[c / 2]), tb = c & 1 ? high_half(sb.w[c / 2]) : low_half(sb.w[c / 2]);
+        const float fa = see_a ? ta : 0.f, fb_ = see_b ? tb : 0.f;
         const unsigned x = transpose8(hb::pack_bf16(p[0] * fa, p[1] * fa)), y = transpose8(hb::pack_bf16(p[2] * fb_, p[3] * fb_));
         unsigned wa = va.w[c], wb = vb.w[c];
         if (mt == MT - 1) spent ^= wa ^ wb ^ x ^ y;
@@ -313,6 +334,9 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
         hb::mma_bf16(eight, a2, x, y);
       }
     }
+    };
+    if (key + STEP - 1 <= pos && (key >= lo || key + STEP - 1 < a.keep)) step(Const<true>());
+    else step(Const<false>());
     __syncwarp();                                                 // all lanes are through with the stage
     if (asked < steps) bring(asked++, spent & a.zero);
   }
@@ -355,6 +379,21 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
       *reinterpret_cast<float4*>(o_s + (warp * HEADS + 2 * q4 + h) * HD + c * 32 + g * 4) =
           make_float4(o[2 * c][h], o[2 * c][2 + h], o[2 * c + 1][h], o[2 * c + 1][2 + h]);
   __syncthreads();
+  float* joined = o_s + WARPS * HEADS * HD;                       // CLUSTER: [HEADS][HD], and (maximum, sum) of every head
+  __shared__ float2 joined_ml[CLUSTER ? HEADS : 1];
+  auto finish = [&](int h, int d, float m_nat, float l, const float4& sum) {
+    if (a.sink && l > 0.f) l += expf((a.sink_values ? a.sink_values[kvh * per + h0 + h] : 0.f) - m_nat);
+    const float inv = l > 0.f ? 1.f / l : l;                      // (a NaN stays one)
+    *reinterpret_cast<uint2*>(a.out + (row0 + h) * HD + d) =
+        make_uint2(hb::pack_bf16(sum.x * inv, sum.y * inv), hb::pack_bf16(sum.z * inv, sum.w * inv));
+  };
+  auto add = [](float4& sum, float& l, const float4& v, float w, float f) {
+    l = fmaf(w, f, l);
+    sum.x = fmaf(v.x, f, sum.x);
+    sum.y = fmaf(v.y, f, sum.y);
+    sum.z = fmaf(v.z, f, sum.z);
+    sum.w = fmaf(v.w, f, sum.w);
+  };
   for (int i = threadIdx.x; i < heads * (HD / 4); i += WARPS * 32) {
     const int h = i / (HD / 4), d = i % (HD / 4) * 4;
     float m = -INFINITY;
@@ -363,28 +402,47 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
     float l = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (ml_s[w][h][1] == 0.f) continue;                         // no key of its steps is the token's
-      const float f = exp2_fast(ml_s[w][h][0] - m);
-      const float4 v = *reinterpret_cast<const float4*>(o_s + (w * HEADS + h) * HD + d);
-      l = fmaf(ml_s[w][h][1], f, l);
-      sum.x = fmaf(v.x, f, sum.x);
-      sum.y = fmaf(v.y, f, sum.y);
-      sum.z = fmaf(v.z, f, sum.z);
-      sum.w = fmaf(v.w, f, sum.w);
-    }
+    for (int w = 0; w < WARPS; ++w)
+      if (ml_s[w][h][1] != 0.f)                                   // (0: no key of its steps is the token's)
+        add(sum, l, *reinterpret_cast<const float4*>(o_s + (w * HEADS + h) * HD + d), ml_s[w][h][1], exp2_fast(ml_s[w][h][0] - m));
     // of scores, not of their base-2 form; a row with a NaN says so in both numbers
     const float m_nat = l != l ? l : m * 0.6931471805599453f;
-    if (a.splits > 1) {
+    if constexpr (CLUSTER) {
+      *reinterpret_cast<float4*>(joined + h * HD + d) = sum;
+      if (d == 0) joined_ml[h] = make_float2(m_nat, l);
+    } else if (a.splits > 1) {
       const size_t at = (part0 + h) * a.splits + split;
       *reinterpret_cast<float4*>(a.part_acc + at * HD + d) = sum;
       if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_nat, l);
     } else {
-      if (a.sink && l > 0.f) l += expf((a.sink_values ? a.sink_values[kvh * per + h0 + h] : 0.f) - m_nat);
-      const float inv = l > 0.f ? 1.f / l : l;                    // (a NaN stays one)
-      *reinterpret_cast<uint2*>(a.out + (row0 + h) * HD + d) =
-          make_uint2(hb::pack_bf16(sum.x * inv, sum.y * inv), hb::pack_bf16(sum.z * inv, sum.w * inv));
+      finish(h, d, m_nat, l, sum);
     }
+  }
+  if constexpr (CLUSTER) {
+    // the blocks share out the heads' rows and add the splits in their order
+    tc::cluster_meet();
+    for (int i = threadIdx.x * a.splits + split; i < heads * (HD / 4); i += WARPS * 32 * a.splits) {
+      const int h = i / (HD / 4), d = i % (HD / 4) * 4;
+      float m[MOST_CLUSTER], w[MOST_CLUSTER], top = -INFINITY;
+      float4 v[MOST_CLUSTER];
+#pragma unroll
+      for (int r = 0; r < MOST_CLUSTER; ++r) {
+        if (r >= a.splits) break;
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m[r]), "=f"(w[r]) : "r"(in_block(&joined_ml[h], r)) : "memory");
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w)
+                     : "r"(in_block(joined + h * HD + d, r)) : "memory");
+        top = fmaxf(top, m[r]);
+      }
+      float l = 0.f;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int r = 0; r < MOST_CLUSTER; ++r) {
+        if (r >= a.splits) break;
+        if (w[r] != 0.f) add(sum, l, v[r], w[r], __expf(m[r] - top));
+      }
+      finish(h, d, top, l, sum);
+    }
+    tc::cluster_meet();                                           // a block's rows are there until all have read them
   }
 }
 
@@ -393,28 +451,40 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
 extern "C" int hb_attention_decode_4bit(const void* q, const void* pages, const int* block_table, int table_stride,
                                         const int* seq_of_token, const int* positions, void* out, int n_tokens, int nh, int nkv, int hd,
                                         int page_size, int chunk, int window, int keep, float scale, int sink,
-                                        const float* sink_values, int split_tiles, int splits, float* part_acc, float* part_ml,
+                                        const float* sink_values, int split_tiles, int splits, int cluster, float* part_acc, float* part_ml,
                                         int* status, const long long* rows, int step_tokens, cudaStream_t stream) {
   if (!q || !pages || !block_table || !seq_of_token || !positions || !out || !status || n_tokens < 0 || nh <= 0 || nkv <= 0 ||
-      nh % nkv || table_stride <= 0 || chunk < 0 || window < 0 || keep < 0 || split_tiles < 1 || splits < 1 ||
-      (splits > 1 && (!part_acc || !part_ml)))
+      nh % nkv || table_stride <= 0 || chunk < 0 || window < 0 || keep < 0 || split_tiles < 1 || splits < 1 || !(scale > 0.f) ||
+      (cluster && (splits < 2 || splits > MOST_CLUSTER)) || (splits > 1 && !cluster && (!part_acc || !part_ml)))
     return HB_ERR_BAD_ARG;
   if ((hd != 64 && hd != 128) || !(page_size == 16 || page_size == 32 || (page_size > 0 && page_size % 64 == 0))) return HB_ERR_UNSUPPORTED;
   const int tiles = (nh / nkv + HEADS - 1) / HEADS;
   if (n_tokens > 65535 || (long long)nkv * tiles > 65535) return HB_ERR_UNSUPPORTED;
   if (n_tokens == 0) return HB_OK;
+  const int shift = page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size);
   const Args a{(const __nv_bfloat16*)q, (const uint8_t*)pages, block_table, seq_of_token, positions, (__nv_bfloat16*)out, part_acc,
-               part_ml, status, rows, sink_values, rows ? step_tokens : n_tokens, table_stride, nh, nkv, page_size, chunk, window, keep,
+               part_ml, status, rows, sink_values, rows ? step_tokens : n_tokens, table_stride, nh, nkv, page_size, shift, chunk, window, keep,
                split_tiles, splits, sink, scale, 0u};
-  const dim3 grid(splits, nkv * tiles, n_tokens);
   const int smem = WARPS * STAGES * (STEP / 16) * 20 * hd;        // blocks of 20 hd bytes; the sums at the end take less
-  auto* kernel = hd == 128 ? attn_decode_4bit_kernel<4> : attn_decode_4bit_kernel<2>;
-  static std::atomic<unsigned long long> allowed[2]{};
-  const cudaError_t e = hb::allow_smem(kernel, smem, allowed[hd == 128]);
+  auto* kernel = cluster ? (hd == 128 ? attn_decode_4bit_kernel<4, true> : attn_decode_4bit_kernel<2, true>)
+                         : (hd == 128 ? attn_decode_4bit_kernel<4, false> : attn_decode_4bit_kernel<2, false>);
+  static std::atomic<unsigned long long> allowed[4]{};
+  cudaError_t e = hb::allow_smem(kernel, smem, allowed[2 * (hd == 128) + (cluster != 0)]);
   if (e != cudaSuccess) return (int)e;
-  kernel<<<grid, WARPS * 32, smem, stream>>>(a);
-  HB_LAUNCH_CHECK();
-  if (splits > 1)
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(splits, nkv * tiles, n_tokens);
+  config.blockDim = dim3(WARPS * 32);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = splits;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = cluster ? 1 : 0;
+  e = cudaLaunchKernelEx(&config, kernel, a);
+  if (e != cudaSuccess) return (int)e;
+  if (splits > 1 && !cluster)
     return hb_attention_merge_rows(part_acc, part_ml, out, HB_DTYPE_BF16, n_tokens * nh, hd, splits, sink, nh, sink_values, rows, step_tokens,
                                    stream);
   return HB_OK;

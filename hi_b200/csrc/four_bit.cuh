@@ -32,6 +32,20 @@ __device__ __forceinline__ void mma_codes(float (&c)[4], unsigned word_a, unsign
   const unsigned a1[4] = {word_a & LOW, word_b & LOW, word_a & HIGH, word_b & HIGH};
   hb::mma_bf16(c, a1, x.z, x.w);
 }
+// the first products of a sum
+__device__ __forceinline__ void mma_first(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_codes_first(float (&c)[4], unsigned word_a, unsigned word_b, const uint4& x) {
+  const unsigned a0[4] = {word_a & LOW, word_b & LOW, word_a & HIGH, word_b & HIGH};
+  mma_first(c, a0, x.x, x.y);
+  word_a >>= 8;
+  word_b >>= 8;
+  const unsigned a1[4] = {word_a & LOW, word_b & LOW, word_a & HIGH, word_b & HIGH};
+  hb::mma_bf16(c, a1, x.z, x.w);
+}
 __device__ __forceinline__ uint4 raised(const uint4& x) {
   return make_uint4(raised(x.x, false), raised(x.y, true), raised(x.z, false), raised(x.w, true));
 }

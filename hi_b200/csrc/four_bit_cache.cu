@@ -45,7 +45,8 @@ __device__ __forceinline__ Quantised quantise(const float (&y)[4]) {
   bool finite = true;
 #pragma unroll
   for (int i = 0; i < 4; ++i) finite = finite && fabsf(y[i]) <= 3.4028234663852886e38f;
-  const unsigned all = __ballot_sync(0xffffffffu, finite);
+  // (a range that float32 does not hold counts as such)
+  const unsigned all = __ballot_sync(0xffffffffu, finite && high - low <= 3.3e38f);
   const bool whole = (all >> (threadIdx.x & 24) & 0xffu) == 0xffu;
   Quantised r;
   r.scale = __float2bfloat16_rn((high - low) / 15.f);

@@ -39,7 +39,7 @@ _SIGNATURES = {
     "hb_qkv_post_4bit": [P, P, I, I, I, F, I, F, F, P, P, I, I, F, I, P, P, P, I, P, P, I, I, I, I, I, I, P],
     "hb_expand_pages_4bit": [P, P, I, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P],
     "hb_prefill_attention_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, I, F, I, I, P, I, I, I, P, c_longlong, P, P],
-    "hb_attention_decode_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, P, I, I, P, P, P, P, I, P],
+    "hb_attention_decode_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, P, I, I, I, P, P, P, P, I, P],
     "hb_four_bit_linear": [P, c_longlong, P, P, P, I, I, I, I, I, P],
     "hb_four_bit_linear_tc": [P, c_longlong, P, P, P, I, I, I, I, I, P, P],
     "hb_paged_attention": [P, I, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, F, P, P, I, I, P, P, P],
@@ -2750,8 +2750,8 @@ def decode_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table: 
     n, nh, hd = q.shape
     step_tokens = n
     _, nkv, page_size = _four_bit_pages(kv_pages, hd)
-    if nh % nkv:
-        raise KernelError(f"{nh} query heads are not a multiple of {nkv} kv heads")
+    if nh % nkv or not scale > 0:
+        raise KernelError(f"{nh} query heads on {nkv} kv heads (a multiple) and a scale above zero are taken, not {scale}")
     seq_of_token, positions = seq_of_token.contiguous(), positions.contiguous()
     _step_tables(n, block_table, seq_of_token, positions)
     if rows is not None:
@@ -2782,7 +2782,8 @@ def decode_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table: 
     if n == 0:
         return out
     part_acc = part_ml = None
-    if splits > 1:
+    cluster = 1 < splits <= DECODE_CLUSTER and n * nkv * -(-(nh // nkv) // 8) * splits <= 592
+    if splits > 1 and not cluster:
         rows_of = n * nh * splits
         scratch = torch.empty(rows_of * (hd + 2), dtype=torch.float32, device=q.device)
         part_acc = scratch.data_ptr()
@@ -2790,7 +2791,7 @@ def decode_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table: 
     TC_USED[0] = True
     _check(lib().hb_attention_decode_4bit(_ptr(q), _ptr(kv_pages), _ptr(block_table), block_table.shape[1], _ptr(seq_of_token),
                                           _ptr(positions), _ptr(out), n, nh, nkv, hd, page_size, chunk, window, keep, scale,
-                                          bool(sink) or sink_values is not None, _ptr(sink_values), split_tiles, splits, part_acc,
+                                          bool(sink) or sink_values is not None, _ptr(sink_values), split_tiles, splits, cluster, part_acc,
                                           part_ml, _ptr(_tc_status(q.device)), _ptr(rows), step_tokens, _stream()),
            "attention_decode_4bit")
     return out
