@@ -96,7 +96,7 @@ template <bool B> struct Const { static constexpr bool value = B; };
 
 // CLUSTER: the splits of a token's heads are a cluster
 template <int G, bool CLUSTER>
-__global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const Args a) {
+__global__ void __launch_bounds__(WARPS * 32, 3) attn_decode_4bit_kernel(const Args a) {
   using B = fb::Block<G>;
   constexpr int HD = 32 * G, MT = STEP / 16;
   constexpr float RAISE = 18446744073709551616.f;                 // 2^64, of weights that meet codes (four_bit.cuh)
@@ -315,6 +315,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
 #pragma unroll
       for (int e = 0; e < 4; ++e) p[e] *= RAISE;
       const Words<G / 2> sa(b + B::scale(g, 1, 0)), sb(b + B::scale(g + 8, 1, 0));
+      if (mt == MT - 1) spent = va.w[0] ^ vb.w[0] ^ sa.w[0] ^ sb.w[0] ^ la ^ lb;      // of every load
       const bool see_a = whole || seen(mt * 16 + g), see_b = whole || seen(mt * 16 + g + 8);
 #pragma unroll
       for (int c = 0; c < G; ++c) {
@@ -322,7 +323,6 @@ __global__ void __launch_bounds__(WARPS * 32, 4) attn_decode_4bit_kernel(const A
         const float fa = see_a ? ta : 0.f, fb_ = see_b ? tb : 0.f;
         const unsigned x = transpose8(hb::pack_bf16(p[0] * fa, p[1] * fa)), y = transpose8(hb::pack_bf16(p[2] * fb_, p[3] * fb_));
         unsigned wa = va.w[c], wb = vb.w[c];
-        if (mt == MT - 1) spent ^= wa ^ wb ^ x ^ y;
         const unsigned a0[4] = {wa & fb::LOW, wa & fb::HIGH, wb & fb::LOW, wb & fb::HIGH};
         hb::mma_bf16(o[2 * c], a0, x, y);
         wa >>= 8;

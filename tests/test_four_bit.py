@@ -326,7 +326,7 @@ def test_decode_in_any_cut(splits, monkeypatch):
     from hi_b200.kernels import ops
 
     step = Step([(1, 2100), (1, 64), (1, 700)], 16, 4, 128, 64, seed=splits).fill()
-    monkeypatch.setattr(ops, "_four_bit_splits", lambda tiles, groups: (-(-tiles // splits), splits))
+    monkeypatch.setattr(ops, "_four_bit_splits", lambda tiles, groups, hd: (-(-tiles // splits), splits))
     got = ops.decode_attention_4bit(step.q, step.pages, step.table, step.seq, step.positions, 0, 0, 0.1, 2101)
     ops.check_tc_status()
     _check_decode(step, got, {}, 0.1)

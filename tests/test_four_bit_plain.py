@@ -65,6 +65,6 @@ def test_refusals_without_a_gpu():
 
 def test_cuts_cover_the_keys():
     for tiles in (1, 2, 3, 7, 16, 63, 100, 513, 2048, 40000):
-        for groups in (1, 8, 40, 64, 512, 8192):
-            size, splits = ops._four_bit_splits(tiles, groups)
+        for groups, hd in ((1, 64), (8, 128), (40, 64), (64, 128), (512, 64), (8192, 128)):
+            size, splits = ops._four_bit_splits(tiles, groups, hd)
             assert size >= 1 and splits >= 1 and size * splits >= tiles and size * (splits - 1) < tiles
