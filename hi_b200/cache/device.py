@@ -3,7 +3,7 @@ mixer with fixed-size state a [max_requests, ...] tensor.
 
 Page layout [pages, kv_heads, page_size, head_dim] (one kv head's page_size rows are
 contiguous; address rule as crates/hi-cuda/src/kernels.cu:4214-4219). One page id addresses
-the same place in every cache slot of its group.
+the same place in every cache slot of its group. A cache in four bits is one pool of bytes for keys and values.
 """
 from __future__ import annotations
 
@@ -11,6 +11,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from ..kernels import ops
 from ..parts.context import CacheView
 from ..parts.spec import CacheSpec
 
@@ -37,7 +38,8 @@ def bytes_per_token(cache_specs: Dict[int, Optional[CacheSpec]], element_size: i
     out = [0] * len(groups)
     for slot, spec in cache_specs.items():
         if spec is not None and spec.paged:
-            out[group_of[slot]] += (2 if spec.values else 1) * spec.kv_heads * spec.head_dim * element_size
+            out[group_of[slot]] += spec.kv_heads * spec.head_dim * 5 // 4 if spec.bits == 4 else \
+                (2 if spec.values else 1) * spec.kv_heads * spec.head_dim * element_size
     return out
 
 
@@ -96,9 +98,14 @@ class DeviceCache:
                 g = self.group_of[slot]
                 shape = (pages_per_group[g], spec.kv_heads, page_size, spec.head_dim)
                 view.group = g
-                view.k_pages = torch.zeros(shape, dtype=dtype, device=self.device)
-                self.bytes += view.k_pages.numel() * view.k_pages.element_size()
-                if spec.values:
+                if spec.bits == 4:
+                    view.kv_pages = torch.zeros((*shape[:2], ops.four_bit_page_bytes(page_size, spec.head_dim)), dtype=torch.uint8,
+                                                device=self.device)
+                    self.bytes += view.kv_pages.numel()
+                else:
+                    view.k_pages = torch.zeros(shape, dtype=dtype, device=self.device)
+                    self.bytes += view.k_pages.numel() * view.k_pages.element_size()
+                if spec.values and spec.bits != 4:
                     view.v_pages = torch.zeros(shape, dtype=dtype, device=self.device)
                     self.bytes += view.v_pages.numel() * view.v_pages.element_size()
             if spec is not None and spec.state_shape:
@@ -132,6 +139,9 @@ class DeviceCache:
             pages = by_group.get(view.group) if view.group is not None else None
             if pages:
                 idx = torch.tensor(pages, device=self.device, dtype=torch.long)
+                if view.kv_pages is not None:
+                    view.kv_pages[idx] = 255             # scales and lows that are NaN
+                    continue
                 view.k_pages[idx] = float("nan")
                 if view.v_pages is not None:
                     view.v_pages[idx] = float("nan")

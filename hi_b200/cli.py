@@ -52,6 +52,9 @@ def build_parser() -> argparse.ArgumentParser:
     r.add_argument("--max-active-requests", type=int, default=None)
     r.add_argument("--max-batched-tokens", type=int, default=8192)
     r.add_argument("--kv-page-size", type=int, default=64)
+    r.add_argument("--weight-bits", type=int, default=16, choices=[4, 16], help="4: dense projections are quantised as they are loaded")
+    r.add_argument("--weight-group", type=int, default=64, choices=[32, 64, 128], help="inputs that share a scale with --weight-bits 4")
+    r.add_argument("--kv-cache-bits", type=int, default=16, choices=[4, 16], help="4: keys and values are cached in four bits")
     r.add_argument("--cpu", action="store_true",
                    help="run the float32 CPU reference (plain C++ loops, whole sequences, no GPU) instead of the engine")
     r.add_argument("--random-weights", action="store_true",
@@ -153,7 +156,8 @@ def cmd_run(args) -> int:
             model = json.load(f)
     llm = LLM(model, random_seed=args.weights_seed, random_std=args.weights_std, dtype=args.dtype, max_batch_size=args.max_batch_size,
               max_active_requests=args.max_active_requests, max_batched_tokens=args.max_batched_tokens,
-              kv_page_size=args.kv_page_size,
+              kv_page_size=args.kv_page_size, weight_bits=args.weight_bits, weight_group=args.weight_group,
+              kv_cache_bits=args.kv_cache_bits,
               kv_cache_tokens=max(args.max_batched_tokens, len(tokens) + args.max_tokens + args.kv_page_size))
     logits = llm.engine.step([StepEntry("inspect", tokens, [len(tokens) - 1])])[0]
     llm.engine.finish("inspect")

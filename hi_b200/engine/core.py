@@ -140,19 +140,23 @@ class Engine:
 
     # ------------------------------------------------------------------ construction
     @staticmethod
-    def from_dir(model_dir: str, dtype="bfloat16", device="cuda:0", **options) -> "Engine":
-        """Load a model folder (config.json + safetensors); the model class is chosen by config.json."""
+    def from_dir(model_dir: str, dtype="bfloat16", device="cuda:0", weight_bits: int = 16, weight_group: int = 64,
+                 kv_cache_bits: int = 16, **options) -> "Engine":
+        """Load a model folder (config.json + safetensors); the model class is chosen by config.json. ``weight_bits=4``: attention's
+        projections, dense feed-forwards and shared experts are quantised to four bits as they are loaded, ``weight_group`` inputs
+        to a scale (routed experts, embeddings, the head and other mixers stay as they are). ``kv_cache_bits=4``: keys and values are
+        cached in four bits (models whose mixers with a paged cache are plain softmax attention, heads of up to 128)."""
         arch, cfg, _raw = load_architecture(model_dir)
-        model = Model(arch.build_spec(cfg), parse_dtype(dtype), device)
+        model = Model(arch.build_spec(cfg), parse_dtype(dtype), device, weight_bits, weight_group, kv_cache_bits)
         load_from_dir(model, model_dir, arch.normalize_tensor_name, arch.derive_tensors)
         return Engine(model, **options)
 
     @staticmethod
     def from_config(config: dict, seed: int = 0, std: float = 0.02, dtype="bfloat16", device="cuda:0",
-                    **options) -> "Engine":
-        """Random weights generated on the device from ``seed`` (no files): for large benchmarks."""
+                    weight_bits: int = 16, weight_group: int = 64, kv_cache_bits: int = 16, **options) -> "Engine":
+        """Random weights generated on the device from ``seed`` (no files): for large benchmarks. Bits as :meth:`from_dir`."""
         arch = lookup(config)
-        model = Model(arch.build_spec(arch.parse_config(config, None)), parse_dtype(dtype), device)
+        model = Model(arch.build_spec(arch.parse_config(config, None)), parse_dtype(dtype), device, weight_bits, weight_group, kv_cache_bits)
         load_random(model, seed, std)
         return Engine(model, **options)
 

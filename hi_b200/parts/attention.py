@@ -9,7 +9,7 @@ import torch
 
 from ..kernels import ops
 from .basic import Part
-from .linear import linear
+from .linear import linear, packed
 from .registry import build, register
 from .spec import CacheSpec, PartSpec, TensorSpec
 
@@ -342,6 +342,14 @@ class AttentionMixer(Part):
                 self.hd = next((r for r in ops.TC_ROW_LENGTHS if r >= self.hd), self.hd)
         elif self.dim != self.vdim or self.dim % 16:
             self.hd = -(-max(self.dim, self.vdim) // 16) * 16                  # rows of the cache and of q
+        # a cache in four bits: rows of its sizes, for what its kernels take
+        self.four_bit = env.cache_bits == 4 and not self.sigmoid and not self.unpadded
+        if self.four_bit:
+            self.hd = next((r for r in ops.FOUR_BIT_ROW_LENGTHS if r >= self.hd), self.hd)
+            if self.hd > ops.FOUR_BIT_ROW_LENGTHS[-1]:
+                raise ValueError(f"{prefix}: a cache in four bits has heads of up to {ops.FOUR_BIT_ROW_LENGTHS[-1]}, not {self.hd}")
+            # pages of portions are expanded for the step's prefill kernels: room for 262,144 tokens (portions behind more ask for more)
+            self.scratch_bytes = 262144 * 4 * self.nkv * self.hd
         if self.hd > (1024 if self.hd != self.dim or self.norm_weighted or self.unpadded or self.values_are_keys else 256):
             raise ValueError(f"{prefix}: head size {self.hd} is not supported")
         self.window = tuple(p["window"]) if p.get("window") else None
@@ -360,7 +368,8 @@ class AttentionMixer(Part):
 
     def cache_spec(self):
         state = (self.taps - 1) * self.channels if self.taps > 1 else 0
-        return CacheSpec(kv_heads=self.nkv, head_dim=self.hd, window=self.window, state_shape=(state,) if state else ())
+        return CacheSpec(kv_heads=self.nkv, head_dim=self.hd, window=self.window, state_shape=(state,) if state else (),
+                         bits=4 if self.four_bit else 16)
 
     @property
     def channels(self) -> int:
@@ -449,7 +458,12 @@ class AttentionMixer(Part):
 
     def load(self, fetch):
         if self.unpadded:
-            return self._load_unpadded(fetch)
+            self._load_unpadded(fetch)
+        else:
+            self._load_padded(fetch)
+        self.w_qkv, self.w_o = packed(self.w_qkv, self.env), packed(self.w_o, self.env)
+
+    def _load_padded(self, fetch):
         names = "qk" if self.values_are_keys else "qkv"
         rows = [fetch(self._name(n)) for n in names]
         if len({t.dtype for t in rows}) > 1:
@@ -539,6 +553,14 @@ class AttentionMixer(Part):
                              v_interleaved=v_inter)
             o = sigmoid_attend_over_pages(q, cache.k_pages, cache.v_pages, block_table, ctx, self.nh, self.nkv, self.hd,
                                           chunk, sliding, self.scale, self.head_bias, self._v_table, v_inter)
+            return linear(o.view(o.shape[0], self.nh * self.hd), self.w_o, bias=self.b_o)
+        if self.four_bit:
+            q = ops.qkv_post_4bit(qkv, self.nh, self.nkv, self.hd, positions, inv_freq, interleaved, self.qk_norm, self.qk_norm_eps,
+                                  self.temperature, ctx.seq_of_token, block_table, cache.kv_pages, cache.writes, self.w_qnorm, self.w_knorm,
+                                  self.norm_weighted, self.dim, rot_mul, self.values_are_keys)
+            o = attend_over_four_bit_pages(q, cache.kv_pages, block_table, ctx, self.nh, self.nkv, self.hd, chunk, sliding, self.scale,
+                                           sink=self.sink, softcap=self.softcap, slopes=self.slopes, sink_values=self.sink_values,
+                                           keep=self.keep)
             return linear(o.view(o.shape[0], self.nh * self.hd), self.w_o, bias=self.b_o)
         extras = self.keep > 0 or bool(self.softcap) or self.slopes is not None or self.sink_values is not None
         if self.hd == self.dim and ctx.max_new == 1 and cache.writes and self.FUSED_DECODE and qkv.dtype == torch.bfloat16 \

@@ -56,6 +56,7 @@ class CacheView:
     group: Optional[int] = None                  # page group (None: no paged cache)
     k_pages: Optional[torch.Tensor] = None       # [pages, kv_heads, page_size, head_dim]
     v_pages: Optional[torch.Tensor] = None
+    kv_pages: Optional[torch.Tensor] = None      # a cache in four bits: uint8 [pages, kv_heads, ops.four_bit_page_bytes], the two above are None
     state: Optional[torch.Tensor] = None         # [max_slots, *state_shape]
     writes: bool = True                          # False: read another entry's cache, do not append
     slot: Optional[int] = None                   # the cache slot's number (a key for per-pass scratch)

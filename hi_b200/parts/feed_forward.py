@@ -8,7 +8,7 @@ import torch
 from ..kernels import ops
 from .basic import Part
 from .context import Pending
-from .linear import linear
+from .linear import linear, packed
 from .registry import register
 from .spec import TensorSpec
 
@@ -23,7 +23,8 @@ class _SwiGLU:
     of the down projection."""
 
     def __init__(self, prefix: str, hidden: int, inter: int, short_names: bool = False, limit: Optional[float] = None,
-                 token_gate: bool = False):
+                 token_gate: bool = False, env=None):
+        self.env = env
         self.limit, self.token_gate = limit, token_gate
         if token_gate and limit is None:
             raise ValueError(f"{prefix}: a gate per token is built for the clamped unit")
@@ -48,8 +49,8 @@ class _SwiGLU:
             rows += [sg, torch.zeros((-(2 * self.inter + 1) % 8, self.hidden), dtype=sg.dtype, device=sg.device)]
         if len({t.dtype for t in rows}) > 1:
             rows = [t.float() for t in rows]
-        self.w_gate_up = torch.cat(rows, dim=0).contiguous()
-        self.w_down = fetch(self._name("down")).contiguous()
+        self.w_gate_up = packed(torch.cat(rows, dim=0).contiguous(), self.env)
+        self.w_down = packed(fetch(self._name("down")).contiguous(), self.env)
 
     def forward(self, x):
         if self.limit is not None:
@@ -69,7 +70,7 @@ class DenseSwiGLU(Part):
     def __init__(self, params, prefix, env):
         super().__init__(params, prefix, env)
         self.mlp = _SwiGLU(prefix, int(params["hidden_size"]), int(params["intermediate_size"]),
-                           short_names=params.get("names", "proj") == "short")
+                           short_names=params.get("names", "proj") == "short", env=env)
 
     def tensor_specs(self):
         return self.mlp.tensor_specs()
@@ -109,8 +110,8 @@ class DenseMLP(Part):
         return specs + ([TensorSpec(f"{self.prefix}.act", (2,))] if self.activation == "xielu" else [])
 
     def load(self, fetch):
-        self.w_up = fetch(f"{self.prefix}.up").contiguous()
-        self.w_down = fetch(f"{self.prefix}.down").contiguous()
+        self.w_up = packed(fetch(f"{self.prefix}.up").contiguous(), self.env)
+        self.w_down = packed(fetch(f"{self.prefix}.down").contiguous(), self.env)
         if self.activation != "xielu":
             return
         pq = fetch(f"{self.prefix}.act").to(torch.float64)
@@ -177,7 +178,7 @@ class SigmoidRoutedExperts(Part):
             limit = float(params["shared_limit"]) if params.get("shared_limit") is not None else None
             self.shared = _SwiGLU(f"{prefix}.shared" if self.per_expert_names else f"{prefix}.shared_expert", self.hidden,
                                   shared_inter, short_names=self.per_expert_names, limit=limit,
-                                  token_gate=bool(params.get("shared_gate", False)))
+                                  token_gate=bool(params.get("shared_gate", False)), env=env)
         score, scale = params.get("score", "sigmoid"), params.get("scale", "input")
         if score not in ("sigmoid", "softmax") or scale not in ("input", "output"):
             raise ValueError(f"{prefix}: score {score!r} / scale {scale!r} are not known (sigmoid | softmax; input | output)")

@@ -21,6 +21,15 @@ def configure_matmul_precision() -> None:
     torch.backends.cuda.matmul.allow_fp16_reduced_precision_reduction = False
 
 
+def packed(weight: torch.Tensor, env) -> torch.Tensor | ops.FourBitWeight:
+    """``weight`` [M, K] as the model is asked to hold it (``env.weight_bits``): in four bits where it is bfloat16 and K a multiple of 32,
+    in groups of ``env.weight_group`` inputs or the next smaller size that divides K."""
+    if env is None or env.weight_bits != 4 or weight.dtype != torch.bfloat16 or weight.shape[1] % 32:
+        return weight
+    group = max(g for g in ops.FOUR_BIT_GROUPS if g <= env.weight_group and weight.shape[1] % g == 0)
+    return ops.quantize_weight(weight, group)
+
+
 def linear(x: torch.Tensor, weight: torch.Tensor | ops.FourBitWeight, out_dtype: torch.dtype | None = None,
            bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` (``+ bias`` [M], added to the float32 sums by the library's epilogue) for

@@ -14,6 +14,7 @@ from . import latent_attention as _latent  # noqa: F401
 from . import mamba2 as _mamba2         # noqa: F401
 from . import mlstm as _mlstm          # noqa: F401
 from . import pair as _pair            # noqa: F401
+from ..kernels import ops
 from .context import CacheView, StepContext
 from .registry import BuildEnv, build
 from .spec import CacheSpec, ModelSpec, PartSpec, TensorSpec
@@ -46,11 +47,17 @@ class Layer:
 
 
 class Model:
-    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device):
+    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device, weight_bits: int = 16, weight_group: int = 64, cache_bits: int = 16):
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError(f"dtype {dtype} is not supported (bfloat16 or float32)")
+        if weight_bits not in (4, 16) or cache_bits not in (4, 16) or weight_group not in ops.FOUR_BIT_GROUPS:
+            raise ValueError(f"weights of {weight_bits} bits in groups of {weight_group}, a cache of {cache_bits}: 4 or 16 bits and groups of "
+                             f"{ops.FOUR_BIT_GROUPS} are built")
+        if dtype != torch.bfloat16 and (weight_bits != 16 or cache_bits != 16):
+            raise ValueError("weights and a cache in four bits are built for bfloat16; the float32 path is 32-bit throughout")
         self.spec, self.dtype, self.device = spec, dtype, torch.device(device)
-        self.env = BuildEnv(dtype=dtype, device=self.device, hidden_size=spec.hidden_size)
+        self.env = BuildEnv(dtype=dtype, device=self.device, hidden_size=spec.hidden_size, weight_bits=weight_bits,
+                            weight_group=weight_group, cache_bits=cache_bits)
         self.embedding = build("embedding", spec.embedding, self.env, spec.embedding.params.get("name", ""))
         self.layers = [Layer(ls, self.env) for ls in spec.layers]
         self.final_norm = build("norm", spec.final_norm, self.env, spec.final_norm.params.get("name", ""))
@@ -70,6 +77,11 @@ class Model:
                     raise ValueError(f"cache slot {entry.cache} is shared by mixers with different cache needs")
             else:
                 self.cache_specs[entry.cache] = cs
+        for slot, cs in self.cache_specs.items():
+            if cs is not None and cs.paged and cs.bits != cache_bits:
+                layer = next(e.layer for e in spec.schedule if e.cache == slot)
+                raise ValueError(f"layer {layer} ('{spec.layers[layer].mixer.kind}'): its cache is not built in {cache_bits} bits (plain "
+                                 f"softmax attention is: without sigmoid weights, a convolution, a second map or an output gate)")
         # fixed-size state of a block arrangement (what its layer keeps per request beside the mixer's), by cache slot
         self.block_state_sizes: Dict[int, int] = {}
         for entry in spec.schedule:
@@ -123,7 +135,7 @@ class Model:
                 ctx.tap = tap if not n else (lambda name, t, prefix=ctx.run_prefix: tap(prefix + name, t))
             view = caches[entry.cache]
             if view.writes != entry.writes_cache:
-                view = CacheView(group=view.group, k_pages=view.k_pages, v_pages=view.v_pages, state=view.state,
+                view = CacheView(group=view.group, k_pages=view.k_pages, v_pages=view.v_pages, kv_pages=view.kv_pages, state=view.state,
                                  writes=entry.writes_cache, slot=view.slot, block_state=view.block_state)
             if entry.interlude is not None:
                 residual, pending = self.interludes[entry.interlude].forward(residual, pending, ctx, entry.interlude_arg)

@@ -39,6 +39,9 @@ class BuildEnv:
     dtype: torch.dtype          # torch.bfloat16 (serving) or torch.float32 (true 32-bit path)
     device: torch.device
     hidden_size: int
+    weight_bits: int = 16       # 4: the dense projections that are made for it hold their weights in four bits
+    weight_group: int = 64      # inputs of a row that share a scale then (32, 64 or 128; the largest of these that divides the row, if less)
+    cache_bits: int = 16        # 4: keys and values are cached in four bits
 
 
 def register(family: str, name: str):

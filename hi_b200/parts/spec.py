@@ -46,6 +46,7 @@ class CacheSpec:
     keys and values itself); no value pool is allocated and its view has ``v_pages`` None.
     Per request: ``state_shape`` elements of fixed size (``()`` = none).
     Mixers with equal paged needs share a page group (one block table per request).
+    ``bits=4``: keys and values lie in one pool of 4-bit pages (``ops.four_bit_page_bytes``), the view's ``kv_pages``.
     """
 
     kv_heads: int = 0
@@ -54,6 +55,7 @@ class CacheSpec:
     state_shape: Tuple[int, ...] = ()
     state_dtype: str = "float32"
     values: bool = True
+    bits: int = 16
 
     @property
     def paged(self) -> bool:
