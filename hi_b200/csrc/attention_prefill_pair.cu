@@ -129,8 +129,8 @@ __device__ __forceinline__ bool work_of(const PrefillPairArgs& a, int bx, int by
   return true;
 }
 
-// HALF: operands and P in float16, values scaled by a.v_factor
-template <int HD, bool HALF>
+// FP16: operands and P in float16, values scaled by a.v_factor
+template <int HD, bool FP16>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const PrefillPairArgs a) {
@@ -309,8 +309,8 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (!ok && queries > 0) tc::mbar_wait_warp(q_full, (queries - 1) & 1);
       for (int i = max(0, n - STAGES); i < n; ++i) tc::mbar_wait_warp(ok ? &empty[i % STAGES] : &full[i % STAGES], (i / STAGES) & 1);
     } else if (warp == 9) {                     // ---- the products: the whole warp walks, one lane issues
-      constexpr uint32_t idesc_qk = HALF ? tc::idesc_f16(BQ, BK, false) : tc::idesc_bf16(BQ, BK, false);
-      constexpr uint32_t idesc_pv = HALF ? tc::idesc_f16(BQ, HD, true) : tc::idesc_bf16(BQ, HD, true);
+      constexpr uint32_t idesc_qk = FP16 ? tc::idesc_f16(BQ, BK, false) : tc::idesc_bf16(BQ, BK, false);
+      constexpr uint32_t idesc_pv = FP16 ? tc::idesc_f16(BQ, HD, true) : tc::idesc_bf16(BQ, HD, true);
       const uint32_t q_addr = tc::smem_u32(q_s), ring_addr = tc::smem_u32(ring);
       bool ok = true;
       int stage = 0, turn = 0, loads = 0, phase[2] = {0, 0};    // the ring's; Q tiles taken; P tiles taken of either item
@@ -491,7 +491,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const float2 y = __ffma2_rn(make_float2(sv[at], sv[at + 1]), scale2, base2);
             const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));
             part[c & 1] = __fadd2_rn(part[c & 1], p);
-            packed[c] = tc::pack16<HALF>(p.x, p.y);
+            packed[c] = tc::pack16<FP16>(p.x, p.y);
           }
           tc::st16_nowait(s_addr + 16 * h, packed);
           if (32 * (h + 1) == EARLY || 32 * (h + 1) == BK) {
@@ -518,7 +518,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         break;
       }
       tc::fence_after();
-      const float factor = HALF ? a.v_factor[x.head / (a.nh / a.nkv)] : 1.f;
+      const float factor = FP16 ? a.v_factor[x.head / (a.nh / a.nkv)] : 1.f;
       if (a.key_splits > 1) {
         // this share of the keys only: the row as it is, with its maximum and sum, for the merge
         const size_t at = ((size_t)(x.tok0 + r) * a.nh + x.head) * a.key_splits + piece;
@@ -531,7 +531,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           uint32_t o[32];
           tc::ld32_nowait(o_addr + c, o);
           tc::wait_ld();
-          if constexpr (HALF)
+          if constexpr (FP16)
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
 #pragma unroll
@@ -587,7 +587,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   }
 }
 
-template <int HD, bool HALF>
+template <int HD, bool FP16>
 int launch(const void* q, const void* k_pages, const void* v_pages, const PrefillPairArgs& a, int n_tokens, long long pool_rows,
            int n_seqs, int max_new, cudaStream_t stream) {
   CUtensorMap mq, mk, mv;
@@ -596,11 +596,11 @@ int launch(const void* q, const void* k_pages, const void* v_pages, const Prefil
       !tc::make_map_bf16(&mv, v_pages, (uint64_t)pool_rows, HD, a.box_rows))
     return HB_ERR_UNSUPPORTED;
   const size_t smem = Layout<HD>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute(attn_prefill_pair_kernel<HD, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(attn_prefill_pair_kernel<HD, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   const long long pairs = ((long long)((max_new + BQ - 1) / BQ) * (a.nh / a.nkv) + 1) / 2;
   if (pairs > 65535 || n_seqs > 65535 || (long long)a.nkv * a.key_splits > 0x7fffffffLL) return HB_ERR_UNSUPPORTED;
-  attn_prefill_pair_kernel<HD, HALF><<<dim3(a.nkv * a.key_splits, n_seqs, (unsigned)pairs), THREADS, smem, stream>>>(mq, mk, mv, a);
+  attn_prefill_pair_kernel<HD, FP16><<<dim3(a.nkv * a.key_splits, n_seqs, (unsigned)pairs), THREADS, smem, stream>>>(mq, mk, mv, a);
   HB_LAUNCH_CHECK();
   return HB_OK;
 }

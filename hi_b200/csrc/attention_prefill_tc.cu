@@ -105,14 +105,15 @@ struct Args {
   int newest_first;
   int keep;                  // a sliding window's kept first tokens
   Pair pair;                 // kPair only
-  const float* v_factor;     // HALF only: the values of kv head h have been divided by v_factor[h]
+  const float* v_factor;     // FP16 only: the values of kv head h have been divided by v_factor[h]
 };
 
-// HALF: operands and P in float16
-template <int HD, bool kPair, bool HALF>
+// FP16: operands and P in float16
+template <int HD, bool kPair, bool FP16>
 __global__ void __launch_bounds__(THREADS, 2)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const Args a) {
+  static_assert(!(kPair && FP16), "two maps side by side come in bfloat16");
   constexpr int DBLK = HD / 64;                 // 64-dim blocks of a row
   constexpr int QBYTES = BQ * HD * 2, KBYTES = BKEYS * HD * 2;
   constexpr int QBLOCK = BQ * 128;              // bytes of one [128 rows x 64 elements] swizzled block of Q
@@ -261,8 +262,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     }
   } else if (warp == 1) {
     // ---- MMA issuer: S_j = Q K_j^T, then O += P_{j-1} V_{j-1}; the whole warp walks, one lane issues
-    constexpr uint32_t idesc_qk = HALF ? tc::idesc_f16(BQ, BKEYS, false) : tc::idesc_bf16(BQ, BKEYS, false);
-    constexpr uint32_t idesc_pv = HALF ? tc::idesc_f16(BQ, HD, true) : tc::idesc_bf16(BQ, HD, true);
+    constexpr uint32_t idesc_qk = FP16 ? tc::idesc_f16(BQ, BKEYS, false) : tc::idesc_bf16(BQ, BKEYS, false);
+    constexpr uint32_t idesc_pv = FP16 ? tc::idesc_f16(BQ, HD, true) : tc::idesc_bf16(BQ, HD, true);
     bool ok = true;
     auto wait = [&](uint64_t* bar, int parity, int code) {
       if (ok && !tc::mbar_wait_warp(bar, parity)) {
@@ -467,7 +468,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         uint32_t packed[BKEYS / 2];
 #pragma unroll
         for (int i = 0; i < BKEYS / 2; ++i) {
-          packed[i] = tc::pack16<HALF>(sv[2 * i], sv[2 * i + 1]);
+          packed[i] = tc::pack16<FP16>(sv[2 * i], sv[2 * i + 1]);
         }
         tc::st32_nowait(tmem + lane_addr + sb * S_COLS, packed);
         tc::wait_st();
@@ -512,7 +513,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           float* ex_ss = ex + 2 * TOKENS * EXS;                // [2][64]
           static_assert((2 * TOKENS * EXS + 2 * TOKENS) * 4 <= KST * KBYTES, "the exchange fits the K tiles");
           const int mp = r / TOKENS;
-          const float inv = (l > 0.f ? 1.f / l : 0.f) * (HALF ? a.v_factor[h / (a.nh / a.nkv)] : 1.f);
+          const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
           for (int c = 0; c < HALF; c += 32) {
             float o[32];
@@ -652,7 +653,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             uint32_t o[32];
             tc::ld32_nowait(tmem_o + lane_addr + c, o);
             tc::wait_ld();
-            if constexpr (HALF)
+            if constexpr (FP16)
 #pragma unroll
               for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a.v_factor[h / (a.nh / a.nkv)]);
 #pragma unroll
@@ -672,7 +673,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           }
         } else {
         if (a.sink && l > 0.f) l += exp2f((a.sink_values ? a.sink_values[h] * 1.4426950408889634f : 0.f) - m);   // m is in units of log 2
-        const float inv = (l > 0.f ? 1.f / l : 0.f) * (HALF ? a.v_factor[h / (a.nh / a.nkv)] : 1.f);
+        const float inv = (l > 0.f ? 1.f / l : 0.f) * (FP16 ? a.v_factor[h / (a.nh / a.nkv)] : 1.f);
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           float o[32];
@@ -707,7 +708,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   }
 }
 
-template <int HD, bool kPair = false, bool HALF = false>
+template <int HD, bool kPair = false, bool FP16 = false>
 int launch(const void* q, const void* k_pages, const void* v_pages, const Args& a, int n_tokens, long long pool_rows,
            int n_seqs, int max_new, cudaStream_t stream) {
   CUtensorMap mq, mk, mv;
@@ -716,14 +717,14 @@ int launch(const void* q, const void* k_pages, const void* v_pages, const Args& 
       !tc::make_map_bf16(&mv, v_pages, (uint64_t)pool_rows, HD, a.box_rows))
     return HB_ERR_UNSUPPORTED;
   const size_t smem = (size_t)BQ * HD * 2 + (KST + 2) * (size_t)BKEYS * HD * 2 + 256;
-  cudaError_t e = cudaFuncSetAttribute(attn_prefill_tc_kernel<HD, kPair, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(attn_prefill_tc_kernel<HD, kPair, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   const int tokens = kPair ? BQ / 2 : BQ;
   const int q_tiles = (max_new + tokens - 1) / tokens;
   if (q_tiles > 65535 || n_seqs > 65535) return HB_ERR_UNSUPPORTED;
   if ((long long)a.nh * a.key_splits > 0x7fffffffLL) return HB_ERR_UNSUPPORTED;
   dim3 grid((kPair ? a.nh / 2 : a.nh) * a.key_splits, q_tiles, n_seqs);
-  attn_prefill_tc_kernel<HD, kPair, HALF><<<grid, THREADS, smem, stream>>>(mq, mk, mv, a);
+  attn_prefill_tc_kernel<HD, kPair, FP16><<<grid, THREADS, smem, stream>>>(mq, mk, mv, a);
   HB_LAUNCH_CHECK();
   return HB_OK;
 }

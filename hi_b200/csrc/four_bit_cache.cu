@@ -280,13 +280,13 @@ __device__ __forceinline__ float held(float x) { return fabsf(x) > 65504.f && fa
 
 constexpr int Q_TOKENS = 8;        // of a block that converts queries
 
-template <int G, bool HALF>
+template <int G, bool FP16>
 __global__ void __launch_bounds__(128) expand_4bit_kernel(const Expand a) {
   constexpr int HD = 32 * G;
   using B = fb::Block<G>;
   const int out_page = blockIdx.x, kvh = blockIdx.y;
   float k_down = 1.f, v_down = 1.f;
-  if constexpr (HALF) {
+  if constexpr (FP16) {
     const int ek = power_above(a.most[2 * kvh]), ev = power_above(a.most[2 * kvh + 1]);
     k_down = power_of_two(-ek);
     v_down = power_of_two(-ev);
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(128) expand_4bit_kernel(const Expand a) {
     unsigned o[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      o[e] = tc::pack16<HALF>(fmaf(scale, (float)(w >> (4 * e) & 15), low), fmaf(scale, (float)(w >> (16 + 4 * e) & 15), low));
+      o[e] = tc::pack16<FP16>(fmaf(scale, (float)(w >> (4 * e) & 15), low), fmaf(scale, (float)(w >> (16 + 4 * e) & 15), low));
     *reinterpret_cast<uint4*>(a.k + out + (size_t)row * HD + group * 32 + q * 8) = make_uint4(o[0], o[1], o[2], o[3]);
   }
   for (int i = threadIdx.x; i < a.page_size / 2 * 8 * G; i += blockDim.x) {  // four dims of the values of two tokens
@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(128) expand_4bit_kernel(const Expand a) {
       const float scale = number(block + B::scale(r + e, 1, group)) * v_down, low = number(block + B::value_low(r + e, group)) * v_down;
       const unsigned c = w >> (16 * e);
       *reinterpret_cast<uint2*>(a.v + out + (size_t)(row + e) * HD + group * 32 + g * 4) = make_uint2(
-          tc::pack16<HALF>(fmaf(scale, (float)(c & 15), low), fmaf(scale, (float)(c >> 4 & 15), low)),
-          tc::pack16<HALF>(fmaf(scale, (float)(c >> 8 & 15), low), fmaf(scale, (float)(c >> 12 & 15), low)));
+          tc::pack16<FP16>(fmaf(scale, (float)(c & 15), low), fmaf(scale, (float)(c >> 4 & 15), low)),
+          tc::pack16<FP16>(fmaf(scale, (float)(c >> 8 & 15), low), fmaf(scale, (float)(c >> 12 & 15), low)));
     }
   }
 }

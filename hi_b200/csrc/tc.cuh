@@ -273,8 +273,8 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn_major) 
   return idesc_bf16(m, n, b_mn_major) & ~((1u << 7) | (1u << 10));
 }
 // two floats as the 16-bit pair that the products take
-template <bool HALF> __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-  if constexpr (HALF) {
+template <bool FP16> __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (FP16) {
     __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
   } else {
