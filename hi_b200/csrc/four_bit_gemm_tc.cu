@@ -7,18 +7,22 @@
 // block of weights a row tile of 16:
 //   warp 0        brings the tokens' tile by TMA (two boxes of 64 k, 128-byte swizzle)
 //   warp 2        brings the 8 row tiles' blocks of codes as one bulk copy each, stages ahead, into a ring of their own
-//   warps 3 .. 18 unpack: eight of them the stage's first 64 k, the others the rest, each a row tile; a word of eight codes becomes eight bfloat16
-//                 and one 16-byte store into the swizzled tile; eight lanes take rows i and i + 4, which meet eight banks of 16 bytes
+//   warps 3 .. 18 unpack: eight of them the stage's first 64 k, the others the rest, each a row tile
 //   warp 1        issues the products, eight of 16 k a stage, and the commits
 //   warps 19 .. 22 read the sums back, add the bias and store: the next tile accumulates into the other half of tensor memory
 // A pair of codes is a pair of denormals after an AND (four_bit.cuh), and code * 2^-133 times scale * 2^73 minus 8 scale * 2^-60 is one
-// instruction with one rounding: the tile holds 2^-60 of the weights, the results are multiplied by 2^60. 9 instructions a word (code in
-// the mantissa of 128, minus 136, times the scale: 15, and the tile of 64 tokens waited for them: 16,384 x 5,120 28 us -> XX).
-// Every row tile is unpacked once per tile of tokens. Eight unpacking warps with their loads in registers took 2,100 cycles a stage, most of
-// it waiting for the fence that shows their stores to the tensor cores and for loads, against 256 to 1,024 of products.
+// instruction with one rounding: the tile holds 2^-60 of the weights, the results are multiplied by 2^60. 9 instructions a word of eight codes
+// (code in the mantissa of 128, minus 136, times the scale: 15).
+// Every row tile is unpacked once per tile of tokens, and where its weights wait decides what a stage takes. Up to 128 tokens: in tensor
+// memory, from which the products read them: a warp stores its 16 rows x 64 k as one instruction, 64 columns a stage behind the sums, and shared
+// memory has the tokens alone to bring to the tensor cores and room for 4 to 6 stages. (In shared memory, a 16-byte store a word, three
+// stages: 64 x 16,384 x 5,120 25.9 us instead of 22.5, 128 of 30.6 / 23.3, 99 x 7,168 x 5,120 21.1 / 17.9, 17 x 5,120 x 5,120 15.8 / 14.6, where the weights
+// alone take 6.7, 6.7, 3.0 and 2.1.) What is left there is the unpacking warps' work: 0.5 us a stage, 5 % of it the products'.
 // PAIR: two blocks of a cluster on 256 rows x up to 256 tokens (cta_group::2), each with its 128 rows and half of the tokens, for
-// many tokens, where the tokens' way from L2 would bound single blocks. SPLIT: few tiles: the blocks of a cluster share out K, one tile a cluster; each
-// sends its sums to the block that finishes those tokens, which adds them in the order of the blocks.
+// many tokens, where the tokens' way from L2 would bound single blocks; weights in shared memory, swizzled, eight lanes with rows i and i + 4,
+// which meet eight banks of 16 bytes (tensor memory holds two tiles' sums). 2,048 x 16,384 x 5,120 221 to 231 us, 1.48 to 1.55 PFLOP/s.
+// SPLIT: few tiles: the blocks of a cluster share out K, one tile a cluster; each sends its sums to the block that finishes those
+// tokens, which adds them in the order of the blocks.
 // Every wait is bounded; a block that gave up says where in `status` and leaves by the common exit.
 #include <cuda.h>
 
@@ -55,6 +59,13 @@ __device__ __forceinline__ uint2 load8(const uint8_t* p) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(tc::smem_u32(p)) : "memory");
   return v;
 }
+// Four steps of 16 k of rows g and g + 8 into tensor memory, 32 columns of 16 lanes: a step is 8 columns, of which a lane has two neighbours.
+__device__ __forceinline__ void store_rows(uint32_t taddr, const uint4& a0, const uint4& a1, const uint4& b0, const uint4& b1) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(a0.x), "r"(a0.y), "r"(b0.x), "r"(b0.y), "r"(a0.z), "r"(a0.w), "r"(b0.z), "r"(b0.w),
+        "r"(a1.x), "r"(a1.y), "r"(b1.x), "r"(b1.y), "r"(a1.z), "r"(a1.w), "r"(b1.z), "r"(b1.w) : "memory");
+}
 template <int GPC> __device__ __forceinline__ uint2 row_scales(const uint8_t* p) {
   if constexpr (GPC == 1) return make_uint2(*reinterpret_cast<const unsigned short*>(p), 0u);
   else if constexpr (GPC == 2) return make_uint2(*reinterpret_cast<const unsigned*>(p), 0u);
@@ -86,11 +97,11 @@ template <bool PAIR, bool SPLIT, int BT, int STAGES, int RAW, int GPC>
 __global__ void __launch_bounds__(THREADS, 1)
 four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) {
   constexpr int XR = PAIR ? BT / 2 : BT;          // token rows of a stage
-  constexpr int X_BYTES = XR * KB * 2, STAGE_BYTES = A_BYTES + X_BYTES;
+  constexpr int X_BYTES = XR * KB * 2, STAGE_BYTES = (PAIR ? A_BYTES : 0) + X_BYTES, X_AT = STAGE_BYTES - X_BYTES;
   constexpr int BLOCK_BYTES = 1024 + 32 * GPC;
   constexpr int SLOTS = SPLIT ? 1 : 2;
-  constexpr int TMEM_COLS = SPLIT ? 128 : SLOTS * BT;      // (a run of 32 columns of a share may start at the 48th of 64)
-  static_assert(!(PAIR && SPLIT) && TMEM_COLS <= 512, "a form at a time, sums within tensor memory");
+  constexpr int TMEM_COLS = 512, A_COLS = KB / 2;          // sums first, then, without PAIR, the stages' weights
+  static_assert(!(PAIR && SPLIT) && SLOTS * BT + (PAIR ? 0 : STAGES * A_COLS) <= TMEM_COLS, "a form at a time, all within tensor memory");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* raw = smem + STAGES * STAGE_BYTES;     // [RAW][UNPACK][RAW_BLOCK]
@@ -154,7 +165,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
           ok = false;
           break;
         }
-        const uint32_t to = ring + s * STAGE_BYTES + A_BYTES, bar = bars + s * 8;
+        const uint32_t to = ring + s * STAGE_BYTES + X_AT, bar = bars + s * 8;
         if (mine && rank == 0 | !PAIR) tc::mbar_expect_tx(&full_x[s], (PAIR ? 2 : 1) * p.box * KB * 2);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -193,12 +204,13 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
           break;
         }
         tc::fence_after();
-        const uint64_t a = ring + s * (STAGE_BYTES >> 4), x = a + (A_BYTES >> 4);
+        const uint64_t a = ring + s * (STAGE_BYTES >> 4), x = a + (X_AT >> 4);
+        const uint32_t a_tmem = tmem + SLOTS * BT + s * A_COLS;
 #pragma unroll
         for (int k = 0; k < KB / 16; ++k) {
           const uint64_t ka = a + ((k / 4 * (A_BYTES / 2) + k % 4 * 32) >> 4), kx = x + ((k / 4 * (X_BYTES / 2) + k % 4 * 32) >> 4);
           if constexpr (PAIR) tc::mma_pair_if(mine, acc, ka, kx, idesc, (c - c0) | k);
-          else tc::mma_if(mine, acc, ka, kx, idesc, (c - c0) | k);
+          else tc::mma_a_tmem_if(mine, acc, a_tmem + k * 8, kx, idesc, (c - c0) | k);
         }
         if constexpr (PAIR) tc::commit_pair_if(mine, &empty[s]);
         else tc::commit_if(mine, &empty[s]);
@@ -232,7 +244,11 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
     }
     for (int i = max(0, issued - RAW); i < issued; ++i) tc::mbar_wait_warp(&raw_full[i % RAW], (i / RAW) & 1);      // no copy is under way at the end
   } else if (warp < FIRST_EPILOGUE) {             // ---- weights
-    const int part = (warp - FIRST_UNPACK) % UNPACK, half = (warp - FIRST_UNPACK) / UNPACK, g = lane >> 3 | (lane & 4), q4 = lane & 3;
+    // PAIR: row tile `part`, rows g and g + 8 of lanes in an order for the stores. Else the warp's part of tensor memory: its quarter's first or
+    // second 16 lanes, rows as the store's fragments have them.
+    const int half = (warp - FIRST_UNPACK) / UNPACK, q4 = lane & 3;
+    const int part = PAIR ? (warp - FIRST_UNPACK) % UNPACK : (warp & 3) * 2 + (warp - FIRST_UNPACK) / 4 % 2;
+    const int g = PAIR ? lane >> 3 | (lane & 4) : lane >> 2;
     int f0, t0, n;
     const uint32_t bars = PAIR ? tc::even_block(full_a) : tc::smem_u32(full_a);
     uint8_t* const row = smem + half * (A_BYTES / 2) + (part * 16 + g) * 128;
@@ -241,14 +257,24 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
     const int stages = c1 > c0 ? tiles * (c1 - c0) : 0;
     int s = 0, turn = 1, r = 0, r_turn = 0;
     uint4 a0, a1, b0, b1;                         // what goes into the next stage: rows g and g + 8, two words of 32 k each
+    const unsigned pick = q4 & 1 ? 0x7351u : 0x6240u;
     auto next = [&]() {                           // false: the codes did not come
       if (!tc::mbar_wait_warp(&raw_full[r], r_turn)) {
         if (lane == 0) atomicExch(p.status, 57);
         return false;
       }
       const uint8_t* block = raw + (r * UNPACK + part) * RAW_BLOCK;        // (rows past the weight's: whatever is there; they are not written out)
-      const uint8_t* words = block + (g * 4 + q4) * 16 + half * 8;
-      const uint2 lo = load8(words), hi = load8(words + 512);
+      uint2 lo, hi;
+      if constexpr (PAIR) {                       // k 8 q4 .. + 7 of each 32
+        const uint8_t* words = block + (g * 4 + q4) * 16 + half * 8;
+        lo = load8(words);
+        hi = load8(words + 512);
+      } else {                                    // k 4 q4 .. + 3 and 16 + 4 q4 .. + 3: a part of two words, one of k under 16 and one of the rest
+        const uint8_t* words = block + (g * 4 + q4 / 2) * 16 + half * 8;
+        const uint2 l0 = load8(words), l1 = load8(words + 32), h0 = load8(words + 512), h1 = load8(words + 544);
+        lo = make_uint2(__byte_perm(l0.x, l1.x, pick), __byte_perm(l0.y, l1.y, pick));
+        hi = make_uint2(__byte_perm(h0.x, h1.x, pick), __byte_perm(h0.y, h1.y, pick));
+      }
       const uint2 s_lo = row_scales<GPC>(block + 1024 + g * 2 * GPC), s_hi = row_scales<GPC>(block + 1024 + (g + 8) * 2 * GPC);
       const int k0 = GPC == 1 ? 0 : GPC == 2 ? half : 2 * half, k1 = GPC == 4 ? k0 + 1 : k0;
       const Factors lo0 = factors(s_lo, k0), hi0 = factors(s_hi, k0);
@@ -270,13 +296,23 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
         if (lane == 0) atomicExch(p.status, 53);
         break;
       }
-      uint8_t *at0 = row + s * STAGE_BYTES + ((q4 ^ g) << 4), *at1 = row + s * STAGE_BYTES + (((4 | q4) ^ g) << 4);
-      *reinterpret_cast<uint4*>(at0) = a0;
-      *reinterpret_cast<uint4*>(at1) = a1;
-      *reinterpret_cast<uint4*>(at0 + 8 * 128) = b0;
-      *reinterpret_cast<uint4*>(at1 + 8 * 128) = b1;
+      if constexpr (PAIR) {
+        uint8_t *at0 = row + s * STAGE_BYTES + ((q4 ^ g) << 4), *at1 = row + s * STAGE_BYTES + (((4 | q4) ^ g) << 4);
+        *reinterpret_cast<uint4*>(at0) = a0;
+        *reinterpret_cast<uint4*>(at1) = a1;
+        *reinterpret_cast<uint4*>(at0 + 8 * 128) = b0;
+        *reinterpret_cast<uint4*>(at1 + 8 * 128) = b1;
+      } else {
+        tc::fence_after();
+        store_rows(tmem + SLOTS * BT + s * A_COLS + half * (A_COLS / 2) + ((uint32_t)(part * 16) << 16), a0, a1, b0, b1);
+      }
       if (i + 1 < stages) ok = next();            // while the stores are on their way: the fence waits for them
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if constexpr (PAIR) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      } else {
+        tc::wait_st();
+        tc::fence_before();
+      }
       __syncwarp();
       if (lane == 0) {
         if constexpr (PAIR) arrive_pair(bars + s * 8);
@@ -389,7 +425,7 @@ int launch(const void* x, long long x_ld, int K, Params p, int blocks, int clust
   CUtensorMap map;
   p.box = (p.most + 15) / 16 * (PAIR ? 8 : 16);
   if (!make_map_rows(&map, x, p.tokens, K, x_ld, p.box)) return HB_ERR_UNSUPPORTED;
-  const size_t smem = STAGES * (size_t)(A_BYTES + (PAIR ? BT / 2 : BT) * KB * 2) + RAW * UNPACK * RAW_BLOCK + 1024 + 512;
+  const size_t smem = STAGES * (size_t)((PAIR ? A_BYTES : 0) + (PAIR ? BT / 2 : BT) * KB * 2) + RAW * UNPACK * RAW_BLOCK + 1024 + 512;
   auto* kernel = four_bit_gemm_kernel<PAIR, SPLIT, BT, STAGES, RAW, GPC>;
   static std::atomic<unsigned long long> allowed{0};
   cudaError_t e = hb::allow_smem(kernel, (int)smem, allowed);
@@ -422,11 +458,11 @@ int gemm(const void* x, long long x_ld, int K, Params p, cudaStream_t stream) {
   while (splits > 1 && p.chunks < 4 * splits) splits /= 2;
   if (splits == 1) {
     const int blocks = f_tiles < 148 ? f_tiles : 148;
-    return p.tokens <= 64 ? launch<false, false, 64, 3, 8, GPC>(x, x_ld, K, p, blocks, 1, stream)
-                          : launch<false, false, 128, 3, 3, GPC>(x, x_ld, K, p, blocks, 1, stream);
+    return p.tokens <= 64 ? launch<false, false, 64, 6, 8, GPC>(x, x_ld, K, p, blocks, 1, stream)
+                          : launch<false, false, 128, 4, 8, GPC>(x, x_ld, K, p, blocks, 1, stream);
   }
-  return p.tokens <= 64 ? launch<false, true, 64, 3, 8, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream)
-                        : launch<false, true, 128, 3, 3, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream);
+  return p.tokens <= 64 ? launch<false, true, 64, 6, 8, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream)
+                        : launch<false, true, 128, 4, 8, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream);
 }
 
 }  // namespace
