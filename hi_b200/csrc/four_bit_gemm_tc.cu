@@ -16,13 +16,13 @@
 // Every row tile is unpacked once per tile of tokens, and where its weights wait decides what a stage takes. Up to 128 tokens: in tensor
 // memory, from which the products read them: a warp stores its 16 rows x 64 k as one instruction, 64 columns a stage behind the sums, and shared
 // memory has the tokens alone to bring to the tensor cores and room for 4 to 6 stages. (In shared memory, a 16-byte store a word, three
-// stages: 64 x 16,384 x 5,120 25.9 us instead of 22.5, 128 of 30.6 / 23.3, 99 x 7,168 x 5,120 21.1 / 17.9, 17 x 5,120 x 5,120 15.8 / 14.6, where the weights
+// stages: 64 x 16,384 x 5,120 25.9 us instead of 22.5, 128 of 30.6 / 23.3, 99 x 7,168 x 5,120 21.1 / 17.9, 17 x 5,120 x 5,120 15.8 / 14.6, all with the same splits, where the weights
 // alone take 6.7, 6.7, 3.0 and 2.1.) What is left there is the unpacking warps' work: 0.5 us a stage, 5 % of it the products'.
 // PAIR: two blocks of a cluster on 256 rows x up to 256 tokens (cta_group::2), each with its 128 rows and half of the tokens, for
 // many tokens, where the tokens' way from L2 would bound single blocks; weights in shared memory, swizzled, eight lanes with rows i and i + 4,
 // which meet eight banks of 16 bytes (tensor memory holds two tiles' sums). 2,048 x 16,384 x 5,120 221 to 231 us, 1.48 to 1.55 PFLOP/s.
 // SPLIT: few tiles: the blocks of a cluster share out K, one tile a cluster; each sends its sums to the block that finishes those
-// tokens, which adds them in the order of the blocks.
+// tokens, which adds them in the order of the blocks. Which form when: `gemm`, below.
 // Every wait is bounded; a block that gave up says where in `status` and leaves by the common exit.
 #include <cuda.h>
 
@@ -38,6 +38,8 @@ constexpr int A_BYTES = BF * KB * 2;
 constexpr int UNPACK = 8, EPILOGUE = 4;           // warps: to unpack half a stage, to write results
 constexpr int FIRST_UNPACK = 3, FIRST_EPILOGUE = FIRST_UNPACK + 2 * UNPACK, THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE);
 constexpr int RAW_BLOCK = 1152;                   // room for a block of codes and scales, the largest
+constexpr int MOST_SPLITS = 8;                    // blocks that share out K
+constexpr size_t stage_bytes(bool pair, int bt) { return (pair ? A_BYTES + bt / 2 * KB * 2 : bt * KB * 2); }
 
 struct Params {
   const uint8_t* w;
@@ -358,7 +360,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
     int f0, t0, n;
     const bool there = tile_at(0, f0, t0, n);
     bool ok = true;
-    if (there && c0 < c1 && warp >= FIRST_EPILOGUE) {
+    if (there && c0 < c1 && warp >= FIRST_UNPACK) {
       ok = tc::mbar_wait_warp(&acc_full[0], 0);
       if (!ok && lane == 0) atomicExch(p.status, 55);
     }
@@ -366,8 +368,9 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
     __syncwarp();
     tc::cluster_meet();                           // every block's ring is free
     const int run = (n + splits - 1) / splits;
-    if (there && c0 < c1 && warp >= FIRST_EPILOGUE) {
-      const int quarter = warp & 3;
+    if (there && c0 < c1 && warp >= FIRST_UNPACK) {
+      const int quarter = warp & 3, turns = (FIRST_EPILOGUE + EPILOGUE - FIRST_UNPACK) / 4;     // five warps a quarter of the rows, 32 tokens in turn
+      int turn = (warp - FIRST_UNPACK) / 4;
 #pragma unroll 1
       for (int r = 0; r < splits; ++r) {
         uint32_t at;
@@ -376,6 +379,8 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
         const int end = min(n, (r + 1) * run);
 #pragma unroll 1
         for (int c = r * run; c < end; c += 32) {
+          if (turn-- > 0) continue;
+          turn = turns - 1;
           float v[32];
           tc::ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
 #pragma unroll
@@ -425,7 +430,7 @@ int launch(const void* x, long long x_ld, int K, Params p, int blocks, int clust
   CUtensorMap map;
   p.box = (p.most + 15) / 16 * (PAIR ? 8 : 16);
   if (!make_map_rows(&map, x, p.tokens, K, x_ld, p.box)) return HB_ERR_UNSUPPORTED;
-  const size_t smem = STAGES * (size_t)((PAIR ? A_BYTES : 0) + (PAIR ? BT / 2 : BT) * KB * 2) + RAW * UNPACK * RAW_BLOCK + 1024 + 512;
+  const size_t smem = STAGES * stage_bytes(PAIR, BT) + RAW * UNPACK * RAW_BLOCK + 1024 + 512;
   auto* kernel = four_bit_gemm_kernel<PAIR, SPLIT, BT, STAGES, RAW, GPC>;
   static std::atomic<unsigned long long> allowed{0};
   cudaError_t e = hb::allow_smem(kernel, (int)smem, allowed);
@@ -445,24 +450,69 @@ int launch(const void* x, long long x_ld, int K, Params p, int blocks, int clust
   return e == cudaSuccess ? HB_OK : (int)e;
 }
 
+// How many clusters of `size` blocks live at a time on the current device (0: the runtime does not say).
+int clusters_of(int size) {
+  static std::atomic<int> known[64][MOST_SPLITS + 1];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device > 63) return 0;
+  int n = known[device][size].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  auto* kernel = four_bit_gemm_kernel<false, true, 128, 4, 8, 1>;
+  constexpr size_t smem = stage_bytes(false, 128) * 4 + 8 * UNPACK * RAW_BLOCK + 1536;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 0;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(size * 148);
+  config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = size;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess || n <= 0) return 0;
+  known[device][size].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// The form, the tokens of a tile and the splits of K by a model of the time in us, fitted to 14 sizes of weight and 7 counts of tokens: a block's
+// stage takes 0.43 to 0.46 with 16 to 128 tokens (its unpacking, the products hide behind it), a pair's 0.48 to 0.68 with 32 to 256, in
+// rounds of what lives at a time, and splits meet in 0.5 + 0.04 a token. Of 56 launches what it takes is 1.01 of the best form's time,
+// 1.05 at worst. Measured, as pairs / single blocks / clusters of splits: 128 x 5,120 x 8,192 40.9 / 32.4 / 19.6 (three), 200 x 5,120 x 8,192
+// 45.9 / 31.5 / -, 256 x 7,168 x 5,120 35.7 / 24.6 / -, 512 x 5,120 x 8,192 44.9 (176 tokens a tile; 50.6 with 256) / 60.4 / -, 512 x 16,384 x 5,120
+// 65.4 / 77.7 / -, 512 x 1,024 x 8,192 41.3 / 32.2 / 16.9 (four), 17 x 1,024 x 8,192 - / 29.9 / 10.4 (eight).
 template <int GPC>
 int gemm(const void* x, long long x_ld, int K, Params p, cudaStream_t stream) {
-  const int f_tiles = (p.n_out + BF - 1) / BF;
-  if (p.tokens > 128) {
-    const int t_tiles = (p.tokens + 255) / 256, pairs = (f_tiles + 1) / 2 * t_tiles;
-    p.most = (((p.tokens + t_tiles - 1) / t_tiles) + 15) / 16 * 16;
-    return launch<true, false, 256, 3, 3, GPC>(x, x_ld, K, p, 2 * (pairs < 74 ? pairs : 74), 2, stream);
+  const int f_tiles = (p.n_out + BF - 1) / BF, fewest = (p.tokens + 255) / 256;
+  struct { float us; bool pair; int most, splits; } best{3.4e38f, false, 0, 1};
+  for (int t = fewest; t <= fewest + 8; ++t) {
+    const int most = ((p.tokens + t - 1) / t + 15) / 16 * 16, tiles = (p.tokens + most - 1) / most;
+    auto take = [&](float us, bool pair, int splits) {
+      if (us < best.us) best = {us, pair, most, splits};
+    };
+    take(6.5f + ((f_tiles + 1) / 2 * (long long)tiles + 73) / 74 * p.chunks * (0.45f + 0.0009f * most), true, 1);
+    if (most > 128) continue;
+    const long long all = (long long)f_tiles * tiles;
+    const float stage = 0.42f + 0.0003f * most;
+    take(5.5f + (all + 147) / 148 * p.chunks * stage, false, 1);
+    for (int s = 2; s <= MOST_SPLITS && s * all <= 148 && 2 * s <= p.chunks; ++s)
+      if (all <= clusters_of(s)) take(6.f + 0.04f * most + (p.chunks + s - 1) / s * stage, false, s);
+    if (most <= 16) break;
   }
-  p.most = p.tokens;
-  int splits = f_tiles > 74 ? 1 : f_tiles > 37 ? 2 : 4;
-  while (splits > 1 && p.chunks < 4 * splits) splits /= 2;
-  if (splits == 1) {
-    const int blocks = f_tiles < 148 ? f_tiles : 148;
-    return p.tokens <= 64 ? launch<false, false, 64, 6, 8, GPC>(x, x_ld, K, p, blocks, 1, stream)
-                          : launch<false, false, 128, 4, 8, GPC>(x, x_ld, K, p, blocks, 1, stream);
+  p.most = best.most;
+  if (best.pair) {
+    const long long pairs = (f_tiles + 1) / 2 * (long long)((p.tokens + p.most - 1) / p.most);
+    return launch<true, false, 256, 3, 3, GPC>(x, x_ld, K, p, 2 * (int)(pairs < 74 ? pairs : 74), 2, stream);
   }
-  return p.tokens <= 64 ? launch<false, true, 64, 6, 8, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream)
-                        : launch<false, true, 128, 4, 8, GPC>(x, x_ld, K, p, f_tiles * splits, splits, stream);
+  const long long all = (long long)f_tiles * ((p.tokens + p.most - 1) / p.most);
+  if (best.splits == 1) {
+    const int blocks = (int)(all < 148 ? all : 148);
+    return p.most <= 64 ? launch<false, false, 64, 6, 8, GPC>(x, x_ld, K, p, blocks, 1, stream)
+                        : launch<false, false, 128, 4, 8, GPC>(x, x_ld, K, p, blocks, 1, stream);
+  }
+  const int blocks = (int)all * best.splits;
+  return p.most <= 64 ? launch<false, true, 64, 6, 8, GPC>(x, x_ld, K, p, blocks, best.splits, stream)
+                      : launch<false, true, 128, 4, 8, GPC>(x, x_ld, K, p, blocks, best.splits, stream);
 }
 
 }  // namespace

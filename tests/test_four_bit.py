@@ -81,6 +81,23 @@ def test_linear_of_many_tokens(m, k, group, tokens):
     ops.check_tc_status()
 
 
+@pytest.mark.parametrize("m,k,group", [(128, 8192, 128), (600, 2048, 64), (1024, 4000, 32), (2048, 2048, 64), (5120, 1024, 128), (4090, 1792, 32)])
+@pytest.mark.parametrize("tokens", [17, 100, 200, 384, 530])
+def test_linear_of_few_tiles(m, k, group, tokens):
+    """Two to eight blocks that share K, with one tile of tokens and with several, shares of unlike length, the last ones short."""
+    from hi_b200.kernels import ops
+
+    g = _gen(m + k + tokens + 1)
+    w, codes, scales = _weight(m, k, group, g)
+    x = torch.randn(tokens, k, device=DEV, generator=g).to(BF16)
+    bias = torch.randn(m, device=DEV, generator=g).to(BF16)
+    got = ops.four_bit_linear(x, w, torch.float32, bias)
+    rounded = weight_values(codes, scales).to(BF16).double()
+    want, size = x.double() @ rounded.t() + bias.double(), x.double().abs() @ rounded.abs().t()
+    assert ((got.double() - want).abs() <= 2.0 ** -18 * size + 2.0 ** -24 * want.abs()).all()
+    ops.check_tc_status()
+
+
 def test_linear_edges():
     """No tokens; rows that start anywhere; large and small inputs; a scale of zero and one that is not finite."""
     from hi_b200.kernels import ops
