@@ -9,7 +9,12 @@
 // times the sum of x over the group, which the same instruction computes once from codes of 8; then the group's scale multiplies its sum
 // in float32. No product is rounded. A block is up to 16 warps that share K in turns of a block of weights; x waits in shared memory in
 // the fragments' order, raised by 2^64 once, each warp's own part; the row tiles of a block follow one another and the loads run ahead
-// over their ends. The warps' sums meet in shared memory in a fixed order.
+// over their ends, three blocks a warp, asked for again where they were used (before the use, into copies, with addresses worked out
+// anew: 163 instructions a block of weights, 8 x 16,384 x 5,120 14.5 us instead of 13.1). The warps' sums meet in shared memory in a fixed order.
+// 8 x 16,384 x 5,120 3.3 TB/s, 1 x 2,048 x 2,048 2.9 us of which 2 are the launch; what bounds it is each warp's chain of loads, unpacking and
+// products (a warp takes 900 cycles a block of weights, 8.4 an instruction), not HBM (0.5 of its rate) nor the tensor cores (0.19). Measured
+// and not kept, 8 x 16,384 x 5,120 / 1 x 5,120 x 8,192: a ring of bulk copies a warp and two row tiles at a time 15.3 / 19.7, two or four sums a group
+// of their own 14.9 / 11.6, sums joined by the warps in turn without a barrier 13.5 / 11.6, clusters that share K 19.7 / 13.9.
 #include "api.h"
 #include "common.cuh"
 #include "four_bit.cuh"
@@ -59,16 +64,19 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) four_bit_few_kernel(const 
     const int total = tiles * per;                                // blocks of weights of this warp
     uint4 lo[AHEAD], hi[AHEAD];
     uint2 s_lo[AHEAD], s_hi[AHEAD];
-    int l_tile = 0, l_i = 0, left = total;
+    int l_i = 0, left = total;
+    const uint8_t* b = a.w + ((size_t)blockIdx.x * a.chunks + c0 + warp) * BYTES + lane * 16;
+    const int to_scales = 1024 + g * 2 * GPC - lane * 16, next_block = warps * BYTES;
+    const long long next_tile = ((long long)gridDim.x * a.chunks - (long long)per * warps) * BYTES;
     auto load = [&](int u) {
       if (left <= 0) return;
-      const uint8_t* b = a.w + ((size_t)(blockIdx.x + (size_t)l_tile * gridDim.x) * a.chunks + c0 + warp + l_i * warps) * BYTES;
-      lo[u] = __ldcs(reinterpret_cast<const uint4*>(b) + lane);
-      hi[u] = __ldcs(reinterpret_cast<const uint4*>(b) + 32 + lane);
-      s_lo[u] = load_scales<GPC>(b + 1024 + g * 2 * GPC);
-      s_hi[u] = load_scales<GPC>(b + 1024 + (g + 8) * 2 * GPC);
+      lo[u] = __ldcs(reinterpret_cast<const uint4*>(b));
+      hi[u] = __ldcs(reinterpret_cast<const uint4*>(b + 512));
+      s_lo[u] = load_scales<GPC>(b + to_scales);
+      s_hi[u] = load_scales<GPC>(b + to_scales + 16 * GPC);
       --left;
-      if (++l_i == per) { l_i = 0; ++l_tile; }
+      b += next_block;
+      if (++l_i == per) { l_i = 0; b += next_tile; }
     };
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) load(u);
@@ -135,27 +143,33 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) four_bit_few_kernel(const 
       ++tile;
       i = 0;
     };
+    const uint4* xc = xs + (size_t)warp * NT * 128 + lane;
+    const float2* st = start + (size_t)warp * GPC * NT * 4 + q4;
     for (int it = 0; it < total; it += AHEAD) {
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         if (it + u >= total) break;
-        const int c = warp + i * warps;
-        const unsigned wl[4] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w}, wh[4] = {hi[u].x, hi[u].y, hi[u].z, hi[u].w};
-        const uint2 sl = s_lo[u], sh = s_hi[u];
-        load(u);
-        const uint4* xc = xs + (size_t)c * NT * 128 + lane;
 #pragma unroll
         for (int k = 0; k < GPC; ++k)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const float2 st = start[((size_t)c * GPC + k) * NT * 4 + n * 4 + q4];
-            float part[4] = {st.x, st.y, st.x, st.y};
+            const float2 begin = st[(k * NT + n) * 4];
+            float part[4] = {begin.x, begin.y, begin.x, begin.y};
 #pragma unroll
-            for (int j = k * 4 / GPC; j < (k + 1) * 4 / GPC; ++j) fb::mma_codes(part, wl[j], wh[j], xc[(n * 4 + j) * 32]);
+            for (int j = k * 4 / GPC; j < (k + 1) * 4 / GPC; ++j)
+              fb::mma_codes(part, j == 0 ? lo[u].x : j == 1 ? lo[u].y : j == 2 ? lo[u].z : lo[u].w,
+                            j == 0 ? hi[u].x : j == 1 ? hi[u].y : j == 2 ? hi[u].z : hi[u].w, xc[(n * 4 + j) * 32]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(part[e], scale_of(e < 2 ? sl : sh, k), acc[n][e]);
+            for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(part[e], scale_of(e < 2 ? s_lo[u] : s_hi[u], k), acc[n][e]);
           }
-        if (++i == per) finish();
+        load(u);
+        xc += warps * NT * 128;
+        st += warps * GPC * NT * 4;
+        if (++i == per) {
+          xc -= per * warps * NT * 128;
+          st -= per * warps * GPC * NT * 4;
+          finish();
+        }
       }
     }
     if (per <= 0)

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from array import array
 from ctypes import c_float, c_int, c_longlong, c_uint64, c_void_p
 from typing import Optional, Tuple
 
@@ -2666,8 +2667,8 @@ def _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos,
             positions.numel() < sum(n_new):
         raise KernelError("start_pos, n_new, cu_seqlens and block_table do not speak of the same requests")
     _on_current_device(kv_pages, block_table, cu_seqlens, positions)
-    numbers = I * n_seqs
-    total = lib().hb_expand_total(numbers(*start_pos), numbers(*n_new), n_seqs, block_table.shape[1], page_size, chunk, window, keep, skip_single)
+    starts, counts = array("i", start_pos), array("i", n_new)
+    total = lib().hb_expand_total(starts.buffer_info()[0], counts.buffer_info()[0], n_seqs, block_table.shape[1], page_size, chunk, window, keep, skip_single) if n_seqs else 0
     if total < 0 or total >= 1 << 31:
         raise KernelError(f"positions of {list(zip(start_pos, n_new))[:4]}... (first, count) lie outside the block table's "
                           f"{block_table.shape[1]} pages a request")

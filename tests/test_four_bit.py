@@ -98,6 +98,20 @@ def test_linear_of_few_tiles(m, k, group, tokens):
     ops.check_tc_status()
 
 
+@pytest.mark.parametrize("m,k,group", [(33, 50048, 32), (20, 26112, 128), (1200, 8192, 64), (3000, 2048, 128), (16, 384, 64)])
+@pytest.mark.parametrize("tokens", [1, 8, 16])
+def test_linear_of_blocks_that_share_k(m, k, group, tokens):
+    """One, two and four blocks on a row tile's K, inputs that shared memory holds and such that come in parts, several row tiles a block."""
+    from hi_b200.kernels import ops
+
+    g = _gen(m + k + tokens + 2)
+    w, codes, scales = _weight(m, k, group, g)
+    x = torch.randn(tokens, k, device=DEV, generator=g).to(BF16)
+    bias = torch.randn(m, device=DEV, generator=g).to(BF16)
+    for kind in (torch.float32, BF16):
+        _check_linear(ops.four_bit_linear(x, w, kind, bias), x, codes, scales, bias)
+
+
 def test_linear_edges():
     """No tokens; rows that start anywhere; large and small inputs; a scale of zero and one that is not finite."""
     from hi_b200.kernels import ops
