@@ -138,7 +138,11 @@ def attend_over_pages(q, k_pages, v_pages, block_table, ctx, nh: int, nkv: int, 
                                sink_values=sink_values, keep=keep)
 
 
-FOUR_BIT_DECODED = 8         # new tokens a request up to which all of a step's tokens are decoded one by one from a 4-bit cache
+# New tokens a request up to which all of a step's tokens are decoded one by one from a 4-bit cache, for up to eight query heads a kv head (the
+# decode kernel takes eight at a time). One by one / expanded, 4 requests behind 3,000 keys, 40 heads of 128 on 8: 8 tokens 39 / 68 us, 12
+# 53 / 69, 16 71 / 69; 32 heads of 64 on 8: 28 / 48, 38 / 49, 43 / 49; 1 to 16 requests behind 300 to 16,000 keys have 0.27 to 0.61 of the time
+# with 8 tokens, 0.29 to 0.86 with 12, 0.31 to 1.14 with 16, 0.33 to 2.2 with 32.
+FOUR_BIT_DECODED = 14
 
 
 def attend_over_four_bit_pages(q, kv_pages, block_table, ctx, nh: int, nkv: int, hd: int, chunk: int, sliding: int, scale: float,
@@ -162,7 +166,7 @@ def attend_over_four_bit_pages(q, kv_pages, block_table, ctx, nh: int, nkv: int,
         return ops.prefill_attention_4bit(q, kv_pages, *spans, chunk, sliding, scale, skip_single, key_splits, sink, sink_values, keep,
                                           one_tile)
 
-    if ctx.max_new <= FOUR_BIT_DECODED:
+    if ctx.max_new * -(-(nh // nkv) // 8) <= FOUR_BIT_DECODED:
         return decode(ctx.max_context)
     return attend_over_pages(q, None, None, block_table, ctx, nh, nkv, hd, chunk, sliding, scale, sink=sink, sink_values=sink_values,
                              keep=keep, decode=decode, prefill=prefill)

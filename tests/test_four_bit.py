@@ -408,6 +408,8 @@ PORTIONS = [
     (16, 4, 128, 64, [(200, 1000), (1, 2000)], dict(window=100, keep=70)),
     (16, 4, 64, 32, [(100, 450), (1, 513), (1, 511)], dict(chunk=256)),
     (8, 8, 128, 16, [(70, 20), (1, 99)], {}),
+    (16, 4, 128, 64, [(14, 200), (9, 0), (1, 5)], dict(window=30)),
+    (48, 4, 64, 64, [(9, 300), (12, 90), (1, 64)], {}),
 ]
 
 
@@ -420,7 +422,7 @@ def test_portions(case):
     nh, nkv, hd, page, portions, mask = case
     step = Step(portions, nh, nkv, hd, page, seed=nh + page).fill()
     scale = hd ** -0.5
-    few = max(n for n, _c in portions) <= FOUR_BIT_DECODED
+    few = max(n for n, _c in portions) * -(-(nh // nkv) // 8) <= FOUR_BIT_DECODED
     for sink in (None, torch.randn(nh, device=DEV, generator=_gen(3))):
         got = attend_over_four_bit_pages(step.q, step.pages, step.table, step.ctx, nh, nkv, hd, mask.get("chunk", 0), mask.get("window", 0),
                                          scale, sink_values=sink, keep=mask.get("keep", 0))
