@@ -112,14 +112,15 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn_decode_4bit_kernel(const A
     if (threadIdx.x == 0) atomicExch(a.status, 32);
     return;
   }
-  const int token = (int)chosen, pos = a.positions[token];
+  const int token = (int)chosen, own = a.positions[token];
+  const int pos = (int)min((long long)own, (long long)a.table_stride * a.page_size - 1);      // the last key that the table has a page for
   const int* table = a.block_table + (size_t)a.seq_of_token[token] * a.table_stride;
   int lo = 0;
-  if (a.chunk > 0) lo = pos / a.chunk * a.chunk;
-  if (a.window > 0) lo = max(lo, pos - a.window + 1);
+  if (a.chunk > 0) lo = own / a.chunk * a.chunk;
+  if (a.window > 0) lo = max(lo, own - a.window + 1);
   // tiles of 64 positions: those of the first tokens that the window keeps, then lo's to the token's own
   const int t0 = lo / TILE, kept = min((a.keep + TILE - 1) / TILE, t0);
-  const int n_tiles = pos < 0 ? 0 : kept + pos / TILE - t0 + 1;
+  const int n_tiles = pos < 0 ? 0 : kept + max(pos / TILE - t0 + 1, 0);
   const int first = split * a.split_tiles, mine = min(a.split_tiles, n_tiles - first);
   const size_t part0 = (size_t)t * a.nh + (size_t)kvh * per + h0, row0 = (size_t)token * a.nh + (size_t)kvh * per + h0;
   if (mine <= 0 && !CLUSTER) {                                    // the token has fewer splits

@@ -98,7 +98,8 @@ __global__ void __launch_bounds__(256, 4) qkv_post_4bit_kernel(const Post a) {
   __syncthreads();
   const int heads = a.nh + (a.v_is_k ? 1 : 2) * a.nkv, todo = a.write_kv ? heads : a.nh;
   int page = -1;
-  if (a.write_kv && pos >= 0) page = a.block_table[(size_t)a.seq_of_token[t] * a.table_stride + pos / a.page_size];
+  if (a.write_kv && pos >= 0 && pos / a.page_size < a.table_stride)
+    page = a.block_table[(size_t)a.seq_of_token[t] * a.table_stride + pos / a.page_size];
   float* row = rows[warp] + lane / LPH * HD;
   const int d0 = 4 * li, group = d0 / 32, rot = 2 * a.rot_pairs;
   const float mul = a.temp_on ? logf(floorf(((float)pos + 1.f) / a.floor_scale) + 1.f) * a.attn_scale + 1.f : 1.f;
@@ -333,10 +334,11 @@ __global__ void __launch_bounds__(EXPAND_THREADS) expand_4bit_kernel(const Expan
   }
   int seq, index;
   if (kvh == 0)                    // the entries that no page of the result is for
-    for (int i = out_page * blockDim.x + threadIdx.x; i < a.n_seqs * a.table_stride; i += a.total * blockDim.x) {
+    for (long long i = (long long)out_page * blockDim.x + threadIdx.x; i < (long long)a.n_seqs * a.table_stride; i += (long long)a.total * blockDim.x) {
       int first, count;
-      span(a, i / a.table_stride, first, count);
-      if (i % a.table_stride < first || i % a.table_stride >= first + count) a.table[i] = 0;
+      const int entry = (int)(i % a.table_stride);
+      span(a, (int)(i / a.table_stride), first, count);
+      if (entry < first || entry >= first + count) a.table[i] = 0;
     }
   if (!find_page(a, out_page, seq, index)) return;
   const int page = a.block_table[(size_t)seq * a.table_stride + index];

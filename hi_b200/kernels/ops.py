@@ -2559,7 +2559,8 @@ def four_bit_linear(x: torch.Tensor, weight: FourBitWeight, out_dtype: torch.dty
                     bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ weight.T (+ bias)`` for bfloat16 ``x`` [N, K] (its rows may be a column slice of a wider matrix) and a weight held in
     four bits, with float32 sums, in ``out_dtype`` (bfloat16 or float32); ``bias`` bfloat16 [M]. Up to 16 rows of ``x`` the products are
-    those of the weight's exact values; more rows take each value rounded to bfloat16, as a bfloat16 weight would hold it."""
+    those of the weight's exact values; more rows take each value rounded to bfloat16, as a bfloat16 weight would hold it. Inputs are below
+    2^63 and scales below 2^54 in size; what scales under 2^-60 add is lost."""
     if not x.is_cuda:
         raise KernelError("x must be a CUDA tensor; this engine has no CPU path")
     m, k = weight.shape
@@ -2735,7 +2736,8 @@ def _four_bit_splits(tiles: int, groups: int, hd: int) -> Tuple[int, int]:
     """The cut of ``tiles`` tiles of 64 keys for ``groups`` (token, kv head, 8 query heads) in the 4-bit decode kernel: (tiles of a split,
     splits), the least by a model of its time in us: rounds of the 444 blocks that live at a time or the work of all tiles,
     whichever is more, and what brings the splits together. Fitted to 60 steps of 1 to 64 tokens, even and uneven, up to 22,000 keys, in
-    up to 16 cuts each: what it takes is 1.03 of the best cut's time on average, 1.18 at worst. 64 tokens of 200 to 4,000 keys, 40 heads of 128 on
+    up to 16 cuts each: what it takes is 1.03 of the best cut's time on average, 1.15 at worst, and 1.04 and 1.26 of 150 others' up to 200,000 keys (models by
+    blocks an SM: 1.03 and 1.37). 64 tokens of 200 to 4,000 keys, 40 heads of 128 on
     8, one split / three / eight: 59 / 57 / 63 us; 8 of 8,192, 2 / 6 / 12: 39 / 28 / 33."""
     tile, work = (0.251, 0.000876) if hd == 128 else (0.213, 0.000379)
     best = (None, tiles, 1)

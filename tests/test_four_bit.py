@@ -386,6 +386,12 @@ def test_decode_of_some_rows():
     step.positions[2] = -1
     padded = ops.decode_attention_4bit(step.q, step.pages, step.table, step.seq, step.positions, 0, 0, 0.125, 301)
     assert not padded[2].any() and torch.equal(padded[0], whole[0])
+    # a position behind the pages that the table names: the keys that are there
+    short = step.table[:, :2].contiguous()
+    clipped = torch.tensor([127, 4, -1, 64], dtype=torch.int32, device=DEV)
+    assert torch.equal(ops.decode_attention_4bit(step.q, step.pages, short, step.seq, step.positions, 0, 0, 0.125, 301),
+                       ops.decode_attention_4bit(step.q, step.pages, short, step.seq, clipped, 0, 0, 0.125, 301))
+    assert not ops.decode_attention_4bit(step.q, step.pages, short, step.seq, step.positions, 0, 50, 0.125, 301)[0].any()
 
 
 def test_a_key_that_is_not_finite_shows():
