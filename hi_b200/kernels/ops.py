@@ -2490,7 +2490,10 @@ def ranked_rows(logits: torch.Tensor, temperatures: torch.Tensor, top_ps: torch.
 # --------------------------------------------------------------------------- four bits
 FOUR_BIT_GROUPS = (32, 64, 128)      # inputs of a weight's row that share a scale
 FOUR_BIT_ROW_LENGTHS = (64, 128)     # head sizes of the 4-bit cache
-FOUR_BIT_FEW = 16                    # tokens up to which a product streams the weights through mma.sync; more go through tcgen05
+# Tokens up to which a product streams the weights through mma.sync, with the weights' exact values; more go through tcgen05. us so / there, 8
+# and 16 rows: 2,048 x 2,048 3.5 / 7.4 and 4.3 / 7.8, 5,120 x 5,120 8.5 / 12.3 and 11.3 / 12.8, 16,384 x 5,120 13.3 / 20.6 and 18.8 / 20.8, 1,024 x 8,192
+# 6.5 / 10.5 and 10.3 / 10.5; over at 9 to 16 rows of long inputs: 5,120 x 8,192 19.7 / 16.5, 4,096 x 14,336 24.7 / 18.8.
+FOUR_BIT_FEW = 16
 
 
 def _on_current_device(*tensors) -> None:
