@@ -459,6 +459,7 @@ extern "C" int hb_attention_decode_4bit(const void* q, const void* pages, const 
       nh % nkv || table_stride <= 0 || chunk < 0 || window < 0 || keep < 0 || split_tiles < 1 || splits < 1 || !(scale > 0.f) ||
       (cluster && (splits < 2 || splits > MOST_CLUSTER)) || (splits > 1 && !cluster && (!part_acc || !part_ml)))
     return HB_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(out)) & 15) return HB_ERR_BAD_ARG;
   if ((hd != 64 && hd != 128) || !(page_size == 16 || page_size == 32 || (page_size > 0 && page_size % 64 == 0))) return HB_ERR_UNSUPPORTED;
   const int tiles = (nh / nkv + HEADS - 1) / HEADS;
   if (n_tokens > 65535 || (long long)nkv * tiles > 65535) return HB_ERR_UNSUPPORTED;

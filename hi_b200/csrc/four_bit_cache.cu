@@ -381,7 +381,8 @@ extern "C" int hb_qkv_post_4bit(const void* qkv, const float* inv_freq, int rot_
                                 int norm_first, int norm_dim, float rot_mul, int v_is_k, const int* positions,
                                 const int* seq_of_token, const int* block_table, int table_stride, void* q_out, void* pages,
                                 int page_size, int write_kv, int n_tokens, int nh, int nkv, int hd, cudaStream_t stream) {
-  if (!qkv || !positions || !q_out || n_tokens < 0 || nh <= 0 || nkv <= 0) return HB_ERR_BAD_ARG;
+  if (!qkv || !positions || !q_out || n_tokens < 0 || nh <= 0 || nkv <= 0 || ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & 7))
+    return HB_ERR_BAD_ARG;
   if (write_kv && (!pages || !block_table || !seq_of_token || table_stride <= 0)) return HB_ERR_BAD_ARG;
   if (!inv_freq) rot_pairs = 0;
   if (norm_dim <= 0) norm_dim = hd;

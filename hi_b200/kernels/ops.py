@@ -2511,7 +2511,11 @@ class FourBitWeight:
     dtype = torch.bfloat16           # of what it is multiplied with
 
     def __init__(self, blocks: torch.Tensor, shape, group: int):
-        self.blocks, self.shape, self.group = blocks, tuple(shape), int(group)
+        m, k = shape
+        if group not in FOUR_BIT_GROUPS or m < 1 or k < 1 or k % group or blocks.dtype != torch.uint8 or not blocks.is_contiguous() or \
+                blocks.shape != (-(-m // 16), -(-k // 128), 1024 + 32 * (128 // group)):
+            raise KernelError(f"blocks {blocks.dtype} {tuple(blocks.shape)} are not those of a 4-bit weight [{m}, {k}] in groups of {group}")
+        self.blocks, self.shape, self.group = blocks, (m, k), int(group)
 
     @property
     def device(self):
@@ -2769,8 +2773,8 @@ def decode_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table: 
     n, nh, hd = q.shape
     step_tokens = n
     _, nkv, page_size = _four_bit_pages(kv_pages, hd)
-    if nh % nkv or not scale > 0:
-        raise KernelError(f"{nh} query heads on {nkv} kv heads (a multiple) and a scale above zero are taken, not {scale}")
+    if nh % nkv or not scale > 0 or q.data_ptr() % 16 or (out is not None and out.data_ptr() % 16):
+        raise KernelError(f"{nh} query heads on {nkv} kv heads (a multiple), rows on 16 bytes and a scale above zero are taken, not {scale}")
     seq_of_token, positions = seq_of_token.contiguous(), positions.contiguous()
     _step_tables(n, block_table, seq_of_token, positions)
     if rows is not None:

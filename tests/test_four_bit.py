@@ -481,6 +481,10 @@ def test_cache_refusals():
                dict(sink_values=torch.zeros(7, device=DEV)), dict(q=torch.zeros(2, 8, 96, dtype=BF16, device=DEV))):
         with pytest.raises(ops.KernelError):
             call(**kw)
+    odd = torch.empty(q.numel() + 4, dtype=BF16, device=DEV)[4:].view_as(q)          # rows that start between 16 bytes
+    for kw in (dict(q=odd), dict(rows=torch.zeros(1, dtype=torch.int64, device=DEV), out=odd)):
+        with pytest.raises(ops.KernelError, match="16 bytes"):
+            call(**kw)
     with pytest.raises(ValueError):
         attend_over_four_bit_pages(q, pages, table, step.ctx, 4, 2, 64, 0, 0, 0.1)
     qkv = torch.zeros(2, 12 * 64, dtype=BF16, device=DEV)

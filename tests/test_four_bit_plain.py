@@ -68,3 +68,19 @@ def test_cuts_cover_the_keys():
         for groups, hd in ((1, 64), (8, 128), (40, 64), (64, 128), (512, 64), (8192, 128)):
             size, splits = ops._four_bit_splits(tiles, groups, hd)
             assert size >= 1 and splits >= 1 and size * splits >= tiles and size * (splits - 1) < tiles
+
+
+@pytest.mark.parametrize("shape,group,blocks", [
+    ((17, 100), 64, (2, 1, 1088)), ((16, 128), 64, (2, 1, 1088)), ((16, 128), 64, (1, 1, 1056)), ((16, 256), 128, (1, 1, 1056)),
+    ((16, 128), 16, (1, 1, 1280)), ((0, 128), 128, (0, 1, 1056)), ((33, 64), 32, (2, 1, 1152))])
+def test_blocks_that_are_not_the_weights(shape, group, blocks):
+    with pytest.raises(ops.KernelError):
+        ops.FourBitWeight(torch.zeros(blocks, dtype=torch.uint8), shape, group)
+
+
+def test_blocks_that_are():
+    w = ops.FourBitWeight(torch.zeros(3, 1, 1152, dtype=torch.uint8), (33, 64), 32)
+    assert w.shape == (33, 64) and w.group == 32
+    for blocks in (w.blocks.to(torch.int8), torch.zeros(3, 2, 1152, dtype=torch.uint8)[:, :1]):
+        with pytest.raises(ops.KernelError):
+            ops.FourBitWeight(blocks, (33, 64), 32)
