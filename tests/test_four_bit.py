@@ -537,3 +537,76 @@ def test_captured_and_on_another_stream():
     got = out.clone()
     assert torch.equal(got, once()) and not torch.equal(got, want)
     ops.check_tc_status()
+
+
+def test_calls_side_by_side():
+    """Products, decode attention and portions on two streams at a time, eager and as two captured graphs, with contents of their own."""
+    from hi_b200.kernels import ops
+    from hi_b200.parts.attention import attend_over_four_bit_pages
+    from hi_b200.parts.linear import linear
+
+    nh, nkv, hd = 16, 4, 128
+
+    def work(seed):
+        step = Step([(1, 900 + seed), (70, 200), (1, 0), (300, 40)], nh, nkv, hd, 64, seed=seed).fill()
+        single = Step([(1, 1500), (1, 70 + seed)], nh, nkv, hd, 64, seed=seed + 10).fill()
+        g = _gen(seed)
+        weights = [_weight(m, k, group, g)[0] for m, k, group in ((512, nh * hd, 128), (2000, 512, 32))]
+        rows = [torch.randn(n, nh * hd, device=DEV, generator=g).to(BF16) for n in (3, 60, 200)]
+
+        def run():
+            out = [linear(linear(x, weights[0]), weights[1]) for x in rows]
+            out.append(attend_over_four_bit_pages(step.q, step.pages, step.table, step.ctx, nh, nkv, hd, 0, 0, 0.09))
+            out.append(attend_over_four_bit_pages(single.q, single.pages, single.table, single.ctx, nh, nkv, hd, 0, 0, 0.09))
+            return out
+        return run
+
+    works = [work(1), work(2)]
+    want = [[t.clone() for t in run()] for run in works]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(works[i]())
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for run in works:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run())
+        graphs.append(graph)
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    ops.check_tc_status()
+    for i in (0, 1):
+        for result in got[i] + [outs[i]]:
+            assert all(torch.equal(a, b) for a, b in zip(result, want[i]))
+
+
+def test_offsets_that_pass_32_bits():
+    """A pool and a weight of more than four gigabytes: pages anywhere in the one, every row tile of the other."""
+    from hi_b200.kernels import ops
+    from hi_b200.parts.attention import attend_over_four_bit_pages
+
+    step = Step([(1, 700), (130, 20), (1, 63)], 16, 8, 128, 64, seed=21, spare=56000).fill()
+    assert step.pages.numel() > 1 << 32 and int(step.table.max()) * step.pages[0].numel() > 1 << 32
+    got = attend_over_four_bit_pages(step.q, step.pages, step.table, step.ctx, 16, 8, 128, 0, 0, 0.09)
+    for s, (n, _c) in enumerate(step.portions):
+        _check_rows(step, s, got, {}, 0.09, None, n == 1)
+    ops.check_tc_status()
+    del step
+    g = _gen(22)
+    part, codes, scales = _weight(2048, 65536, 128, g)
+    whole = ops.FourBitWeight(part.blocks.repeat(66, 1, 1), (66 * 2048, 65536), 128)
+    assert whole.blocks.numel() > 1 << 32
+    for n in (3, 40):
+        x = torch.randn(n, 65536, device=DEV, generator=g).to(BF16)
+        y = ops.four_bit_linear(x, whole, torch.float32).view(n, 66, 2048)
+        _check_linear(y[:, 65], x, codes, scales)
+        assert torch.equal(y, y[:, :1].expand_as(y))
+    ops.check_tc_status()
