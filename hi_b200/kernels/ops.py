@@ -2741,20 +2741,30 @@ FOUR_BIT_CLUSTERED = 256
 @functools.lru_cache(maxsize=4096)                 # a step's layers ask the same
 def _four_bit_splits(tiles: int, groups: int, hd: int) -> Tuple[int, int]:
     """The cut of ``tiles`` tiles of 64 keys for ``groups`` (token, kv head, 8 query heads) in the 4-bit decode kernel: (tiles of a split,
-    splits), the least by a model of its time in us: rounds of the 444 blocks that live at a time or the work of all tiles,
-    whichever is more, and what brings the splits together. Fitted to 60 steps of 1 to 64 tokens, even and uneven, up to 22,000 keys, in
-    up to 16 cuts each: what it takes is 1.03 of the best cut's time on average, 1.15 at worst, and 1.04 and 1.26 of 150 others' up to 200,000 keys (models by
-    blocks an SM: 1.03 and 1.37). 64 tokens of 200 to 4,000 keys, 40 heads of 128 on
-    8, one split / three / eight: 59 / 57 / 63 us; 8 of 8,192, 2 / 6 / 12: 39 / 28 / 33."""
-    tile, work = (0.251, 0.000876) if hd == 128 else (0.213, 0.000379)
+    splits), the least by two models of its time in us, multiplied: by the card (rounds of the 444 blocks that live at a time, or
+    the work of all tiles, whichever is more) and by an SM (its blocks three at a time, a tile at the rate of its instructions or of one
+    block's chain), each with what brings the splits together. Fitted to 60 and 150 steps of 1 to 64 tokens, even and uneven, up to 200,000 keys, in
+    up to 20 cuts each: what it takes is 1.03 of the best cut's time on average, 1.24 at worst (the first model alone 1.04 and 1.26, the
+    second 1.03 and 1.37). 64 tokens of 200 to 4,000 keys, 40 heads of 128 on 8, one split / three / eight: 59 / 56 / 63 us; 8 of 8,192, 2 / 6 /
+    12: 40 / 29 / 33; one of 131,072, 32 heads of 64 on 8, 16 / 54 / 94 splits: 60 / 37 / 44."""
+    work_tile, work = (0.251, 0.000876) if hd == 128 else (0.213, 0.000379)
+    rate, chain = (0.243, 0.538) if hd == 128 else (0.172, 0.407)
     best = (None, tiles, 1)
     for s in range(1, max(1, min(tiles, 96)) + 1):
         size = -(-tiles // s)
         real = -(-tiles // size)
-        waves = -(-(real * groups) // 444)
-        cost = max(waves * (4.92 + tile * size), work * groups * tiles + 0.538 * size + 2.03 * waves)
-        if real > 1:
-            cost += 0.212 * real if real <= DECODE_CLUSTER and real * groups <= FOUR_BIT_CLUSTERED else 0.624 + 0.0105 * real * groups
+        blocks = real * groups
+        waves = -(-blocks // 444)
+        card = max(waves * (4.92 + work_tile * size), work * groups * tiles + 0.538 * size + 2.03 * waves)
+        full, rest = divmod(-(-blocks // 148), 3)
+        sm = 3.01 + full * (max(3 * rate, chain) * size + 0.877) + (max(rest * rate, chain) * size + 0.877 if rest else 0.0)
+        if real > 1 and real <= DECODE_CLUSTER and blocks <= FOUR_BIT_CLUSTERED:
+            card += 0.212 * real
+            sm += 0.364 * real
+        elif real > 1:
+            card += 0.624 + 0.0105 * blocks
+            sm += 2.24 + 0.00103 * blocks + 0.131 * real
+        cost = card ** 0.4 * sm ** 0.6
         if best[0] is None or cost < best[0]:
             best = (cost, size, real)
     return best[1], best[2]
