@@ -2,7 +2,7 @@
 // (+ bias[n]), w in the blocks of four_bit_linear.cu, x bfloat16, float32 sums in tensor memory.
 //
 // The product is taken transposed as in grouped_gemm_tc.cu: 128 weight rows are the MMA's M, up to 256 tokens its N. The operand in shared
-// memory has to be bfloat16, so here, unlike for a few tokens, scale * (code - 8) is rounded to it (2^-9 of a weight at most, as a bfloat16
+// memory has to be bfloat16, so here, unlike for a few tokens, scale * (code - 8) is rounded to it (2^-8 of a weight at most, as a bfloat16
 // checkpoint's weights are; the group's scale cannot wait for the sum, which runs over all groups in tensor memory). A stage is 128 k, one
 // block of weights a row tile of 16:
 //   warp 0        brings the tokens' tile by TMA (two boxes of 64 k, 128-byte swizzle)
@@ -16,8 +16,9 @@
 // Every row tile is unpacked once per tile of tokens, and where its weights wait decides what a stage takes. Up to 128 tokens: in tensor
 // memory, from which the products read them: a warp stores its 16 rows x 64 k as one instruction, 64 columns a stage behind the sums, and shared
 // memory has the tokens alone to bring to the tensor cores and room for 4 to 6 stages. (In shared memory, a 16-byte store a word, three
-// stages: 64 x 16,384 x 5,120 25.9 us instead of 22.5, 128 of 30.6 / 23.3, 99 x 7,168 x 5,120 21.1 / 17.9, 17 x 5,120 x 5,120 15.8 / 14.6, all with the same splits, where the weights
-// alone take 6.7, 6.7, 3.0 and 2.1.) What is left there is the unpacking warps' work: 0.5 us a stage, 5 % of it the products'.
+// stages, the same splits: 64 x 16,384 x 5,120 25.9 us instead of 22.5, 128 of 30.6 / 23.3, 99 x 7,168 x 5,120 21.1 / 17.9, 17 x 5,120 x 5,120 15.8 /
+// 14.6, where the weights alone take 6.7, 6.7, 3.0 and 2.1.) What is left there is the unpacking warps' work, 0.43 us a stage, of which the
+// products of 64 tokens take a fifth.
 // PAIR: two blocks of a cluster on 256 rows x up to 256 tokens (cta_group::2), each with its 128 rows and half of the tokens, for
 // many tokens, where the tokens' way from L2 would bound single blocks; weights in shared memory, swizzled, eight lanes with rows i and i + 4,
 // which meet eight banks of 16 bytes (tensor memory holds two tiles' sums). 2,048 x 16,384 x 5,120 221 to 231 us, 1.48 to 1.55 PFLOP/s.
