@@ -138,6 +138,8 @@ def cmd_run(args) -> int:
         raise SystemExit("the prompt must include at least one token")
     args.tokenizer = tokenizer
     if args.cpu:
+        if args.weight_bits != 16 or args.kv_cache_bits != 16:
+            raise SystemExit("--cpu is the float32 reference: weights and a cache in four bits are served on the GPU only")
         return _run_on_cpu(args, tokens)
     import torch
 

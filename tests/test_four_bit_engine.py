@@ -37,6 +37,14 @@ def test_options_that_are_refused():
         build(wide, cache_bits=4)
 
 
+@pytest.mark.parametrize("option", [("--weight-bits", "4"), ("--kv-cache-bits", "4")])
+def test_the_float32_reference_takes_no_four_bits(option, tmp_path):
+    from hi_b200.cli import main
+
+    with pytest.raises(SystemExit, match="four bits"):
+        main(["run", str(tmp_path / "model"), "--tokens", "1,2,3", "--cpu", *option])
+
+
 def test_a_cached_token_takes_five_eighths_of_a_byte_a_number():
     from hi_b200.cache.device import bytes_per_token
     from hi_b200.parts.spec import CacheSpec
