@@ -479,7 +479,7 @@ int clusters_of(int size) {
 // The form, the tokens of a tile and the splits of K by a model of the time in us, fitted to 14 sizes of weight and 7 counts of tokens: a block's
 // stage takes 0.43 to 0.46 with 16 to 128 tokens (its unpacking, the products hide behind it), a pair's 0.48 to 0.68 with 32 to 256, in
 // rounds of what lives at a time, and splits meet in 0.5 + 0.04 a token. Of 56 launches what it takes is 1.01 of the best form's time,
-// 1.05 at worst. Measured, as pairs / single blocks / clusters of splits: 128 x 5,120 x 8,192 40.9 / 32.4 / 19.6 (three), 200 x 5,120 x 8,192
+// 1.08 at worst. Measured, as pairs / single blocks / clusters of splits: 128 x 5,120 x 8,192 40.9 / 32.4 / 19.6 (three), 200 x 5,120 x 8,192
 // 45.9 / 31.5 / -, 256 x 7,168 x 5,120 35.7 / 24.6 / -, 512 x 5,120 x 8,192 44.9 (176 tokens a tile; 50.6 with 256) / 60.4 / -, 512 x 16,384 x 5,120
 // 65.4 / 77.7 / -, 512 x 1,024 x 8,192 41.3 / 32.2 / 16.9 (four), 17 x 1,024 x 8,192 - / 29.9 / 10.4 (eight).
 template <int GPC>
