@@ -260,7 +260,7 @@ __device__ __forceinline__ bool find_page(const Expand& a, int out_page, int& se
 __device__ __forceinline__ float number(const uint8_t* p) { return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p)); }
 
 // The largest magnitudes of a kv head's keys and values on the pages (of rows that are there; a group's ends: its low and fifteen steps
-// above it; one atomic a block, and none where it changes nothing: 29 us for 1,000 pages of 8 heads with one a warp, 7 so), as the bits of floats, whose order is theirs: the least power of two above one divides the head's numbers, so that float16 holds
+// above it; one atomic a block, and none where it changes nothing: 29 us for 144 pages of 8 heads with one a warp, 7 so), as the bits of floats, whose order is theirs: the least power of two above one divides the head's numbers, so that float16 holds
 // them to 2^-11 of their size, or 2^-25 of the largest one's where they are small.
 constexpr int EXPAND_THREADS = 512, MOST_THREADS = 128;
 
