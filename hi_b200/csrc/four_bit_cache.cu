@@ -199,7 +199,10 @@ __global__ void __launch_bounds__(256, 4) qkv_post_4bit_kernel(const Post a) {
 
 // ---- pages of the step's portions as bfloat16. Request s needs its pages first_s .. last_s: from the oldest position that its first
 // new token may read to its last one; they lie side by side in the result, request after request, and `table` [n_seqs, table_stride]
-// says where (entries outside first_s .. last_s are 0: no kernel that is told of the same mask reads them).
+// says where. Every other entry is -1, as that of a page which was given back: kernels that walk tiles larger than a page look at
+// entries in front of first_s, and what they would multiply by weights of zero there has to be a page of the request or none. The grid is
+// made from the host's copies of the requests' positions; where the device's ask for another number of pages, `status` says so
+// (no entry names a page that is not in the result).
 struct Expand {
   const uint8_t* pages;
   const int* block_table;
@@ -215,6 +218,7 @@ struct Expand {
   int* most;                       // [nkv][keys, values]
   uint16_t* q_half;
   float* v_factor;
+  int* status;
 };
 
 __device__ __forceinline__ void span(const Expand& a, int s, int& first, int& count) {
@@ -227,6 +231,17 @@ __device__ __forceinline__ void span(const Expand& a, int s, int& first, int& co
   else if (a.window > 0 && a.keep == 0) lo = max(0, start - a.window + 1);
   first = lo / a.page_size;
   count = (start + n - 1) / a.page_size - first + 1;
+}
+
+// The pages that all requests ask for, by one warp.
+__device__ __forceinline__ int all_pages(const Expand& a) {
+  int all = 0;
+  for (int s = threadIdx.x & 31; s < a.n_seqs; s += 32) {
+    int first, count;
+    span(a, s, first, count);
+    all += count;
+  }
+  return __reduce_add_sync(0xffffffffu, all);
 }
 
 // The request and its page that page `out_page` of the result is; false: none (or the table has no such page). A whole block asks.
@@ -333,13 +348,7 @@ __global__ void __launch_bounds__(EXPAND_THREADS) expand_4bit_kernel(const Expan
     }
   }
   int seq, index;
-  if (kvh == 0)                    // the entries that no page of the result is for
-    for (long long i = (long long)out_page * blockDim.x + threadIdx.x; i < (long long)a.n_seqs * a.table_stride; i += (long long)a.total * blockDim.x) {
-      int first, count;
-      const int entry = (int)(i % a.table_stride);
-      span(a, (int)(i / a.table_stride), first, count);
-      if (entry < first || entry >= first + count) a.table[i] = 0;
-    }
+  if (out_page == 0 && kvh == 0 && threadIdx.x < 32 && all_pages(a) != a.total && threadIdx.x == 0) atomicExch(a.status, 33);
   if (!find_page(a, out_page, seq, index)) return;
   const int page = a.block_table[(size_t)seq * a.table_stride + index];
   if (kvh == 0 && threadIdx.x == 0) a.table[(size_t)seq * a.table_stride + index] = page < 0 ? -1 : out_page;
@@ -405,11 +414,13 @@ extern "C" int hb_qkv_post_4bit(const void* qkv, const float* inv_freq, int rot_
 
 namespace {
 int expand(const Expand& a, int hd, bool half, cudaStream_t stream) {
-  if (!a.pages || !a.block_table || !a.cu_seqlens || !a.positions || !a.table || a.n_seqs < 0 || a.total < 0 || a.nkv <= 0 || a.table_stride <= 0 ||
+  if (!a.pages || !a.block_table || !a.cu_seqlens || !a.positions || !a.table || !a.status || a.n_seqs < 0 || a.total < 0 || a.nkv <= 0 || a.table_stride <= 0 ||
       a.chunk < 0 || a.window < 0 || a.keep < 0 || (a.total > 0 && (!a.k || !a.v)))
     return HB_ERR_BAD_ARG;
   if ((hd != 64 && hd != 128) || !good_page(a.page_size) || a.nkv > 65535) return HB_ERR_UNSUPPORTED;
   if (a.n_seqs == 0 || a.total == 0) return HB_OK;
+  const cudaError_t e = cudaMemsetAsync(a.table, 0xff, (size_t)a.n_seqs * a.table_stride * 4, stream);      // -1
+  if (e != cudaSuccess) return (int)e;
   const dim3 grid(a.total, a.nkv);
   if (half) {
     const dim3 more(a.total + (a.n_tokens + Q_TOKENS - 1) / Q_TOKENS, a.nkv);
@@ -430,9 +441,10 @@ int expand(const Expand& a, int hd, bool half, cudaStream_t stream) {
 
 extern "C" int hb_expand_pages_4bit(const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
                                     const int* positions, int n_seqs, int total, int page_size, int chunk, int window, int keep,
-                                    int skip_single, int nkv, int hd, void* k, void* v, int* table, cudaStream_t stream) {
+                                    int skip_single, int nkv, int hd, void* k, void* v, int* table, int* status,
+                                    cudaStream_t stream) {
   return expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)k, (uint16_t*)v, table, n_seqs,
-                       table_stride, page_size, chunk, window, keep, skip_single, nkv, total, nullptr, 0, 0, nullptr, nullptr, nullptr},
+                       table_stride, page_size, chunk, window, keep, skip_single, nkv, total, nullptr, 0, 0, nullptr, nullptr, nullptr, status},
                 hd, false, stream);
 }
 
@@ -498,7 +510,7 @@ extern "C" int hb_prefill_attention_4bit(const void* q, const void* pages, const
   int* table = reinterpret_cast<int*>(w + room.table);
   int code = expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)(w + room.k), (uint16_t*)(w + room.v), table,
                            n_seqs, table_stride, page_size, chunk, window, keep, skip_single, nkv, total, (const __nv_bfloat16*)q, n_tokens, nh,
-                           most, (uint16_t*)(w + room.q_half), v_factor},
+                           most, (uint16_t*)(w + room.q_half), v_factor, status},
                     hd, true, stream);
   if (code != HB_OK) return code;
   float* part_acc = key_splits > 1 ? reinterpret_cast<float*>(w + room.part_acc) : nullptr;

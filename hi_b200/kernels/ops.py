@@ -38,7 +38,7 @@ _SIGNATURES = {
     "hb_moe_combine": [P, P, P, P, I, P, I, I, I, P],
     "hb_qkv_post": [P, I, P, I, I, I, F, I, F, F, P, P, I, I, F, P, I, I, I, P, P, P, I, P, P, P, I, I, I, I, I, I, P],
     "hb_qkv_post_4bit": [P, P, I, I, I, F, I, F, F, P, P, I, I, F, I, P, P, P, I, P, P, I, I, I, I, I, I, P],
-    "hb_expand_pages_4bit": [P, P, I, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P],
+    "hb_expand_pages_4bit": [P, P, I, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P, P],
     "hb_prefill_attention_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, I, F, I, I, P, I, I, I, P, c_longlong, P, P],
     "hb_attention_decode_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, P, I, I, I, P, P, P, P, I, P],
     "hb_four_bit_linear": [P, c_longlong, P, P, P, I, I, I, I, I, P],
@@ -2273,7 +2273,7 @@ def _tc_status(device: torch.device) -> torch.Tensor:
 def check_tc_status(device=None) -> None:
     """Raise if a kernel with bounded mbarrier waits (the tcgen05 products and attention, the TMA
     and the 4-bit decode attention, the recurrences by chunks) timed out on one of its barriers since the last check, or the decode
-    attention was given a row that its step does not have
+    attention was given a row that its step does not have, or pages of a 4-bit cache were expanded for other positions than the device's
     (synchronises; skipped while a stream is being captured)."""
     TC_USED[0] = False
     if torch.cuda.is_current_stream_capturing():
@@ -2287,6 +2287,9 @@ def check_tc_status(device=None) -> None:
                     buffers[1].zero_()
             if code == 32:
                 raise KernelError("decode attention was given a row outside the step; its output is invalid")
+            if code == 33:
+                raise KernelError("pages of a 4-bit cache were expanded by start_pos and n_new that are not what positions and cu_seqlens "
+                                  "say on the device; the output is invalid")
             where = {1: "grouped product: the TMA producer waiting for a free stage",
                      2: "grouped product: the MMA issuer waiting for a loaded stage",
                      3: "grouped product: the epilogue waiting for the accumulator",
@@ -2687,16 +2690,18 @@ def expand_pages_4bit(kv_pages: torch.Tensor, hd: int, block_table: torch.Tensor
     """The pages that the step's new tokens may read, in bfloat16: ``(k_pages, v_pages, table)`` with pages [P, nkv, page_size, hd],
     request after request from the page of the oldest position that its first new token reads (``chunk``, ``window``, ``keep``
     as in :func:`paged_attention`; with ``keep`` from the request's first page on) to its last token's, and the block table
-    that names them. Rows behind a request's last token hold whatever the pool holds there. ``start_pos`` and ``n_new`` are the host's
-    copies of what ``positions`` and ``cu_seqlens`` say on the device. ``skip_single``: requests of one new token are left out."""
+    that names them (-1: no page). Rows behind a request's last token hold whatever the pool holds there. ``start_pos`` and ``n_new`` are
+    the host's copies of what ``positions`` and ``cu_seqlens`` say on the device; where those ask for another number of pages,
+    :func:`check_tc_status` raises. ``skip_single``: requests of one new token are left out."""
     nkv, page_size, total = _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos, n_new, chunk, window, keep, skip_single)
     k, v = kv_pages.new_empty((2, total, nkv, page_size, hd), dtype=torch.bfloat16).unbind(0)
     if not total:
-        return k, v, torch.zeros_like(block_table)
-    table = torch.empty_like(block_table)
+        return k, v, torch.full_like(block_table, -1)
+    table = torch.empty_like(block_table) if block_table.shape[0] == len(n_new) else torch.full_like(block_table, -1)
+    TC_USED[0] = True
     _check(lib().hb_expand_pages_4bit(_ptr(kv_pages), _ptr(block_table), block_table.shape[1], _ptr(cu_seqlens), _ptr(positions),
                                       len(n_new), total, page_size, chunk, window, keep, skip_single, nkv, hd, _ptr(k), _ptr(v), _ptr(table),
-                                      _stream()), "expand_pages_4bit")
+                                      _ptr(_tc_status(kv_pages.device)), _stream()), "expand_pages_4bit")
     return k, v, table
 
 

@@ -1,0 +1,149 @@
+"""The 4-bit cache where its neighbours could reach a request: tables of expanded pages, positions that the host and the device do not agree on,
+reshaped scores against float64."""
+import math
+
+import pytest
+import torch
+
+from plain_four_bit import quantise, values, visible
+
+BF16 = torch.bfloat16
+DEV = "cuda:0"
+
+
+def _step(portions, nh, nkv, hd, page, **kw):
+    from test_four_bit import Step
+
+    return Step(portions, nh, nkv, hd, page, **kw)
+
+
+def _reshaped(q, k, v, seen, positions, scale, cap=0.0, slopes=None, sink=None):
+    """float64: scores cap tanh(scale q k / cap) - slope (position - key), softmax with the sink's term. Returns the result, the same with |v|, and
+    scale times the largest sum |q| |k| of a row (what roundings of the keys are relative to)."""
+    per = q.shape[1] // k.shape[1]
+    q, k, v = q.double(), k.double().repeat_interleave(per, 1), v.double().repeat_interleave(per, 1)
+    hidden = ~seen.any(0)
+    k, v = k.masked_fill(hidden.view(-1, 1, 1), 0), v.masked_fill(hidden.view(-1, 1, 1), 0)
+    s = torch.einsum("nhd,thd->nht", q, k) * scale
+    size = (scale * torch.einsum("nhd,thd->nht", q.abs(), k.abs())).masked_fill(~seen.unsqueeze(1), 0).amax(-1, keepdim=True)
+    if cap:
+        s = cap * torch.tanh(s / cap)
+    if slopes is not None:
+        distance = positions.view(-1, 1).double() - torch.arange(k.shape[0], device=q.device).double()
+        s = s - slopes.double().view(1, -1, 1) * distance.unsqueeze(1)
+    s = s.masked_fill(~seen.unsqueeze(1), -math.inf)
+    top = s.amax(-1, keepdim=True)
+    if sink is not None:
+        top = torch.maximum(top, sink.double().view(1, -1, 1))
+    p = torch.exp(s - top)
+    total = p.sum(-1, keepdim=True)
+    if sink is not None:
+        total = total + torch.exp(sink.double().view(1, -1, 1) - top)
+    p = p / total
+    return torch.einsum("nht,thd->nhd", p, v), torch.einsum("nht,thd->nhd", p, v.abs()), size
+
+
+def _check_reshaped(step, s, got, mask, scale, cap, slopes=None, sink=None):
+    """Keys rounded to bfloat16 (2^-8 of each, which moves a score by up to 2^-8 of scale sum |q| |k|, less under a cap) and a cap by fast functions
+    (2^-20 of it): a weight against its sum is off by twice that; values and weights rounded to bfloat16, and the result."""
+    a, b = step.cu[s], step.cu[s + 1]
+    k, v = values(quantise(step.k[s])), values(quantise(step.v[s]))
+    seen = visible(step.positions[a:b], k.shape[0], **mask)
+    want, size, scores = _reshaped(step.q[a:b], k, v, seen, step.positions[a:b], scale, cap, slopes, sink)
+    off = 2.0 ** -8 * scores + 2.0 ** -20 * cap
+    tol = 2 * off * (1 + off) * size + 2.0 ** -8 * (2 * size + want.abs()) + 2.0 ** -20 * size.amax()
+    diff = (got[a:b].double() - want).abs()
+    assert (diff <= tol).all(), (s, float((diff / tol).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 32), (64, 64)])
+def test_a_table_of_expanded_pages_names_them_and_nothing_else(hd, page):
+    from hi_b200.kernels import ops
+
+    step = _step([(37, 0), (1, 200), (70, 3), (2, 63), (1, 500)], 4, 2, hd, page, seed=page).fill()
+    ctx = step.ctx
+    wide = torch.cat([step.table, torch.full_like(step.table[:1], 5)])            # a row behind the last request
+    for chunk, window, keep, skip in ((0, 0, 0, False), (64, 0, 0, False), (0, 20, 0, True), (0, 20, 5, False), (100, 0, 0, True)):
+        for given in (step.table, wide):
+            k, _v, table = ops.expand_pages_4bit(step.pages, hd, given, ctx.cu_seqlens, step.positions, ctx.start_pos, ctx.n_new, chunk, window,
+                                                 keep, skip)
+            want, at = torch.full_like(given, -1), 0
+            for s, (n, c) in enumerate(step.portions):
+                if skip and n == 1:
+                    continue
+                low = c // chunk * chunk if chunk else max(0, c - window + 1) if window and not keep else 0
+                count = (c + n - 1) // page - low // page + 1
+                want[s, low // page: low // page + count] = torch.arange(at, at + count, dtype=torch.int32, device=DEV)
+                at += count
+            assert k.shape[0] == at and torch.equal(table, want)
+    none = ops.expand_pages_4bit(step.pages, hd, step.table, ctx.cu_seqlens * 0, step.positions, ctx.start_pos, [0] * 5)[2]
+    assert (none == -1).all()
+    ops.check_tc_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [[0, 0], [300, 380]])
+def test_positions_that_the_device_does_not_have_are_found(host):
+    """More pages on the device than the host asked for, and fewer: no entry names a page that is not there, and the step's check raises."""
+    from hi_b200.kernels import ops
+
+    step = _step([(1, 300), (1, 90)], 4, 2, 64, 64, seed=3).fill()
+    k, _v, table = ops.expand_pages_4bit(step.pages, 64, step.table, step.ctx.cu_seqlens, step.positions, host, [1, 1])
+    assert int(table.max()) < k.shape[0] and int(table.min()) == -1
+    with pytest.raises(ops.KernelError, match="4-bit cache"):
+        ops.check_tc_status()
+    ops.expand_pages_4bit(step.pages, 64, step.table, step.ctx.cu_seqlens, step.positions, [300, 90], [1, 1])
+    ops.check_tc_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,window", [(32, 100), (16, 90), (16, 37)])
+def test_a_request_beside_one_that_is_not_finite(page, window):
+    """Request 0 has groups of NaN on its first pages; request 1's window starts inside a tile of keys, behind pages that nobody needs."""
+    from hi_b200.kernels import ops
+    from hi_b200.parts.attention import attend_over_four_bit_pages
+
+    step = _step([(70, 10), (200, 260), (33, 400)], 8, 2, 64, page, seed=window)
+    step.k[0][3], step.v[0][:20] = float("nan"), float("nan")
+    step.fill()
+    ctx, scale = step.ctx, 0.125
+    slopes = torch.rand(8, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)) * 0.02
+    for cap, slope in ((20.0, None), (0.0, slopes), (5.0, slopes)):
+        got = attend_over_four_bit_pages(step.q, step.pages, step.table, ctx, 8, 2, 64, 0, window, scale, softcap=cap, slopes=slope)
+        ops.check_tc_status()
+        for s in (1, 2):
+            _check_reshaped(step, s, got, dict(window=window), scale, cap, slope)
+    for one_tile in (False, True):
+        got = ops.prefill_attention_4bit(step.q, step.pages, step.table, ctx.cu_seqlens, step.positions, ctx.start_pos, ctx.n_new, 0, window, scale,
+                                         one_tile=one_tile)
+        ops.check_tc_status()
+        for s in (1, 2):
+            _check_reshaped(step, s, got, dict(window=window), scale, 0.0)
+
+
+RESHAPED = [
+    ([(40, 100), (1, 70), (1, 900)], 64, {}),
+    ([(130, 700), (20, 0), (1, 33)], 32, dict(window=90)),
+    ([(1, 300), (1, 64), (1, 2000)], 64, dict(window=100)),
+    ([(1, 300), (1, 64), (1, 129)], 16, dict(chunk=100)),
+    ([(90, 333), (1, 10)], 16, dict(window=50, keep=20)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", RESHAPED, ids=lambda c: f"p{c[1]}n{len(c[0])}" + "".join(f"_{k}{v}" for k, v in c[2].items()))
+def test_reshaped_scores_against_float64(case):
+    from hi_b200.kernels import ops
+    from hi_b200.parts.attention import attend_over_four_bit_pages
+
+    portions, page, mask = case
+    step = _step(portions, 8, 2, 64, page, seed=page + len(portions)).fill()
+    g = torch.Generator(device=DEV).manual_seed(2)
+    slopes, sinks = torch.rand(8, device=DEV, generator=g) * 0.02, torch.randn(8, device=DEV, generator=g)
+    for cap, slope, sink in ((20.0, None, None), (0.0, slopes, None), (3.0, slopes, sinks)):
+        got = attend_over_four_bit_pages(step.q, step.pages, step.table, step.ctx, 8, 2, 64, mask.get("chunk", 0), mask.get("window", 0), 0.125,
+                                         softcap=cap, slopes=slope, sink_values=sink, keep=mask.get("keep", 0))
+        ops.check_tc_status()
+        for s in range(len(portions)):
+            _check_reshaped(step, s, got, mask, 0.125, cap, slope, sink)
