@@ -145,7 +145,8 @@ class Engine:
         """Load a model folder (config.json + safetensors); the model class is chosen by config.json. ``weight_bits=4``: attention's
         projections, dense feed-forwards and shared experts are quantised to four bits as they are loaded, ``weight_group`` inputs
         to a scale (routed experts, embeddings, the head and other mixers stay as they are). ``kv_cache_bits=4``: keys and values are
-        cached in four bits (models whose mixers with a paged cache are plain softmax attention, heads of up to 128)."""
+        cached in four bits (models whose mixers with a paged cache are plain softmax attention, heads of up to 128; where their scores are
+        capped or biased by distance, steps are not captured)."""
         arch, cfg, _raw = load_architecture(model_dir)
         model = Model(arch.build_spec(cfg), parse_dtype(dtype), device, weight_bits, weight_group, kv_cache_bits)
         load_from_dir(model, model_dir, arch.normalize_tensor_name, arch.derive_tensors)

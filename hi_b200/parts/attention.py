@@ -149,7 +149,9 @@ def attend_over_four_bit_pages(q, kv_pages, block_table, ctx, nh: int, nkv: int,
                                sink: bool = False, softcap: float = 0.0, slopes=None, sink_values=None, keep: int = 0):
     """:func:`attend_over_pages` over a cache held in four bits (``ops.qkv_post_4bit`` fills it). Single tokens, and portions of a few,
     read it as it is; for portions of prompts the pages that they may read are expanded to float16 once and go through the tcgen05
-    kernels. Reshaped scores (``softcap``, ``slopes``) are taken by the kernels of the bfloat16 cache, over pages expanded to that."""
+    kernels. Reshaped scores (``softcap``, ``slopes``) are taken by the kernels of the bfloat16 cache, over pages expanded to that, in steps
+    of single tokens too. What is expanded is fixed by ``ctx.start_pos`` and ``ctx.n_new`` of the call: a captured call is replayed at its own positions
+    only (``ops.check_tc_status`` raises where others ask for more or fewer pages)."""
     if q.shape != (ctx.n_tokens, nh, hd) or kv_pages.shape[1] != nkv:
         raise ValueError(f"queries {tuple(q.shape)} and pages of {kv_pages.shape[1]} kv heads for {ctx.n_tokens} tokens, {nh} heads on {nkv}")
     spans = (block_table, ctx.cu_seqlens, ctx.positions, ctx.start_pos, ctx.n_new)
@@ -354,6 +356,8 @@ class AttentionMixer(Part):
                 raise ValueError(f"{prefix}: a cache in four bits has heads of up to {ops.FOUR_BIT_ROW_LENGTHS[-1]}, not {self.hd}")
             # pages of portions are expanded for the step's prefill kernels: room for 262,144 tokens (portions behind more ask for more)
             self.scratch_bytes = 262144 * 4 * self.nkv * self.hd
+            # capped or biased scores go over pages expanded by the host's positions, which a captured step does not know
+            self.graph_safe = not self.softcap and self.distance_bias is None
         if self.hd > (1024 if self.hd != self.dim or self.norm_weighted or self.unpadded or self.values_are_keys else 256):
             raise ValueError(f"{prefix}: head size {self.hd} is not supported")
         self.window = tuple(p["window"]) if p.get("window") else None

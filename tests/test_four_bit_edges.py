@@ -147,3 +147,53 @@ def test_reshaped_scores_against_float64(case):
         ops.check_tc_status()
         for s in range(len(portions)):
             _check_reshaped(step, s, got, mask, 0.125, cap, slope, sink)
+
+
+def _tiny(**kw):
+    import bezasun_configs
+
+    return bezasun_configs.config(131, 64, 1e-5, [bezasun_configs.attention(4, 2, 16, 16, 0.25, mlp=None, **kw)])
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_steps_whose_pages_are_expanded_are_not_captured(bits):
+    """On the CPU: capped or biased scores over a 4-bit cache need the host's positions at every step; other steps do not."""
+    from hi_b200.config.registry import lookup
+    from hi_b200.parts.model import Model
+    from tiny_configs import TINY_A
+
+    def build(cfg):
+        arch = lookup(cfg)
+        return Model(arch.build_spec(arch.parse_config(cfg, None)), BF16, "cpu", cache_bits=bits)
+
+    for cfg in (_tiny(softcap=20.0), _tiny()):
+        model = build(cfg)
+        mixers = [layer.mixer for layer in model.layers]
+        assert all(m.softcap or m.distance_bias is not None for m in mixers)
+        assert model.graph_safe == (bits == 16)
+    assert build(TINY_A).graph_safe
+
+
+@pytest.mark.gpu
+def test_engine_steps_with_reshaped_scores(tmp_path):
+    """Decoding over several pages and across their ends, two and more requests: graphs asked for and not, and a cache in bfloat16 beside them."""
+    import bezasun_configs
+    import harness as h
+    from hi_b200.engine.core import Engine, StepEntry
+
+    mdir = str(tmp_path / "m")
+    bezasun_configs.write_model(mdir, _tiny(softcap=20.0), 4)
+    toks, other = ([(7 * i + s) % 128 for i in range(160)] for s in (1, 5))
+    runs = []
+    for graphs, bits in ((True, 4), (False, 4), (False, 16)):
+        eng = Engine.from_dir(mdir, kv_page_size=16, kv_cache_tokens=640, max_active_requests=4, kv_cache_bits=bits, use_cuda_graphs=graphs,
+                              graph_context_bucket=128)
+        out = [eng.step([StepEntry("a", toks[:70], [69])]), eng.step([StepEntry("b", other[:30], [29])])]
+        for i in range(40):
+            out.append(eng.step([StepEntry("a", [toks[70 + i]], [0]), StepEntry("b", [other[30 + i]], [0])]))
+        assert not eng._graphs
+        eng.snapshot()
+        runs.append(torch.cat(out).float().cpu())
+    assert torch.equal(runs[0], runs[1])
+    # what four bits do to the keys and values of one small layer; a wrong page gives logits that have nothing to do with these
+    assert runs[0].isfinite().all() and torch.corrcoef(torch.stack([runs[0].flatten(), runs[2].flatten()]))[0, 1] > 0.9
