@@ -59,7 +59,7 @@ int hb_expand_pages_4bit(const void* pages, const int* block_table, int table_st
 // how many pages that is (from the host's copies of the requests' positions), or -1
 long long hb_expand_total(const int* start_pos, const int* n_new, int n_seqs, int width, int page_size, int chunk, int window,
                           int keep, int skip_single);
-// attention of portions over it: pages expanded to float16 in the workspace (so many bytes of it), then the tcgen05 prefill kernels on them
+// attention of portions over it: pages expanded in the workspace (so many bytes of it), then the tcgen05 prefill kernels on them
 long long hb_prefill_attention_4bit_bytes(int total, int n_tokens, int n_seqs, int table_stride, int nh, int nkv, int hd,
                                           int page_size, int key_splits);
 int hb_prefill_attention_4bit(const void* q, const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
@@ -67,13 +67,14 @@ int hb_prefill_attention_4bit(const void* q, const void* pages, const int* block
                               int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
                               const float* sink_values, int key_splits, int one_tile, int total, void* workspace,
                               long long workspace_bytes, int* status, cudaStream_t stream);
-// q, k and v in float16, values of kv head h divided by v_factor[h] (attention_prefill_tc.cu)
-int hb_attention_prefill_tc_half(const void* q, const void* k_pages, const void* v_pages, const float* v_factor,
-                                 const int* block_table, int table_stride, const int* cu_seqlens, const int* positions,
-                                 void* out, int n_tokens, int n_pages, int n_seqs, int max_new, int nh, int nkv, int hd,
-                                 int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
-                                 const float* sink_values, int key_splits, float* part_acc, float* part_ml,
-                                 int one_tile, int* status, cudaStream_t stream);
+// q, k and v of request s and kv head h in float16 where form[s][h].y is not 0, else in bfloat16; values divided by form[s][h].x, scores of a
+// row to be multiplied by q_factor[token][head] (attention_prefill_tc.cu)
+int hb_attention_prefill_tc_mixed(const void* q, const void* k_pages, const void* v_pages, const float2* form, const float* q_factor,
+                                  const int* block_table, int table_stride, const int* cu_seqlens, const int* positions,
+                                  void* out, int n_tokens, int n_pages, int n_seqs, int max_new, int nh, int nkv, int hd,
+                                  int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
+                                  const float* sink_values, int key_splits, float* part_acc, float* part_ml,
+                                  int one_tile, int* status, cudaStream_t stream);
 // attention of single tokens over it; splits of split_tiles x 64 positions, brought together in a cluster (2 to 8)
 // or in part_acc and part_ml
 int hb_attention_decode_4bit(const void* q, const void* pages, const int* block_table, int table_stride,

@@ -67,6 +67,7 @@ struct Item {
 struct Work {
   Item x[2];
   int there, begin, end, p_end, seq, kvh, piece;
+  float2 form;                                                 // MIXED only
 };
 
 template <int HD>
@@ -87,6 +88,7 @@ __device__ __forceinline__ int first_visible(const PrefillPairArgs& a, int pos) 
 
 // The work of block (bx, by, bz) of the grid; false if there is none. A row that a share of the keys leaves out weighs nothing in
 // the merge: such an item has tokens and no tiles.
+template <bool MIXED>
 __device__ __forceinline__ bool work_of(const PrefillPairArgs& a, int bx, int by, int bz, Work& w) {
   const int group = a.nh / a.nkv, seq_begin = a.cu_seqlens[by], n_new = a.cu_seqlens[by + 1] - seq_begin;
   const int items = (n_new + BQ - 1) / BQ * group, first = 2 * ((items + 1) / 2 - 1 - bz);   // a request's last tokens first
@@ -97,6 +99,7 @@ __device__ __forceinline__ bool work_of(const PrefillPairArgs& a, int bx, int by
   w.seq = by;
   w.kvh = bx % a.nkv;
   w.piece = bx / a.nkv;
+  if constexpr (MIXED) w.form = a.form[(size_t)by * a.nkv + w.kvh];
   const int p0 = a.positions[seq_begin];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -129,8 +132,10 @@ __device__ __forceinline__ bool work_of(const PrefillPairArgs& a, int bx, int by
   return true;
 }
 
-// FP16: operands and P in float16, values scaled by a.v_factor
-template <int HD, bool FP16>
+template <bool B> struct Const { static constexpr bool value = B; };
+
+// MIXED: operands and P in float16 or bfloat16, by request and key head (a.form)
+template <int HD, bool MIXED>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const PrefillPairArgs a) {
@@ -188,7 +193,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     return boxes && key0 <= job.p_end ? a.block_table[(size_t)job.seq * a.table_stride + key0 / a.page_size] : -1;
   };
   if (warp == 8) {
-    if (!work_of(a, blockIdx.x, blockIdx.y, blockIdx.z, job)) job.there = 0;
+    if (!work_of<MIXED>(a, blockIdx.x, blockIdx.y, blockIdx.z, job)) job.there = 0;
     else if (job.begin < job.end) page = page_of(job.begin);
   }
   if (warp == 9) tc::alloc(tmem_slot, 512);
@@ -228,7 +233,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         some = got != 0;
-        if (!some || !work_of(a, bx, by, bz, job)) job.there = 0;
+        if (!some || !work_of<MIXED>(a, bx, by, bz, job)) job.there = 0;
         else if (job.begin < job.end) page = page_of(job.begin);
       };
       for (int w = 0; ok; ) {
@@ -309,8 +314,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (!ok && queries > 0) tc::mbar_wait_warp(q_full, (queries - 1) & 1);
       for (int i = max(0, n - STAGES); i < n; ++i) tc::mbar_wait_warp(ok ? &empty[i % STAGES] : &full[i % STAGES], (i / STAGES) & 1);
     } else if (warp == 9) {                     // ---- the products: the whole warp walks, one lane issues
-      constexpr uint32_t idesc_qk = FP16 ? tc::idesc_f16(BQ, BK, false) : tc::idesc_bf16(BQ, BK, false);
-      constexpr uint32_t idesc_pv = FP16 ? tc::idesc_f16(BQ, HD, true) : tc::idesc_bf16(BQ, HD, true);
+      uint32_t idesc_qk = tc::idesc_bf16(BQ, BK, false), idesc_pv = tc::idesc_bf16(BQ, HD, true);
       const uint32_t q_addr = tc::smem_u32(q_s), ring_addr = tc::smem_u32(ring);
       bool ok = true;
       int stage = 0, turn = 0, loads = 0, phase[2] = {0, 0};    // the ring's; Q tiles taken; P tiles taken of either item
@@ -335,6 +339,11 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           x_end[i] = tc::uniform(job.x[i].end);
           x_first[i] = tc::uniform(job.x[i].first);
           x_last[i] = tc::uniform(job.x[i].p_last);
+        }
+        if constexpr (MIXED) {
+          const bool half = tc::uniform(job.form.y != 0.f);
+          idesc_qk = half ? tc::idesc_f16(BQ, BK, false) : tc::idesc_bf16(BQ, BK, false);
+          idesc_pv = half ? tc::idesc_f16(BQ, HD, true) : tc::idesc_bf16(BQ, HD, true);
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&work_read[w & 1]);
@@ -424,12 +433,15 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const bool there = job.there;
       const Item x = job.x[i];
       const int piece = job.piece;
+      const float2 form = MIXED ? job.form : make_float2(1.f, 0.f);
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&work_read[w & 1]);
       if (!there) break;
       const bool row_ok = r < x.n_valid;
       const int pos = x.p_first + r, warp_first = x.p_first + (warp & 3) * 32;
       const int lo = first_visible(a, pos), warp_lo = first_visible(a, warp_first + 31);
+      float scale_log2 = a.scale_log2;
+      if constexpr (MIXED) scale_log2 *= row_ok ? a.q_factor[(size_t)(x.tok0 + r) * a.nh + x.head] : 1.f;
       // rows without a token start above every score, so they never move the maximum
       float m = row_ok ? -INFINITY : INFINITY, l = 0.f;
       for (int j = x.begin; j < x.end; ++j, ++phase) {
@@ -460,7 +472,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
           for (int c = 0; c < BK; ++c) sv[c] = c >= least ? sv[c] : -INFINITY;
         }
-        const float mx = fmaxf(m, row_max(sv) * a.scale_log2);           // the scale is positive
+        const float mx = fmaxf(m, row_max(sv) * scale_log2);           // the scale is positive
         // The exponentials are taken against `m`, which follows the maximum only when a row of the warp has grown by more than 2^8:
         // P stays below 256 and most tiles leave O as it is. A row that has seen nothing yet has nothing to move to.
         const bool move = __any_sync(0xffffffffu, mx > m + 8.f);
@@ -480,8 +492,9 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
         }
         const float base = m == -INFINITY ? 0.f : -m;                    // of a row that has seen nothing: 2^-inf = 0 all the same
-        const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(base, base);
+        const float2 scale2 = make_float2(scale_log2, scale_log2), base2 = make_float2(base, base);
         float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        auto weigh = [&](auto half) {
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
           uint32_t packed[16];
@@ -491,7 +504,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const float2 y = __ffma2_rn(make_float2(sv[at], sv[at + 1]), scale2, base2);
             const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));
             part[c & 1] = __fadd2_rn(part[c & 1], p);
-            packed[c] = tc::pack16<FP16>(p.x, p.y);
+            packed[c] = tc::pack16<decltype(half)::value>(p.x, p.y);
           }
           tc::st16_nowait(s_addr + 16 * h, packed);
           if (32 * (h + 1) == EARLY || 32 * (h + 1) == BK) {
@@ -501,6 +514,9 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (lane == 0) tc::mbar_arrive(32 * (h + 1) == BK ? &p_rest[i] : &p_ready[i]);
           }
         }
+        };
+        if (MIXED && form.y != 0.f) weigh(Const<true>());
+        else weigh(Const<false>());
         const float2 both = __fadd2_rn(part[0], part[1]);
         l = l * corr + (both.x + both.y);
       }
@@ -518,7 +534,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         break;
       }
       tc::fence_after();
-      const float factor = FP16 ? a.v_factor[x.head / (a.nh / a.nkv)] : 1.f;
+      const float factor = form.x;
       if (a.key_splits > 1) {
         // this share of the keys only: the row as it is, with its maximum and sum, for the merge
         const size_t at = ((size_t)(x.tok0 + r) * a.nh + x.head) * a.key_splits + piece;
@@ -531,7 +547,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           uint32_t o[32];
           tc::ld32_nowait(o_addr + c, o);
           tc::wait_ld();
-          if constexpr (FP16)
+          if constexpr (MIXED)
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
 #pragma unroll
@@ -587,7 +603,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   }
 }
 
-template <int HD, bool FP16>
+template <int HD, bool MIXED>
 int launch(const void* q, const void* k_pages, const void* v_pages, const PrefillPairArgs& a, int n_tokens, long long pool_rows,
            int n_seqs, int max_new, cudaStream_t stream) {
   CUtensorMap mq, mk, mv;
@@ -596,11 +612,11 @@ int launch(const void* q, const void* k_pages, const void* v_pages, const Prefil
       !tc::make_map_bf16(&mv, v_pages, (uint64_t)pool_rows, HD, a.box_rows))
     return HB_ERR_UNSUPPORTED;
   const size_t smem = Layout<HD>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute(attn_prefill_pair_kernel<HD, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(attn_prefill_pair_kernel<HD, MIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   const long long pairs = ((long long)((max_new + BQ - 1) / BQ) * (a.nh / a.nkv) + 1) / 2;
   if (pairs > 65535 || n_seqs > 65535 || (long long)a.nkv * a.key_splits > 0x7fffffffLL) return HB_ERR_UNSUPPORTED;
-  attn_prefill_pair_kernel<HD, FP16><<<dim3(a.nkv * a.key_splits, n_seqs, (unsigned)pairs), THREADS, smem, stream>>>(mq, mk, mv, a);
+  attn_prefill_pair_kernel<HD, MIXED><<<dim3(a.nkv * a.key_splits, n_seqs, (unsigned)pairs), THREADS, smem, stream>>>(mq, mk, mv, a);
   HB_LAUNCH_CHECK();
   return HB_OK;
 }
@@ -609,8 +625,8 @@ int launch(const void* q, const void* k_pages, const void* v_pages, const Prefil
 
 int hb_prefill_pair_launch(const void* q, const void* k_pages, const void* v_pages, const PrefillPairArgs& a, int n_tokens,
                            long long pool_rows, int n_seqs, int max_new, int hd, cudaStream_t stream) {
-  if (hd == 128 && a.v_factor) return launch<128, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
-  if (hd == 64 && a.v_factor) return launch<64, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
+  if (hd == 128 && a.form) return launch<128, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
+  if (hd == 64 && a.form) return launch<64, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
   if (hd == 128) return launch<128, false>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
   if (hd == 64) return launch<64, false>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
   return HB_ERR_UNSUPPORTED;

@@ -18,8 +18,10 @@ struct PrefillPairArgs {
   float* part_ml;
   int sink;                  // 1: the denominator has one more term, e^0, or e^sink_values[head]
   const float* sink_values;
-  // not null: q, k and v are float16 (four_bit_cache.cu), and the values of kv head h have been divided by v_factor[h]
-  const float* v_factor;
+  // not null: requests and kv heads have forms of their own (four_bit_cache.cu). form[seq][kv head]: what the values have been divided by, and
+  // 1 for q, k and v in float16; q_factor[token][head]: what a row's scores are multiplied by
+  const float2* form;
+  const float* q_factor;
 };
 
 // head_dim 64 or 128; HB_ERR_UNSUPPORTED for others

@@ -105,15 +105,16 @@ struct Args {
   int newest_first;
   int keep;                  // a sliding window's kept first tokens
   Pair pair;                 // kPair only
-  const float* v_factor;     // FP16 only: the values of kv head h have been divided by v_factor[h]
+  const float2* form;        // MIXED only: see PrefillPairArgs
+  const float* q_factor;
 };
 
-// FP16: operands and P in float16
-template <int HD, bool kPair, bool FP16>
+// MIXED: operands and P in float16 or bfloat16, by request and key head (a.form)
+template <int HD, bool kPair, bool MIXED>
 __global__ void __launch_bounds__(THREADS, 2)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const Args a) {
-  static_assert(!(kPair && FP16), "two maps side by side come in bfloat16");
+  static_assert(!(kPair && MIXED), "two maps side by side come in bfloat16");
   constexpr int DBLK = HD / 64;                 // 64-dim blocks of a row
   constexpr int QBYTES = BQ * HD * 2, KBYTES = BKEYS * HD * 2;
   constexpr int QBLOCK = BQ * 128;              // bytes of one [128 rows x 64 elements] swizzled block of Q
@@ -173,6 +174,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     return;
   }
   const int kvh = (kPair ? 2 * h : h) / (a.nh / a.nkv);
+  const float2 form = MIXED ? a.form[(size_t)seq * a.nkv + kvh] : make_float2(1.f, 0.f);
+  const bool half = MIXED && tc::uniform(form.y != 0.f);
   const int p_first = a.positions[tok0];
   const int p_last = p_first + n_valid - 1;
   auto first_visible = [&](int pos) {
@@ -262,8 +265,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     }
   } else if (warp == 1) {
     // ---- MMA issuer: S_j = Q K_j^T, then O += P_{j-1} V_{j-1}; the whole warp walks, one lane issues
-    constexpr uint32_t idesc_qk = FP16 ? tc::idesc_f16(BQ, BKEYS, false) : tc::idesc_bf16(BQ, BKEYS, false);
-    constexpr uint32_t idesc_pv = FP16 ? tc::idesc_f16(BQ, HD, true) : tc::idesc_bf16(BQ, HD, true);
+    const uint32_t idesc_qk = half ? tc::idesc_f16(BQ, BKEYS, false) : tc::idesc_bf16(BQ, BKEYS, false);
+    const uint32_t idesc_pv = half ? tc::idesc_f16(BQ, HD, true) : tc::idesc_bf16(BQ, HD, true);
     bool ok = true;
     auto wait = [&](uint64_t* bar, int parity, int code) {
       if (ok && !tc::mbar_wait_warp(bar, parity)) {
@@ -327,7 +330,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const float bias_log2 = (sigmoid && a.head_bias) ? a.head_bias[h] * 1.4426950408889634f : 0.f;
     // reshaped scores are brought to units of log 2 first and the code below then takes them with a scale of one
     const bool reshaped = a.softcap > 0.f || a.slopes != nullptr;
-    const float scale_l2 = reshaped ? 1.f : a.scale_log2;
+    float scale_l2 = reshaped ? 1.f : a.scale_log2;
+    if constexpr (MIXED) scale_l2 *= row_ok ? a.q_factor[(size_t)(tok0 + row) * a.nh + h] : 1.f;     // (never reshaped)
     const float slope_l2 = a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
     const float cap_l2 = a.softcap * 1.4426950408889634f;
     const float twice_over_cap = a.softcap > 0.f ? 2.f * a.scale_log2 / a.softcap : 0.f;
@@ -466,9 +470,12 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       // columns ran before the Q K^T that refilled them (one thread issues them, in that order).
       {
         uint32_t packed[BKEYS / 2];
+        if (half) {
 #pragma unroll
-        for (int i = 0; i < BKEYS / 2; ++i) {
-          packed[i] = tc::pack16<FP16>(sv[2 * i], sv[2 * i + 1]);
+          for (int i = 0; i < BKEYS / 2; ++i) packed[i] = tc::pack16<true>(sv[2 * i], sv[2 * i + 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < BKEYS / 2; ++i) packed[i] = tc::pack16<false>(sv[2 * i], sv[2 * i + 1]);
         }
         tc::st32_nowait(tmem + lane_addr + sb * S_COLS, packed);
         tc::wait_st();
@@ -653,9 +660,9 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             uint32_t o[32];
             tc::ld32_nowait(tmem_o + lane_addr + c, o);
             tc::wait_ld();
-            if constexpr (FP16)
+            if constexpr (MIXED)
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a.v_factor[h / (a.nh / a.nkv)]);
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * form.x);
 #pragma unroll
             for (int i = 0; i < 32; i += 16) {
               uint4 v[4];
@@ -673,7 +680,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           }
         } else {
         if (a.sink && l > 0.f) l += exp2f((a.sink_values ? a.sink_values[h] * 1.4426950408889634f : 0.f) - m);   // m is in units of log 2
-        const float inv = (l > 0.f ? 1.f / l : 0.f) * (FP16 ? a.v_factor[h / (a.nh / a.nkv)] : 1.f);
+        const float inv = (l > 0.f ? 1.f / l : 0.f) * form.x;
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           float o[32];
@@ -708,7 +715,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   }
 }
 
-template <int HD, bool kPair = false, bool FP16 = false>
+template <int HD, bool kPair = false, bool MIXED = false>
 int launch(const void* q, const void* k_pages, const void* v_pages, const Args& a, int n_tokens, long long pool_rows,
            int n_seqs, int max_new, cudaStream_t stream) {
   CUtensorMap mq, mk, mv;
@@ -717,14 +724,14 @@ int launch(const void* q, const void* k_pages, const void* v_pages, const Args& 
       !tc::make_map_bf16(&mv, v_pages, (uint64_t)pool_rows, HD, a.box_rows))
     return HB_ERR_UNSUPPORTED;
   const size_t smem = (size_t)BQ * HD * 2 + (KST + 2) * (size_t)BKEYS * HD * 2 + 256;
-  cudaError_t e = cudaFuncSetAttribute(attn_prefill_tc_kernel<HD, kPair, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(attn_prefill_tc_kernel<HD, kPair, MIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   const int tokens = kPair ? BQ / 2 : BQ;
   const int q_tiles = (max_new + tokens - 1) / tokens;
   if (q_tiles > 65535 || n_seqs > 65535) return HB_ERR_UNSUPPORTED;
   if ((long long)a.nh * a.key_splits > 0x7fffffffLL) return HB_ERR_UNSUPPORTED;
   dim3 grid((kPair ? a.nh / 2 : a.nh) * a.key_splits, q_tiles, n_seqs);
-  attn_prefill_tc_kernel<HD, kPair, FP16><<<grid, THREADS, smem, stream>>>(mq, mk, mv, a);
+  attn_prefill_tc_kernel<HD, kPair, MIXED><<<grid, THREADS, smem, stream>>>(mq, mk, mv, a);
   HB_LAUNCH_CHECK();
   return HB_OK;
 }
@@ -743,7 +750,7 @@ int prefill_tc(const void* q, const void* k_pages, const void* v_pages, const in
                int nh, int nkv, int hd, int page_size, int chunk, int window, float scale, int skip_single, int sink,
                const float* head_bias, int key_splits, float* part_acc, float* part_ml, int* status, int turn_inside,
                const float* v_inv_freq, int v_pairs, int v_interleaved, float softcap, const float* slopes,
-               const float* sink_values, int keep, const Pair* pair, int one_tile, const float* v_factor, cudaStream_t stream);
+               const float* sink_values, int keep, const Pair* pair, int one_tile, const float2* form, const float* q_factor, cudaStream_t stream);
 }  // namespace
 
 // one_tile: plain softmax rows of 64 and 128 too go one query tile a block (ops.prefill_one_tile says where that is faster)
@@ -755,7 +762,7 @@ extern "C" int hb_attention_prefill_tc(const void* q, const void* k_pages, const
                                        float* part_ml, int one_tile, int* status, cudaStream_t stream) {
   return prefill_tc(q, k_pages, v_pages, block_table, table_stride, cu_seqlens, positions, out, n_tokens, n_pages, n_seqs,
                     max_new, nh, nkv, hd, page_size, chunk, window, scale, skip_single, sink, head_bias, key_splits,
-                    part_acc, part_ml, status, 0, nullptr, 0, 0, 0.f, nullptr, nullptr, 0, nullptr, one_tile, nullptr, stream);
+                    part_acc, part_ml, status, 0, nullptr, 0, 0, 0.f, nullptr, nullptr, 0, nullptr, one_tile, nullptr, nullptr, stream);
 }
 
 // The same with reshaped scores (see Args): a cap, a distance bias per head, a sink with a score per head.
@@ -768,20 +775,20 @@ extern "C" int hb_attention_prefill_tc_reshaped(const void* q, const void* k_pag
                                                 float* part_acc, float* part_ml, int one_tile, int* status, cudaStream_t stream) {
   return prefill_tc(q, k_pages, v_pages, block_table, table_stride, cu_seqlens, positions, out, n_tokens, n_pages, n_seqs,
                     max_new, nh, nkv, hd, page_size, chunk, window, scale, skip_single, sink, nullptr, key_splits,
-                    part_acc, part_ml, status, 0, nullptr, 0, 0, softcap, slopes, sink_values, keep, nullptr, one_tile, nullptr, stream);
+                    part_acc, part_ml, status, 0, nullptr, 0, 0, softcap, slopes, sink_values, keep, nullptr, one_tile, nullptr, nullptr, stream);
 }
 
-// q, k and v in float16, the values of kv head h divided by v_factor[h] (hb_prefill_attention_4bit makes them); hd 64 or 128.
-extern "C" int hb_attention_prefill_tc_half(const void* q, const void* k_pages, const void* v_pages, const float* v_factor,
-                                            const int* block_table, int table_stride, const int* cu_seqlens, const int* positions,
-                                            void* out, int n_tokens, int n_pages, int n_seqs, int max_new, int nh, int nkv, int hd,
-                                            int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
-                                            const float* sink_values, int key_splits, float* part_acc, float* part_ml,
-                                            int one_tile, int* status, cudaStream_t stream) {
-  if (!v_factor || sink < 0 || sink > 1) return HB_ERR_BAD_ARG;
+// q, k and v by request and key head in float16 or bfloat16 (hb_prefill_attention_4bit makes them); hd 64 or 128.
+extern "C" int hb_attention_prefill_tc_mixed(const void* q, const void* k_pages, const void* v_pages, const float2* form, const float* q_factor,
+                                             const int* block_table, int table_stride, const int* cu_seqlens, const int* positions,
+                                             void* out, int n_tokens, int n_pages, int n_seqs, int max_new, int nh, int nkv, int hd,
+                                             int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
+                                             const float* sink_values, int key_splits, float* part_acc, float* part_ml,
+                                             int one_tile, int* status, cudaStream_t stream) {
+  if (!form || !q_factor || sink < 0 || sink > 1) return HB_ERR_BAD_ARG;
   return prefill_tc(q, k_pages, v_pages, block_table, table_stride, cu_seqlens, positions, out, n_tokens, n_pages, n_seqs,
                     max_new, nh, nkv, hd, page_size, chunk, window, scale, skip_single, sink, nullptr, key_splits,
-                    part_acc, part_ml, status, 0, nullptr, 0, 0, 0.f, nullptr, sink_values, keep, nullptr, one_tile, v_factor, stream);
+                    part_acc, part_ml, status, 0, nullptr, 0, 0, 0.f, nullptr, sink_values, keep, nullptr, one_tile, form, q_factor, stream);
 }
 
 // Sigmoid weights with the result written by the kernel itself: `out` [n_tokens, nh, hd] bfloat16 takes every
@@ -798,7 +805,7 @@ extern "C" int hb_sigmoid_prefill_tc(const void* q, const void* k_pages, const v
   if (v_pairs > 0 && !v_interleaved && 2 * v_pairs != hd) return HB_ERR_UNSUPPORTED;
   return prefill_tc(q, k_pages, v_pages, block_table, table_stride, cu_seqlens, positions, out, n_tokens, n_pages, n_seqs,
                     max_new, nh, nkv, hd, page_size, chunk, window, scale, skip_single, 2, head_bias, 1, nullptr, nullptr,
-                    status, 1, v_inv_freq, v_pairs, v_interleaved, 0.f, nullptr, nullptr, 0, nullptr, 1, nullptr, stream);
+                    status, 1, v_inv_freq, v_pairs, v_interleaved, 0.f, nullptr, nullptr, 0, nullptr, 1, nullptr, nullptr, stream);
 }
 
 // Differential attention: q [n_tokens, nh, hd] holds the two maps of head a as heads 2a and 2a + 1, both over the same
@@ -817,7 +824,7 @@ extern "C" int hb_diff_prefill_tc(const void* q, const void* k_pages, const void
   const Pair pair{lambda, eps, mul, vdim, vec ? 1 : 0, (const __nv_bfloat16*)gate, gate_stride};
   return prefill_tc(q, k_pages, v_pages, block_table, table_stride, cu_seqlens, positions, out, n_tokens, n_pages, n_seqs,
                     max_new, nh, nkv, hd, page_size, chunk, window, scale, skip_single, 0, nullptr, 1, nullptr, nullptr,
-                    status, 0, nullptr, 0, 0, 0.f, nullptr, nullptr, keep, &pair, 1, nullptr, stream);
+                    status, 0, nullptr, 0, 0, 0.f, nullptr, nullptr, keep, &pair, 1, nullptr, nullptr, stream);
 }
 
 namespace {
@@ -826,7 +833,7 @@ int prefill_tc(const void* q, const void* k_pages, const void* v_pages, const in
                int nh, int nkv, int hd, int page_size, int chunk, int window, float scale, int skip_single, int sink,
                const float* head_bias, int key_splits, float* part_acc, float* part_ml, int* status, int turn_inside,
                const float* v_inv_freq, int v_pairs, int v_interleaved, float softcap, const float* slopes,
-               const float* sink_values, int keep, const Pair* pair, int one_tile, const float* v_factor, cudaStream_t stream) {
+               const float* sink_values, int keep, const Pair* pair, int one_tile, const float2* form, const float* q_factor, cudaStream_t stream) {
   if (sink == 2 && (softcap > 0.f || slopes || sink_values)) return HB_ERR_UNSUPPORTED;
   if (!q || !k_pages || !v_pages || !block_table || !cu_seqlens || !positions || !out || !status) return HB_ERR_BAD_ARG;
   if (n_tokens < 0 || n_pages <= 0 || n_seqs < 0 || max_new < 0 || nh <= 0 || nkv <= 0 || nh % nkv != 0 ||
@@ -840,13 +847,13 @@ int prefill_tc(const void* q, const void* k_pages, const void* v_pages, const in
   if (n_seqs == 0 || max_new == 0 || n_tokens == 0) return HB_OK;
   Args a{block_table, cu_seqlens, positions, (__nv_bfloat16*)out, status, table_stride, nh, nkv, page_size, chunk,
          window, skip_single, page_size < BKEYS ? page_size : BKEYS, scale * 1.4426950408889634f, key_splits, part_acc, part_ml, sink, head_bias,
-         turn_inside, v_pairs, v_interleaved, v_inv_freq, softcap, slopes, sink_values, slopes ? 1 : 0, keep, pair ? *pair : Pair{}, v_factor};
+         turn_inside, v_pairs, v_interleaved, v_inv_freq, softcap, slopes, sink_values, slopes ? 1 : 0, keep, pair ? *pair : Pair{}, form, q_factor};
   const long long pool_rows = (long long)n_pages * nkv * page_size;
   // (a launch of more pairs than a grid holds goes one tile a block)
   const long long pairs = ((max_new + 127LL) / 128 * (nh / nkv) + 1) / 2;
   if (!one_tile && !pair && !turn_inside && sink != 2 && softcap <= 0.f && !slopes && keep == 0 && hd <= 128 && pairs <= 65535) {
     const PrefillPairArgs b{block_table, cu_seqlens, positions, (__nv_bfloat16*)out, status, table_stride, nh, nkv, page_size, chunk, window,
-                            skip_single, a.box_rows, a.scale_log2, key_splits, part_acc, part_ml, sink, sink_values, v_factor};
+                            skip_single, a.box_rows, a.scale_log2, key_splits, part_acc, part_ml, sink, sink_values, form, q_factor};
     return hb_prefill_pair_launch(q, k_pages, v_pages, b, n_tokens, pool_rows, n_seqs, max_new, hd, stream);
   }
   if (pair) {
@@ -855,7 +862,7 @@ int prefill_tc(const void* q, const void* k_pages, const void* v_pages, const in
     if (hd == 64) return launch<64, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
     return HB_ERR_UNSUPPORTED;
   }
-  if (v_factor) {
+  if (form) {
     if (hd == 128) return launch<128, false, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
     if (hd == 64) return launch<64, false, true>(q, k_pages, v_pages, a, n_tokens, pool_rows, n_seqs, max_new, stream);
     return HB_ERR_UNSUPPORTED;

@@ -208,16 +208,17 @@ struct Expand {
   const int* block_table;
   const int* cu_seqlens;
   const int* positions;
-  uint16_t* k;                     // bfloat16, or float16
+  uint16_t* k;                     // bfloat16, or for the prefill kernels float16
   uint16_t* v;
   int* table;
   int n_seqs, table_stride, page_size, chunk, window, keep, skip_single, nkv, total;
-  // float16 only
+  // for the prefill kernels only
   const __nv_bfloat16* q;
   int n_tokens, nh;
-  int* most;                       // [nkv][keys, values]
-  uint16_t* q_half;
-  float* v_factor;
+  int4* most;                      // [n_seqs][nkv]: see most_4bit_kernel
+  uint16_t* q_out;
+  float* q_factor;                 // [n_tokens][nh]
+  float2* form;                    // [n_seqs][nkv]: what the values have been divided by, 1 for float16
   int* status;
 };
 
@@ -245,11 +246,12 @@ __device__ __forceinline__ int all_pages(const Expand& a) {
 }
 
 // The request and its page that page `out_page` of the result is; false: none (or the table has no such page). A whole block asks.
-__device__ __forceinline__ bool find_page(const Expand& a, int out_page, int& seq, int& index) {
-  __shared__ int found[2];
+// `leads`: it is the request's first.
+__device__ __forceinline__ bool find_page(const Expand& a, int out_page, int& seq, int& index, bool& leads) {
+  __shared__ int found[3];
   const int lane = threadIdx.x & 31;
   if (threadIdx.x < 32) {          // the requests' counts are summed 32 at a time
-    int before = 0, who_seq = -1, at = 0;
+    int before = 0, who_seq = -1, at = 0, led = 0;
     for (int s0 = 0; s0 < a.n_seqs && who_seq < 0; s0 += 32) {
       int first = 0, count = 0;
       if (s0 + lane < a.n_seqs) span(a, s0 + lane, first, count);
@@ -262,94 +264,142 @@ __device__ __forceinline__ bool find_page(const Expand& a, int out_page, int& se
       const unsigned hit = __ballot_sync(0xffffffffu, before + upto > out_page);
       const int who = hit ? __ffs(hit) - 1 : 0;
       const int start = __shfl_sync(0xffffffffu, before + upto - count, who), from = __shfl_sync(0xffffffffu, first, who);
-      if (hit) { who_seq = s0 + who; at = from + out_page - start; }
+      if (hit) { who_seq = s0 + who; at = from + out_page - start; led = out_page == start; }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    if (lane == 0) { found[0] = who_seq; found[1] = at; }
+    if (lane == 0) { found[0] = who_seq; found[1] = at; found[2] = led; }
   }
   __syncthreads();
   seq = found[0];
   index = found[1];
+  leads = found[2];
   return seq >= 0 && index < a.table_stride;
 }
 __device__ __forceinline__ float number(const uint8_t* p) { return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p)); }
 
-// The largest magnitudes of a kv head's keys and values on the pages (of rows that are there; a group's ends: its low and fifteen steps
-// above it; one atomic a block, and none where it changes nothing: 29 us for 144 pages of 8 heads with one a warp, 7 so), as the bits of floats, whose order is theirs: the least power of two above one divides the head's numbers, so that float16 holds
-// them to 2^-11 of their size, or 2^-25 of the largest one's where they are small.
+// ---- for the tcgen05 prefill kernels: float16, which keeps 11 of a cached value's up to 13 bits where bfloat16 keeps 8. Keys and values of a
+// request's kv head are divided by the least power of two above the largest of them, so float16 holds a group to 2^-11 of its largest
+// magnitude where that is at least 2^-14 of the head's. A request with a smaller one, or with a largest one out of 2^-100 .. 2^100, is
+// expanded to bfloat16 for that head instead, and its products are taken in it. What a request's result is rounded to depends on its own rows
+// alone. A query's row of a head is multiplied by a power of two of its own, which the scores' scale takes back: it keeps all bits of elements
+// down to 2^-32 of its largest.
+//
+// The magnitudes of a request's kv head on the pages, of rows that are there (a group's ends: its low and fifteen steps above it): one atomic a
+// block and number, and none where it changes nothing (29 us for 144 pages of 8 heads with one a warp, 7 so). `most` holds the bits of floats, whose
+// order is theirs: keys' largest, keys' smallest group's above zero (taken from that of infinity, so that it only grows too), then values'; -1: none.
 constexpr int EXPAND_THREADS = 512, MOST_THREADS = 128;
 
 template <int G>
 __global__ void __launch_bounds__(MOST_THREADS) most_4bit_kernel(const Expand a) {
   using B = fb::Block<G>;
+  constexpr int INFINITE = 0x7f800000;
   const int kvh = blockIdx.y;
   int seq, index;
-  if (!find_page(a, blockIdx.x, seq, index)) return;
+  bool leads;
+  if (!find_page(a, blockIdx.x, seq, index, leads)) return;
   const int page = a.block_table[(size_t)seq * a.table_stride + index];
   if (page < 0) return;
   const int begin = a.cu_seqlens[seq], last = a.positions[begin] + a.cu_seqlens[seq + 1] - begin - 1;
   const int rows = min(a.page_size, last - index * a.page_size + 1);
   const uint8_t* from = a.pages + ((size_t)page * a.nkv + kvh) * (a.page_size / fb::BLOCK_ROWS) * B::BYTES;
-  float k_most = 0.f, v_most = 0.f;
+  float k_most = 0.f, k_least = INFINITY, v_most = 0.f, v_least = INFINITY;
+  auto take = [](float low, float scale, float& most, float& least) {
+    const float size = fmaxf(fabsf(low), fabsf(fmaf(scale, 15.f, low)));      // (of a group of NaN: NaN)
+    most = fmaxf(most, size);
+    if (size > 0.f) least = fminf(least, size);
+  };
   for (int i = threadIdx.x; i < rows * G; i += blockDim.x) {
     const int row = i / G, r = row % fb::BLOCK_ROWS, group = i % G;
     const uint8_t* block = from + row / fb::BLOCK_ROWS * B::BYTES;
-    const float k = number(block + B::key_low(r, group)), v = number(block + B::value_low(r, group));
-    k_most = fmaxf(k_most, fmaxf(fabsf(k), fabsf(fmaf(number(block + B::scale(r, 0, group)), 15.f, k))));
-    v_most = fmaxf(v_most, fmaxf(fabsf(v), fabsf(fmaf(number(block + B::scale(r, 1, group)), 15.f, v))));
+    take(number(block + B::key_low(r, group)), number(block + B::scale(r, 0, group)), k_most, k_least);
+    take(number(block + B::value_low(r, group)), number(block + B::scale(r, 1, group)), v_most, v_least);
   }
-  k_most = hb::warp_max(k_most);
-  v_most = hb::warp_max(v_most);
-  __shared__ float both[2][MOST_THREADS / 32];
-  if (threadIdx.x % 32 == 0) { both[0][threadIdx.x / 32] = k_most; both[1][threadIdx.x / 32] = v_most; }
+  __shared__ int all[4][MOST_THREADS / 32];
+  const int mine[4] = {__reduce_max_sync(0xffffffffu, __float_as_int(k_most)), __reduce_max_sync(0xffffffffu, INFINITE - __float_as_int(k_least)),
+                       __reduce_max_sync(0xffffffffu, __float_as_int(v_most)), __reduce_max_sync(0xffffffffu, INFINITE - __float_as_int(v_least))};
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+    if (threadIdx.x % 32 == n) all[n][threadIdx.x / 32] = mine[n];
   __syncthreads();
-  if (threadIdx.x < 2) {
-    float most = 0.f;
-    for (int w = 0; w < MOST_THREADS / 32; ++w) most = fmaxf(most, both[threadIdx.x][w]);
-    int* to = a.most + 2 * kvh + threadIdx.x;
-    if (__float_as_int(most) > *reinterpret_cast<volatile int*>(to)) atomicMax(to, __float_as_int(most));      // it only grows
+  if (threadIdx.x < 4) {
+    int most = 0;
+    for (int w = 0; w < MOST_THREADS / 32; ++w) most = max(most, all[threadIdx.x][w]);
+    int* to = reinterpret_cast<int*>(a.most + (size_t)seq * a.nkv + kvh) + threadIdx.x;
+    if (most > *reinterpret_cast<volatile int*>(to)) atomicMax(to, most);      // it only grows
   }
 }
-// two to the power that is the least above a magnitude of these bits, within what a float can be divided by
-__device__ __forceinline__ int power_above(int bits) {
-  const int e = (bits >> 23) - 126;
-  return bits == 0 ? 0 : max(-100, min(e, 120));
+// two to the power that is the least above a magnitude of these bits (of a normal float); of zero and none: 0
+__device__ __forceinline__ int power_above(int bits) { return bits <= 0 ? 0 : (bits >> 23) - 126; }
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((max(-126, min(e, 127)) + 127) << 23); }
+
+// How a request's kv head is held: float16, keys and values divided by 2^k and 2^v, or (half false) bfloat16.
+struct Held { bool half; int k, v; };
+__device__ __forceinline__ Held held(const int4& most) {
+  auto fits = [](int largest, int smallest) {                      // as `most` has them
+    const int e = power_above(largest), least = 0x7f800000 - smallest;
+    return largest <= 0 || (e >= -100 && e <= 100 && (largest >> 23) - (least >> 23) <= 13);
+  };
+  if (!fits(most.x, most.y) || !fits(most.z, most.w)) return Held{false, 0, 0};
+  return Held{true, power_above(most.x), power_above(most.z)};
 }
-__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
-// a float as float16, a finite one too large for it as its largest
-__device__ __forceinline__ float held(float x) { return fabsf(x) > 65504.f && fabsf(x) < INFINITY ? copysignf(65504.f, x) : x; }
+__device__ __forceinline__ uint32_t pack_as(bool half, float lo, float hi) { return half ? tc::pack16<true>(lo, hi) : tc::pack16<false>(lo, hi); }
 
 constexpr int Q_TOKENS = 8;        // of a block that converts queries
 
-template <int G, bool FP16>
+// PREFILL: in the form that `most` asks for, and the queries beside it; else bfloat16
+template <int G, bool PREFILL>
 __global__ void __launch_bounds__(EXPAND_THREADS) expand_4bit_kernel(const Expand a) {
   constexpr int HD = 32 * G;
   using B = fb::Block<G>;
   const int out_page = blockIdx.x, kvh = blockIdx.y;
-  float k_down = 1.f, v_down = 1.f;
-  if constexpr (FP16) {
-    const int ek = power_above(a.most[2 * kvh]), ev = power_above(a.most[2 * kvh + 1]);
-    k_down = power_of_two(-ek);
-    v_down = power_of_two(-ev);
-    if (out_page == 0 && threadIdx.x == 0) a.v_factor[kvh] = power_of_two(ev);
-    if (out_page >= a.total) {     // queries of this kv head
-      const float up = power_of_two(ek - 8);
-      const int per = a.nh / a.nkv, t0 = (out_page - a.total) * Q_TOKENS, words = per * HD / 8;
-      for (int i = threadIdx.x; i < min(Q_TOKENS, a.n_tokens - t0) * words; i += blockDim.x) {
-        const size_t at = ((size_t)(t0 + i / words) * a.nh + kvh * per) * HD + i % words * 8;
-        float x[8];
+  if constexpr (PREFILL) {
+    if (out_page >= a.total) {       // queries of this kv head
+      __shared__ Held forms[Q_TOKENS];
+      const int per = a.nh / a.nkv, t0 = (out_page - a.total) * Q_TOKENS, tokens = min(Q_TOKENS, min(a.n_tokens, a.cu_seqlens[a.n_seqs]) - t0);
+      if ((int)threadIdx.x < tokens) {
+        int s = 0, end = a.n_seqs;                                  // the last request that does not begin behind the token
+        while (end - s > 1) {
+          const int mid = (s + end) / 2;
+          if (a.cu_seqlens[mid] <= t0 + (int)threadIdx.x) s = mid;
+          else end = mid;
+        }
+        forms[threadIdx.x] = held(a.most[(size_t)s * a.nkv + kvh]);
+      }
+      __syncthreads();
+      constexpr int WORDS = HD / 8;                                 // of a row, as many lanes
+      const unsigned row_lanes = (WORDS == 16 ? 0xffffu : 0xffu) << (threadIdx.x & 31 & ~(WORDS - 1));
+      for (int i = threadIdx.x; i < tokens * per * WORDS; i += blockDim.x) {
+        const int token = i / WORDS / per, head = kvh * per + i / WORDS % per;
+        const Held form = forms[token];
+        const size_t row = (size_t)(t0 + token) * a.nh + head, at = row * HD + i % WORDS * 8;
+        const uint4 raw = *reinterpret_cast<const uint4*>(a.q + at);
+        float x[8], most = 0.f;
         hb::load8(a.q + at, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
+#pragma unroll
+        for (int o = WORDS / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(row_lanes, most, o));
+        const int e_q = max(-100, power_above(__float_as_int(most)));
+        const float up = power_of_two(15 - e_q);                    // (an infinity stays one)
         unsigned o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = tc::pack16<true>(held(x[2 * e] * up), held(x[2 * e + 1] * up));
-        *reinterpret_cast<uint4*>(a.q_half + at) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int e = 0; e < 4; ++e) o[e] = tc::pack16<true>(x[2 * e] * up, x[2 * e + 1] * up);
+        *reinterpret_cast<uint4*>(a.q_out + at) = form.half ? make_uint4(o[0], o[1], o[2], o[3]) : raw;
+        if (i % WORDS == 0) a.q_factor[row] = form.half ? power_of_two(e_q - 15 + form.k) : 1.f;
       }
       return;
     }
   }
   int seq, index;
+  bool leads;
   if (out_page == 0 && kvh == 0 && threadIdx.x < 32 && all_pages(a) != a.total && threadIdx.x == 0) atomicExch(a.status, 33);
-  if (!find_page(a, out_page, seq, index)) return;
+  if (!find_page(a, out_page, seq, index, leads)) return;
+  Held form{false, 0, 0};
+  if constexpr (PREFILL) {
+    form = held(a.most[(size_t)seq * a.nkv + kvh]);
+    if (leads && threadIdx.x == 0) a.form[(size_t)seq * a.nkv + kvh] = make_float2(power_of_two(form.v), form.half ? 1.f : 0.f);
+  }
+  const float k_down = power_of_two(-form.k), v_down = power_of_two(-form.v);
   const int page = a.block_table[(size_t)seq * a.table_stride + index];
   if (kvh == 0 && threadIdx.x == 0) a.table[(size_t)seq * a.table_stride + index] = page < 0 ? -1 : out_page;
   const size_t out = ((size_t)out_page * a.nkv + kvh) * a.page_size * HD;
@@ -363,7 +413,7 @@ __global__ void __launch_bounds__(EXPAND_THREADS) expand_4bit_kernel(const Expan
     unsigned o[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      o[e] = tc::pack16<FP16>(fmaf(scale, (float)(w >> (4 * e) & 15), low), fmaf(scale, (float)(w >> (16 + 4 * e) & 15), low));
+      o[e] = pack_as(form.half, fmaf(scale, (float)(w >> (4 * e) & 15), low), fmaf(scale, (float)(w >> (16 + 4 * e) & 15), low));
     *reinterpret_cast<uint4*>(a.k + out + (size_t)row * HD + group * 32 + q * 8) = make_uint4(o[0], o[1], o[2], o[3]);
   }
   for (int i = threadIdx.x; i < a.page_size / 2 * 8 * G; i += blockDim.x) {  // four dims of the values of two tokens
@@ -375,8 +425,8 @@ __global__ void __launch_bounds__(EXPAND_THREADS) expand_4bit_kernel(const Expan
       const float scale = number(block + B::scale(r + e, 1, group)) * v_down, low = number(block + B::value_low(r + e, group)) * v_down;
       const unsigned c = w >> (16 * e);
       *reinterpret_cast<uint2*>(a.v + out + (size_t)(row + e) * HD + group * 32 + g * 4) = make_uint2(
-          tc::pack16<FP16>(fmaf(scale, (float)(c & 15), low), fmaf(scale, (float)(c >> 4 & 15), low)),
-          tc::pack16<FP16>(fmaf(scale, (float)(c >> 8 & 15), low), fmaf(scale, (float)(c >> 12 & 15), low)));
+          pack_as(form.half, fmaf(scale, (float)(c & 15), low), fmaf(scale, (float)(c >> 4 & 15), low)),
+          pack_as(form.half, fmaf(scale, (float)(c >> 8 & 15), low), fmaf(scale, (float)(c >> 12 & 15), low)));
     }
   }
 }
@@ -413,16 +463,18 @@ extern "C" int hb_qkv_post_4bit(const void* qkv, const float* inv_freq, int rot_
 }
 
 namespace {
-int expand(const Expand& a, int hd, bool half, cudaStream_t stream) {
+int expand(const Expand& a, int hd, bool prefill, cudaStream_t stream) {
   if (!a.pages || !a.block_table || !a.cu_seqlens || !a.positions || !a.table || !a.status || a.n_seqs < 0 || a.total < 0 || a.nkv <= 0 || a.table_stride <= 0 ||
       a.chunk < 0 || a.window < 0 || a.keep < 0 || (a.total > 0 && (!a.k || !a.v)))
     return HB_ERR_BAD_ARG;
   if ((hd != 64 && hd != 128) || !good_page(a.page_size) || a.nkv > 65535) return HB_ERR_UNSUPPORTED;
   if (a.n_seqs == 0 || a.total == 0) return HB_OK;
-  const cudaError_t e = cudaMemsetAsync(a.table, 0xff, (size_t)a.n_seqs * a.table_stride * 4, stream);      // -1
+  // the table's entries are -1, and (behind them) the magnitudes
+  const size_t unset = prefill ? (uint8_t*)(a.most + (size_t)a.n_seqs * a.nkv) - (uint8_t*)a.table : (size_t)a.n_seqs * a.table_stride * 4;
+  const cudaError_t e = cudaMemsetAsync(a.table, 0xff, unset, stream);
   if (e != cudaSuccess) return (int)e;
   const dim3 grid(a.total, a.nkv);
-  if (half) {
+  if (prefill) {
     const dim3 more(a.total + (a.n_tokens + Q_TOKENS - 1) / Q_TOKENS, a.nkv);
     if (hd == 128) most_4bit_kernel<4><<<grid, MOST_THREADS, 0, stream>>>(a);
     else most_4bit_kernel<2><<<grid, MOST_THREADS, 0, stream>>>(a);
@@ -444,23 +496,24 @@ extern "C" int hb_expand_pages_4bit(const void* pages, const int* block_table, i
                                     int skip_single, int nkv, int hd, void* k, void* v, int* table, int* status,
                                     cudaStream_t stream) {
   return expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)k, (uint16_t*)v, table, n_seqs,
-                       table_stride, page_size, chunk, window, keep, skip_single, nkv, total, nullptr, 0, 0, nullptr, nullptr, nullptr, status},
+                       table_stride, page_size, chunk, window, keep, skip_single, nkv, total, nullptr, 0, 0, nullptr, nullptr, nullptr, nullptr, status},
                 hd, false, stream);
 }
 
 // What hb_prefill_attention_4bit needs of its workspace, in order, each part on 1,024 bytes.
 namespace {
 struct Room {
-  size_t k, v, q_half, table, most, v_factor, part_acc, part_ml, all;
+  size_t k, v, q, q_factor, table, most, form, part_acc, part_ml, all;
   Room(int total, int n_tokens, int n_seqs, int table_stride, int nh, int nkv, int hd, int page_size, int key_splits) {
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 1023) / 1024 * 1024; return here; };
     k = take((size_t)total * nkv * page_size * hd * 2);
     v = take((size_t)total * nkv * page_size * hd * 2);
-    q_half = take((size_t)n_tokens * nh * hd * 2);
+    q = take((size_t)n_tokens * nh * hd * 2);
+    q_factor = take((size_t)n_tokens * nh * 4);
     table = take((size_t)n_seqs * table_stride * 4);
-    most = take((size_t)nkv * 8);
-    v_factor = take((size_t)nkv * 4);
+    most = take((size_t)n_seqs * nkv * 16);
+    form = take((size_t)n_seqs * nkv * 8);
     part_acc = take(key_splits > 1 ? (size_t)n_tokens * nh * key_splits * hd * 4 : 0);
     part_ml = take(key_splits > 1 ? (size_t)n_tokens * nh * key_splits * 8 : 0);
     all = at;
@@ -489,9 +542,8 @@ extern "C" long long hb_prefill_attention_4bit_bytes(int total, int n_tokens, in
   return (long long)Room(total, n_tokens, n_seqs, table_stride, nh, nkv, hd, page_size, key_splits).all;
 }
 
-// The pages in float16 (a 4-bit cache's values have up to 13 bits, of which bfloat16 keeps 8 and float16 11), keys and values divided by a
-// power of two per kv head that brings the largest of them under 1, q times the keys' over 256; then the tcgen05 prefill attention on them,
-// whose scores are a 256th of q k^T, and the merge of shared keys.
+// Pages and queries in the form that each request's kv head is held in (float16 or bfloat16, above), then the tcgen05 prefill attention on them
+// and the merge of shared keys.
 extern "C" int hb_prefill_attention_4bit(const void* q, const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
                                          const int* positions, void* out, int n_tokens, int n_seqs, int max_new, int nh, int nkv, int hd,
                                          int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
@@ -503,20 +555,18 @@ extern "C" int hb_prefill_attention_4bit(const void* q, const void* pages, const
   const Room room(total, n_tokens, n_seqs, table_stride, nh, nkv, hd, page_size, key_splits);
   if ((long long)room.all > workspace_bytes) return HB_ERR_BAD_ARG;
   uint8_t* w = static_cast<uint8_t*>(workspace);
-  int* most = reinterpret_cast<int*>(w + room.most);
-  float* v_factor = reinterpret_cast<float*>(w + room.v_factor);
-  const cudaError_t e = cudaMemsetAsync(most, 0, (size_t)nkv * 8, stream);
-  if (e != cudaSuccess) return (int)e;
+  float* q_factor = reinterpret_cast<float*>(w + room.q_factor);
+  float2* form = reinterpret_cast<float2*>(w + room.form);
   int* table = reinterpret_cast<int*>(w + room.table);
   int code = expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)(w + room.k), (uint16_t*)(w + room.v), table,
                            n_seqs, table_stride, page_size, chunk, window, keep, skip_single, nkv, total, (const __nv_bfloat16*)q, n_tokens, nh,
-                           most, (uint16_t*)(w + room.q_half), v_factor, status},
+                           (int4*)(w + room.most), (uint16_t*)(w + room.q), q_factor, form, status},
                     hd, true, stream);
   if (code != HB_OK) return code;
   float* part_acc = key_splits > 1 ? reinterpret_cast<float*>(w + room.part_acc) : nullptr;
   float* part_ml = key_splits > 1 ? reinterpret_cast<float*>(w + room.part_ml) : nullptr;
-  code = hb_attention_prefill_tc_half(w + room.q_half, w + room.k, w + room.v, v_factor, table, table_stride, cu_seqlens, positions, out,
-                                      n_tokens, total, n_seqs, max_new, nh, nkv, hd, page_size, chunk, window, keep, 256.f * scale, skip_single,
+  code = hb_attention_prefill_tc_mixed(w + room.q, w + room.k, w + room.v, form, q_factor, table, table_stride, cu_seqlens, positions, out,
+                                      n_tokens, total, n_seqs, max_new, nh, nkv, hd, page_size, chunk, window, keep, scale, skip_single,
                                       sink, sink_values, key_splits, part_acc, part_ml, one_tile, status, stream);
   if (code != HB_OK || key_splits == 1) return code;
   return hb_attention_merge(part_acc, part_ml, out, HB_DTYPE_BF16, n_tokens * nh, hd, key_splits, sink, nh, sink_values, stream);

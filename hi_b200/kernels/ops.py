@@ -2710,8 +2710,9 @@ def prefill_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table:
                            key_splits: int = 1, sink: bool = False, sink_values: Optional[torch.Tensor] = None, keep: int = 0,
                            one_tile: bool = False) -> torch.Tensor:
     """:func:`prefill_attention_tc` over a cache held in four bits: the pages that the step's new tokens may read (``start_pos`` and
-    ``n_new`` as in :func:`expand_pages_4bit`) are expanded to float16 first, keys and values of a kv head divided by a power of two, and
-    the tcgen05 kernels run on those. Rows of requests that ``skip_single`` leaves out are not written."""
+    ``n_new`` as in :func:`expand_pages_4bit`) are expanded first, and the tcgen05 kernels run on those. Keys and values of a request's kv head are
+    expanded to float16, divided by a power of two each, where their groups' magnitudes lie within 2^13 of one another, else to bfloat16; which of
+    them a request gets depends on its own rows alone. Rows of requests that ``skip_single`` leaves out are not written."""
     _need(q, "q", torch.bfloat16)
     n, nh, hd = q.shape
     nkv, page_size, total = _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos, n_new, chunk, window, keep, skip_single)

@@ -148,8 +148,8 @@ FOUR_BIT_DECODED = 14
 def attend_over_four_bit_pages(q, kv_pages, block_table, ctx, nh: int, nkv: int, hd: int, chunk: int, sliding: int, scale: float,
                                sink: bool = False, softcap: float = 0.0, slopes=None, sink_values=None, keep: int = 0):
     """:func:`attend_over_pages` over a cache held in four bits (``ops.qkv_post_4bit`` fills it). Single tokens, and portions of a few,
-    read it as it is; for portions of prompts the pages that they may read are expanded to float16 once and go through the tcgen05
-    kernels. Reshaped scores (``softcap``, ``slopes``) are taken by the kernels of the bfloat16 cache, over pages expanded to that, in steps
+    read it as it is; for portions of prompts the pages that they may read are expanded once and go through the tcgen05
+    kernels (``ops.prefill_attention_4bit``). Reshaped scores (``softcap``, ``slopes``) are taken by the kernels of the bfloat16 cache, over pages expanded to that, in steps
     of single tokens too. What is expanded is fixed by ``ctx.start_pos`` and ``ctx.n_new`` of the call: a captured call is replayed at its own positions
     only (``ops.check_tc_status`` raises where others ask for more or fewer pages)."""
     if q.shape != (ctx.n_tokens, nh, hd) or kv_pages.shape[1] != nkv:
