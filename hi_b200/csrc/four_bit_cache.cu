@@ -227,6 +227,7 @@ __device__ __forceinline__ void span(const Expand& a, int s, int& first, int& co
   first = count = 0;
   if (n <= 0 || (n == 1 && a.skip_single)) return;
   const int start = a.positions[begin];
+  if (start < 0) return;
   int lo = 0;
   if (a.chunk > 0) lo = start / a.chunk * a.chunk;
   else if (a.window > 0 && a.keep == 0) lo = max(0, start - a.window + 1);
@@ -234,15 +235,24 @@ __device__ __forceinline__ void span(const Expand& a, int s, int& first, int& co
   count = (start + n - 1) / a.page_size - first + 1;
 }
 
-// The pages that all requests ask for, by one warp.
-__device__ __forceinline__ int all_pages(const Expand& a) {
+// Whether the requests ask for as many pages as the grid has, by one warp. If not, `status` says so, and entries of pages behind the grid's are -1.
+__device__ void check_total(const Expand& a) {
   int all = 0;
-  for (int s = threadIdx.x & 31; s < a.n_seqs; s += 32) {
+  for (int s = threadIdx.x; s < a.n_seqs; s += 32) {
     int first, count;
     span(a, s, first, count);
     all += count;
   }
-  return __reduce_add_sync(0xffffffffu, all);
+  if (__reduce_add_sync(0xffffffffu, all) == a.total) return;
+  if (threadIdx.x == 0) atomicExch(a.status, 33);
+  int before = 0;
+  for (int s = 0; s < a.n_seqs; ++s) {
+    int first, count;
+    span(a, s, first, count);
+    for (int i = max(0, a.total - before) + threadIdx.x; i < count && first + i < a.table_stride; i += 32)
+      a.table[(size_t)s * a.table_stride + first + i] = -1;
+    before += count;
+  }
 }
 
 // The request and its page that page `out_page` of the result is; false: none (or the table has no such page). A whole block asks.
@@ -392,7 +402,14 @@ __global__ void __launch_bounds__(EXPAND_THREADS) expand_4bit_kernel(const Expan
   }
   int seq, index;
   bool leads;
-  if (out_page == 0 && kvh == 0 && threadIdx.x < 32 && all_pages(a) != a.total && threadIdx.x == 0) atomicExch(a.status, 33);
+  if (out_page == 0 && kvh == 0 && threadIdx.x < 32) check_total(a);
+  if (!PREFILL && kvh == 0)          // the entries that no page of the result is for (with PREFILL: -1 already)
+    for (long long i = (long long)out_page * blockDim.x + threadIdx.x; i < (long long)a.n_seqs * a.table_stride; i += (long long)a.total * blockDim.x) {
+      int first, count;
+      const int entry = (int)(i % a.table_stride);
+      span(a, (int)(i / a.table_stride), first, count);
+      if (entry < first || entry >= first + count) a.table[i] = -1;
+    }
   if (!find_page(a, out_page, seq, index, leads)) return;
   Held form{false, 0, 0};
   if constexpr (PREFILL) {
@@ -469,12 +486,11 @@ int expand(const Expand& a, int hd, bool prefill, cudaStream_t stream) {
     return HB_ERR_BAD_ARG;
   if ((hd != 64 && hd != 128) || !good_page(a.page_size) || a.nkv > 65535) return HB_ERR_UNSUPPORTED;
   if (a.n_seqs == 0 || a.total == 0) return HB_OK;
-  // the table's entries are -1, and (behind them) the magnitudes
-  const size_t unset = prefill ? (uint8_t*)(a.most + (size_t)a.n_seqs * a.nkv) - (uint8_t*)a.table : (size_t)a.n_seqs * a.table_stride * 4;
-  const cudaError_t e = cudaMemsetAsync(a.table, 0xff, unset, stream);
-  if (e != cudaSuccess) return (int)e;
   const dim3 grid(a.total, a.nkv);
   if (prefill) {
+    // the table's entries are -1, and (behind them) the magnitudes
+    const cudaError_t e = cudaMemsetAsync(a.table, 0xff, (uint8_t*)(a.most + (size_t)a.n_seqs * a.nkv) - (uint8_t*)a.table, stream);
+    if (e != cudaSuccess) return (int)e;
     const dim3 more(a.total + (a.n_tokens + Q_TOKENS - 1) / Q_TOKENS, a.nkv);
     if (hd == 128) most_4bit_kernel<4><<<grid, MOST_THREADS, 0, stream>>>(a);
     else most_4bit_kernel<2><<<grid, MOST_THREADS, 0, stream>>>(a);

@@ -95,6 +95,11 @@ def test_positions_that_the_device_does_not_have_are_found(host):
         ops.check_tc_status()
     ops.expand_pages_4bit(step.pages, 64, step.table, step.ctx.cu_seqlens, step.positions, [300, 90], [1, 1])
     ops.check_tc_status()
+    for kw in ({}, dict(chunk=64), dict(window=70)):              # positions before the first: no pages
+        table = ops.expand_pages_4bit(step.pages, 64, step.table, step.ctx.cu_seqlens, torch.full_like(step.positions, -1000), [300, 90], [1, 1], **kw)[2]
+        assert (table == -1).all()
+        with pytest.raises(ops.KernelError, match="4-bit cache"):
+            ops.check_tc_status()
 
 
 @pytest.mark.gpu
