@@ -67,9 +67,9 @@ int hb_prefill_attention_4bit(const void* q, const void* pages, const int* block
                               int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
                               const float* sink_values, int key_splits, int one_tile, int total, void* workspace,
                               long long workspace_bytes, int* status, cudaStream_t stream);
-// q, k and v of request s and kv head h in float16 where form[s][h].y is not 0, else in bfloat16; values divided by form[s][h].x, scores of a
-// row to be multiplied by q_factor[token][head] (attention_prefill_tc.cu)
-int hb_attention_prefill_tc_mixed(const void* q, const void* k_pages, const void* v_pages, const float2* form, const float* q_factor,
+// q, k and v of request s and kv head h in float16 where form[s][h].y is not 0, else in bfloat16; values divided by form[s][h].x; a row's scores
+// times q_scale[token][head] are in units of log 2, `scale` is not used (attention_prefill_tc.cu)
+int hb_attention_prefill_tc_mixed(const void* q, const void* k_pages, const void* v_pages, const float2* form, const float* q_scale,
                                   const int* block_table, int table_stride, const int* cu_seqlens, const int* positions,
                                   void* out, int n_tokens, int n_pages, int n_seqs, int max_new, int nh, int nkv, int hd,
                                   int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,

@@ -441,7 +441,8 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const int pos = x.p_first + r, warp_first = x.p_first + (warp & 3) * 32;
       const int lo = first_visible(a, pos), warp_lo = first_visible(a, warp_first + 31);
       float scale_log2 = a.scale_log2;
-      if constexpr (MIXED) scale_log2 *= row_ok ? a.q_factor[(size_t)(x.tok0 + r) * a.nh + x.head] : 1.f;
+      if constexpr (MIXED)
+        if (row_ok) scale_log2 = a.q_scale[(size_t)(x.tok0 + r) * a.nh + x.head];
       // rows without a token start above every score, so they never move the maximum
       float m = row_ok ? -INFINITY : INFINITY, l = 0.f;
       for (int j = x.begin; j < x.end; ++j, ++phase) {
@@ -475,7 +476,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const float mx = fmaxf(m, row_max(sv) * scale_log2);           // the scale is positive
         // The exponentials are taken against `m`, which follows the maximum only when a row of the warp has grown by more than 2^8:
         // P stays below 256 and most tiles leave O as it is. A row that has seen nothing yet has nothing to move to.
-        const bool move = __any_sync(0xffffffffu, mx > m + 8.f);
+        const bool move = __any_sync(0xffffffffu, MIXED ? mx - m > 8.f : mx > m + 8.f);      // (MIXED: exact for large ones too)
         float corr = 1.f;
         if (move) {
           corr = m == -INFINITY ? 0.f : fast_exp2(m - mx);
@@ -491,7 +492,8 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
           }
         }
-        const float base = m == -INFINITY ? 0.f : -m;                    // of a row that has seen nothing: 2^-inf = 0 all the same
+        // (of a row that has seen nothing: 2^-inf = 0 all the same)
+        const float base = (m == -INFINITY ? 0.f : -m) + (MIXED ? RAISE : 0.f);
         const float2 scale2 = make_float2(scale_log2, scale_log2), base2 = make_float2(base, base);
         float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         auto weigh = [&](auto half) {
@@ -535,6 +537,7 @@ attn_prefill_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       tc::fence_after();
       const float factor = form.x;
+      if constexpr (MIXED) m -= RAISE;            // what the sum and O are relative to
       if (a.key_splits > 1) {
         // this share of the keys only: the row as it is, with its maximum and sum, for the merge
         const size_t at = ((size_t)(x.tok0 + r) * a.nh + x.head) * a.key_splits + piece;

@@ -106,7 +106,7 @@ struct Args {
   int keep;                  // a sliding window's kept first tokens
   Pair pair;                 // kPair only
   const float2* form;        // MIXED only: see PrefillPairArgs
-  const float* q_factor;
+  const float* q_scale;
 };
 
 // MIXED: operands and P in float16 or bfloat16, by request and key head (a.form)
@@ -331,7 +331,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // reshaped scores are brought to units of log 2 first and the code below then takes them with a scale of one
     const bool reshaped = a.softcap > 0.f || a.slopes != nullptr;
     float scale_l2 = reshaped ? 1.f : a.scale_log2;
-    if constexpr (MIXED) scale_l2 *= row_ok ? a.q_factor[(size_t)(tok0 + row) * a.nh + h] : 1.f;     // (never reshaped)
+    if constexpr (MIXED)
+      if (row_ok) scale_l2 = a.q_scale[(size_t)(tok0 + row) * a.nh + h];      // (never reshaped)
     const float slope_l2 = a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
     const float cap_l2 = a.softcap * 1.4426950408889634f;
     const float twice_over_cap = a.softcap > 0.f ? 2.f * a.scale_log2 / a.softcap : 0.f;
@@ -405,7 +406,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       // sum, scaled by a common factor that the final division removes.
       // A row that has seen nothing yet, -inf on both sides, has nothing to move to. (While it did, the rows past a portion's
       // end started over in every tile: a portion of 513 tokens behind 7,000, 16 heads, took 219 us where it takes 66.)
-      const bool move = !sigmoid && __any_sync(0xffffffffu, mx > m + 8.f);
+      const bool move = !sigmoid && __any_sync(0xffffffffu, MIXED ? mx - m > 8.f : mx > m + 8.f);      // (MIXED: exact for large ones too)
       float corr = 1.f;
       if (move) {
         corr = (m == -INFINITY) ? 0.f : fast_exp2(m - mx);
@@ -425,7 +426,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       } else {
         // two scores an instruction where the hardware has it (fma and add on pairs of floats);
         // the sum runs in four chains
-        const float2 scale2 = make_float2(scale_l2, scale_l2), neg_m2 = make_float2(-m, -m);
+        const float base = -m + (MIXED ? RAISE : 0.f);
+        const float2 scale2 = make_float2(scale_l2, scale_l2), neg_m2 = make_float2(base, base);
         float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int i = 0; i < BKEYS; i += 4) {
@@ -507,6 +509,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(p_ready);
     }
+    if constexpr (MIXED) m -= RAISE;            // what the sum and O are relative to
     if (ok) {
       if (!tc::mbar_wait_warp(pv_done, (nt - 1) & 1)) {
         if (lane == 0) atomicExch(a.status, 18);
@@ -750,7 +753,7 @@ int prefill_tc(const void* q, const void* k_pages, const void* v_pages, const in
                int nh, int nkv, int hd, int page_size, int chunk, int window, float scale, int skip_single, int sink,
                const float* head_bias, int key_splits, float* part_acc, float* part_ml, int* status, int turn_inside,
                const float* v_inv_freq, int v_pairs, int v_interleaved, float softcap, const float* slopes,
-               const float* sink_values, int keep, const Pair* pair, int one_tile, const float2* form, const float* q_factor, cudaStream_t stream);
+               const float* sink_values, int keep, const Pair* pair, int one_tile, const float2* form, const float* q_scale, cudaStream_t stream);
 }  // namespace
 
 // one_tile: plain softmax rows of 64 and 128 too go one query tile a block (ops.prefill_one_tile says where that is faster)
@@ -779,16 +782,16 @@ extern "C" int hb_attention_prefill_tc_reshaped(const void* q, const void* k_pag
 }
 
 // q, k and v by request and key head in float16 or bfloat16 (hb_prefill_attention_4bit makes them); hd 64 or 128.
-extern "C" int hb_attention_prefill_tc_mixed(const void* q, const void* k_pages, const void* v_pages, const float2* form, const float* q_factor,
+extern "C" int hb_attention_prefill_tc_mixed(const void* q, const void* k_pages, const void* v_pages, const float2* form, const float* q_scale,
                                              const int* block_table, int table_stride, const int* cu_seqlens, const int* positions,
                                              void* out, int n_tokens, int n_pages, int n_seqs, int max_new, int nh, int nkv, int hd,
                                              int page_size, int chunk, int window, int keep, float scale, int skip_single, int sink,
                                              const float* sink_values, int key_splits, float* part_acc, float* part_ml,
                                              int one_tile, int* status, cudaStream_t stream) {
-  if (!form || !q_factor || sink < 0 || sink > 1) return HB_ERR_BAD_ARG;
+  if (!form || !q_scale || sink < 0 || sink > 1) return HB_ERR_BAD_ARG;
   return prefill_tc(q, k_pages, v_pages, block_table, table_stride, cu_seqlens, positions, out, n_tokens, n_pages, n_seqs,
                     max_new, nh, nkv, hd, page_size, chunk, window, scale, skip_single, sink, nullptr, key_splits,
-                    part_acc, part_ml, status, 0, nullptr, 0, 0, 0.f, nullptr, sink_values, keep, nullptr, one_tile, form, q_factor, stream);
+                    part_acc, part_ml, status, 0, nullptr, 0, 0, 0.f, nullptr, sink_values, keep, nullptr, one_tile, form, q_scale, stream);
 }
 
 // Sigmoid weights with the result written by the kernel itself: `out` [n_tokens, nh, hd] bfloat16 takes every
@@ -833,7 +836,7 @@ int prefill_tc(const void* q, const void* k_pages, const void* v_pages, const in
                int nh, int nkv, int hd, int page_size, int chunk, int window, float scale, int skip_single, int sink,
                const float* head_bias, int key_splits, float* part_acc, float* part_ml, int* status, int turn_inside,
                const float* v_inv_freq, int v_pairs, int v_interleaved, float softcap, const float* slopes,
-               const float* sink_values, int keep, const Pair* pair, int one_tile, const float2* form, const float* q_factor, cudaStream_t stream) {
+               const float* sink_values, int keep, const Pair* pair, int one_tile, const float2* form, const float* q_scale, cudaStream_t stream) {
   if (sink == 2 && (softcap > 0.f || slopes || sink_values)) return HB_ERR_UNSUPPORTED;
   if (!q || !k_pages || !v_pages || !block_table || !cu_seqlens || !positions || !out || !status) return HB_ERR_BAD_ARG;
   if (n_tokens < 0 || n_pages <= 0 || n_seqs < 0 || max_new < 0 || nh <= 0 || nkv <= 0 || nh % nkv != 0 ||
@@ -847,13 +850,13 @@ int prefill_tc(const void* q, const void* k_pages, const void* v_pages, const in
   if (n_seqs == 0 || max_new == 0 || n_tokens == 0) return HB_OK;
   Args a{block_table, cu_seqlens, positions, (__nv_bfloat16*)out, status, table_stride, nh, nkv, page_size, chunk,
          window, skip_single, page_size < BKEYS ? page_size : BKEYS, scale * 1.4426950408889634f, key_splits, part_acc, part_ml, sink, head_bias,
-         turn_inside, v_pairs, v_interleaved, v_inv_freq, softcap, slopes, sink_values, slopes ? 1 : 0, keep, pair ? *pair : Pair{}, form, q_factor};
+         turn_inside, v_pairs, v_interleaved, v_inv_freq, softcap, slopes, sink_values, slopes ? 1 : 0, keep, pair ? *pair : Pair{}, form, q_scale};
   const long long pool_rows = (long long)n_pages * nkv * page_size;
   // (a launch of more pairs than a grid holds goes one tile a block)
   const long long pairs = ((max_new + 127LL) / 128 * (nh / nkv) + 1) / 2;
   if (!one_tile && !pair && !turn_inside && sink != 2 && softcap <= 0.f && !slopes && keep == 0 && hd <= 128 && pairs <= 65535) {
     const PrefillPairArgs b{block_table, cu_seqlens, positions, (__nv_bfloat16*)out, status, table_stride, nh, nkv, page_size, chunk, window,
-                            skip_single, a.box_rows, a.scale_log2, key_splits, part_acc, part_ml, sink, sink_values, form, q_factor};
+                            skip_single, a.box_rows, a.scale_log2, key_splits, part_acc, part_ml, sink, sink_values, form, q_scale};
     return hb_prefill_pair_launch(q, k_pages, v_pages, b, n_tokens, pool_rows, n_seqs, max_new, hd, stream);
   }
   if (pair) {

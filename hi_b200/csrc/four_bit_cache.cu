@@ -217,7 +217,8 @@ struct Expand {
   int n_tokens, nh;
   int4* most;                      // [n_seqs][nkv]: see most_4bit_kernel
   uint16_t* q_out;
-  float* q_factor;                 // [n_tokens][nh]
+  float* q_scale;                  // [n_tokens][nh]: of a row's scores, to units of log 2
+  float scale_log2;
   float2* form;                    // [n_seqs][nkv]: what the values have been divided by, 1 for float16
   int* status;
 };
@@ -291,8 +292,9 @@ __device__ __forceinline__ float number(const uint8_t* p) { return __bfloat162fl
 // request's kv head are divided by the least power of two above the largest of them, so float16 holds a group to 2^-11 of its largest
 // magnitude where that is at least 2^-14 of the head's. A request with a smaller one, or with a largest one out of 2^-100 .. 2^100, is
 // expanded to bfloat16 for that head instead, and its products are taken in it. What a request's result is rounded to depends on its own rows
-// alone. A query's row of a head is multiplied by a power of two of its own, which the scores' scale takes back: it keeps all bits of elements
-// down to 2^-32 of its largest.
+// alone. A query's row of a head is multiplied by a power of two of its own, which the row's scale takes back: it keeps all bits of elements
+// down to 2^-32 of its largest. Where its scores could pass 2^20 the mantissa of the scale goes into the row, rounded to float16 as the keys
+// are: their maximum times a power of two is exact, and so are the differences to it. (Rounded, it would be off by more than float16's weights can grow.)
 //
 // The magnitudes of a request's kv head on the pages, of rows that are there (a group's ends: its low and fifteen steps above it): one atomic a
 // block and number, and none where it changes nothing (29 us for 144 pages of 8 heads with one a warp, 7 so). `most` holds the bits of floats, whose
@@ -390,12 +392,15 @@ __global__ void __launch_bounds__(EXPAND_THREADS) expand_4bit_kernel(const Expan
 #pragma unroll
         for (int o = WORDS / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(row_lanes, most, o));
         const int e_q = max(-100, power_above(__float_as_int(most)));
-        const float up = power_of_two(15 - e_q);                    // (an infinity stays one)
+        const float e_scale = power_of_two((__float_as_int(a.scale_log2) >> 23) - 127), rest = a.scale_log2 / e_scale;      // rest: 1 to 2
+        const bool large = (float)HD * a.scale_log2 * power_of_two(e_q + form.k) > 1048576.f;
+        const float up = large ? power_of_two(14 - e_q) * rest : power_of_two(15 - e_q);                   // (an infinity stays one)
         unsigned o[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = tc::pack16<true>(x[2 * e] * up, x[2 * e + 1] * up);
         *reinterpret_cast<uint4*>(a.q_out + at) = form.half ? make_uint4(o[0], o[1], o[2], o[3]) : raw;
-        if (i % WORDS == 0) a.q_factor[row] = form.half ? power_of_two(e_q - 15 + form.k) : 1.f;
+        if (i % WORDS == 0)
+          a.q_scale[row] = !form.half ? a.scale_log2 : large ? power_of_two(e_q - 14 + form.k) * e_scale : power_of_two(e_q - 15 + form.k) * a.scale_log2;
       }
       return;
     }
@@ -512,21 +517,21 @@ extern "C" int hb_expand_pages_4bit(const void* pages, const int* block_table, i
                                     int skip_single, int nkv, int hd, void* k, void* v, int* table, int* status,
                                     cudaStream_t stream) {
   return expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)k, (uint16_t*)v, table, n_seqs,
-                       table_stride, page_size, chunk, window, keep, skip_single, nkv, total, nullptr, 0, 0, nullptr, nullptr, nullptr, nullptr, status},
+                       table_stride, page_size, chunk, window, keep, skip_single, nkv, total, nullptr, 0, 0, nullptr, nullptr, nullptr, 0.f, nullptr, status},
                 hd, false, stream);
 }
 
 // What hb_prefill_attention_4bit needs of its workspace, in order, each part on 1,024 bytes.
 namespace {
 struct Room {
-  size_t k, v, q, q_factor, table, most, form, part_acc, part_ml, all;
+  size_t k, v, q, q_scale, table, most, form, part_acc, part_ml, all;
   Room(int total, int n_tokens, int n_seqs, int table_stride, int nh, int nkv, int hd, int page_size, int key_splits) {
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 1023) / 1024 * 1024; return here; };
     k = take((size_t)total * nkv * page_size * hd * 2);
     v = take((size_t)total * nkv * page_size * hd * 2);
     q = take((size_t)n_tokens * nh * hd * 2);
-    q_factor = take((size_t)n_tokens * nh * 4);
+    q_scale = take((size_t)n_tokens * nh * 4);
     table = take((size_t)n_seqs * table_stride * 4);
     most = take((size_t)n_seqs * nkv * 16);
     form = take((size_t)n_seqs * nkv * 8);
@@ -571,17 +576,17 @@ extern "C" int hb_prefill_attention_4bit(const void* q, const void* pages, const
   const Room room(total, n_tokens, n_seqs, table_stride, nh, nkv, hd, page_size, key_splits);
   if ((long long)room.all > workspace_bytes) return HB_ERR_BAD_ARG;
   uint8_t* w = static_cast<uint8_t*>(workspace);
-  float* q_factor = reinterpret_cast<float*>(w + room.q_factor);
+  float* q_scale = reinterpret_cast<float*>(w + room.q_scale);
   float2* form = reinterpret_cast<float2*>(w + room.form);
   int* table = reinterpret_cast<int*>(w + room.table);
   int code = expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)(w + room.k), (uint16_t*)(w + room.v), table,
                            n_seqs, table_stride, page_size, chunk, window, keep, skip_single, nkv, total, (const __nv_bfloat16*)q, n_tokens, nh,
-                           (int4*)(w + room.most), (uint16_t*)(w + room.q), q_factor, form, status},
+                           (int4*)(w + room.most), (uint16_t*)(w + room.q), q_scale, scale * 1.4426950408889634f, form, status},
                     hd, true, stream);
   if (code != HB_OK) return code;
   float* part_acc = key_splits > 1 ? reinterpret_cast<float*>(w + room.part_acc) : nullptr;
   float* part_ml = key_splits > 1 ? reinterpret_cast<float*>(w + room.part_ml) : nullptr;
-  code = hb_attention_prefill_tc_mixed(w + room.q, w + room.k, w + room.v, form, q_factor, table, table_stride, cu_seqlens, positions, out,
+  code = hb_attention_prefill_tc_mixed(w + room.q, w + room.k, w + room.v, form, q_scale, table, table_stride, cu_seqlens, positions, out,
                                       n_tokens, total, n_seqs, max_new, nh, nkv, hd, page_size, chunk, window, keep, scale, skip_single,
                                       sink, sink_values, key_splits, part_acc, part_ml, one_tile, status, stream);
   if (code != HB_OK || key_splits == 1) return code;

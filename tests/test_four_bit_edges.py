@@ -235,8 +235,9 @@ def test_a_portion_does_not_depend_on_other_requests(hd, page, one_tile):
     for size in (2.0 ** 20, 2.0 ** -20, 2.0 ** 90, 2.0 ** -90):
         got = run((1, 2), size)
         assert torch.equal(got[:40], want[:40]) and torch.equal(got[191:224], want[191:224])
-    got = run((), 1.0, 2.0 ** 10)
-    assert torch.equal(got[:32], want[:32]) and torch.equal(got[40:224], want[40:224])
+    for query in (2.0 ** 10, 2.0 ** 30):                          # (scores of 2^34: their maxima's own rounding is more than float16 holds)
+        got = run((), 1.0, query)
+        assert torch.equal(got[:32], want[:32]) and torch.equal(got[40:224], want[40:224])
 
 
 @pytest.mark.gpu
@@ -281,3 +282,35 @@ def test_portions_of_uneven_sizes(form, one_tile):
                     _check_reshaped(late, 0, got[5:], mask, scale, 0.0)
             else:
                 _check_reshaped(step, s, got, mask, scale, 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,page", [(128, 64), (64, 32)])
+@pytest.mark.parametrize("one_tile,shares", [(False, 1), (False, 3), (True, 1), (True, 3)])
+def test_many_small_weights(hd, page, one_tile, shares):
+    """One key of no value that weighs 2^26 times as much as each of 6,000 others: they are all that the result is made of. Keys, values and scores
+    are held exactly; a weight in float16 is off by 2^-32 of the largest or 2^-11 of itself, the exponential by 2^-17, the result is rounded."""
+    from hi_b200.kernels import ops
+
+    step = _step([(150, 6000), (40, 300)], 4, 2, hd, page, seed=5)
+    for s in (0, 1):
+        step.k[s].zero_()
+        step.k[s][0, :, 0] = 15.0
+        step.v[s].fill_(1.0)
+        step.v[s][0] = 0.0
+    step.fill()
+    step.q.zero_()
+    step.q[:, :, 0] = 1.0
+    scale = 26 * math.log(2) / 15
+    ctx = step.ctx
+    for sink in (None, torch.full((4,), 26 * math.log(2), device=DEV), torch.full((4,), 0.0, device=DEV)):
+        got = ops.prefill_attention_4bit(step.q, step.pages, step.table, ctx.cu_seqlens, step.positions, ctx.start_pos, ctx.n_new, 0, 0, scale,
+                                         key_splits=shares, sink_values=sink, one_tile=one_tile)
+        ops.check_tc_status()
+        for s in (0, 1):
+            a, b = step.cu[s], step.cu[s + 1]
+            others = step.positions[a:b].double() * 2.0 ** -26
+            extra = 0.0 if sink is None else math.exp(float(sink[0]) - 26 * math.log(2))
+            want = (others / (1 + others + extra)).view(-1, 1, 1)
+            tol = want * (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -16) + others.view(-1, 1, 1) * 2.0 ** -6
+            assert ((got[a:b].double() - want).abs() <= tol).all(), (s, float(got[a:b].min()), float(want.min()))
