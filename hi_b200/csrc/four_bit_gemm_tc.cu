@@ -164,7 +164,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
       const int row = tc::uniform(t0 + (PAIR ? rank * ((n + 15) / 16 * 8) : 0));      // a pair's tokens are half in one block, half in the other
       for (int c = tc::uniform(c0); c < c1; ++c) {
         if (!tc::mbar_wait_warp(&empty[s], turn)) {
-          if (lane == 0) atomicExch(p.status, 51);
+          if (lane == 0) atomicExch(p.status, 81);
           ok = false;
           break;
         }
@@ -195,14 +195,14 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
     for (int i = 0; (rank == 0 || !PAIR) && ok && tile_at(i, f0, t0, n); ++i) {
       const int b = i % SLOTS;
       if (i >= SLOTS && !tc::mbar_wait_warp(&acc_empty[b], (i / SLOTS - 1) & 1)) {
-        if (lane == 0) atomicExch(p.status, 54);
+        if (lane == 0) atomicExch(p.status, 84);
         break;
       }
       tc::fence_after();
       const uint32_t idesc = tc::idesc_bf16(FEATURES, tc::uniform((n + 15) & ~15), false), acc = tmem + b * BT;
       for (int c = c0; c < c1; ++c) {
         if (!tc::mbar_wait_warp(&full_x[s], turn) || !tc::mbar_wait_warp(&full_a[s], turn)) {
-          if (lane == 0) atomicExch(p.status, 52);
+          if (lane == 0) atomicExch(p.status, 82);
           ok = false;
           break;
         }
@@ -231,7 +231,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
       const uint8_t* from = p.w + ((size_t)(tile + lane) * p.chunks + c0) * BLOCK_BYTES;
       for (int c = c0; c < c1; ++c, from += BLOCK_BYTES) {
         if (!tc::mbar_wait_warp(&raw_empty[r], turn)) {
-          if (lane == 0) atomicExch(p.status, 56);
+          if (lane == 0) atomicExch(p.status, 86);
           ok = false;
           break;
         }
@@ -263,7 +263,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
     const unsigned pick = q4 & 1 ? 0x7351u : 0x6240u;
     auto next = [&]() {                           // false: the codes did not come
       if (!tc::mbar_wait_warp(&raw_full[r], r_turn)) {
-        if (lane == 0) atomicExch(p.status, 57);
+        if (lane == 0) atomicExch(p.status, 87);
         return false;
       }
       const uint8_t* block = raw + (r * UNPACK + part) * RAW_BLOCK;        // (rows past the weight's: whatever is there; they are not written out)
@@ -296,7 +296,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
     bool ok = stages > 0 && next();
     for (int i = 0; ok && i < stages; ++i) {
       if (!tc::mbar_wait_warp(&empty[s], turn)) {
-        if (lane == 0) atomicExch(p.status, 53);
+        if (lane == 0) atomicExch(p.status, 83);
         break;
       }
       if constexpr (PAIR) {
@@ -331,7 +331,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
       const bool f_ok = f < p.n_out;
       const float bias = p.bias && f_ok ? __bfloat162float(p.bias[f]) : 0.f;
       if (!tc::mbar_wait_warp(&acc_full[b], (i / SLOTS) & 1)) {
-        if (lane == 0) atomicExch(p.status, 55);
+        if (lane == 0) atomicExch(p.status, 85);
         break;
       }
       tc::fence_after();
@@ -363,7 +363,7 @@ four_bit_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const Params p) 
     bool ok = true;
     if (there && c0 < c1 && warp >= FIRST_UNPACK) {
       ok = tc::mbar_wait_warp(&acc_full[0], 0);
-      if (!ok && lane == 0) atomicExch(p.status, 55);
+      if (!ok && lane == 0) atomicExch(p.status, 85);
     }
     tc::fence_after();
     __syncwarp();

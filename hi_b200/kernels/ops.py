@@ -2296,13 +2296,13 @@ def check_tc_status(device=None) -> None:
                      4: "grouped product: the MMA issuer waiting for a free accumulator",
                      31: "decode attention: the warps waiting for a tile's TMA loads",
                      41: "recurrence by chunks: the warps waiting for a chunk's copies",
-                     51: "4-bit product: the TMA producer waiting for a free stage",
-                     52: "4-bit product: the MMA issuer waiting for a stage",
-                     53: "4-bit product: the warps that unpack weights waiting for a free stage",
-                     54: "4-bit product: the MMA issuer waiting for a free accumulator",
-                     55: "4-bit product: the epilogue waiting for the accumulator",
-                     56: "4-bit product: the warp that brings codes waiting for a free place",
-                     57: "4-bit product: the warps that unpack weights waiting for their codes"}.get(
+                     81: "4-bit product: the TMA producer waiting for a free stage",
+                     82: "4-bit product: the MMA issuer waiting for a stage",
+                     83: "4-bit product: the warps that unpack weights waiting for a free stage",
+                     84: "4-bit product: the MMA issuer waiting for a free accumulator",
+                     85: "4-bit product: the epilogue waiting for the accumulator",
+                     86: "4-bit product: the warp that brings codes waiting for a free place",
+                     87: "4-bit product: the warps that unpack weights waiting for their codes"}.get(
                 code, f"prefill attention, wait {code}" if code >= 11 else f"code {code}")
             raise KernelError(f"a kernel gave up a bounded wait ({where}); its output is invalid")
 

@@ -314,3 +314,31 @@ def test_many_small_weights(hd, page, one_tile, shares):
             want = (others / (1 + others + extra)).view(-1, 1, 1)
             tol = want * (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -16) + others.view(-1, 1, 1) * 2.0 ** -6
             assert ((got[a:b].double() - want).abs() <= tol).all(), (s, float(got[a:b].min()), float(want.min()))
+
+
+def test_a_status_names_one_kernel():
+    """On the CPU, from the sources: no two kernels report the same number, and those that have words of their own are what reports them."""
+    import inspect
+    import os
+    import re
+
+    from hi_b200.kernels import build, ops
+
+    def numbers(name):
+        with open(os.path.join(build.CSRC, name)) as f:
+            text = f.read()
+        found = set()
+        for first, plus in re.findall(r"atomicExch\((?:\w+\.)?status, (\d+)( \+ i)?\)", text):
+            found |= {int(first), int(first) + 1} if plus else {int(first)}
+        for first, plus in re.findall(r"wait\([^;]*?, (\d+)( \+ i)?\);", text):           # waits that hand their number on
+            found |= {int(first), int(first) + 1} if plus else {int(first)}
+        return found
+
+    product, pair, one = (numbers(f) for f in ("four_bit_gemm_tc.cu", "attention_prefill_pair.cu", "attention_prefill_tc.cu"))
+    grouped, cache = numbers("grouped_gemm_tc.cu"), numbers("four_bit_cache.cu")
+    assert {51, 57, 59, 60, 61, 71} <= pair and {11, 21, 24} <= one and cache == {33}
+    kinds = [product, pair, one, grouped, cache, numbers("attention_decode_tma.cu"), numbers("recurrence_chunked.cu")]
+    assert all(not a & b for i, a in enumerate(kinds) for b in kinds[:i])
+    words = {int(n): w for n, w in re.findall(r'(\d+): "([^"]+)"', inspect.getsource(ops.check_tc_status))}
+    assert {n for n, w in words.items() if w.startswith("4-bit product")} == product
+    assert not (pair | one) & set(words)
