@@ -2535,9 +2535,11 @@ def pack_weight(codes: torch.Tensor, scales: torch.Tensor) -> FourBitWeight:
     group = k // groups if groups and k % groups == 0 else 0
     if m == 0 or group not in FOUR_BIT_GROUPS:
         raise KernelError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)}: groups of {FOUR_BIT_GROUPS} are taken")
+    if int(codes.max()) > 15:
+        raise KernelError(f"a code of {int(codes.max())}: codes are 0 .. 15")
     tiles, chunks, per = -(-m // 16), -(-k // 128), 128 // group
     c = torch.full((tiles * 16, chunks * 128), 8, dtype=torch.uint8, device=codes.device)
-    c[:m, :k] = codes & 15
+    c[:m, :k] = codes
     c = c.view(tiles, 16, chunks, 4, 4, 8).permute(0, 2, 1, 4, 3, 5)          # [tile, chunk, row, lane, word, eight k]
     c = c[..., [0, 4, 1, 5]] | c[..., [2, 6, 3, 7]] << 4
     s = torch.zeros((tiles * 16, chunks * per), dtype=torch.bfloat16, device=codes.device)

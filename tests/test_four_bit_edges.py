@@ -342,3 +342,15 @@ def test_a_status_names_one_kernel():
     words = {int(n): w for n, w in re.findall(r'(\d+): "([^"]+)"', inspect.getsource(ops.check_tc_status))}
     assert {n for n, w in words.items() if w.startswith("4-bit product")} == product
     assert not (pair | one) & set(words)
+
+
+def test_codes_of_more_than_four_bits_are_refused():
+    from hi_b200.kernels import ops
+
+    codes = torch.full((3, 64), 15, dtype=torch.uint8)
+    scales = torch.ones(3, 2, dtype=BF16)
+    ops.pack_weight(codes, scales)
+    for wrong in (16, 255):
+        codes[2, 63] = wrong
+        with pytest.raises(ops.KernelError, match="0 .. 15"):
+            ops.pack_weight(codes, scales)
