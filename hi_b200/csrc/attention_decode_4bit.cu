@@ -456,7 +456,7 @@ extern "C" int hb_attention_decode_4bit(const void* q, const void* pages, const 
                                         const float* sink_values, int split_tiles, int splits, int cluster, float* part_acc, float* part_ml,
                                         int* status, const long long* rows, int step_tokens, cudaStream_t stream) {
   if (!q || !pages || !block_table || !seq_of_token || !positions || !out || !status || n_tokens < 0 || nh <= 0 || nkv <= 0 ||
-      nh % nkv || table_stride <= 0 || chunk < 0 || window < 0 || keep < 0 || split_tiles < 1 || splits < 1 || !(scale > 0.f) ||
+      nh % nkv || table_stride <= 0 || chunk < 0 || window < 0 || keep < 0 || (keep > 0 && chunk > 0) || split_tiles < 1 || splits < 1 || !(scale > 0.f) ||
       (cluster && (splits < 2 || splits > MOST_CLUSTER)) || (splits > 1 && !cluster && (!part_acc || !part_ml)))
     return HB_ERR_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(out)) & 15) return HB_ERR_BAD_ARG;

@@ -487,7 +487,7 @@ extern "C" int hb_qkv_post_4bit(const void* qkv, const float* inv_freq, int rot_
 namespace {
 int expand(const Expand& a, int hd, bool prefill, cudaStream_t stream) {
   if (!a.pages || !a.block_table || !a.cu_seqlens || !a.positions || !a.table || !a.status || a.n_seqs < 0 || a.total < 0 || a.nkv <= 0 || a.table_stride <= 0 ||
-      a.chunk < 0 || a.window < 0 || a.keep < 0 || (a.total > 0 && (!a.k || !a.v)))
+      a.chunk < 0 || a.window < 0 || a.keep < 0 || (a.keep > 0 && a.chunk > 0) || (a.total > 0 && (!a.k || !a.v)))
     return HB_ERR_BAD_ARG;
   if ((hd != 64 && hd != 128) || !good_page(a.page_size) || a.nkv > 65535) return HB_ERR_UNSUPPORTED;
   if (a.n_seqs == 0 || a.total == 0) return HB_OK;
@@ -543,11 +543,11 @@ struct Room {
 }  // namespace
 
 // How many pages the requests' new tokens may read, by what the host knows of them (cu_seqlens and positions on the device say the same);
-// -1: a position lies outside a block table of `width` pages a request.
+// -1: a position lies outside a block table of `width` pages a request, or the mask is not one (first tokens are kept beside a sliding window, not beside chunks).
 extern "C" long long hb_expand_total(const int* start_pos, const int* n_new, int n_seqs, int width, int page_size, int chunk, int window,
                                      int keep, int skip_single) {
   long long total = 0;
-  if (!start_pos || !n_new || n_seqs < 0 || page_size <= 0) return -1;
+  if (!start_pos || !n_new || n_seqs < 0 || page_size <= 0 || chunk < 0 || window < 0 || keep < 0 || (keep > 0 && chunk > 0)) return -1;
   for (int s = 0; s < n_seqs; ++s) {
     const long long start = start_pos[s], n = n_new[s];
     if (n <= 0 || (n == 1 && skip_single)) continue;

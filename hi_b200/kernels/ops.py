@@ -2683,7 +2683,7 @@ def _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos,
     total = lib().hb_expand_total(starts.buffer_info()[0], counts.buffer_info()[0], n_seqs, block_table.shape[1], page_size, chunk, window, keep, skip_single) if n_seqs else 0
     if total < 0 or total >= 1 << 31:
         raise KernelError(f"positions of {list(zip(start_pos, n_new))[:4]}... (first, count) lie outside the block table's "
-                          f"{block_table.shape[1]} pages a request")
+                          f"{block_table.shape[1]} pages a request, or a mask of {chunk}, {window} and {keep} tokens is not one")
     return nkv, page_size, total
 
 
@@ -2783,7 +2783,7 @@ def decode_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table: 
                           out: Optional[torch.Tensor] = None, most_keys: int = 0) -> torch.Tensor:
     """:func:`decode_attention` over a cache held in four bits: every row of bfloat16 ``q`` [N, nh, hd] (or with ``rows``, int64 and distinct,
     those tokens, into ``out``) is one request's token. ``chunk``, ``window``, ``keep``, ``sink``, ``sink_values``, ``max_context``,
-    ``most_keys`` as there."""
+    ``most_keys`` as there; first tokens are kept beside a sliding window, not beside chunks."""
     _need(q, "q", torch.bfloat16)
     if q.dim() != 3:
         raise KernelError("q is [tokens, heads, head_dim]")

@@ -354,3 +354,34 @@ def test_codes_of_more_than_four_bits_are_refused():
         codes[2, 63] = wrong
         with pytest.raises(ops.KernelError, match="0 .. 15"):
             ops.pack_weight(codes, scales)
+
+
+NO_MASK = [dict(chunk=512, keep=5), dict(chunk=64, window=1000, keep=200)]
+
+
+@pytest.mark.parametrize("wrong", NO_MASK, ids=str)
+def test_kept_tokens_beside_chunks_are_refused_by_the_entries(wrong):
+    """On the CPU: the entry points look at the mask before anything is launched or read."""
+    from hi_b200.kernels import ops
+
+    some = torch.zeros(64, dtype=torch.int64)
+    p = (some.data_ptr() + 15) // 16 * 16
+    chunk, window, keep = wrong.get("chunk", 0), wrong.get("window", 0), wrong["keep"]
+    lib = ops.lib()
+    assert lib.hb_attention_decode_4bit(p, p, p, 4, p, p, p, 1, 8, 2, 64, 64, chunk, window, keep, 0.1, 0, None, 1, 1, 0, None, None, p, None, 1,
+                                        None) == 1001
+    assert lib.hb_expand_pages_4bit(p, p, 4, p, p, 1, 1, 64, chunk, window, keep, 0, 2, 64, p, p, p, p, None) == 1001
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wrong", NO_MASK, ids=str)
+def test_kept_tokens_beside_chunks_are_refused(wrong):
+    from hi_b200.kernels import ops
+    from hi_b200.parts.attention import attend_over_four_bit_pages
+
+    for portions in ([(1, 700), (1, 20)], [(40, 700), (20, 64)]):
+        step = _step(portions, 8, 2, 64, 64).fill()
+        for cap in (0.0, 8.0):
+            with pytest.raises(ops.KernelError):
+                attend_over_four_bit_pages(step.q, step.pages, step.table, step.ctx, 8, 2, 64, wrong.get("chunk", 0), wrong.get("window", 0), 0.125,
+                                           softcap=cap, keep=wrong["keep"])
