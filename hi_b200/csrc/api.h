@@ -51,14 +51,15 @@ int hb_qkv_post_4bit(const void* qkv, const float* inv_freq, int rot_pairs, int 
                      int norm_first, int norm_dim, float rot_mul, int v_is_k, const int* positions,
                      const int* seq_of_token, const int* block_table, int table_stride, void* q_out, void* pages,
                      int page_size, int write_kv, int n_tokens, int nh, int nkv, int hd, cudaStream_t stream);
-// the pages that the requests' new tokens may read, as bfloat16 pages [total, nkv, page_size, hd], and the table of them (-1: no page);
+// the pages that the requests' new tokens may read, as bfloat16 pages [total, nkv, page_size, hd], and the table of them (-1: no page); whole:
+// with kept first tokens all pages from a request's first on, else without those between them and the window;
 // status 33: the device's positions ask for another number of pages than `total`
 int hb_expand_pages_4bit(const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
                          const int* positions, int n_seqs, int total, int page_size, int chunk, int window, int keep,
-                         int skip_single, int nkv, int hd, void* k, void* v, int* table, int* status, cudaStream_t stream);
+                         int whole, int skip_single, int nkv, int hd, void* k, void* v, int* table, int* status, cudaStream_t stream);
 // how many pages that is (from the host's copies of the requests' positions), or -1
 long long hb_expand_total(const int* start_pos, const int* n_new, int n_seqs, int width, int page_size, int chunk, int window,
-                          int keep, int skip_single);
+                          int keep, int whole, int skip_single);
 // attention of portions over it: pages expanded in the workspace (so many bytes of it), then the tcgen05 prefill kernels on them
 long long hb_prefill_attention_4bit_bytes(int total, int n_tokens, int n_seqs, int table_stride, int nh, int nkv, int hd,
                                           int page_size, int key_splits);

@@ -198,7 +198,8 @@ __global__ void __launch_bounds__(256, 4) qkv_post_4bit_kernel(const Post a) {
 }
 
 // ---- pages of the step's portions as bfloat16. Request s needs its pages first_s .. last_s: from the oldest position that its first
-// new token may read to its last one; they lie side by side in the result, request after request, and `table` [n_seqs, table_stride]
+// new token may read to its last one, and in front of them the pages of the first tokens that it keeps (`whole`: with kept tokens all pages
+// from the request's first on); they lie side by side in the result, request after request, and `table` [n_seqs, table_stride]
 // says where. Every other entry is -1, as that of a page which was given back: kernels that walk tiles larger than a page look at
 // entries in front of first_s, and what they would multiply by weights of zero there has to be a page of the request or none. The grid is
 // made from the host's copies of the requests' positions; where the device's ask for another number of pages, `status` says so
@@ -211,7 +212,7 @@ struct Expand {
   uint16_t* k;                     // bfloat16, or for the prefill kernels float16
   uint16_t* v;
   int* table;
-  int n_seqs, table_stride, page_size, chunk, window, keep, skip_single, nkv, total;
+  int n_seqs, table_stride, page_size, chunk, window, keep, whole, skip_single, nkv, total;
   // for the prefill kernels only
   const __nv_bfloat16* q;
   int n_tokens, nh;
@@ -223,36 +224,45 @@ struct Expand {
   int* status;
 };
 
-__device__ __forceinline__ void span(const Expand& a, int s, int& first, int& count) {
+// The pages of a request: `lead` of them from its first on, then those from `first` on, `count` in all.
+struct Span {
+  int lead, first, count;
+  __host__ __device__ int page(int i) const { return i < lead ? i : first + i - lead; }
+  __host__ __device__ bool has(int page) const { return page < lead || (page >= first && page < first + count - lead); }
+};
+template <typename I>              // int on the device, where divisions of 64 bits are slow
+__host__ __device__ inline Span span_of(I start, I n, int page_size, int chunk, int window, int keep, int whole) {
+  I low = 0;
+  if (chunk > 0) low = start / chunk * chunk;
+  else if (window > 0 && start - window + 1 > 0) low = start - window + 1;
+  if (whole && keep > 0) low = 0;
+  Span s;
+  s.first = (int)(low / page_size);
+  const int kept = keep / page_size + (keep % page_size != 0);
+  s.lead = kept < s.first ? kept : s.first;
+  s.count = s.lead + (int)((start + n - 1) / page_size) - s.first + 1;
+  return s;
+}
+__device__ __forceinline__ Span span(const Expand& a, int s) {
   const int begin = a.cu_seqlens[s], n = a.cu_seqlens[s + 1] - begin;
-  first = count = 0;
-  if (n <= 0 || (n == 1 && a.skip_single)) return;
+  if (n <= 0 || (n == 1 && a.skip_single)) return Span{0, 0, 0};
   const int start = a.positions[begin];
-  if (start < 0) return;
-  int lo = 0;
-  if (a.chunk > 0) lo = start / a.chunk * a.chunk;
-  else if (a.window > 0 && a.keep == 0) lo = max(0, start - a.window + 1);
-  first = lo / a.page_size;
-  count = (start + n - 1) / a.page_size - first + 1;
+  if (start < 0) return Span{0, 0, 0};
+  return span_of(start, n, a.page_size, a.chunk, a.window, a.keep, a.whole);
 }
 
 // Whether the requests ask for as many pages as the grid has, by one warp. If not, `status` says so, and entries of pages behind the grid's are -1.
 __device__ void check_total(const Expand& a) {
   int all = 0;
-  for (int s = threadIdx.x; s < a.n_seqs; s += 32) {
-    int first, count;
-    span(a, s, first, count);
-    all += count;
-  }
+  for (int s = threadIdx.x; s < a.n_seqs; s += 32) all += span(a, s).count;
   if (__reduce_add_sync(0xffffffffu, all) == a.total) return;
   if (threadIdx.x == 0) atomicExch(a.status, 33);
   int before = 0;
   for (int s = 0; s < a.n_seqs; ++s) {
-    int first, count;
-    span(a, s, first, count);
-    for (int i = max(0, a.total - before) + threadIdx.x; i < count && first + i < a.table_stride; i += 32)
-      a.table[(size_t)s * a.table_stride + first + i] = -1;
-    before += count;
+    const Span x = span(a, s);
+    for (int i = max(0, a.total - before) + threadIdx.x; i < x.count && x.page(i) < a.table_stride; i += 32)
+      a.table[(size_t)s * a.table_stride + x.page(i)] = -1;
+    before += x.count;
   }
 }
 
@@ -264,18 +274,18 @@ __device__ __forceinline__ bool find_page(const Expand& a, int out_page, int& se
   if (threadIdx.x < 32) {          // the requests' counts are summed 32 at a time
     int before = 0, who_seq = -1, at = 0, led = 0;
     for (int s0 = 0; s0 < a.n_seqs && who_seq < 0; s0 += 32) {
-      int first = 0, count = 0;
-      if (s0 + lane < a.n_seqs) span(a, s0 + lane, first, count);
-      int upto = count;
+      Span x{0, 0, 0};
+      if (s0 + lane < a.n_seqs) x = span(a, s0 + lane);
+      int upto = x.count;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
+        const int below = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += below;
       }
       const unsigned hit = __ballot_sync(0xffffffffu, before + upto > out_page);
       const int who = hit ? __ffs(hit) - 1 : 0;
-      const int start = __shfl_sync(0xffffffffu, before + upto - count, who), from = __shfl_sync(0xffffffffu, first, who);
-      if (hit) { who_seq = s0 + who; at = from + out_page - start; led = out_page == start; }
+      const int mine = out_page - (before + upto - x.count), here = __shfl_sync(0xffffffffu, x.page(mine), who);
+      if (hit) { who_seq = s0 + who; at = here; led = __shfl_sync(0xffffffffu, mine, who) == 0; }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
     if (lane == 0) { found[0] = who_seq; found[1] = at; found[2] = led; }
@@ -410,10 +420,7 @@ __global__ void __launch_bounds__(EXPAND_THREADS) expand_4bit_kernel(const Expan
   if (out_page == 0 && kvh == 0 && threadIdx.x < 32) check_total(a);
   if (!PREFILL && kvh == 0)          // the entries that no page of the result is for (with PREFILL: -1 already)
     for (long long i = (long long)out_page * blockDim.x + threadIdx.x; i < (long long)a.n_seqs * a.table_stride; i += (long long)a.total * blockDim.x) {
-      int first, count;
-      const int entry = (int)(i % a.table_stride);
-      span(a, (int)(i / a.table_stride), first, count);
-      if (entry < first || entry >= first + count) a.table[i] = -1;
+      if (!span(a, (int)(i / a.table_stride)).has((int)(i % a.table_stride))) a.table[i] = -1;
     }
   if (!find_page(a, out_page, seq, index, leads)) return;
   Held form{false, 0, 0};
@@ -514,10 +521,10 @@ int expand(const Expand& a, int hd, bool prefill, cudaStream_t stream) {
 
 extern "C" int hb_expand_pages_4bit(const void* pages, const int* block_table, int table_stride, const int* cu_seqlens,
                                     const int* positions, int n_seqs, int total, int page_size, int chunk, int window, int keep,
-                                    int skip_single, int nkv, int hd, void* k, void* v, int* table, int* status,
+                                    int whole, int skip_single, int nkv, int hd, void* k, void* v, int* table, int* status,
                                     cudaStream_t stream) {
   return expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)k, (uint16_t*)v, table, n_seqs,
-                       table_stride, page_size, chunk, window, keep, skip_single, nkv, total, nullptr, 0, 0, nullptr, nullptr, nullptr, 0.f, nullptr, status},
+                       table_stride, page_size, chunk, window, keep, whole, skip_single, nkv, total, nullptr, 0, 0, nullptr, nullptr, nullptr, 0.f, nullptr, status},
                 hd, false, stream);
 }
 
@@ -545,16 +552,14 @@ struct Room {
 // How many pages the requests' new tokens may read, by what the host knows of them (cu_seqlens and positions on the device say the same);
 // -1: a position lies outside a block table of `width` pages a request, or the mask is not one (first tokens are kept beside a sliding window, not beside chunks).
 extern "C" long long hb_expand_total(const int* start_pos, const int* n_new, int n_seqs, int width, int page_size, int chunk, int window,
-                                     int keep, int skip_single) {
+                                     int keep, int whole, int skip_single) {
   long long total = 0;
   if (!start_pos || !n_new || n_seqs < 0 || page_size <= 0 || chunk < 0 || window < 0 || keep < 0 || (keep > 0 && chunk > 0)) return -1;
   for (int s = 0; s < n_seqs; ++s) {
     const long long start = start_pos[s], n = n_new[s];
     if (n <= 0 || (n == 1 && skip_single)) continue;
-    const long long last = (start + n - 1) / page_size;
-    if (start < 0 || last >= width) return -1;
-    const long long low = chunk > 0 ? start / chunk * chunk : window > 0 && keep == 0 ? (start - window + 1 > 0 ? start - window + 1 : 0) : 0;
-    total += last - low / page_size + 1;
+    if (start < 0 || (start + n - 1) / page_size >= width) return -1;
+    total += span_of(start, n, page_size, chunk, window, keep, whole).count;
   }
   return total;
 }
@@ -580,7 +585,7 @@ extern "C" int hb_prefill_attention_4bit(const void* q, const void* pages, const
   float2* form = reinterpret_cast<float2*>(w + room.form);
   int* table = reinterpret_cast<int*>(w + room.table);
   int code = expand(Expand{(const uint8_t*)pages, block_table, cu_seqlens, positions, (uint16_t*)(w + room.k), (uint16_t*)(w + room.v), table,
-                           n_seqs, table_stride, page_size, chunk, window, keep, skip_single, nkv, total, (const __nv_bfloat16*)q, n_tokens, nh,
+                           n_seqs, table_stride, page_size, chunk, window, keep, 0, skip_single, nkv, total, (const __nv_bfloat16*)q, n_tokens, nh,
                            (int4*)(w + room.most), (uint16_t*)(w + room.q), q_scale, scale * 1.4426950408889634f, form, status},
                     hd, true, stream);
   if (code != HB_OK) return code;

@@ -38,7 +38,7 @@ _SIGNATURES = {
     "hb_moe_combine": [P, P, P, P, I, P, I, I, I, P],
     "hb_qkv_post": [P, I, P, I, I, I, F, I, F, F, P, P, I, I, F, P, I, I, I, P, P, P, I, P, P, P, I, I, I, I, I, I, P],
     "hb_qkv_post_4bit": [P, P, I, I, I, F, I, F, F, P, P, I, I, F, I, P, P, P, I, P, P, I, I, I, I, I, I, P],
-    "hb_expand_pages_4bit": [P, P, I, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P, P],
+    "hb_expand_pages_4bit": [P, P, I, P, P, I, I, I, I, I, I, I, I, I, I, P, P, P, P, P],
     "hb_prefill_attention_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, I, F, I, I, P, I, I, I, P, c_longlong, P, P],
     "hb_attention_decode_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, P, I, I, I, P, P, P, P, I, P],
     "hb_four_bit_linear": [P, c_longlong, P, P, P, I, I, I, I, I, P],
@@ -126,7 +126,7 @@ def lib():
         handle.hb_recurrence_chunked_scratch_floats.restype = c_longlong
         handle.hb_prefill_pair_idle_us.argtypes = [P, I, I, I, I, I, I, I, ctypes.c_double]
         handle.hb_prefill_pair_idle_us.restype = ctypes.c_double
-        handle.hb_expand_total.argtypes = [P, P, I, I, I, I, I, I, I]
+        handle.hb_expand_total.argtypes = [P, P, I, I, I, I, I, I, I, I]
         handle.hb_expand_total.restype = c_longlong
         handle.hb_prefill_attention_4bit_bytes.argtypes = [I, I, I, I, I, I, I, I, I]
         handle.hb_prefill_attention_4bit_bytes.restype = c_longlong
@@ -2669,7 +2669,7 @@ def qkv_post_4bit(qkv: torch.Tensor, nh: int, nkv: int, hd: int, positions: torc
     return q
 
 
-def _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos, n_new, chunk, window, keep, skip_single):
+def _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos, n_new, chunk, window, keep, whole, skip_single):
     """What the expansions of :func:`expand_pages_4bit` have in common: kv heads, page size and how many pages they make."""
     _, nkv, page_size = _four_bit_pages(kv_pages, hd)
     for t, nm in ((block_table, "block_table"), (cu_seqlens, "cu_seqlens"), (positions, "positions")):
@@ -2680,7 +2680,8 @@ def _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos,
         raise KernelError("start_pos, n_new, cu_seqlens and block_table do not speak of the same requests")
     _on_current_device(kv_pages, block_table, cu_seqlens, positions)
     starts, counts = array("i", start_pos), array("i", n_new)
-    total = lib().hb_expand_total(starts.buffer_info()[0], counts.buffer_info()[0], n_seqs, block_table.shape[1], page_size, chunk, window, keep, skip_single) if n_seqs else 0
+    total = lib().hb_expand_total(starts.buffer_info()[0], counts.buffer_info()[0], n_seqs, block_table.shape[1], page_size, chunk, window,
+                                  keep, whole, skip_single) if n_seqs else 0
     if total < 0 or total >= 1 << 31:
         raise KernelError(f"positions of {list(zip(start_pos, n_new))[:4]}... (first, count) lie outside the block table's "
                           f"{block_table.shape[1]} pages a request, or a mask of {chunk}, {window} and {keep} tokens is not one")
@@ -2688,21 +2689,21 @@ def _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos,
 
 
 def expand_pages_4bit(kv_pages: torch.Tensor, hd: int, block_table: torch.Tensor, cu_seqlens: torch.Tensor, positions: torch.Tensor,
-                      start_pos, n_new, chunk: int = 0, window: int = 0, keep: int = 0, skip_single: bool = False):
+                      start_pos, n_new, chunk: int = 0, window: int = 0, keep: int = 0, skip_single: bool = False, whole: bool = True):
     """The pages that the step's new tokens may read, in bfloat16: ``(k_pages, v_pages, table)`` with pages [P, nkv, page_size, hd],
     request after request from the page of the oldest position that its first new token reads (``chunk``, ``window``, ``keep``
-    as in :func:`paged_attention`; with ``keep`` from the request's first page on) to its last token's, and the block table
-    that names them (-1: no page). Rows behind a request's last token hold whatever the pool holds there. ``start_pos`` and ``n_new`` are
+    as in :func:`paged_attention`; with ``keep`` from the request's first page on, or with ``whole=False`` the kept tokens' pages in front
+    of the window's and none between them) to its last token's, and the block table that names them (-1: no page). Rows behind a request's last token hold whatever the pool holds there. ``start_pos`` and ``n_new`` are
     the host's copies of what ``positions`` and ``cu_seqlens`` say on the device; where those ask for another number of pages,
     :func:`check_tc_status` raises. ``skip_single``: requests of one new token are left out."""
-    nkv, page_size, total = _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos, n_new, chunk, window, keep, skip_single)
+    nkv, page_size, total = _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos, n_new, chunk, window, keep, whole, skip_single)
     k, v = kv_pages.new_empty((2, total, nkv, page_size, hd), dtype=torch.bfloat16).unbind(0)
     if not total:
         return k, v, torch.full_like(block_table, -1)
     table = torch.empty_like(block_table) if block_table.shape[0] == len(n_new) else torch.full_like(block_table, -1)
     TC_USED[0] = True
     _check(lib().hb_expand_pages_4bit(_ptr(kv_pages), _ptr(block_table), block_table.shape[1], _ptr(cu_seqlens), _ptr(positions),
-                                      len(n_new), total, page_size, chunk, window, keep, skip_single, nkv, hd, _ptr(k), _ptr(v), _ptr(table),
+                                      len(n_new), total, page_size, chunk, window, keep, whole, skip_single, nkv, hd, _ptr(k), _ptr(v), _ptr(table),
                                       _ptr(_tc_status(kv_pages.device)), _stream()), "expand_pages_4bit")
     return k, v, table
 
@@ -2717,7 +2718,7 @@ def prefill_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table:
     them a request gets depends on its own rows alone. Rows of requests that ``skip_single`` leaves out are not written."""
     _need(q, "q", torch.bfloat16)
     n, nh, hd = q.shape
-    nkv, page_size, total = _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos, n_new, chunk, window, keep, skip_single)
+    nkv, page_size, total = _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos, n_new, chunk, window, keep, False, skip_single)
     if nh % nkv or q.data_ptr() % 16 or not scale > 0:
         raise KernelError(f"{nh} query heads on {nkv} kv heads (a multiple), q on 16 bytes and a scale above zero are taken")
     if sink_values is not None:

@@ -156,7 +156,7 @@ def attend_over_four_bit_pages(q, kv_pages, block_table, ctx, nh: int, nkv: int,
         raise ValueError(f"queries {tuple(q.shape)} and pages of {kv_pages.shape[1]} kv heads for {ctx.n_tokens} tokens, {nh} heads on {nkv}")
     spans = (block_table, ctx.cu_seqlens, ctx.positions, ctx.start_pos, ctx.n_new)
     if softcap or slopes is not None:
-        k, v, table = ops.expand_pages_4bit(kv_pages, hd, *spans, chunk, sliding, keep)
+        k, v, table = ops.expand_pages_4bit(kv_pages, hd, *spans, chunk, sliding, keep, whole=False)
         return attend_over_pages(q, k, v, table, ctx, nh, nkv, hd, chunk, sliding, scale, sink=sink, softcap=softcap, slopes=slopes,
                                  sink_values=sink_values, keep=keep)
 

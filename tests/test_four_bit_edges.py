@@ -359,6 +359,26 @@ def test_codes_of_more_than_four_bits_are_refused():
 NO_MASK = [dict(chunk=512, keep=5), dict(chunk=64, window=1000, keep=200)]
 
 
+def test_pages_between_kept_tokens_and_a_window_are_not_asked_for():
+    """On the CPU: the count grows with the window, not with the context; and with every page of the request where all are wanted."""
+    from array import array
+
+    from hi_b200.kernels import ops
+
+    def total(start, n, page, chunk=0, window=0, keep=0, whole=0):
+        starts, counts = array("i", start), array("i", n)
+        return ops.lib().hb_expand_total(starts.buffer_info()[0], counts.buffer_info()[0], len(n), 1 << 24, page, chunk, window, keep, whole, 0)
+
+    for start, n, page, window, keep in ((10_000_000, 20, 64, 1024, 4), (5000, 300, 16, 100, 70), (90, 40, 64, 64, 130), (200, 1, 32, 20, 33)):
+        last, first = (start + n - 1) // page, (start - window + 1) // page
+        kept = -(-keep // page)
+        assert total([start], [n], page, window=window, keep=keep) == len(set(range(kept)) | set(range(first, last + 1)) - set(range(first)))
+        assert total([start], [n], page, window=window, keep=keep, whole=1) == last + 1
+    assert total([700, 40], [10, 0], 64) == total([700, 40], [10, 0], 64, keep=5) == 12
+    for wrong in (dict(chunk=-1), dict(window=-1), dict(keep=-1), *NO_MASK):
+        assert total([700], [10], 64, **wrong) == -1
+
+
 @pytest.mark.parametrize("wrong", NO_MASK, ids=str)
 def test_kept_tokens_beside_chunks_are_refused_by_the_entries(wrong):
     """On the CPU: the entry points look at the mask before anything is launched or read."""
@@ -370,7 +390,7 @@ def test_kept_tokens_beside_chunks_are_refused_by_the_entries(wrong):
     lib = ops.lib()
     assert lib.hb_attention_decode_4bit(p, p, p, 4, p, p, p, 1, 8, 2, 64, 64, chunk, window, keep, 0.1, 0, None, 1, 1, 0, None, None, p, None, 1,
                                         None) == 1001
-    assert lib.hb_expand_pages_4bit(p, p, 4, p, p, 1, 1, 64, chunk, window, keep, 0, 2, 64, p, p, p, p, None) == 1001
+    assert lib.hb_expand_pages_4bit(p, p, 4, p, p, 1, 1, 64, chunk, window, keep, 1, 0, 2, 64, p, p, p, p, None) == 1001
 
 
 @pytest.mark.gpu
@@ -385,3 +405,52 @@ def test_kept_tokens_beside_chunks_are_refused(wrong):
             with pytest.raises(ops.KernelError):
                 attend_over_four_bit_pages(step.q, step.pages, step.table, step.ctx, 8, 2, 64, wrong.get("chunk", 0), wrong.get("window", 0), 0.125,
                                            softcap=cap, keep=wrong["keep"])
+
+
+KEPT = [
+    ([(40, 3000), (150, 20), (1, 2000)], 64, dict(window=100, keep=4)),
+    ([(40, 3000), (16, 64), (33, 700)], 16, dict(window=100, keep=70)),
+    ([(40, 300), (150, 20)], 32, dict(window=90, keep=200)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", KEPT, ids=lambda c: f"p{c[1]}" + "".join(f"_{k}{v}" for k, v in c[2].items()))
+def test_portions_with_kept_tokens(case):
+    """Kept tokens in front of a window, more and fewer than a page, also where no page lies between them; what nobody may read is
+    not finite."""
+    from hi_b200.kernels import ops
+    from hi_b200.parts.attention import attend_over_four_bit_pages
+
+    portions, page, mask = case
+    step = _step(portions, 8, 2, 64, page, seed=page + len(portions))
+    window, keep = mask["window"], mask["keep"]
+    hidden = []
+    for s, (n, c) in enumerate(portions):
+        seen = visible(step.positions[step.cu[s]: step.cu[s + 1]], n + c, **mask)
+        unseen = (~seen.any(0)).nonzero().flatten()
+        whole = [int(p) for p in unseen if p // page * page + page <= n + c and (~seen.any(0))[p // page * page: p // page * page + page].all()]
+        step.k[s][whole], step.v[s][whole] = float("nan"), float("nan")
+        hidden.append(len(whole))
+    assert any(hidden) or keep == 200
+    step.fill()
+    for s, (n, c) in enumerate(portions):                        # and their pages are given back
+        seen = visible(step.positions[step.cu[s]: step.cu[s + 1]], n + c, **mask).any(0)
+        for p in range((n + c) // page):
+            if not seen[p * page: p * page + page].any():
+                step.table[s, p] = -1
+    for cap in (0.0, 8.0):
+        got = attend_over_four_bit_pages(step.q, step.pages, step.table, step.ctx, 8, 2, 64, 0, window, 0.125, softcap=cap, keep=keep)
+        ops.check_tc_status()
+        for s in range(len(portions)):
+            if cap:
+                _check_reshaped(step, s, got, mask, 0.125, cap)
+            else:
+                from test_four_bit import _check_rows
+
+                rows = slice(step.cu[s], step.cu[s + 1])
+                seen = visible(step.positions[rows], step.k[s].shape[0], **mask).any(0)
+                k, v = step.k[s], step.v[s]
+                step.k[s], step.v[s] = k.masked_fill(~seen.view(-1, 1, 1), 0), v.masked_fill(~seen.view(-1, 1, 1), 0)
+                _check_rows(step, s, got, mask, 0.125, None, portions[s][0] == 1)
+                step.k[s], step.v[s] = k, v
