@@ -85,6 +85,30 @@ def pool_tokens_for_budget(cache_specs: Dict[int, Optional[CacheSpec]], element_
     return [-(-t // page_size) * page_size for t in tokens]
 
 
+def pool_tokens_that_fit(cache_specs: Dict[int, Optional[CacheSpec]], element_size: int, free_bytes: int, fraction: float,
+                         scratch_bytes: int, scratch_per_token: Dict[int, int], page_size: int, max_requests: int,
+                         most_tokens: Optional[int] = None) -> List[int]:
+    """Pool sizes (tokens per group) from the free memory: :func:`pool_tokens_for_budget` of :func:`pool_budget`, or of less where a workspace
+    that grows with the pools (``scratch_per_token``: bytes a token by cache slot, one slot at a time) would not fit beside them."""
+    _, group_of = plan_groups(cache_specs)
+
+    def tokens(budget):
+        return pool_tokens_for_budget(cache_specs, element_size, budget, page_size, max_requests, most_tokens)
+
+    def fits(budget):
+        t = tokens(budget)
+        return budget + scratch_bytes + max((each * t[group_of[slot]] for slot, each in scratch_per_token.items()), default=0) <= free_bytes
+
+    most = pool_budget(free_bytes, fraction, scratch_bytes)
+    if fits(most):
+        return tokens(most)
+    low = 0
+    while most - low > 1 << 16:                                  # the largest budget that leaves room, to 64 KB
+        mid = (low + most) // 2
+        low, most = (mid, most) if fits(mid) else (low, mid)
+    return tokens(low)
+
+
 class DeviceCache:
     def __init__(self, cache_specs: Dict[int, Optional[CacheSpec]], pages_per_group: Sequence[int], page_size: int,
                  max_requests: int, dtype: torch.dtype, device, block_state_sizes: Optional[Dict[int, int]] = None):

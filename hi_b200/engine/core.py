@@ -18,7 +18,7 @@ from typing import Dict, Hashable, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
-from ..cache.device import DeviceCache, plan_groups, pool_budget, pool_tokens_for_budget
+from ..cache.device import DeviceCache, plan_groups, pool_tokens_that_fit
 from ..cache.pages import CacheManager, OutOfPages
 from ..config.registry import load_architecture, lookup
 from ..parts.context import StepContext
@@ -108,9 +108,9 @@ class Engine:
                 raise ValueError("cache_memory_fraction must lie in (0, 1]")
             free, _total = torch.cuda.mem_get_info(self.device)
             longest = model.spec.max_position_embeddings
-            auto = pool_tokens_for_budget(model.cache_specs, torch.empty((), dtype=model.dtype).element_size(),
-                                          pool_budget(free, cache_memory_fraction, model.scratch_bytes), self.page_size, max_active_requests,
-                                          most_tokens=None if longest is None else longest * max_active_requests)
+            auto = pool_tokens_that_fit(model.cache_specs, torch.empty((), dtype=model.dtype).element_size(), free, cache_memory_fraction,
+                                        model.scratch_bytes, model.scratch_per_token, self.page_size, max_active_requests,
+                                        most_tokens=None if longest is None else longest * max_active_requests)
         pages = []
         for g, spec in enumerate(groups):
             if auto is not None:

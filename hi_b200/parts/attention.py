@@ -354,8 +354,10 @@ class AttentionMixer(Part):
             self.hd = next((r for r in ops.FOUR_BIT_ROW_LENGTHS if r >= self.hd), self.hd)
             if self.hd > ops.FOUR_BIT_ROW_LENGTHS[-1]:
                 raise ValueError(f"{prefix}: a cache in four bits has heads of up to {ops.FOUR_BIT_ROW_LENGTHS[-1]}, not {self.hd}")
-            # pages of portions are expanded for the step's prefill kernels: room for 262,144 tokens (portions behind more ask for more)
-            self.scratch_bytes = 262144 * 4 * self.nkv * self.hd
+            # what portions may read is expanded for the step's prefill kernels: every page of the pool at most, once; beside it their queries and
+            # their scales, of 8,192 tokens
+            self.scratch_per_token = 4 * self.nkv * self.hd
+            self.scratch_bytes = 8192 * self.nh * (2 * self.hd + 4)
             # capped or biased scores go over pages expanded by the host's positions, which a captured step does not know
             self.graph_safe = not self.softcap and self.distance_bias is None
         if self.hd > (1024 if self.hd != self.dim or self.norm_weighted or self.unpadded or self.values_are_keys else 256):

@@ -95,6 +95,12 @@ class Model:
         self.loaded = False
         self.graph_safe = all(getattr(p, "graph_safe", False) for p in self.all_parts())
         self.scratch_bytes = max(getattr(p, "scratch_bytes", 0) for p in self.all_parts())       # one part at a time
+        # the part of a cache slot asks for so many bytes a token that its page group has room for
+        self.scratch_per_token: Dict[int, int] = {}
+        for entry in spec.schedule:
+            each = getattr(self.layers[entry.layer].mixer, "scratch_per_token", 0)
+            if each:
+                self.scratch_per_token[entry.cache] = each
 
     # ---- weights
     def all_parts(self):

@@ -454,3 +454,33 @@ def test_portions_with_kept_tokens(case):
                 step.k[s], step.v[s] = k.masked_fill(~seen.view(-1, 1, 1), 0), v.masked_fill(~seen.view(-1, 1, 1), 0)
                 _check_rows(step, s, got, mask, 0.125, None, portions[s][0] == 1)
                 step.k[s], step.v[s] = k, v
+
+
+def test_pools_leave_room_for_the_pages_that_portions_expand():
+    """On the CPU: every page of a layer's pool as bfloat16 keys and values, and the portions' queries, fit beside the pools, whatever fraction of the
+    memory they may take; pools in 16 bits are as large as before."""
+    from hi_b200.cache.device import bytes_per_token, plan_groups, pool_budget, pool_tokens_for_budget, pool_tokens_that_fit
+    from hi_b200.config.registry import lookup
+    from hi_b200.parts.model import Model
+    from tiny_configs import TINY_A
+
+    cfg = dict(TINY_A, head_dim=128, attention_chunk_size=1 << 20)
+    arch = lookup(cfg)
+    spec = arch.build_spec(arch.parse_config(cfg, None))
+    for bits in (16, 4):
+        model = Model(spec, BF16, "cpu", cache_bits=bits)
+        _, group_of = plan_groups(model.cache_specs)
+        cost = bytes_per_token(model.cache_specs, 2)
+        for free in (1 << 26, 1 << 30, 5 << 30):
+            for fraction in (0.5, 0.9, 1.0):
+                args = (model.cache_specs, 2, free, fraction, model.scratch_bytes, model.scratch_per_token, 64, 2)
+                tokens = pool_tokens_that_fit(*args)
+                plain = pool_tokens_for_budget(model.cache_specs, 2, pool_budget(free, fraction, model.scratch_bytes), 64, 2)
+                if bits == 16:
+                    assert tokens == plain
+                    continue
+                need = max(each * tokens[group_of[slot]] for slot, each in model.scratch_per_token.items())
+                assert all(model.scratch_per_token[slot] == 4 * cs.kv_heads * cs.head_dim for slot, cs in model.cache_specs.items() if cs.paged)
+                taken = sum(c * t for c, t in zip(cost, tokens)) + need + model.scratch_bytes
+                assert free - (1 << 20) <= taken <= free + (1 << 17) if tokens != plain else taken <= free + (1 << 17)
+                assert pool_tokens_that_fit(*args, most_tokens=4096) == [min(t, 4096) for t in tokens]
