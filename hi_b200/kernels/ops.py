@@ -2571,8 +2571,9 @@ def four_bit_linear(x: torch.Tensor, weight: FourBitWeight, out_dtype: torch.dty
                     bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ weight.T (+ bias)`` for bfloat16 ``x`` [N, K] (its rows may be a column slice of a wider matrix) and a weight held in
     four bits, with float32 sums, in ``out_dtype`` (bfloat16 or float32); ``bias`` bfloat16 [M]. Up to 16 rows of ``x`` the products are
-    those of the weight's exact values; more rows take each value rounded to bfloat16, as a bfloat16 weight would hold it. Inputs are below
-    2^63 and scales below 2^54 in size; what scales under 2^-60 add is lost."""
+    those of the weight's exact values; more rows take each value rounded to bfloat16, as a bfloat16 weight would hold it. Scales are below
+    2^54 in size; what scales under 2^-60 add is lost. Inputs of 2^64 and more, and infinities, are multiplied as any other (a row that has one takes its
+    sums one product after the other, up to 16 rows)."""
     if not x.is_cuda:
         raise KernelError("x must be a CUDA tensor; this engine has no CPU path")
     m, k = weight.shape

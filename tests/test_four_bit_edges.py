@@ -484,3 +484,41 @@ def test_pools_leave_room_for_the_pages_that_portions_expand():
                 taken = sum(c * t for c, t in zip(cost, tokens)) + need + model.scratch_bytes
                 assert free - (1 << 20) <= taken <= free + (1 << 17) if tokens != plain else taken <= free + (1 << 17)
                 assert pool_tokens_that_fit(*args, most_tokens=4096) == [min(t, 4096) for t in tokens]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,group", [(40, 256, 32), (300, 2112, 64), (33, 50048, 128), (17, 50048, 32)])
+@pytest.mark.parametrize("tokens", [1, 8, 13, 16, 20])
+def test_linear_of_inputs_that_are_large_or_infinite(m, k, group, tokens):
+    """Infinite outputs where the definition has them, NaN where infinities of both signs meet or one meets a weight of zero; finite ones to the
+    float32 sums' rounding (K steps of 2^-24 of all magnitudes; the weight's rounding to bfloat16 from 17 rows on). Other rows do not change."""
+    from hi_b200.kernels import ops
+    from plain_four_bit import weight_values
+
+    g = torch.Generator(device=DEV).manual_seed(m + k + tokens)
+    codes = torch.randint(0, 16, (m, k), device=DEV, generator=g).to(torch.uint8)
+    scales = ((0.5 + torch.rand(m, k // group, device=DEV, generator=g)) * 0.2 * k ** -0.5).to(BF16)
+    w = ops.pack_weight(codes, scales)
+    x = torch.randn(tokens, k, device=DEV, generator=g).to(BF16)
+    bias = torch.randn(m, device=DEV, generator=g).to(BF16)
+    plain = ops.four_bit_linear(x, w, torch.float32, bias)
+    changed = sorted({0, tokens // 2, tokens - 1})
+    x[changed[0], k - 1] = math.inf
+    if len(changed) > 1:
+        x[changed[1], 5], x[changed[1], k // 2] = 2.0 ** 100, -(2.0 ** 90)
+        x[changed[2], 3], x[changed[2], k - 30] = math.inf, -math.inf
+    got = ops.four_bit_linear(x, w, torch.float32, bias)
+    ops.check_tc_status()
+    exact = weight_values(codes, scales)
+    for t in range(tokens):
+        if t not in changed:
+            assert torch.equal(got[t], plain[t])
+            continue
+        products = x[t].double() * exact
+        want = products.sum(1) + bias.double()
+        finite = want.isfinite()
+        assert torch.equal(got[t].isnan(), want.isnan()) and torch.equal(got[t][want.isinf()].double(), want[want.isinf()])
+        tol = (k * 2.0 ** -24 + (2.0 ** -8 if tokens > 16 else 0.0)) * products.abs().sum(1) + 2.0 ** -23 * want.abs()
+        assert ((got[t].double() - want).abs() <= tol)[finite].all()
+    if tokens == 1:
+        assert got.isinf().any()
