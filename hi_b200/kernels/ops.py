@@ -2718,6 +2718,9 @@ def prefill_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table:
     expanded to float16, divided by a power of two each, where their groups' magnitudes lie within 2^13 of one another, else to bfloat16; which of
     them a request gets depends on its own rows alone. Rows of requests that ``skip_single`` leaves out are not written."""
     _need(q, "q", torch.bfloat16)
+    if q.dim() != 3 or q.shape[0] < sum(n_new) or key_splits < 1:
+        raise KernelError(f"q is [tokens, heads, head_dim] with a row for each of {sum(n_new)} tokens, not {tuple(q.shape)}, and keys are shared by "
+                          f"one block or more, not {key_splits}")
     n, nh, hd = q.shape
     nkv, page_size, total = _four_bit_spans(kv_pages, hd, block_table, cu_seqlens, positions, start_pos, n_new, chunk, window, keep, False, skip_single)
     if nh % nkv or q.data_ptr() % 16 or not scale > 0:

@@ -522,3 +522,19 @@ def test_linear_of_inputs_that_are_large_or_infinite(m, k, group, tokens):
         assert ((got[t].double() - want).abs() <= tol)[finite].all()
     if tokens == 1:
         assert got.isinf().any()
+
+
+@pytest.mark.gpu
+def test_portions_of_more_tokens_than_queries_are_refused():
+    from hi_b200.kernels import ops
+
+    step = _step([(40, 100), (30, 0)], 8, 2, 64, 64, seed=7).fill()
+    ctx = step.ctx
+    call = lambda q, **kw: ops.prefill_attention_4bit(q, step.pages, step.table, ctx.cu_seqlens, step.positions, ctx.start_pos, ctx.n_new, 0, 0, 0.1, **kw)
+    for q in (step.q[:69], step.q[0], step.q[:, :7].contiguous()):
+        with pytest.raises(ops.KernelError):
+            call(q)
+    with pytest.raises(ops.KernelError):
+        call(step.q, key_splits=0)
+    call(step.q)
+    ops.check_tc_status()
