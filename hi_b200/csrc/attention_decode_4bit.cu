@@ -176,15 +176,37 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn_decode_4bit_kernel(const A
   look(0);
   for (int i = 0; i < min(STAGES, steps); ++i) bring(i, 0u);
 
-  // the heads' queries as columns, raised; their sums over a group in three pieces
+  // the heads' queries as columns, raised; their sums over a group in three pieces. A row whose largest element is not 2^-30 .. 2^60 is brought there
+  // by a power of two, which its scale takes back: smaller ones lost pieces of their sums, larger ones would be infinite where they are raised.
   uint4 qf[G];
   uint2 q_sums;
+  float to_log2[2];                                               // of the lane's two heads
   {
     float sums[G];
+    unsigned most = 0u;
 #pragma unroll
     for (int c = 0; c < G; ++c) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (g < heads) v = *reinterpret_cast<const uint4*>(a.q + (row0 + g) * HD + c * 32 + q4 * 8);
+      qf[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (g < heads) qf[c] = *reinterpret_cast<const uint4*>(a.q + (row0 + g) * HD + c * 32 + q4 * 8);
+      const unsigned w[4] = {qf[c].x, qf[c].y, qf[c].z, qf[c].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = __vmaxu2(most, w[i] & 0x7fff7fffu);
+    }
+    most = max(most >> 16, most & 0xffffu);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const int e_q = (int)(most >> 7) - 127;                       // (zero and numbers that are not normal: -127)
+    const int down = most == 0u || e_q == 128 ? 0 : e_q < -30 ? e_q + 30 : max(0, e_q - 59);      // infinite: as it is
+    const unsigned factor = (unsigned)(127 - down) << 7 | (unsigned)(127 - down) << 23;           // 2^-down, twice
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int theirs = min(__shfl_sync(0xffffffffu, down, (2 * q4 + h) * 4), 56);               // (2^(69 + 56) times the scale: a float)
+      to_log2[h] = a.scale * 1.4426950408889634f * fb::UNSCALE * __int_as_float((127 + theirs) << 23);
+    }
+#pragma unroll
+    for (int c = 0; c < G; ++c) {
+      uint4 v = qf[c];
+      if (down != 0) v = make_uint4(fb::times(v.x, factor), fb::times(v.y, factor), fb::times(v.z, factor), fb::times(v.w, factor));
       const unsigned w[4] = {v.x, v.y, v.z, v.w};
       float sum = 0.f;
 #pragma unroll
@@ -204,8 +226,6 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn_decode_4bit_kernel(const A
       q_sums = make_uint2(q4 == 0 ? p[0] : q4 == 1 ? p[1] : q4 == 2 ? p[2] : 0u, 0u);
     }
   }
-  const float to_log2 = a.scale * 1.4426950408889634f * fb::UNSCALE;
-
   float m_run[2] = {-INFINITY, -INFINITY};
   float o[2 * G][4];                                              // dims 4 g + (0, 1) and (2, 3) of every group
   float low[4] = {0.f, 0.f, 0.f, 0.f};                            // rows g < G: lows' sums, G .. 2 G - 1: scales'; row 8: the weights'
@@ -268,7 +288,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn_decode_4bit_kernel(const A
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-      m_new[h] = m * to_log2;                                     // (the scale is positive)
+      m_new[h] = m * to_log2[h];                                     // (the scale is positive)
       grows = grows || m_new[h] > m_run[h] + 1.f;                 // (of a head that has seen nothing yet: any)
     }
     if (__any_sync(0xffffffffu, grows)) {
@@ -291,7 +311,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn_decode_4bit_kernel(const A
       const uint8_t* b = blocks + mt * B::BYTES;
       float p[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = exp2_fast(fmaf(s[mt][e], to_log2, base[e & 1]));
+      for (int e = 0; e < 4; ++e) p[e] = exp2_fast(fmaf(s[mt][e], to_log2[e & 1], base[e & 1]));
       // rows of the bare weights' product: a group's lows, a group's scales (columns of the records of 8 keys), at 8 ones
       unsigned la, lb;
       {

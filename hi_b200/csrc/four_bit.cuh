@@ -15,13 +15,13 @@ constexpr unsigned LOW = 0x000f000fu, HIGH = 0x00f000f0u;      // pairs of codes
 // a sum of products of 2^64 x and codes, put back to its size
 constexpr float UNSCALE = 590295810358705651712.f;             // 2^69
 
-// a pair of bfloat16 times 2^64 or 2^60
-__device__ __forceinline__ unsigned raised(unsigned pair, bool by_60) {
-  const unsigned factor = by_60 ? 0x5d805d80u : 0x5f805f80u;
+__device__ __forceinline__ unsigned times(unsigned pair, unsigned by) {
   unsigned r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(pair), "r"(factor));
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(pair), "r"(by));
   return r;
 }
+// a pair of bfloat16 times 2^64 or 2^60
+__device__ __forceinline__ unsigned raised(unsigned pair, bool by_60) { return times(pair, by_60 ? 0x5d805d80u : 0x5f805f80u); }
 // c[0..3] += rows (word_a: rows lane / 4, word_b: rows + 8) of 32 codes a row, eight a lane, times eight columns: x holds the lane's
 // eight elements of its column (lane / 4), raised by 64, 60, 64, 60
 __device__ __forceinline__ void mma_codes(float (&c)[4], unsigned word_a, unsigned word_b, const uint4& x) {

@@ -2637,7 +2637,8 @@ def qkv_post_4bit(qkv: torch.Tensor, nh: int, nkv: int, hd: int, positions: torc
                   norm_first: bool = False, norm_dim: int = 0, rot_mul: float = 1.0, values_are_keys: bool = False) -> torch.Tensor:
     """:func:`qkv_post` for a cache held in four bits: the same encoding of q, k and v from bfloat16 ``qkv``, after which the rows of
     k and v are quantised in groups of 32 dims (a bfloat16 scale and a bfloat16 least value each) and appended to ``kv_pages``
-    (uint8 [pages, nkv, :func:`four_bit_page_bytes`]). Returns q [N, nh, hd]."""
+    (uint8 [pages, nkv, :func:`four_bit_page_bytes`]). A group with a value that is not finite, or whose values span more than 3.3e38, is
+    cached as NaN. Returns q [N, nh, hd]."""
     _need(qkv, "qkv", torch.bfloat16)
     _, nkv2, page_size = _four_bit_pages(kv_pages, hd)
     n, columns = qkv.shape[0], (nh + (1 if values_are_keys else 2) * nkv) * hd
@@ -2788,7 +2789,8 @@ def decode_attention_4bit(q: torch.Tensor, kv_pages: torch.Tensor, block_table: 
                           out: Optional[torch.Tensor] = None, most_keys: int = 0) -> torch.Tensor:
     """:func:`decode_attention` over a cache held in four bits: every row of bfloat16 ``q`` [N, nh, hd] (or with ``rows``, int64 and distinct,
     those tokens, into ``out``) is one request's token. ``chunk``, ``window``, ``keep``, ``sink``, ``sink_values``, ``max_context``,
-    ``most_keys`` as there; first tokens are kept beside a sliding window, not beside chunks."""
+    ``most_keys`` as there; first tokens are kept beside a sliding window, not beside chunks. The scales of cached values lie between 2^-60 and 2^62
+    (what smaller ones add is lost, larger ones give infinities)."""
     _need(q, "q", torch.bfloat16)
     if q.dim() != 3:
         raise KernelError("q is [tokens, heads, head_dim]")

@@ -538,3 +538,37 @@ def test_portions_of_more_tokens_than_queries_are_refused():
         call(step.q, key_splits=0)
     call(step.q)
     ops.check_tc_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_decode_with_queries_of_any_size(hd):
+    """Keys times a power of two and queries divided by it give the same numbers bit by bit. Beside a head whose query is zero or not finite: so do
+    other tokens and other kv heads; heads of the same one follow their maxima together, and stay within a decode step's roundings."""
+    from hi_b200.kernels import ops
+    from test_four_bit import _check_rows
+
+    def run(e, change=None):
+        step = _step([(1, 300), (1, 40), (1, 1000)], 16, 2, hd, 64, seed=51)
+        step.k, q = [k * 2.0 ** e for k in step.k], step.q * 2.0 ** -e
+        step.fill()
+        if change is not None:
+            q[1, 3], q[2, 9, 5] = 0.0, change
+        out = ops.decode_attention_4bit(q, step.pages, step.table, step.seq, step.positions, 0, 0, hd ** -0.5, 1001)
+        ops.check_tc_status()
+        if change is not None:
+            step.q = q
+            _check_rows(step, 1, out, {}, hd ** -0.5, None, True)           # the token with a query of zeros
+        return out
+
+    want, largest = run(0), _step([(1, 300), (1, 40), (1, 1000)], 16, 2, hd, 64, seed=51).v[2]
+    for e in (60, -60, 64, -64, 100, -100):
+        assert torch.equal(run(e), want)
+    for change in (math.inf, float("nan")):
+        got = run(0, change)
+        others = torch.ones(3, 16, dtype=torch.bool, device=DEV)
+        others[1, :8] = others[2, 8:] = False
+        assert torch.equal(got[others], want[others]) and got[2, 9].isnan().all()
+        mates = [8, 10, 11, 12, 13, 14, 15]
+        # either is within 2^-8 of the values' parts, up to 3 of the largest, and twice 2^-8 of itself
+        assert ((got[2, mates].double() - want[2, mates].double()).abs() <= 2 * 2.0 ** -8 * 5 * values(quantise(largest)).abs().amax()).all()
