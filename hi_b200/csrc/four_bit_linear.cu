@@ -11,7 +11,7 @@
 // the fragments' order, raised by 2^64 once, each warp's own part; the row tiles of a block follow one another and the loads run ahead
 // over their ends, three blocks a warp, asked for again where they were used (before the use, into copies, with addresses worked out
 // anew: 163 instructions a block of weights, 8 x 16,384 x 5,120 14.5 us instead of 13.1). The warps' sums meet in shared memory in a fixed order.
-// 8 x 16,384 x 5,120 3.3 TB/s, 1 x 2,048 x 2,048 2.9 us of which 2 are the launch; what bounds it is each warp's chain of loads, unpacking and
+// 8 x 16,384 x 5,120 3.2 TB/s (13.5 us), 1 x 2,048 x 2,048 2.9 us of which 2 are the launch; what bounds it is each warp's chain of loads, unpacking and
 // products (a warp takes 900 cycles a block of weights, 8.4 an instruction), not HBM (0.5 of its rate) nor the tensor cores (0.19). Measured
 // and not kept, 8 x 16,384 x 5,120 / 1 x 5,120 x 8,192: a ring of bulk copies a warp and two row tiles at a time 15.3 / 19.7, two or four sums a group
 // of their own 14.9 / 11.6, sums joined by the warps in turn without a barrier 13.5 / 11.6, clusters that share K 19.7 / 13.9.

@@ -144,7 +144,8 @@ class Engine:
                  kv_cache_bits: int = 16, **options) -> "Engine":
         """Load a model folder (config.json + safetensors); the model class is chosen by config.json. ``weight_bits=4``: attention's
         projections, dense feed-forwards and shared experts are quantised to four bits as they are loaded, ``weight_group`` inputs
-        to a scale (routed experts, embeddings, the head and other mixers stay as they are). ``kv_cache_bits=4``: keys and values are
+        to a scale (routed experts, embeddings, the head and other mixers stay as they are, and weights stored in 32 bits or with inputs that are
+        not a multiple of 32). ``kv_cache_bits=4``: keys and values are
         cached in four bits (models whose mixers with a paged cache are plain softmax attention, heads of up to 128; where their scores are
         capped or biased by distance, steps are not captured)."""
         arch, cfg, _raw = load_architecture(model_dir)
