@@ -90,6 +90,16 @@ int hb_four_bit_linear(const void* x, long long x_ld, const void* w, const void*
 int hb_four_bit_linear_tc(const void* x, long long x_ld, const void* w, const void* bias, void* out, int out_dtype, int tokens,
                           int n_out, int K, int group, int* status, cudaStream_t stream);
 
+// Microscaled 4-bit floats (mx.cuh): rows to codes and scales (in an expert plan's order, if given), back to values, and their product with such
+// weights, plain or as a gated unit that leaves quantised. status: nonzero after a wait that ran out.
+int hb_mx_quantize(const void* x, int dtype, long long x_ld, int rows, int K, const int* sorted_entry, int top_k, const int* offsets,
+                   int experts, void* codes, void* scales, cudaStream_t stream);
+int hb_mx_values(const void* codes, const void* scales, int rows, int K, const int* offsets, int experts, void* out, int out_dtype,
+                 cudaStream_t stream);
+int hb_mx_gemm(const void* x, const void* x_scales, int rows, const int* offsets, int experts, const void* w, const void* w_scales, int n_out,
+               int K, const void* bias, const int* sorted_entry, const float* scores, int glu, float limit, void* out, int out_dtype,
+               void* out_scales, int* status, cudaStream_t stream);
+
 // sink != 0 (every attention entry point): the softmax's denominator has one more term of score 0,
 // p_j = e^{s_j} / (1 + sum e^{s_j}); the term has no value. The general kernel and the merge also take
 // sink_values (float32 [nh] or null): the term's score is the head's own number instead of 0. The general

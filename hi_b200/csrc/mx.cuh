@@ -1,0 +1,80 @@
+// Microscaled 4-bit floats: blocks of 32 values along a row share a power of two (a byte, 127 + e; 255: not a number), a value is 2^e times
+// an e2m1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives, 8 being the sign). Rows lie as the tensor cores read them:
+//   codes   [rows, K / 2]: two to a byte, the even one in the low half;
+//   scales  [tiles][chunks(K)][512]: a tile is 128 rows, a chunk 128 values, and row r's byte of block b of a chunk at
+//           (r % 32) 16 + r / 32 * 4 + b: lanes of tensor memory are r % 32, columns r / 32 (tcgen05.cp 32x128b.warpx4). Chunks are an
+//           even number, those past K are zeros. Rows of several experts begin a tile each, so tile numbers follow from the plan's offsets.
+#pragma once
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace mx {
+
+constexpr int BLOCK = 32, TILE = 128, CHUNK = 128, ATOM = 512;
+
+__host__ __device__ constexpr int chunks(int k) { return (k + 2 * CHUNK - 1) / (2 * CHUNK) * 2; }
+// where a row of a tile has its bytes
+__host__ __device__ constexpr int row_at(int r) { return (r % 32) * 16 + r / 32 * 4; }
+
+// The scale's byte of a block whose largest magnitude has these bits: floor(log2) - 2, and 255 for infinities and what is not a number.
+__device__ __forceinline__ uint32_t scale_of(uint32_t top_bits) {
+  const uint32_t e = top_bits >> 23;
+  return e == 255 ? 255u : e > 2 ? e - 2 : 0u;
+}
+// 2^-e of a scale's byte (up to 253): exact as a float, and so is its product with a value that does not become zero as a code
+__device__ __forceinline__ float inverse(uint32_t scale) { return __uint_as_float((254u - scale) << 23); }
+__device__ __forceinline__ float value_of(uint32_t scale) {
+  return __uint_as_float(scale == 0 ? 0x00400000u : scale == 255 ? 0x7fffffffu : scale << 23);
+}
+// eight values to codes, nearest with ties to even, 6 at most
+__device__ __forceinline__ uint32_t codes8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n.reg .b8 a, b, c, d;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+      "mov.b32 %0, {a, b, c, d};\n}"
+      : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// what eight codes stand for
+__device__ __forceinline__ void values8(uint32_t codes, float scale, float (&v)[8]) {
+  uint32_t h[4];
+  asm("{\n.reg .b8 a, b, c, d;\n"
+      "mov.b32 {a, b, c, d}, %4;\n"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(codes));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    v[2 * i] = f.x * scale;
+    v[2 * i + 1] = f.y * scale;
+  }
+}
+
+// The tile of a row of expert-sorted rows and its place there, by a whole warp; `offsets` null: one run of rows.
+__device__ __forceinline__ void place_of(const int* offsets, int experts, int row, int& tile, int& at) {
+  if (!offsets) {
+    tile = row / TILE;
+    at = row_at(row % TILE);
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  int tiles = 0, first = 0;
+  for (int e = lane; e < experts; e += 32) {
+    const int a = offsets[e], b = offsets[e + 1];
+    if (b <= row) tiles += (b - a + TILE - 1) / TILE;
+    else if (a <= row) first = a + 1;
+  }
+  tiles = __reduce_add_sync(0xffffffffu, tiles);
+  first = row - (int)__reduce_max_sync(0xffffffffu, first) + 1;
+  tile = tiles + first / TILE;
+  at = row_at(first % TILE);
+}
+
+}  // namespace mx

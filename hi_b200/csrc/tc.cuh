@@ -283,6 +283,42 @@ template <bool FP16> __device__ __forceinline__ uint32_t pack16(float lo, float 
   }
 }
 
+// ---- microscaled 4-bit floats (kind::mxf4, scales of two blocks of 32 for every 64 k): both operands packed, 128-byte rows of 256 k with the
+// 128-byte swizzle (desc_kmajor), scales in tensor memory.
+// Instruction descriptor: A and B e2m1 (bits 7, 10), N / 8 (17-22), scales powers of two (23), M / 16 (24-28); which half of a column's
+// four scales the product takes, 0 or 2, for B in bits 4-5, for A in bits 29-30.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n, int half) {
+  return ((uint32_t)half << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) |
+         ((uint32_t)half << 29);
+}
+__device__ __forceinline__ void mma_mx_if(uint32_t mine, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
+                                          uint32_t b_scales, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred e, p;\n"
+      "setp.ne.b32 e, %7, 0;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(a_scales), "r"(b_scales), "r"(mine) : "memory");
+}
+// 512 bytes of scales (128 rows x 4, mx.cuh) to four columns of all four quarters of tensor memory; products issued later see them
+__device__ __forceinline__ void copy_scales_if(uint32_t mine, uint32_t d_tmem, uint64_t desc) {
+  asm volatile(
+      "{\n.reg .pred e;\n"
+      "setp.ne.b32 e, %2, 0;\n"
+      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}" ::"r"(d_tmem), "l"(desc), "r"(mine) : "memory");
+}
+// descriptor of such 512 bytes: rows of 16 bytes, no swizzle, 128 bytes between groups of eight
+__device__ __forceinline__ uint64_t desc_scales(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFF) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+__device__ __forceinline__ void bulk_load_if(uint32_t mine, uint32_t smem_dst, const void* from, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "{\n.reg .pred e;\n"
+      "setp.ne.b32 e, %4, 0;\n"
+      "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n}"
+      ::"r"(smem_dst), "l"(from), "r"(bytes), "r"(bar), "r"(mine) : "memory");
+}
+
 // ---- tensor maps (the driver's encoder, looked up through the runtime: no link against libcuda)
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -310,6 +346,17 @@ inline bool make_map_bf16(CUtensorMap* map, const void* base, uint64_t rows, uin
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, elem,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// [rows, bytes] row-major; box [box_rows, 128 bytes]; else the same
+inline bool make_map_bytes(CUtensorMap* map, const void* base, uint64_t rows, uint64_t bytes, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {bytes, rows};
+  const cuuint64_t strides[1] = {bytes};
+  const cuuint32_t box[2] = {128, box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace tc

@@ -43,6 +43,9 @@ _SIGNATURES = {
     "hb_attention_decode_4bit": [P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, P, I, I, I, P, P, P, P, I, P],
     "hb_four_bit_linear": [P, c_longlong, P, P, P, I, I, I, I, I, P],
     "hb_four_bit_linear_tc": [P, c_longlong, P, P, P, I, I, I, I, I, P, P],
+    "hb_mx_quantize": [P, I, c_longlong, I, I, P, I, P, I, P, P, P],
+    "hb_mx_values": [P, P, I, I, P, I, P, I, P],
+    "hb_mx_gemm": [P, P, I, P, I, P, P, I, I, P, P, P, I, F, P, I, P, P, P],
     "hb_paged_attention": [P, I, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, F, P, P, I, I, P, P, P],
     "hb_attention_portions": [P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, F, I, F, P, P, I, P, P, P],
     "hb_attention_merge": [P, P, P, I, I, I, I, I, I, P, P],
@@ -2302,7 +2305,11 @@ def check_tc_status(device=None) -> None:
                      84: "4-bit product: the MMA issuer waiting for a free accumulator",
                      85: "4-bit product: the epilogue waiting for the accumulator",
                      86: "4-bit product: the warp that brings codes waiting for a free place",
-                     87: "4-bit product: the warps that unpack weights waiting for their codes"}.get(
+                     87: "4-bit product: the warps that unpack weights waiting for their codes",
+                     91: "microscaled product: the TMA producer waiting for a free stage",
+                     92: "microscaled product: the MMA issuer waiting for a loaded stage",
+                     93: "microscaled product: the epilogue waiting for the accumulator",
+                     94: "microscaled product: the MMA issuer waiting for a free accumulator"}.get(
                 code, f"prefill attention, wait {code}" if code >= 11 else f"code {code}")
             raise KernelError(f"a kernel gave up a bounded wait ({where}); its output is invalid")
 
@@ -2603,6 +2610,232 @@ def four_bit_linear(x: torch.Tensor, weight: FourBitWeight, out_dtype: torch.dty
         _check(lib().hb_four_bit_linear_tc(_ptr(x), x.stride(0), _ptr(weight.blocks), _ptr(bias), _ptr(out), _dt(out), n, m, k,
                                            weight.group, _ptr(_tc_status(x.device)), _stream()), "four_bit_linear_tc")
     return out
+
+
+# --------------------------------------------------------------------------- microscaled 4-bit floats
+MX_BLOCK, MX_TILE, MX_CHUNK = 32, 128, 128     # values that share a power of two; rows and values of 512 bytes of scales (csrc/mx.cuh)
+
+
+def _mx_chunks(k: int) -> int:
+    return -(-k // (2 * MX_CHUNK)) * 2
+
+
+class MxRows:
+    """Rows [N, K] in microscaled 4-bit floats: blocks of 32 values along a row are 2^e times e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
+    their negatives) with e = floor(log2(largest magnitude)) - 2, at least -127; a block with a value that is not finite is not a number.
+    ``codes`` uint8 [N, K / 2] (the even value in the low half), ``scales`` as the tensor cores read them (csrc/mx.cuh). Rows in the order
+    of a :class:`MoePlan` carry its ``offsets``: every expert's scales begin a tile. ``mx_quantize``, ``mx_glu`` and ``mx_experts_glu`` make them."""
+
+    __slots__ = ("codes", "scales", "shape", "offsets")
+
+    def __init__(self, codes, scales, shape, offsets=None):
+        self.codes, self.scales, self.shape, self.offsets = codes, scales, shape, offsets
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def experts(self) -> int:
+        return 1 if self.offsets is None else self.offsets.numel() - 1
+
+
+class MxWeight:
+    """A weight [M, K], or a stack [E, M, K] of experts', in microscaled 4-bit floats (:class:`MxRows`). ``codes`` uint8 [E, M, K / 2],
+    ``scales`` uint8 [E, ceil(M / 128), chunks, 512]. ``glu``: its rows are 32 of a gate and 32 of an up projection in turn
+    (``mx_interleave``). ``mx_pack_weight`` and ``mx_quantize_weight`` make one; ``parts.linear.linear`` takes one in a weight's place."""
+
+    dtype = torch.bfloat16           # of what it is multiplied with
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, glu: bool = False):
+        e, m, k = (1, *shape) if len(shape) == 2 else tuple(shape)
+        if min(e, m, k) < 1 or k % MX_BLOCK or (glu and m % (2 * MX_BLOCK)) or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or \
+                codes.shape != (e, m, k // 2) or scales.shape != (e, -(-m // MX_TILE), _mx_chunks(k), 512) or \
+                not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device:
+            raise KernelError(f"codes {codes.dtype} {tuple(codes.shape)} and scales {scales.dtype} {tuple(scales.shape)} are not those of a "
+                              f"microscaled weight {tuple(shape)}" + (", of which a gated unit has a multiple of 64 rows" if glu else ""))
+        self.codes, self.scales, self.shape, self.glu, self.experts = codes, scales, tuple(shape), bool(glu), e
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def mx_interleave(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """[..., I, X] and [..., I, X] as [..., 2 I, X]: 32 rows of ``gate``, 32 of ``up``, and so on (I a multiple of 32). Of weights, or of their codes and
+    exponents each."""
+    if gate.shape != up.shape or gate.dtype != up.dtype or gate.dim() < 2 or gate.shape[-2] % MX_BLOCK:
+        raise KernelError(f"gate {tuple(gate.shape)} and up {tuple(up.shape)}: alike, with a multiple of {MX_BLOCK} rows")
+    return torch.stack([gate.unflatten(-2, (-1, MX_BLOCK)), up.unflatten(-2, (-1, MX_BLOCK))], dim=-3).flatten(-4, -2)
+
+
+def mx_pack_weight(codes: torch.Tensor, exponents: torch.Tensor, glu: bool = False) -> MxWeight:
+    """``codes`` uint8 [M, K] or [E, M, K] of 0 .. 15 (e2m1, 8 is the sign) and ``exponents`` uint8 [..., K / 32] (127 + e; 255: not a number) as
+    an :class:`MxWeight`. Once, when a model is loaded; works on any device."""
+    if codes.dim() not in (2, 3) or codes.dtype != torch.uint8 or exponents.dtype != torch.uint8 or codes.device != exponents.device or \
+            codes.numel() == 0 or codes.shape[-1] % MX_BLOCK or exponents.shape != (*codes.shape[:-1], codes.shape[-1] // MX_BLOCK):
+        raise KernelError(f"a microscaled weight is uint8 codes [M, K] or [E, M, K] and exponents [..., K / {MX_BLOCK}] on one device, not "
+                          f"{codes.dtype} {tuple(codes.shape)} and {exponents.dtype} {tuple(exponents.shape)}")
+    if int(codes.max()) > 15:
+        raise KernelError(f"a code of {int(codes.max())}: codes are 0 .. 15")
+    e, (m, k) = codes.shape[0] if codes.dim() == 3 else 1, codes.shape[-2:]
+    tiles, chunks = -(-m // MX_TILE), _mx_chunks(k)
+    s = exponents.new_zeros((e, tiles * MX_TILE, chunks * 4))
+    s[:, :m, : k // MX_BLOCK] = exponents.view(e, m, -1)
+    s = s.view(e, tiles, 4, 32, chunks, 4).permute(0, 1, 4, 3, 2, 5).reshape(e, tiles, chunks, 512).contiguous()
+    c = codes.view(e, m, k // 2, 2)
+    return MxWeight((c[..., 0] | c[..., 1] << 4).contiguous(), s, codes.shape, glu)
+
+
+def _mx_scales(x: torch.Tensor, rows: int, k: int, experts: int) -> torch.Tensor:
+    tiles = -(-rows // MX_TILE) + min(experts, max(rows, 1)) - 1       # as many as `experts` runs of these rows can begin
+    return x.new_empty((tiles, _mx_chunks(k), 512), dtype=torch.uint8)
+
+
+def _mx_input(x: torch.Tensor, k: Optional[int] = None) -> torch.Tensor:
+    if not x.is_cuda:
+        raise KernelError("x must be a CUDA tensor; this engine has no CPU path")
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32) or x.shape[1] % MX_BLOCK or not x.shape[1] or k not in (None, x.shape[1]):
+        raise KernelError(f"rows of {f'{k} values' if k else f'a multiple of {MX_BLOCK} values'} in bfloat16 or float32 are quantised, not "
+                          f"{x.dtype} {tuple(x.shape)}")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise KernelError("quantised rows have no gradients")
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) * x.element_size() % 16) or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x
+
+
+def _mx_quantize(x: torch.Tensor, rows: int, sorted_entry, top_k: int, offsets) -> MxRows:
+    k, experts = x.shape[1], 1 if offsets is None else offsets.numel() - 1
+    codes, scales = x.new_empty((rows, k // 2), dtype=torch.uint8), _mx_scales(x, rows, k, experts)
+    if rows:
+        _check(lib().hb_mx_quantize(_ptr(x), _dt(x), x.stride(0) if x.shape[0] > 1 else k, rows, k, _ptr(sorted_entry), top_k, _ptr(offsets), experts,
+                                    _ptr(codes), _ptr(scales), _stream()), "mx_quantize")
+    return MxRows(codes, scales, (rows, k), offsets)
+
+
+def _mx_plan(plan: MoePlan, rows: int) -> None:
+    for t, name in ((plan.offsets, "plan.offsets"), (plan.sorted_entry, "plan.sorted_entry")):
+        _need(t, name, torch.int32)
+    if plan.offsets.numel() < 2 or plan.sorted_entry.numel() != max(rows, 1):
+        raise KernelError(f"a plan of {plan.sorted_entry.numel()} entries for {rows} rows")
+
+
+def mx_quantize(x: torch.Tensor, plan: Optional[MoePlan] = None, top_k: int = 1) -> MxRows:
+    """The rows of ``x`` [N, K] (bfloat16 or float32, K a multiple of 32; its rows may be a column slice of a wider matrix) in microscaled 4-bit
+    floats. With ``plan``: the N * top_k rows of its experts, sorted, row i from token sorted_entry[i] // top_k."""
+    x = _mx_input(x)
+    if plan is None:
+        _on_current_device(x)
+        return _mx_quantize(x, x.shape[0], None, 1, None)
+    rows = x.shape[0] * top_k
+    _mx_plan(plan, rows)
+    _on_current_device(x, plan.offsets, plan.sorted_entry)
+    return _mx_quantize(x, rows, plan.sorted_entry, top_k, plan.offsets)
+
+
+def mx_values(rows: MxRows, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that quantised rows stand for, [N, K] in bfloat16 or float32 (both hold them exactly)."""
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise KernelError(f"values are bfloat16 or float32, not {out_dtype}")
+    _on_current_device(rows.codes)
+    n, k = rows.shape
+    out = torch.empty((n, k), dtype=out_dtype, device=rows.device)
+    if n:
+        _check(lib().hb_mx_values(_ptr(rows.codes), _ptr(rows.scales), n, k, _ptr(rows.offsets), rows.experts, _ptr(out), _dt(out), _stream()),
+               "mx_values")
+    return out
+
+
+def mx_quantize_weight(weight: torch.Tensor, glu: bool = False) -> MxWeight:
+    """A weight [M, K], or experts' [E, M, K], on a GPU (bfloat16 or float32, K a multiple of 32) in microscaled 4-bit floats."""
+    if weight.dim() not in (2, 3) or weight.numel() == 0:
+        raise KernelError(f"a weight [M, K] or [E, M, K] is quantised, not {tuple(weight.shape)}")
+    e, (m, k) = weight.shape[0] if weight.dim() == 3 else 1, weight.shape[-2:]
+    x = _mx_input(weight.detach().reshape(e * m, k))
+    _on_current_device(x)
+    offsets = entries = None
+    if e > 1:
+        offsets = torch.arange(0, (e + 1) * m, m, dtype=torch.int32, device=x.device)
+        entries = torch.arange(e * m, dtype=torch.int32, device=x.device)
+    rows = _mx_quantize(x, e * m, entries, 1, offsets)
+    tiles = -(-m // MX_TILE)
+    return MxWeight(rows.codes.view(e, m, k // 2), rows.scales[: e * tiles].view(e, tiles, _mx_chunks(k), 512), weight.shape, glu)
+
+
+def _mx_gemm(rows: MxRows, weight: MxWeight, name: str, out_dtype=None, bias=None, sorted_entry=None, scores=None, limit: float = 0.0):
+    """The product; without ``out_dtype`` the gated unit, as :class:`MxRows`."""
+    (n, k), m = rows.shape, weight.shape[-2]
+    if rows.experts != weight.experts or k != weight.shape[-1] or (len(weight.shape) == 3) != (rows.offsets is not None):
+        raise KernelError(f"{name}: rows {rows.shape} of {rows.experts} experts do not go with a weight {weight.shape}")
+    if bias is not None:
+        if torch.is_grad_enabled() and bias.requires_grad:
+            raise KernelError(f"{name}: products with microscaled weights have no gradients")
+        _need(bias, "bias", torch.bfloat16)
+        if bias.numel() != m:
+            raise KernelError(f"{name}: bias has {bias.numel()} elements for {m} outputs")
+    _on_current_device(rows.codes, rows.offsets, weight.codes, bias, sorted_entry, scores)
+    act = None
+    if out_dtype is None:
+        out = rows.codes.new_empty((n, m // 4))
+        act = MxRows(out, _mx_scales(rows.codes, n, m // 2, rows.experts), (n, m // 2), rows.offsets)
+    else:
+        out = rows.codes.new_empty((n, m), dtype=out_dtype)
+    if n:
+        TC_USED[0] = True
+        _check(lib().hb_mx_gemm(_ptr(rows.codes), _ptr(rows.scales), n, _ptr(rows.offsets), rows.experts, _ptr(weight.codes), _ptr(weight.scales), m, k,
+                                _ptr(bias), _ptr(sorted_entry), _ptr(scores), int(act is not None), float(limit), _ptr(out),
+                                0 if act is not None else _dt(out), _ptr(act.scales) if act is not None else None,
+                                _ptr(_tc_status(rows.device)), _stream()), name)
+    return out if act is None else act
+
+
+def _mx_rows_for(x, weight: MxWeight, name: str, glu: bool, stack: bool = False) -> None:
+    if not isinstance(weight, MxWeight) or weight.glu != glu or (len(weight.shape) == 3) != stack:
+        raise KernelError(f"{name} takes {'experts' if stack else 'a weight'} in microscaled 4-bit floats" + (" with gate and up rows in turn" if glu else ""))
+
+
+def mx_linear(x, weight: MxWeight, out_dtype: torch.dtype = torch.bfloat16, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x @ weight.T (+ bias)`` for ``x`` [N, K] (:class:`MxRows`, or bfloat16 or float32 rows, which are quantised first) with float32 sums, in
+    ``out_dtype`` (bfloat16 or float32); ``bias`` bfloat16 [M]."""
+    _mx_rows_for(x, weight, "mx_linear", False)
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise KernelError(f"mx_linear returns bfloat16 or float32, not {out_dtype}")
+    if not isinstance(x, MxRows):
+        x = mx_quantize(_mx_input(x, weight.shape[-1]))
+    return _mx_gemm(x, weight, "mx_linear", out_dtype, bias)
+
+
+def mx_glu(x, weight: MxWeight, limit: float = 0.0) -> MxRows:
+    """silu(x Wg^T) (x Wu^T), or with ``limit`` > 0 the clamped unit min(g, limit) sigmoid(1.702 min(g, limit)) (clamp(u, +-limit) + 1), from float32
+    sums, quantised as it is: what the down projection reads. ``weight`` has gate and up rows in turn (``mx_interleave``)."""
+    _mx_rows_for(x, weight, "mx_glu", True)
+    if not isinstance(x, MxRows):
+        x = mx_quantize(_mx_input(x, weight.shape[-1]))
+    return _mx_gemm(x, weight, "mx_glu", limit=limit)
+
+
+def mx_experts_glu(x: torch.Tensor, plan: MoePlan, top_k: int, weight: MxWeight, scores: Optional[torch.Tensor] = None,
+                   limit: float = 0.0) -> MxRows:
+    """:func:`mx_glu` by expert: the rows of ``x`` [N, K] go to their experts' order quantised, and an entry's sums are multiplied by its score
+    (float32 [N, top_k], or None) before the unit."""
+    _mx_rows_for(x, weight, "mx_experts_glu", True, True)
+    if scores is not None:
+        _need(scores, "scores", torch.float32)
+        if scores.numel() != x.shape[0] * top_k:
+            raise KernelError(f"mx_experts_glu: {scores.numel()} scores for {x.shape[0]} tokens of {top_k} experts")
+    rows = mx_quantize(_mx_input(x, weight.shape[-1]), plan, top_k)
+    return _mx_gemm(rows, weight, "mx_experts_glu", sorted_entry=plan.sorted_entry, scores=scores, limit=limit)
+
+
+def mx_experts_linear(rows: MxRows, weight: MxWeight, plan: MoePlan) -> torch.Tensor:
+    """y[slot] = rows[slot] W[e]^T, float32 [N*k, M], for rows in the plan's order (:func:`mx_experts_glu`); ``moe_combine`` sums a token's."""
+    _mx_rows_for(rows, weight, "mx_experts_linear", False, True)
+    if rows.offsets is not plan.offsets:
+        raise KernelError("mx_experts_linear: the rows are in another plan's order")
+    return _mx_gemm(rows, weight, "mx_experts_linear", torch.float32)
 
 
 def four_bit_page_bytes(page_size: int, hd: int) -> int:

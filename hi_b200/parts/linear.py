@@ -30,17 +30,20 @@ def packed(weight: torch.Tensor, env) -> torch.Tensor | ops.FourBitWeight:
     return ops.quantize_weight(weight, group)
 
 
-def linear(x: torch.Tensor, weight: torch.Tensor | ops.FourBitWeight, out_dtype: torch.dtype | None = None,
+def linear(x: torch.Tensor, weight: torch.Tensor | ops.FourBitWeight | ops.MxWeight, out_dtype: torch.dtype | None = None,
            bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` (``+ bias`` [M], added to the float32 sums by the library's epilogue) for
     ``x`` [N, K] and ``weight`` [M, K].
 
     A weight kept in float32 while activations are bfloat16 (a tensor stored in 32-bit stays
     so) is multiplied in float32. ``out_dtype=torch.float32`` asks for a float32 result from
-    bfloat16 operands (the logits). A weight held in four bits is multiplied by ``ops.four_bit_linear``.
+    bfloat16 operands (the logits). A weight held in four bits is multiplied by ``ops.four_bit_linear``, one in microscaled
+    4-bit floats, with ``x`` quantised alike, by ``ops.mx_linear``.
     """
     if isinstance(weight, ops.FourBitWeight):
         return ops.four_bit_linear(x, weight, out_dtype or x.dtype, None if bias is None else bias.to(x.dtype))
+    if isinstance(weight, ops.MxWeight):
+        return ops.mx_linear(x, weight, out_dtype or x.dtype, None if bias is None else bias.to(torch.bfloat16))
     if not x.is_cuda:
         raise RuntimeError("hi_b200 runs on a CUDA device only")
     if torch.backends.cuda.matmul.allow_tf32:
