@@ -26,6 +26,12 @@ constexpr int A_BYTES = BM * KB / 2, SCALES = KB / mx::CHUNK * mx::ATOM;        
 constexpr int EPILOGUE = 8, THREADS = 64 + 32 * EPILOGUE;
 constexpr int MOST_EXPERTS = 1024;
 
+// hb::clamped_glu with a division that has no second path (its denominator is 1 at least; past 2^126 the result is 0)
+__device__ __forceinline__ float clamped(float gate, float up, float limit) {
+  const float g = fminf(gate, limit), u = fminf(fmaxf(up, -limit), limit);
+  return __fdividef(g, 1.f + expf(-1.702f * g)) * (u + 1.f);
+}
+
 struct Params {
   const uint8_t *x_scales, *w_scales;
   const int* offsets;            // [experts + 1] first row of every expert, or null: one
@@ -216,7 +222,7 @@ mx_gemm_kernel(const __grid_constant__ Maps maps, const Params p) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               const float gs = score * __uint_as_float(g[j]), us = score * __uint_as_float(u[j]);
-              act[j] = p.limit > 0.f ? hb::clamped_glu(gs, us, p.limit) : gs / (1.f + expf(-gs)) * us;
+              act[j] = p.limit > 0.f ? clamped(gs, us, p.limit) : __fdividef(gs, 1.f + expf(-gs)) * us;
               top = max(top, __float_as_uint(act[j]) & 0x7fffffffu);
             }
             const uint32_t scale = mx::scale_of(top);

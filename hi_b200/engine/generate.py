@@ -69,7 +69,7 @@ class LLM:
     (crates/hi-local/src/main.rs:28-59): ``max_batch_size``, ``max_active_requests``,
     ``max_batched_tokens``, ``kv_page_size``; plus ``kv_cache_tokens`` (pool capacity; by default
     nine tenths of the device memory that is free after loading) and ``max_prefill_portion``;
-    ``weight_bits``, ``weight_group`` and ``kv_cache_bits``: weights and cache in four bits (:meth:`Engine.from_dir`).
+    ``weight_bits``, ``weight_group``, ``weight_format`` and ``kv_cache_bits``: weights and cache in four bits (:meth:`Engine.from_dir`).
     """
 
     def __init__(self, model: Union[str, dict, Engine], *, dtype="bfloat16", device="cuda:0",
@@ -77,7 +77,7 @@ class LLM:
                  kv_cache_tokens: Optional[int] = None, windowed_cache_tokens: Optional[int] = None,
                  max_batch_size: int = 8, max_active_requests: Optional[int] = None,
                  max_batched_tokens: int = 8192, max_prefill_portion: Optional[int] = None, lookahead: bool = True,
-                 weight_bits: int = 16, weight_group: int = 64, kv_cache_bits: int = 16):
+                 weight_bits: int = 16, weight_group: int = 64, kv_cache_bits: int = 16, weight_format: str = "int4"):
         self.config = SchedulerConfig(max_batch_size=max_batch_size, max_active_requests=max_active_requests,
                                       max_batched_tokens=max_batched_tokens, max_prefill_portion=max_prefill_portion)
         self.config.validate()
@@ -88,7 +88,7 @@ class LLM:
             opts = dict(kv_page_size=kv_page_size, max_active_requests=slots,
                         kv_cache_tokens=kv_cache_tokens,      # None: sized from the memory that is free
                         windowed_cache_tokens=windowed_cache_tokens, weight_bits=weight_bits, weight_group=weight_group,
-                        kv_cache_bits=kv_cache_bits)
+                        kv_cache_bits=kv_cache_bits, weight_format=weight_format)
             if isinstance(model, dict):
                 self.engine = Engine.from_config(model, seed=random_seed or 0, std=random_std, dtype=dtype,
                                                  device=device, **opts)

@@ -2627,6 +2627,7 @@ class MxRows:
     of a :class:`MoePlan` carry its ``offsets``: every expert's scales begin a tile. ``mx_quantize``, ``mx_glu`` and ``mx_experts_glu`` make them."""
 
     __slots__ = ("codes", "scales", "shape", "offsets")
+    dtype = torch.bfloat16           # of what is computed from them, unless it is said
 
     def __init__(self, codes, scales, shape, offsets=None):
         self.codes, self.scales, self.shape, self.offsets = codes, scales, shape, offsets

@@ -8,7 +8,7 @@ import torch
 from ..kernels import ops
 from .basic import Part
 from .context import Pending
-from .linear import linear, packed
+from .linear import linear, microscaled, microscaled_stack, packed
 from .registry import register
 from .spec import TensorSpec
 
@@ -49,10 +49,16 @@ class _SwiGLU:
             rows += [sg, torch.zeros((-(2 * self.inter + 1) % 8, self.hidden), dtype=sg.dtype, device=sg.device)]
         if len({t.dtype for t in rows}) > 1:
             rows = [t.float() for t in rows]
-        self.w_gate_up = packed(torch.cat(rows, dim=0).contiguous(), self.env)
+        if not self.token_gate and self.inter % ops.MX_BLOCK == 0 and microscaled(rows[0], self.env):
+            self.w_gate_up = ops.mx_quantize_weight(ops.mx_interleave(*rows), glu=True)
+        else:
+            self.w_gate_up = packed(torch.cat(rows, dim=0).contiguous(), self.env)
         self.w_down = packed(fetch(self._name("down")).contiguous(), self.env)
 
     def forward(self, x):
+        if isinstance(self.w_gate_up, ops.MxWeight) and self.w_gate_up.glu:
+            act = ops.mx_glu(x, self.w_gate_up, self.limit or 0.0)
+            return linear(act if isinstance(self.w_down, ops.MxWeight) else ops.mx_values(act), self.w_down)
         if self.limit is not None:
             return linear(ops.glu_limit(linear(x, self.w_gate_up), self.inter, self.limit,
                                         2 * self.inter if self.token_gate else -1), self.w_down)
@@ -204,6 +210,7 @@ class SigmoidRoutedExperts(Part):
         self.score_scale = float(params.get("score_scale", 1.0))
         self._ones: Optional[torch.Tensor] = None
         self.w_router = self.w_gate = self.w_up = self.w_down = None
+        self.w_gate_up: Optional[ops.MxWeight] = None       # in microscaled 4-bit floats instead of w_gate and w_up
         self._side_stream = None
 
     def tensor_specs(self):
@@ -247,6 +254,10 @@ class SigmoidRoutedExperts(Part):
             self.w_gate = expert_tensor(f"{p}.experts.gate_proj.weight") if gated else None
             self.w_up = expert_tensor(f"{p}.experts.up_proj.weight")
             self.w_down = expert_tensor(f"{p}.experts.down_proj.weight")
+        if gated and self.inter % ops.MX_BLOCK == 0 and microscaled(self.w_up, self.env):
+            self.w_gate_up = microscaled_stack((ops.mx_interleave(g, u) for g, u in zip(self.w_gate, self.w_up)), glu=True)
+            self.w_gate = self.w_up = None
+            self.w_down = microscaled_stack(self.w_down)
         if self.shared:
             self.shared.load(fetch)
 
@@ -290,6 +301,10 @@ class SigmoidRoutedExperts(Part):
         if ctx.tap is not None:
             ctx.tap(f"{self.prefix}.router_ids", ids)
         entry_weights = None
+        if self.w_gate_up is not None:
+            act = ops.mx_experts_glu(normed, plan, self.top_k, self.w_gate_up, None if self.scale_output else scores, self.limit)
+            return self._joined(normed, ops.mx_experts_linear(act, self.w_down, plan), plan, side, shared if side is not None else None,
+                                scores.view(-1) if self.scale_output else None)
         if self.scale_output:
             # the experts read the unscaled rows (a factor of one); their outputs take the score in the sum
             if self._ones is None or self._ones.numel() < scores.numel():
@@ -307,6 +322,9 @@ class SigmoidRoutedExperts(Part):
         else:
             act = ops.moe_gate_up(normed, plan, self.top_k, self.w_gate, self.w_up, scores, few, self.activation, self.limit)
             y = ops.moe_down(act, self.w_down, plan, few)
+        return self._joined(normed, y, plan, side, shared if side is not None else None, entry_weights)
+
+    def _joined(self, normed, y, plan, side, shared, entry_weights) -> Pending:
         if side is not None:
             torch.cuda.current_stream().wait_stream(side)
         else:

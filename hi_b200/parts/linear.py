@@ -21,13 +21,27 @@ def configure_matmul_precision() -> None:
     torch.backends.cuda.matmul.allow_fp16_reduced_precision_reduction = False
 
 
-def packed(weight: torch.Tensor, env) -> torch.Tensor | ops.FourBitWeight:
-    """``weight`` [M, K] as the model is asked to hold it (``env.weight_bits``): in four bits where it is bfloat16 and K a multiple of 32,
-    in groups of ``env.weight_group`` inputs or the next smaller size that divides K."""
+def microscaled(weight: torch.Tensor, env) -> bool:
+    """Whether ``weight`` [..., M, K] is to be held in microscaled 4-bit floats: bfloat16 with K a multiple of 32."""
+    return env is not None and env.weight_bits == 4 and env.weight_format == "mxfp4" and weight.dtype == torch.bfloat16 and \
+        weight.shape[-1] % ops.MX_BLOCK == 0
+
+
+def packed(weight: torch.Tensor, env) -> torch.Tensor | ops.FourBitWeight | ops.MxWeight:
+    """``weight`` [M, K] as the model is asked to hold it (``env.weight_bits``, ``env.weight_format``): in four bits where it is bfloat16 and K a
+    multiple of 32, whole numbers in groups of ``env.weight_group`` inputs or the next smaller size that divides K."""
     if env is None or env.weight_bits != 4 or weight.dtype != torch.bfloat16 or weight.shape[1] % 32:
         return weight
+    if microscaled(weight, env):
+        return ops.mx_quantize_weight(weight)
     group = max(g for g in ops.FOUR_BIT_GROUPS if g <= env.weight_group and weight.shape[1] % g == 0)
     return ops.quantize_weight(weight, group)
+
+
+def microscaled_stack(weights, glu: bool = False) -> ops.MxWeight:
+    """Experts' weights [M, K], one after the other, as one stack in microscaled 4-bit floats (one's 16-bit copy at a time)."""
+    parts = [ops.mx_quantize_weight(w, glu) for w in weights]
+    return ops.MxWeight(torch.cat([p.codes for p in parts]), torch.cat([p.scales for p in parts]), (len(parts), *parts[0].shape), glu)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor | ops.FourBitWeight | ops.MxWeight, out_dtype: torch.dtype | None = None,

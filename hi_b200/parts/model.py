@@ -46,18 +46,24 @@ class Layer:
         return [p for p in parts if p is not None]
 
 
+WEIGHT_FORMATS = ("int4", "mxfp4")      # of weights in four bits
+
+
 class Model:
-    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device, weight_bits: int = 16, weight_group: int = 64, cache_bits: int = 16):
+    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device, weight_bits: int = 16, weight_group: int = 64, cache_bits: int = 16,
+                 weight_format: str = "int4"):
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError(f"dtype {dtype} is not supported (bfloat16 or float32)")
         if weight_bits not in (4, 16) or cache_bits not in (4, 16) or weight_group not in ops.FOUR_BIT_GROUPS:
             raise ValueError(f"weights of {weight_bits} bits in groups of {weight_group}, a cache of {cache_bits}: 4 or 16 bits and groups of "
                              f"{ops.FOUR_BIT_GROUPS} are built")
+        if weight_format not in WEIGHT_FORMATS:
+            raise ValueError(f"weight format {weight_format!r} is not known: {WEIGHT_FORMATS}")
         if dtype != torch.bfloat16 and (weight_bits != 16 or cache_bits != 16):
             raise ValueError("weights and a cache in four bits are built for bfloat16; the float32 path is 32-bit throughout")
         self.spec, self.dtype, self.device = spec, dtype, torch.device(device)
         self.env = BuildEnv(dtype=dtype, device=self.device, hidden_size=spec.hidden_size, weight_bits=weight_bits,
-                            weight_group=weight_group, cache_bits=cache_bits)
+                            weight_group=weight_group, weight_format=weight_format, cache_bits=cache_bits)
         self.embedding = build("embedding", spec.embedding, self.env, spec.embedding.params.get("name", ""))
         self.layers = [Layer(ls, self.env) for ls in spec.layers]
         self.final_norm = build("norm", spec.final_norm, self.env, spec.final_norm.params.get("name", ""))

@@ -41,6 +41,7 @@ class BuildEnv:
     hidden_size: int
     weight_bits: int = 16       # 4: the dense projections that are made for it hold their weights in four bits
     weight_group: int = 64      # inputs of a row that share a scale then (32, 64 or 128; the largest of these that divides the row, if less)
+    weight_format: str = "int4" # of weights in four bits: "int4" (whole numbers with group scales) or "mxfp4" (microscaled floats, routed experts too)
     cache_bits: int = 16        # 4: keys and values are cached in four bits
 
 
