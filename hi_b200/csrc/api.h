@@ -96,7 +96,7 @@ int hb_mx_quantize(const void* x, int dtype, long long x_ld, int rows, int K, co
                    int experts, void* codes, void* scales, cudaStream_t stream);
 int hb_mx_values(const void* codes, const void* scales, int rows, int K, const int* offsets, int experts, void* out, int out_dtype,
                  cudaStream_t stream);
-int hb_mx_gemm(const void* x, const void* x_scales, int rows, const int* offsets, int experts, const void* w, const void* w_scales, int n_out,
+int hb_mx_gemm(const void* raw, int raw_dtype, long long raw_ld, int top_k, void* x, void* x_scales, int rows, const int* offsets, int experts, const void* w, const void* w_scales, int n_out,
                int K, const void* bias, const int* sorted_entry, const float* scores, int glu, float limit, void* out, int out_dtype,
                void* out_scales, int* status, cudaStream_t stream);
 

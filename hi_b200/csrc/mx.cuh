@@ -21,7 +21,7 @@ __device__ __forceinline__ uint32_t scale_of(uint32_t top_bits) {
   const uint32_t e = top_bits >> 23;
   return e == 255 ? 255u : e > 2 ? e - 2 : 0u;
 }
-// 2^-e of a scale's byte (up to 253): exact as a float, and so is its product with a value that does not become zero as a code
+// 2^-e of a scale's byte (255: anything): exact as a float, and so is its product with a value that does not become zero as a code
 __device__ __forceinline__ float inverse(uint32_t scale) { return __uint_as_float((254u - scale) << 23); }
 __device__ __forceinline__ float value_of(uint32_t scale) {
   return __uint_as_float(scale == 0 ? 0x00400000u : scale == 255 ? 0x7fffffffu : scale << 23);

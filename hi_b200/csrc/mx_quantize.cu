@@ -19,57 +19,140 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-constexpr int SPAN = 256;          // values a warp takes at a time, eight a lane
-constexpr int THREADS = 256;
+// Eight values as they are read, their largest magnitude's bits as a float's, and themselves as floats.
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = reinterpret_cast<const float4*>(p)[0];
+    b = reinterpret_cast<const float4*>(p)[1];
+  }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void floats(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  __device__ __forceinline__ uint32_t top() const {
+    float v[8];
+    floats(v);
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t = max(t, __float_as_uint(v[i]) & 0x7fffffffu);
+    return t;
+  }
+};
+template <> struct Eight<__nv_bfloat16> {
+  uint4 w;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { w = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void floats(float (&v)[8]) const {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(u[i] << 16);
+      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ uint32_t top() const {       // two 16-bit halves at a time: bits of magnitudes are in the order of the magnitudes
+    constexpr uint32_t M = 0x7fff7fffu;
+    const uint32_t t = __vmaxu2(__vmaxu2(w.x & M, w.y & M), __vmaxu2(w.z & M, w.w & M));
+    return max(t & 0xffff0000u, t << 16);
+  }
+};
 
-// Row blockIdx.x (of `rows` in the order of `sorted_entry`, if there is one), SPANs blockIdx.y * 8 + warp, ... Four lanes have a block of 32.
-template <typename T>
+constexpr int SPAN = 256;          // values a warp takes at a time, eight a lane
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+
+// A warp takes MANY spans of 256 values of a row. Four lanes have a block of 32.
+template <typename T, int MANY>
 __global__ void __launch_bounds__(THREADS)
-mx_quantize_kernel(const T* __restrict__ x, long long x_ld, int k, const int* __restrict__ sorted_entry, int top_k,
+mx_quantize_kernel(const T* __restrict__ x, long long x_ld, int rows, int k, const int* __restrict__ sorted_entry, int top_k,
                    const int* __restrict__ offsets, int experts, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int span = blockIdx.y * (THREADS / 32) + warp, all = mx::chunks(k);
-  if (span * 2 >= all) return;
+  asm volatile("griddepcontrol.launch_dependents;");       // the product behind this launch may begin to bring its weights
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, all = mx::chunks(k), groups = (all / 2 + MANY - 1) / MANY;
+  const long long item = (long long)blockIdx.x * WARPS + warp;
+  const int row = (int)(item / groups), first = (int)(item % groups) * MANY;
+  if (row >= rows) return;
   const size_t from = sorted_entry ? sorted_entry[row] / top_k : row;
+  const T* const in = x + from * x_ld + lane * 8;
+  Eight<T> x8[MANY];
+#pragma unroll
+  for (int m = 0; m < MANY; ++m) {
+    const int k0 = (first + m) * SPAN + lane * 8;
+    if (k0 < k) x8[m].load(in + (first + m) * SPAN);
+    else x8[m].zero();
+  }
   int tile, at;
   mx::place_of(offsets, experts, row, tile, at);
-  const int k0 = span * SPAN + lane * 8;
-  float v[8] = {};
-  if (k0 < k) hb::load8(x + from * x_ld + k0, v);
-  uint32_t top = 0;
+  uint8_t* const to = codes + (size_t)row * (k / 2) + lane * 4;
+  uint8_t* const scale_to = scales + (size_t)tile * all * mx::ATOM + at;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const uint32_t scale = mx::scale_of(top);
-  const float by = scale == 255 ? 0.f : mx::inverse(scale);
+  for (int m = 0; m < MANY; ++m) {
+    const int span = first + m, k0 = span * SPAN + lane * 8;
+    if (span * 2 >= all) break;
+    uint32_t top = x8[m].top();
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t scale = mx::scale_of(top);
+    const float by = mx::inverse(scale);          // (what is multiplied by the scale 255 does not matter)
+    float v[8];
+    x8[m].floats(v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = scale == 255 ? 0.f : v[i] * by;
-  if (k0 < k) *reinterpret_cast<uint32_t*>(codes + (size_t)row * (k / 2) + k0 / 2) = mx::codes8(v);
-  // the four blocks of 16 lanes: a word of scales
-  uint32_t word = scale << (lane / 4 % 4 * 8);
-  word |= __shfl_xor_sync(0xffffffffu, word, 4);
-  word |= __shfl_xor_sync(0xffffffffu, word, 8);
-  if (lane % 16 == 0)
-    *reinterpret_cast<uint32_t*>(scales + ((size_t)tile * all + span * 2 + lane / 16) * mx::ATOM + at) = word;
+    for (int i = 0; i < 8; ++i) v[i] *= by;
+    if (k0 < k) *reinterpret_cast<uint32_t*>(to + span * (SPAN / 2)) = mx::codes8(v);
+    // the four blocks of 16 lanes: a word of scales
+    uint32_t word = scale << (lane / 4 % 4 * 8);
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(scale_to + (size_t)(span * 2 + lane / 16) * mx::ATOM) = word;
+  }
 }
 
-template <typename T>
+template <typename T, int MANY>
 __global__ void __launch_bounds__(THREADS)
-mx_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int k, const int* __restrict__ offsets, int experts,
-                 T* __restrict__ out) {
-  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int span = blockIdx.y * (THREADS / 32) + warp, all = mx::chunks(k);
-  if (span * 2 >= all) return;
+mx_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int k, const int* __restrict__ offsets,
+                 int experts, T* __restrict__ out) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, all = mx::chunks(k), groups = (all / 2 + MANY - 1) / MANY;
+  const long long item = (long long)blockIdx.x * WARPS + warp;
+  const int row = (int)(item / groups), first = (int)(item % groups) * MANY;
+  if (row >= rows) return;
   int tile, at;
   mx::place_of(offsets, experts, row, tile, at);
-  const int k0 = span * SPAN + lane * 8;
-  if (k0 >= k) return;
-  const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + (size_t)row * (k / 2) + k0 / 2);
-  const float scale = mx::value_of(scales[((size_t)tile * all + span * 2 + lane / 16) * mx::ATOM + at + lane / 4 % 4]);
-  float v[8];
-  mx::values8(word, scale, v);
-  store8(out + (size_t)row * k + k0, v);
+  const uint8_t* const from = codes + (size_t)row * (k / 2) + lane * 4;
+  const uint8_t* const scale_from = scales + (size_t)tile * all * mx::ATOM + at + lane / 4 % 4;
+  uint32_t word[MANY], scale[MANY];
+#pragma unroll
+  for (int m = 0; m < MANY; ++m) {
+    const bool there = (first + m) * SPAN + lane * 8 < k;
+    word[m] = there ? *reinterpret_cast<const uint32_t*>(from + (first + m) * (SPAN / 2)) : 0u;
+    scale[m] = there ? scale_from[(size_t)((first + m) * 2 + lane / 16) * mx::ATOM] : 0u;
+  }
+#pragma unroll
+  for (int m = 0; m < MANY; ++m) {
+    const int k0 = (first + m) * SPAN + lane * 8;
+    if (k0 >= k) break;
+    float v[8];
+    mx::values8(word[m], mx::value_of(scale[m]), v);
+    store8(out + (size_t)row * k + k0, v);
+  }
+}
+
+// Spans of a warp: as many as keep the card full. (One span a warp, 8,192 x 16,384 bfloat16: QUANT1 us, four QUANT4; 1 x 5,120: 1.4 and the same.)
+int blocks_of(int rows, int k, int many) {
+  const long long items = (long long)rows * ((mx::chunks(k) / 2 + many - 1) / many), blocks = (items + WARPS - 1) / WARPS;
+  return blocks > 0x7fffffffll ? 0 : (int)blocks;
+}
+bool much(int rows, int k) { return (long long)rows * (mx::chunks(k) / 2) >= 4 * 148 * 32; }
+
+template <typename T, int MANY>
+void quantize(const void* x, long long x_ld, int rows, int k, const int* sorted_entry, int top_k, const int* offsets, int experts, void* codes,
+              void* scales, int blocks, cudaStream_t stream) {
+  mx_quantize_kernel<T, MANY><<<blocks, THREADS, 0, stream>>>((const T*)x, x_ld, rows, k, sorted_entry, top_k, offsets, experts, (uint8_t*)codes,
+                                                              (uint8_t*)scales);
+}
+template <typename T, int MANY>
+void values(const void* codes, const void* scales, int rows, int k, const int* offsets, int experts, void* out, int blocks, cudaStream_t stream) {
+  mx_values_kernel<T, MANY><<<blocks, THREADS, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, rows, k, offsets, experts, (T*)out);
 }
 
 }  // namespace
@@ -83,12 +166,11 @@ extern "C" int hb_mx_quantize(const void* x, int dtype, long long x_ld, int rows
     return HB_ERR_BAD_ARG;
   if (K % mx::BLOCK || (reinterpret_cast<uintptr_t>(x) & 15) || x_ld * (dtype == HB_DTYPE_F32 ? 4 : 2) % 16) return HB_ERR_UNSUPPORTED;
   if (rows == 0) return HB_OK;
-  const dim3 grid(rows, (mx::chunks(K) / 2 + THREADS / 32 - 1) / (THREADS / 32));
-  if (dtype == HB_DTYPE_F32)
-    mx_quantize_kernel<<<grid, THREADS, 0, stream>>>((const float*)x, x_ld, K, sorted_entry, top_k, offsets, experts, (uint8_t*)codes, (uint8_t*)scales);
-  else
-    mx_quantize_kernel<<<grid, THREADS, 0, stream>>>((const __nv_bfloat16*)x, x_ld, K, sorted_entry, top_k, offsets, experts, (uint8_t*)codes,
-                                                     (uint8_t*)scales);
+  const bool four = much(rows, K);
+  const int blocks = blocks_of(rows, K, four ? 4 : 1);
+  if (blocks == 0) return HB_ERR_UNSUPPORTED;
+  auto* launch = dtype == HB_DTYPE_F32 ? (four ? quantize<float, 4> : quantize<float, 1>) : (four ? quantize<__nv_bfloat16, 4> : quantize<__nv_bfloat16, 1>);
+  launch(x, x_ld, rows, K, sorted_entry, top_k, offsets, experts, codes, scales, blocks, stream);
   HB_LAUNCH_CHECK();
   return HB_OK;
 }
@@ -100,11 +182,11 @@ extern "C" int hb_mx_values(const void* codes, const void* scales, int rows, int
     return HB_ERR_BAD_ARG;
   if (K % mx::BLOCK) return HB_ERR_UNSUPPORTED;
   if (rows == 0) return HB_OK;
-  const dim3 grid(rows, (mx::chunks(K) / 2 + THREADS / 32 - 1) / (THREADS / 32));
-  if (out_dtype == HB_DTYPE_F32)
-    mx_values_kernel<<<grid, THREADS, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, K, offsets, experts, (float*)out);
-  else
-    mx_values_kernel<<<grid, THREADS, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, K, offsets, experts, (__nv_bfloat16*)out);
+  const bool four = much(rows, K);
+  const int blocks = blocks_of(rows, K, four ? 4 : 1);
+  if (blocks == 0) return HB_ERR_UNSUPPORTED;
+  auto* launch = out_dtype == HB_DTYPE_F32 ? (four ? values<float, 4> : values<float, 1>) : (four ? values<__nv_bfloat16, 4> : values<__nv_bfloat16, 1>);
+  launch(codes, scales, rows, K, offsets, experts, out, blocks, stream);
   HB_LAUNCH_CHECK();
   return HB_OK;
 }

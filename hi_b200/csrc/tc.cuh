@@ -307,6 +307,22 @@ __device__ __forceinline__ void copy_scales_if(uint32_t mine, uint32_t d_tmem, u
       "setp.ne.b32 e, %2, 0;\n"
       "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}" ::"r"(d_tmem), "l"(desc), "r"(mine) : "memory");
 }
+__device__ __forceinline__ void mma_mx_pair_if(uint32_t mine, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
+                                               uint32_t b_scales, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred e, p;\n"
+      "setp.ne.b32 e, %7, 0;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(a_scales), "r"(b_scales), "r"(mine) : "memory");
+}
+// the same offsets of both blocks of a pair, each to its own tensor memory
+__device__ __forceinline__ void copy_scales_pair_if(uint32_t mine, uint32_t d_tmem, uint64_t desc) {
+  asm volatile(
+      "{\n.reg .pred e;\n"
+      "setp.ne.b32 e, %2, 0;\n"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n}" ::"r"(d_tmem), "l"(desc), "r"(mine) : "memory");
+}
 // descriptor of such 512 bytes: rows of 16 bytes, no swizzle, 128 bytes between groups of eight
 __device__ __forceinline__ uint64_t desc_scales(uint32_t saddr) {
   return (uint64_t)((saddr & 0x3FFFF) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
@@ -347,7 +363,18 @@ inline bool make_map_bf16(CUtensorMap* map, const void* base, uint64_t rows, uin
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// [rows, bytes] row-major; box [box_rows, 128 bytes]; else the same
+// [rows, 512 bytes] of scales, a box of `box_rows`, as they lie
+inline bool make_map_scales(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {128, rows};
+  const cuuint64_t strides[1] = {512};
+  const cuuint32_t box[2] = {128, box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// [rows, bytes] row-major; box [box_rows, 128 bytes]; else the same as make_map_bf16
 inline bool make_map_bytes(CUtensorMap* map, const void* base, uint64_t rows, uint64_t bytes, uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;

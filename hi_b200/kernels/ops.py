@@ -45,7 +45,7 @@ _SIGNATURES = {
     "hb_four_bit_linear_tc": [P, c_longlong, P, P, P, I, I, I, I, I, P, P],
     "hb_mx_quantize": [P, I, c_longlong, I, I, P, I, P, I, P, P, P],
     "hb_mx_values": [P, P, I, I, P, I, P, I, P],
-    "hb_mx_gemm": [P, P, I, P, I, P, P, I, I, P, P, P, I, F, P, I, P, P, P],
+    "hb_mx_gemm": [P, I, c_longlong, I, P, P, I, P, I, P, P, I, I, P, P, P, I, F, P, I, P, P, P],
     "hb_paged_attention": [P, I, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, F, P, P, I, I, P, P, P],
     "hb_attention_portions": [P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, F, I, F, P, P, I, P, P, P],
     "hb_attention_merge": [P, P, P, I, I, I, I, I, I, P, P],
@@ -2709,12 +2709,17 @@ def _mx_input(x: torch.Tensor, k: Optional[int] = None) -> torch.Tensor:
 
 
 def _mx_quantize(x: torch.Tensor, rows: int, sorted_entry, top_k: int, offsets) -> MxRows:
-    k, experts = x.shape[1], 1 if offsets is None else offsets.numel() - 1
-    codes, scales = x.new_empty((rows, k // 2), dtype=torch.uint8), _mx_scales(x, rows, k, experts)
+    out = _mx_empty(x, rows, offsets)
     if rows:
-        _check(lib().hb_mx_quantize(_ptr(x), _dt(x), x.stride(0) if x.shape[0] > 1 else k, rows, k, _ptr(sorted_entry), top_k, _ptr(offsets), experts,
-                                    _ptr(codes), _ptr(scales), _stream()), "mx_quantize")
-    return MxRows(codes, scales, (rows, k), offsets)
+        k = x.shape[1]
+        _check(lib().hb_mx_quantize(_ptr(x), _dt(x), x.stride(0) if x.shape[0] > 1 else k, rows, k, _ptr(sorted_entry), top_k, _ptr(offsets),
+                                    out.experts, _ptr(out.codes), _ptr(out.scales), _stream()), "mx_quantize")
+    return out
+
+
+def _mx_empty(x: torch.Tensor, rows: int, offsets) -> MxRows:
+    k, experts = x.shape[1], 1 if offsets is None else offsets.numel() - 1
+    return MxRows(x.new_empty((rows, k // 2), dtype=torch.uint8), _mx_scales(x, rows, k, experts), (rows, k), offsets)
 
 
 def _mx_plan(plan: MoePlan, rows: int) -> None:
@@ -2766,8 +2771,9 @@ def mx_quantize_weight(weight: torch.Tensor, glu: bool = False) -> MxWeight:
     return MxWeight(rows.codes.view(e, m, k // 2), rows.scales[: e * tiles].view(e, tiles, _mx_chunks(k), 512), weight.shape, glu)
 
 
-def _mx_gemm(rows: MxRows, weight: MxWeight, name: str, out_dtype=None, bias=None, sorted_entry=None, scores=None, limit: float = 0.0):
-    """The product; without ``out_dtype`` the gated unit, as :class:`MxRows`."""
+def _mx_gemm(rows: MxRows, weight: MxWeight, name: str, out_dtype=None, bias=None, plan=None, scores=None, limit: float = 0.0, raw=None,
+             top_k: int = 1):
+    """The product; without ``out_dtype`` the gated unit, as :class:`MxRows`. With ``raw`` the rows are quantised from it first, by the same call."""
     (n, k), m = rows.shape, weight.shape[-2]
     if rows.experts != weight.experts or k != weight.shape[-1] or (len(weight.shape) == 3) != (rows.offsets is not None):
         raise KernelError(f"{name}: rows {rows.shape} of {rows.experts} experts do not go with a weight {weight.shape}")
@@ -2777,6 +2783,7 @@ def _mx_gemm(rows: MxRows, weight: MxWeight, name: str, out_dtype=None, bias=Non
         _need(bias, "bias", torch.bfloat16)
         if bias.numel() != m:
             raise KernelError(f"{name}: bias has {bias.numel()} elements for {m} outputs")
+    sorted_entry = None if plan is None else plan.sorted_entry
     _on_current_device(rows.codes, rows.offsets, weight.codes, bias, sorted_entry, scores)
     act = None
     if out_dtype is None:
@@ -2786,7 +2793,8 @@ def _mx_gemm(rows: MxRows, weight: MxWeight, name: str, out_dtype=None, bias=Non
         out = rows.codes.new_empty((n, m), dtype=out_dtype)
     if n:
         TC_USED[0] = True
-        _check(lib().hb_mx_gemm(_ptr(rows.codes), _ptr(rows.scales), n, _ptr(rows.offsets), rows.experts, _ptr(weight.codes), _ptr(weight.scales), m, k,
+        _check(lib().hb_mx_gemm(_ptr(raw), 0 if raw is None else _dt(raw), 0 if raw is None else raw.stride(0) if raw.shape[0] > 1 else k, top_k,
+                                _ptr(rows.codes), _ptr(rows.scales), n, _ptr(rows.offsets), rows.experts, _ptr(weight.codes), _ptr(weight.scales), m, k,
                                 _ptr(bias), _ptr(sorted_entry), _ptr(scores), int(act is not None), float(limit), _ptr(out),
                                 0 if act is not None else _dt(out), _ptr(act.scales) if act is not None else None,
                                 _ptr(_tc_status(rows.device)), _stream()), name)
@@ -2804,18 +2812,22 @@ def mx_linear(x, weight: MxWeight, out_dtype: torch.dtype = torch.bfloat16, bias
     _mx_rows_for(x, weight, "mx_linear", False)
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise KernelError(f"mx_linear returns bfloat16 or float32, not {out_dtype}")
+    raw = None
     if not isinstance(x, MxRows):
-        x = mx_quantize(_mx_input(x, weight.shape[-1]))
-    return _mx_gemm(x, weight, "mx_linear", out_dtype, bias)
+        raw = _mx_input(x, weight.shape[-1])
+        x = _mx_empty(raw, raw.shape[0], None)
+    return _mx_gemm(x, weight, "mx_linear", out_dtype, bias, raw=raw)
 
 
 def mx_glu(x, weight: MxWeight, limit: float = 0.0) -> MxRows:
     """silu(x Wg^T) (x Wu^T), or with ``limit`` > 0 the clamped unit min(g, limit) sigmoid(1.702 min(g, limit)) (clamp(u, +-limit) + 1), from float32
     sums, quantised as it is: what the down projection reads. ``weight`` has gate and up rows in turn (``mx_interleave``)."""
     _mx_rows_for(x, weight, "mx_glu", True)
+    raw = None
     if not isinstance(x, MxRows):
-        x = mx_quantize(_mx_input(x, weight.shape[-1]))
-    return _mx_gemm(x, weight, "mx_glu", limit=limit)
+        raw = _mx_input(x, weight.shape[-1])
+        x = _mx_empty(raw, raw.shape[0], None)
+    return _mx_gemm(x, weight, "mx_glu", limit=limit, raw=raw)
 
 
 def mx_experts_glu(x: torch.Tensor, plan: MoePlan, top_k: int, weight: MxWeight, scores: Optional[torch.Tensor] = None,
@@ -2827,8 +2839,9 @@ def mx_experts_glu(x: torch.Tensor, plan: MoePlan, top_k: int, weight: MxWeight,
         _need(scores, "scores", torch.float32)
         if scores.numel() != x.shape[0] * top_k:
             raise KernelError(f"mx_experts_glu: {scores.numel()} scores for {x.shape[0]} tokens of {top_k} experts")
-    rows = mx_quantize(_mx_input(x, weight.shape[-1]), plan, top_k)
-    return _mx_gemm(rows, weight, "mx_experts_glu", sorted_entry=plan.sorted_entry, scores=scores, limit=limit)
+    raw, rows = _mx_input(x, weight.shape[-1]), x.shape[0] * top_k
+    _mx_plan(plan, rows)
+    return _mx_gemm(_mx_empty(raw, rows, plan.offsets), weight, "mx_experts_glu", plan=plan, scores=scores, limit=limit, raw=raw, top_k=top_k)
 
 
 def mx_experts_linear(rows: MxRows, weight: MxWeight, plan: MoePlan) -> torch.Tensor:
