@@ -176,8 +176,8 @@ mx_gemm_kernel(const __grid_constant__ Maps maps, const Params p) {
     if constexpr (PAIR) tc::alloc_pair(tmem_slot, TMEM_COLS);
     else tc::alloc(tmem_slot, TMEM_COLS);
   }
-  if (warp == 3 && lane < (PAIR ? 7 : 5)) {
-    const CUtensorMap* map = lane < 4 ? &maps.x[lane] : lane == 4 ? &maps.w : lane == 5 ? &maps.x_scales : &maps.w_scales;
+  if (warp == 3 && lane < (PAIR ? 3 : 1)) {
+    const CUtensorMap* map = lane == 0 ? &maps.w : lane == 1 ? &maps.x_scales : &maps.w_scales;
     tc::prefetch_map(map);
   }
   if (warp == 2) {
@@ -498,11 +498,15 @@ struct Call {
 template <bool GLU, bool PAIR, bool SPLIT, int BN, int STAGES>
 int launch(const Call& c, const Params& p, int blocks, int cluster) {
   Maps maps;
-  for (int b = 0; b < 4; ++b)
-    if (!tc::make_map_bytes(&maps.x[b], c.x, (uint64_t)p.rows, (uint64_t)c.K / 2, 16u << b)) return HB_ERR_UNSUPPORTED;
-  if (!tc::make_map_bytes(&maps.w, c.w, (uint64_t)p.experts * p.n_out, (uint64_t)c.K / 2, PAIR ? BN / 2 : BN) ||
-      !tc::make_map_scales(&maps.x_scales, c.x_scales, (uint64_t)c.scale_tiles * p.chunks, KB / mx::CHUNK) ||
-      !tc::make_map_scales(&maps.w_scales, c.w_scales, (uint64_t)p.experts * p.w_tiles * p.chunks, KB / mx::CHUNK))
+  // a map costs the host 0.3 us: those that tiles of these rows ask for
+  const int rest = p.rows % BM, last = rest == 0 ? 3 : rest <= 16 ? 0 : rest <= 32 ? 1 : rest <= 64 ? 2 : 3;
+  for (int b = 0; b < 4; ++b) {
+    const bool asked = PAIR ? b == 3 : p.offsets ? b == 0 || p.rows > 8 << b : b == last || (b == 3 && p.rows >= BM);
+    if (asked && !tc::make_map_bytes(&maps.x[b], c.x, (uint64_t)p.rows, (uint64_t)c.K / 2, 16u << b)) return HB_ERR_UNSUPPORTED;
+  }
+  if (!tc::make_map_bytes(&maps.w, c.w, (uint64_t)p.experts * p.n_out, (uint64_t)c.K / 2, PAIR ? BN / 2 : BN)) return HB_ERR_UNSUPPORTED;
+  if (PAIR && (!tc::make_map_scales(&maps.x_scales, c.x_scales, (uint64_t)c.scale_tiles * p.chunks, KB / mx::CHUNK) ||
+               !tc::make_map_scales(&maps.w_scales, c.w_scales, (uint64_t)p.experts * p.w_tiles * p.chunks, KB / mx::CHUNK)))
     return HB_ERR_UNSUPPORTED;
   static_assert((2 * STAGES + 5) * 8 + 8 <= 256, "the barriers fit");
   static_assert(STAGES * stage_bytes<PAIR, BN>() + 1280 + 12 * 128 <= 227 * 1024, "128 experts at least");

@@ -2623,18 +2623,32 @@ def _mx_chunks(k: int) -> int:
 class MxRows:
     """Rows [N, K] in microscaled 4-bit floats: blocks of 32 values along a row are 2^e times e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
     their negatives) with e = floor(log2(largest magnitude)) - 2, at least -127; a block with a value that is not finite is not a number.
-    ``codes`` uint8 [N, K / 2] (the even value in the low half), ``scales`` as the tensor cores read them (csrc/mx.cuh). Rows in the order
-    of a :class:`MoePlan` carry its ``offsets``: every expert's scales begin a tile. ``mx_quantize``, ``mx_glu`` and ``mx_experts_glu`` make them."""
+    ``codes`` uint8 [N, K / 2] (the even value in the low half), ``scales`` [tiles, chunks, 512] as the tensor cores read them
+    (csrc/mx.cuh), one behind the other in ``data``. Rows in the order of a :class:`MoePlan` carry its ``offsets``: every expert's scales
+    begin a tile. ``mx_quantize``, ``mx_glu`` and ``mx_experts_glu`` make them."""
 
-    __slots__ = ("codes", "scales", "shape", "offsets")
+    __slots__ = ("data", "shape", "offsets", "scales_at")
     dtype = torch.bfloat16           # of what is computed from them, unless it is said
 
-    def __init__(self, codes, scales, shape, offsets=None):
-        self.codes, self.scales, self.shape, self.offsets = codes, scales, shape, offsets
+    def __init__(self, like: torch.Tensor, n: int, k: int, offsets=None):
+        """Room for ``n`` rows of ``k`` values beside ``like``, nothing written."""
+        runs = 1 if offsets is None else min(offsets.numel() - 1, n or 1)
+        self.shape, self.offsets, self.scales_at = (n, k), offsets, -(-n * k // 1024) * 512
+        tiles = -(-n // MX_TILE) + runs - 1                 # as many as runs of these rows can begin
+        self.data = like.new_empty(self.scales_at + tiles * _mx_chunks(k) * 512, dtype=torch.uint8)      # (one allocation: 1.5 us less)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        n, k = self.shape
+        return self.data[: n * k // 2].view(n, k // 2)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.data[self.scales_at:].view(-1, _mx_chunks(self.shape[1]), 512)
 
     @property
     def device(self):
-        return self.codes.device
+        return self.data.device
 
     @property
     def experts(self) -> int:
@@ -2688,38 +2702,28 @@ def mx_pack_weight(codes: torch.Tensor, exponents: torch.Tensor, glu: bool = Fal
     return MxWeight((c[..., 0] | c[..., 1] << 4).contiguous(), s, codes.shape, glu)
 
 
-def _mx_scales(x: torch.Tensor, rows: int, k: int, experts: int) -> torch.Tensor:
-    tiles = -(-rows // MX_TILE) + min(experts, max(rows, 1)) - 1       # as many as `experts` runs of these rows can begin
-    return x.new_empty((tiles, _mx_chunks(k), 512), dtype=torch.uint8)
-
-
 def _mx_input(x: torch.Tensor, k: Optional[int] = None) -> torch.Tensor:
     if not x.is_cuda:
         raise KernelError("x must be a CUDA tensor; this engine has no CPU path")
-    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32) or x.shape[1] % MX_BLOCK or not x.shape[1] or k not in (None, x.shape[1]):
+    shape, dtype = x.shape, x.dtype
+    if len(shape) != 2 or (dtype != torch.bfloat16 and dtype != torch.float32) or (shape[1] != k if k else shape[1] % MX_BLOCK or not shape[1]):
         raise KernelError(f"rows of {f'{k} values' if k else f'a multiple of {MX_BLOCK} values'} in bfloat16 or float32 are quantised, not "
-                          f"{x.dtype} {tuple(x.shape)}")
-    if torch.is_grad_enabled() and x.requires_grad:
+                          f"{dtype} {tuple(shape)}")
+    if x.requires_grad and torch.is_grad_enabled():
         raise KernelError("quantised rows have no gradients")
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) * x.element_size() % 16) or x.data_ptr() % 16:
+    if not x.is_contiguous() and (x.stride(1) != 1 or (shape[0] > 1 and x.stride(0) * x.element_size() % 16)):
         x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
-    return x
+    return x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
 
 
 def _mx_quantize(x: torch.Tensor, rows: int, sorted_entry, top_k: int, offsets) -> MxRows:
-    out = _mx_empty(x, rows, offsets)
+    k = x.shape[1]
+    out = MxRows(x, rows, k, offsets)
     if rows:
-        k = x.shape[1]
-        _check(lib().hb_mx_quantize(_ptr(x), _dt(x), x.stride(0) if x.shape[0] > 1 else k, rows, k, _ptr(sorted_entry), top_k, _ptr(offsets),
-                                    out.experts, _ptr(out.codes), _ptr(out.scales), _stream()), "mx_quantize")
+        to = out.data.data_ptr()
+        _check(lib().hb_mx_quantize(x.data_ptr(), _dt(x), x.stride(0) if x.shape[0] > 1 else k, rows, k, _ptr(sorted_entry), top_k, _ptr(offsets),
+                                    out.experts, to, to + out.scales_at, _stream()), "mx_quantize")
     return out
-
-
-def _mx_empty(x: torch.Tensor, rows: int, offsets) -> MxRows:
-    k, experts = x.shape[1], 1 if offsets is None else offsets.numel() - 1
-    return MxRows(x.new_empty((rows, k // 2), dtype=torch.uint8), _mx_scales(x, rows, k, experts), (rows, k), offsets)
 
 
 def _mx_plan(plan: MoePlan, rows: int) -> None:
@@ -2746,12 +2750,13 @@ def mx_values(rows: MxRows, out_dtype: torch.dtype = torch.bfloat16) -> torch.Te
     """The values that quantised rows stand for, [N, K] in bfloat16 or float32 (both hold them exactly)."""
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise KernelError(f"values are bfloat16 or float32, not {out_dtype}")
-    _on_current_device(rows.codes)
+    data = rows.data
+    _on_current_device(data)
     n, k = rows.shape
-    out = torch.empty((n, k), dtype=out_dtype, device=rows.device)
+    out = data.new_empty((n, k), dtype=out_dtype)
     if n:
-        _check(lib().hb_mx_values(_ptr(rows.codes), _ptr(rows.scales), n, k, _ptr(rows.offsets), rows.experts, _ptr(out), _dt(out), _stream()),
-               "mx_values")
+        at = data.data_ptr()
+        _check(lib().hb_mx_values(at, at + rows.scales_at, n, k, _ptr(rows.offsets), rows.experts, out.data_ptr(), _dt(out), _stream()), "mx_values")
     return out
 
 
@@ -2784,21 +2789,22 @@ def _mx_gemm(rows: MxRows, weight: MxWeight, name: str, out_dtype=None, bias=Non
         if bias.numel() != m:
             raise KernelError(f"{name}: bias has {bias.numel()} elements for {m} outputs")
     sorted_entry = None if plan is None else plan.sorted_entry
-    _on_current_device(rows.codes, rows.offsets, weight.codes, bias, sorted_entry, scores)
-    act = None
+    data, codes = rows.data, weight.codes
+    _on_current_device(data, codes, rows.offsets, bias, sorted_entry, scores)
     if out_dtype is None:
-        out = rows.codes.new_empty((n, m // 4))
-        act = MxRows(out, _mx_scales(rows.codes, n, m // 2, rows.experts), (n, m // 2), rows.offsets)
+        out = MxRows(data, n, m // 2, rows.offsets)
+        to, kind, scales_to = out.data.data_ptr(), 0, out.scales_at
     else:
-        out = rows.codes.new_empty((n, m), dtype=out_dtype)
+        out = data.new_empty((n, m), dtype=out_dtype)
+        to, kind, scales_to = out.data_ptr(), _dt(out), 0
     if n:
         TC_USED[0] = True
-        _check(lib().hb_mx_gemm(_ptr(raw), 0 if raw is None else _dt(raw), 0 if raw is None else raw.stride(0) if raw.shape[0] > 1 else k, top_k,
-                                _ptr(rows.codes), _ptr(rows.scales), n, _ptr(rows.offsets), rows.experts, _ptr(weight.codes), _ptr(weight.scales), m, k,
-                                _ptr(bias), _ptr(sorted_entry), _ptr(scores), int(act is not None), float(limit), _ptr(out),
-                                0 if act is not None else _dt(out), _ptr(act.scales) if act is not None else None,
-                                _ptr(_tc_status(rows.device)), _stream()), name)
-    return out if act is None else act
+        at = data.data_ptr()
+        raw_at, raw_kind, raw_ld = (None, 0, 0) if raw is None else (raw.data_ptr(), _dt(raw), raw.stride(0) if raw.shape[0] > 1 else k)
+        _check(lib().hb_mx_gemm(raw_at, raw_kind, raw_ld, top_k, at, at + rows.scales_at, n, _ptr(rows.offsets), weight.experts, codes.data_ptr(),
+                                weight.scales.data_ptr(), m, k, _ptr(bias), _ptr(sorted_entry), _ptr(scores), out_dtype is None, limit, to, kind,
+                                to + scales_to if scales_to else None, _ptr(_tc_status(data.device)), _stream()), name)
+    return out
 
 
 def _mx_rows_for(x, weight: MxWeight, name: str, glu: bool, stack: bool = False) -> None:
@@ -2815,7 +2821,7 @@ def mx_linear(x, weight: MxWeight, out_dtype: torch.dtype = torch.bfloat16, bias
     raw = None
     if not isinstance(x, MxRows):
         raw = _mx_input(x, weight.shape[-1])
-        x = _mx_empty(raw, raw.shape[0], None)
+        x = MxRows(raw, raw.shape[0], raw.shape[1])
     return _mx_gemm(x, weight, "mx_linear", out_dtype, bias, raw=raw)
 
 
@@ -2826,7 +2832,7 @@ def mx_glu(x, weight: MxWeight, limit: float = 0.0) -> MxRows:
     raw = None
     if not isinstance(x, MxRows):
         raw = _mx_input(x, weight.shape[-1])
-        x = _mx_empty(raw, raw.shape[0], None)
+        x = MxRows(raw, raw.shape[0], raw.shape[1])
     return _mx_gemm(x, weight, "mx_glu", limit=limit, raw=raw)
 
 
@@ -2841,7 +2847,7 @@ def mx_experts_glu(x: torch.Tensor, plan: MoePlan, top_k: int, weight: MxWeight,
             raise KernelError(f"mx_experts_glu: {scores.numel()} scores for {x.shape[0]} tokens of {top_k} experts")
     raw, rows = _mx_input(x, weight.shape[-1]), x.shape[0] * top_k
     _mx_plan(plan, rows)
-    return _mx_gemm(_mx_empty(raw, rows, plan.offsets), weight, "mx_experts_glu", plan=plan, scores=scores, limit=limit, raw=raw, top_k=top_k)
+    return _mx_gemm(MxRows(raw, rows, raw.shape[1], plan.offsets), weight, "mx_experts_glu", plan=plan, scores=scores, limit=limit, raw=raw, top_k=top_k)
 
 
 def mx_experts_linear(rows: MxRows, weight: MxWeight, plan: MoePlan) -> torch.Tensor:
