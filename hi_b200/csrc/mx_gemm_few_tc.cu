@@ -78,14 +78,16 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
   // tile i of this block, by a whole warp
   auto tile_at = [&](int i, Tile& t) {
     const int at = unit_id + i * unit_count;
+    if (!p.offsets) {                             // one run of rows: no table (the first copies leave 0.4 us earlier)
+      const int units = (p.rows + BT - 1) / BT, f = units == 1 ? at : at / units, m = at - f * units;
+      if (f >= f_tiles) return false;
+      t = {0, m * BT, min(BT, p.rows - m * BT), m * BT / mx::TILE, f * BF};
+      return true;
+    }
     if (at >= first_unit[p.experts] * f_tiles) return false;
-    const int e = mx::expert_of(p, first_unit, f_tiles, at);
+    const int e = mx::expert_of(p, first_unit, f_tiles, at), row = first_row[e];
     const int units = first_unit[e + 1] - first_unit[e], here = at - first_unit[e] * f_tiles, f = here / units, m = here - f * units;
-    t.expert = e;
-    t.row0 = first_row[e] + m * BT;
-    t.rows = min(BT, first_row[e + 1] - t.row0);
-    t.scale_tile = first_tile[e] + m * BT / mx::TILE;
-    t.f0 = f * BF;
+    t = {e, row + m * BT, min(BT, first_row[e + 1] - row - m * BT), first_tile[e] + m * BT / mx::TILE, f * BF};
     return true;
   };
   const uint32_t mine = tc::elect_one(), ring = tc::smem_u32(smem), bars = tc::smem_u32(full);
@@ -113,12 +115,10 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
   int ahead = 0;                                  // warp 0: stages on their way before the warps meet
   if (warp == 0) {
     if (lane == 0) {
-      for (int s = 0; s < STAGES; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
-      for (int b = 0; b < 2; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], EPILOGUE); }
-      tc::mbar_init(acc_shared, EPILOGUE);
-      asm volatile("fence.mbarrier_init.release.cluster;\nfence.proxy.async.shared::cta;" ::: "memory");
+      for (int s = 0; s < STAGES; ++s) tc::mbar_init(&full[s], 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    mx::place_experts(p, BT, first_row, first_tile, first_unit);
+    if (p.offsets) mx::place_experts(p, BT, first_row, first_tile, first_unit);
     __syncwarp();
     if (tile_at(0, t)) {
       ahead = min(STAGES, kb1 - kb0);
@@ -135,6 +135,12 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
     }
   }
   if (warp == 1) tc::alloc(tmem_slot, TMEM_COLS);
+  if (warp == 2 && lane == 0) {
+    for (int s = 0; s < STAGES; ++s) tc::mbar_init(&empty[s], 1);
+    for (int b = 0; b < 2; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], EPILOGUE); }
+    tc::mbar_init(acc_shared, EPILOGUE);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();

@@ -338,11 +338,11 @@ int pairs(const Call& c, const Params& p, int pairs) {
 }
 
 // The form by a model of the time in us. Few rows (mx_gemm_few_tc.cu): a stage of 128 weight rows by n rows takes a block 0.12 + 0.0014 n, 0.2 at least, and
-// the first stage's way and the last results 4.4; blocks that share K meet in 2 + 0.045 a row more. Pairs: a stage 0.34 in the first round and 0.44 in
+// the first stage's way and the last results 3.4; blocks that share K meet in 2.6 + 0.045 a row more. Pairs: a stage 0.34 in the first round and 0.44 in
 // others (the card is at its power limit then), a tile 6 at least (its results), 6.5 besides. An expert's last tile is taken to be half full.
 // Measured, as pairs / single blocks: 512 x 16,384 x 5,120 24.1 / 24.2, 700 x 5,120 x 8,192 18.8 / 18.4, 2,048 x 16,384 x 5,120 67.5 / 72.7, units of 2,047 x 8,192
-// x 5,120 64.4 / 75.0, of 99 x 5,120 x 8,192 17.7 / 12.8; 4,096 rows of 16 experts of 5,120 x 8,192: up 209 / 218, down 118 / 110, 2,048: 157 / 147 and 87 / 75; 8 x
-// 5,120 x 8,192 10.8, in two and three parts 9.9 and 9.1. Tiles of up to 64, 128 and 256 rows: 8 x 7,168 x 5,120 8.4 / 8.8 / 10.3, 2,048 x 16,384 x 5,120
+// x 5,120 64.4 / 75.0, 99 x 5,120 x 8,192 17.7 / 11.5; 4,096 rows of 16 experts of 5,120 x 8,192: up 209 / 218, down 118 / 110, 2,048: 157 / 147 and 87 / 75; 8 x
+// 5,120 x 8,192 9.9, in two and three parts 9.0 and 8.5. Tiles of up to 64, 128 and 256 rows: 8 x 7,168 x 5,120 7.5 / 7.8 / 9.4, 2,048 x 16,384 x 5,120
 // - / 84.6 / 72.7.
 int gemm(const Call& c, const Params& p, bool glu) {
   const int runs = p.experts < p.rows ? p.experts : p.rows, each = (p.rows + runs - 1) / runs, stages = p.chunks / 2;
@@ -352,18 +352,18 @@ int gemm(const Call& c, const Params& p, bool glu) {
   float single, pair;
   if (runs == 1) {
     const int tiles = (p.rows + most_rows - 1) / most_rows, n = (p.rows + tiles - 1) / tiles;
-    single = 4.4f + (f_tiles * tiles + 147) / 148 * stages * fmaxf(0.2f, 0.12f + 0.0014f * n);
+    single = 3.4f + (f_tiles * tiles + 147) / 148 * stages * fmaxf(0.2f, 0.12f + 0.0014f * n);
     pair = 6.5f + (most_pairs + 73) / 74 * fmaxf(6.f, stages * 0.44f) - stages * 0.1f;
   } else {
     const float tiles = runs * (each > most_rows ? (float)each / most_rows + 0.5f : 1.f), pairs = runs * ((float)each / (2 * BM) + 0.5f);
-    single = 4.4f + f_tiles / 148.f * stages * fmaxf(0.2f * tiles, 0.12f * tiles + 0.0014f * p.rows);
+    single = 3.4f + f_tiles / 148.f * stages * fmaxf(0.2f * tiles, 0.12f * tiles + 0.0014f * p.rows);
     pair = 6.5f + f_pairs / 74.f * pairs * fmaxf(6.f, stages * 0.44f);
   }
   int splits = 1;
   float best = fminf(single, pair);
   const long long most = ((p.rows + BM - 1) / BM + runs - 1LL) * f_tiles;
   for (int n = 2; n <= MOST_SPLITS && n <= stages && n * most <= 148; ++n) {
-    const float shared = 6.4f + 0.045f * each + (stages + n - 1) / n * 0.2f;
+    const float shared = 6.f + 0.045f * each + (stages + n - 1) / n * 0.2f;
     if (shared < best) { best = shared; splits = n; }
   }
   if (splits > 1 || single <= pair) return hb_mx_gemm_few(c, p, glu, splits, most_rows);
