@@ -239,7 +239,8 @@ mx_gemm_kernel(const __grid_constant__ Maps maps, const Params p) {
       const bool another = pair_id + (i + 1) * pair_count < all;
       for (int kb = 0; kb < stages; ++kb) {
         const int next = s + 1 == STAGES ? 0 : s + 1, next_turn = s + 1 == STAGES ? turn ^ 1 : turn;
-        if ((kb + 1 < stages || another) && !scales(next, next_turn, set ^ 1)) {
+        const bool more = kb + 1 < stages || another;
+        if (kb > 0 && more && !scales(next, next_turn, set ^ 1)) {
           ok = false;
           break;
         }
@@ -250,6 +251,10 @@ mx_gemm_kernel(const __grid_constant__ Maps maps, const Params p) {
           tc::mma_mx_pair_if(mine, acc, a + (k * 32 >> 4), w + (k * 32 >> 4), tc::idesc_mxf4(2 * BM, BN, k % 2 * 2), sa + k / 2 * 4, sb + k / 2 * CHUNK_COLS,
                              kb | k);
         tc::commit_pair_if(mine, &empty[s]);
+        if (kb == 0 && more && !scales(next, next_turn, set ^ 1)) {        // (a tile's first products have waited long enough)
+          ok = false;
+          break;
+        }
         s = next;
         turn = next_turn;
         set ^= 1;
@@ -258,10 +263,11 @@ mx_gemm_kernel(const __grid_constant__ Maps maps, const Params p) {
     }
   } else {                                        // ---- results
     const int quarter = warp & 3, half = (warp - 2) >> 2, r = quarter * 32 + lane;
+    // What has been read is in registers when the warp arrives; a release towards the cluster would wait for the results' stores, 1,700 cycles a tile.
     auto arrive = [&](uint64_t* bar) {
       tc::fence_before();
       __syncwarp();
-      if (lane == 0) tc::arrive_even(tc::even_block(bar));
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(tc::even_block(bar)) : "memory");
     };
     for (int i = 0; tile_at(i, t); ++i) {
       const int b = i & 1;
