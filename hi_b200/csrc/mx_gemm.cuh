@@ -116,4 +116,5 @@ int start(Kernel* kernel, const Maps& maps, const Params& p, int threads, int bl
 }  // namespace mx
 
 // Few rows, and experts: `splits` blocks share K (1: none do), up to `most` rows a tile.
+int hb_mx_clusters(int size);      // clusters of so many blocks that live at a time
 int hb_mx_gemm_few(const mx::Call& c, const mx::Params& p, bool glu, int splits, int most);

@@ -418,7 +418,7 @@ int launch(const Call& c, const Params& p, int blocks, int cluster) {
 
 template <bool GLU>
 int few(const Call& c, const Params& p, int splits, int most) {
-  auto grid = [&](int bt) {       // tiles that there may be
+  auto grid = [&](int bt) {        // tiles that there may be
     const long long units = (p.rows + bt - 1) / bt + (p.experts < p.rows ? p.experts : p.rows) - 1LL;
     return units * ((p.n_out + BF - 1) / BF);
   };
@@ -430,6 +430,31 @@ int few(const Call& c, const Params& p, int splits, int most) {
 }
 
 }  // namespace
+
+// How many clusters of `size` blocks live at a time on the current device; without one, as many as its blocks would make.
+int hb_mx_clusters(int size) {
+  static std::atomic<int> known[64][16];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device > 63 || size > 15) return 148 / size;
+  int n = known[device][size].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  auto* kernel = mx_gemm_few_kernel<false, true, 128, 6>;
+  constexpr size_t smem = 6 * stage_bytes<128>() + 1280 + 24;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return 148 / size;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(size * 148);
+  config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = size;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess || n <= 0) return 148 / size;
+  known[device][size].store(n, std::memory_order_relaxed);
+  return n;
+}
 
 // splits: blocks that share K (1: none do); most: rows of a tile, 64 (where there are no more in all), 128 or 256.
 int hb_mx_gemm_few(const Call& c, const Params& p, bool glu, int splits, int most) {

@@ -344,36 +344,45 @@ int pairs(const Call& c, const Params& p, int pairs) {
 }
 
 // The form by a model of the time in us. Few rows (mx_gemm_few_tc.cu): a stage of 128 weight rows by n rows takes a block 0.12 + 0.0014 n, 0.2 at least, and
-// the first stage's way and the last results 3.4; blocks that share K meet in 2.6 + 0.045 a row more. Pairs: a stage 0.34 in the first round and 0.44 in
+// the first stage's way and the last results 3.4; n blocks that share K 4.3, 0.07 a tile, 0.17 a stage and 0.02 + 0.05 / n a row. Pairs: a stage 0.34 in the first round and 0.44 in
 // others (the card is at its power limit then), a tile 6 at least (its results), 6.5 besides. An expert's last tile is taken to be half full.
 // Measured, as pairs / single blocks: 512 x 16,384 x 5,120 24.1 / 24.2, 700 x 5,120 x 8,192 18.8 / 18.4, 2,048 x 16,384 x 5,120 67.5 / 72.7, units of 2,047 x 8,192
-// x 5,120 64.4 / 75.0, 99 x 5,120 x 8,192 17.7 / 11.5; 4,096 rows of 16 experts of 5,120 x 8,192: up 209 / 218, down 118 / 110, 2,048: 157 / 147 and 87 / 75; 8 x
-// 5,120 x 8,192 9.9, in two and three parts 9.0 and 8.5. Tiles of up to 64, 128 and 256 rows: 8 x 7,168 x 5,120 7.5 / 7.8 / 9.4, 2,048 x 16,384 x 5,120
+// x 5,120 64.4 / 75.0, 99 x 5,120 x 8,192 17.7 / 11.5; 4,096 rows of 16 experts of 5,120 x 8,192: up 209 / 218, down 118 / 110, 2,048: 157 / 147 and 87 / 75; in one, two, four and
+// eight parts 1 x 256 x 8,192 7.9 / 6.7 / 5.9 / 5.5, 16 x 2,048 x 8,192 9.0 / 8.7 / 7.5 / 12.4 (more clusters than live at a time), 60 x 2,048 x 4,096 6.8 / 9.1 /
+// 7.9 / 13.3, in three 1 x 5,120 x 8,192 9.5 -> 8.6, 60 rows 10.2 -> 10.8. Tiles of up to 64, 128 and 256 rows: 8 x 7,168 x 5,120 7.5 / 7.8 / 9.4, 2,048 x 16,384 x 5,120
 // - / 84.6 / 72.7.
-int gemm(const Call& c, const Params& p, bool glu) {
-  const int runs = p.experts < p.rows ? p.experts : p.rows, each = (p.rows + runs - 1) / runs, stages = p.chunks / 2;
-  const int most_rows = p.rows <= 64 ? 64 : each <= 128 ? 128 : 256;
-  const long long f_tiles = (p.n_out + 127) / 128, f_pairs = (p.n_out + BN - 1) / BN;
-  const long long most_pairs = ((p.rows + 2 * BM - 1) / (2 * BM) + runs - 1LL) * f_pairs;      // that there may be
+// `runs`: experts that may have rows. splits 0: pairs of blocks; else single ones, so many of them on a tile, with up to `most_rows` rows of it.
+struct Form { int splits, most_rows; };
+Form form(int rows, int experts, int n_out, int chunks) {
+  const int runs = experts < rows ? experts : rows, each = (rows + runs - 1) / runs, stages = chunks / 2;
+  const int most_rows = rows <= 64 ? 64 : each <= 128 ? 128 : 256;
+  const long long f_tiles = (n_out + 127) / 128, f_pairs = (n_out + BN - 1) / BN;
   float single, pair;
   if (runs == 1) {
-    const int tiles = (p.rows + most_rows - 1) / most_rows, n = (p.rows + tiles - 1) / tiles;
+    const int tiles = (rows + most_rows - 1) / most_rows, n = (rows + tiles - 1) / tiles;
     single = 3.4f + (f_tiles * tiles + 147) / 148 * stages * fmaxf(0.2f, 0.12f + 0.0014f * n);
-    pair = 6.5f + (most_pairs + 73) / 74 * fmaxf(6.f, stages * 0.44f) - stages * 0.1f;
+    pair = 6.5f + ((rows + 2 * BM - 1) / (2 * BM) * f_pairs + 73) / 74 * fmaxf(6.f, stages * 0.44f) - stages * 0.1f;
   } else {
     const float tiles = runs * (each > most_rows ? (float)each / most_rows + 0.5f : 1.f), pairs = runs * ((float)each / (2 * BM) + 0.5f);
-    single = 3.4f + f_tiles / 148.f * stages * fmaxf(0.2f * tiles, 0.12f * tiles + 0.0014f * p.rows);
+    single = 3.4f + f_tiles / 148.f * stages * fmaxf(0.2f * tiles, 0.12f * tiles + 0.0014f * rows);
     pair = 6.5f + f_pairs / 74.f * pairs * fmaxf(6.f, stages * 0.44f);
   }
-  int splits = 1;
-  float best = fminf(single, pair);
-  const long long most = ((p.rows + BM - 1) / BM + runs - 1LL) * f_tiles;
+  Form best{single <= pair ? 1 : 0, most_rows};
+  float least = fminf(single, pair);
+  const long long most = ((rows + BM - 1) / BM + runs - 1LL) * f_tiles;                // tiles that there may be
   for (int n = 2; n <= MOST_SPLITS && n <= stages && n * most <= 148; ++n) {
-    const float shared = 6.f + 0.045f * each + (stages + n - 1) / n * 0.2f;
-    if (shared < best) { best = shared; splits = n; }
+    const float shared = 4.3f + 0.07f * most + (stages + n - 1) / n * 0.17f + each * (0.02f + 0.05f / n);
+    if (shared < least && most <= hb_mx_clusters(n)) { least = shared; best = {n, 128}; }
   }
-  if (splits > 1 || single <= pair) return hb_mx_gemm_few(c, p, glu, splits, most_rows);
-  const int n = (int)(most_pairs < 74 ? most_pairs : 74);
+  return best;
+}
+
+int gemm(const Call& c, const Params& p, bool glu) {
+  const Form f = form(p.rows, p.experts, p.n_out, p.chunks);
+  if (f.splits) return hb_mx_gemm_few(c, p, glu, f.splits, f.most_rows);
+  const int runs = p.experts < p.rows ? p.experts : p.rows;
+  const long long most = ((p.rows + 2 * BM - 1) / (2 * BM) + runs - 1LL) * ((p.n_out + BN - 1) / BN);      // tiles that there may be
+  const int n = (int)(most < 74 ? most : 74);
   return glu ? pairs<true>(c, p, n) : pairs<false>(c, p, n);
 }
 
@@ -405,4 +414,11 @@ extern "C" int hb_mx_gemm(const void* raw, int raw_dtype, long long raw_ld, int 
                  experts, n_out, mx::chunks(K), (n_out + 127) / 128, limit, raw != nullptr};
   const Call c{x, x_scales, w, w_scales, K, (rows + BM - 1) / BM + (experts < rows ? experts : rows) - 1, stream};
   return gemm(c, p, glu != 0);
+}
+
+// The form that hb_mx_gemm takes: 0 pairs of blocks, else 1000 times the blocks that share a tile's K and the rows of a tile.
+extern "C" int hb_mx_gemm_form(int rows, int experts, int n_out, int K) {
+  if (rows < 1 || experts < 1 || n_out < 1 || K < 1) return -1;
+  const Form f = form(rows, experts, n_out, mx::chunks(K));
+  return f.splits ? f.splits * 1000 + f.most_rows : 0;
 }

@@ -121,6 +121,59 @@ def test_linear(m, k, n):
     ops.check_tc_status()
 
 
+@pytest.mark.parametrize("m,k,n", [(128, 8192, 5), (600, 10272, 9), (5120, 8192, 1), (1000, 8192, 33), (2048, 9248, 17), (300, 13312, 70)])
+def test_linear_of_blocks_that_share_k(m, k, n):
+    """Shares of unlike length, the last one short; every block finishes some rows, or has none to finish."""
+    from hi_b200.kernels import ops
+
+    assert ops.lib().hb_mx_gemm_form(n, 1, m, k) >= 2000
+    g = _gen(m + k + n)
+    x, (codes, exps) = _rows(g, n, k), _weight(g, m, k)
+    bias = torch.randn(m, device=DEV, generator=g).to(BF16)
+    w, xv, wv = ops.mx_pack_weight(codes, exps), plain_mx.held(x), plain_mx.values(codes, exps)
+    y = ops.mx_linear(x, w, F32, bias)
+    _near(y, xv, wv, bias)
+    assert torch.equal(ops.mx_linear(x, w, bias=bias), y.to(BF16)) and torch.equal(ops.mx_linear(ops.mx_quantize(x), w, F32, bias), y)
+    if m % 64 == 0:
+        act = ops.mx_values(ops.mx_glu(x, ops.mx_pack_weight(codes, exps, glu=True), 1.5), F32).double()
+        gate, up = (wv.view(-1, 2, 32, k)[:, i].flatten(0, 1) for i in (0, 1))
+        _check_unit(act, xv, gate, up, 1.5)
+    ops.check_tc_status()
+
+
+@pytest.mark.parametrize("m,k,n", [(16400, 5152, 2221), (16385, 4800, 2147), (24576, 5120, 1500)])
+def test_linear_of_many_rows(m, k, n):
+    """Pairs of blocks: several tiles a pair, tiles that are not full in rows, features and k, an odd number of features."""
+    from hi_b200.kernels import ops
+
+    assert ops.lib().hb_mx_gemm_form(n, 1, m, k) == 0
+    g = _gen(m + k + n)
+    x, (codes, exps) = _rows(g, n, k), _weight(g, m, k)
+    bias = torch.randn(m, device=DEV, generator=g).to(BF16)
+    w, xv, wv = ops.mx_pack_weight(codes, exps), plain_mx.held(x), plain_mx.values(codes, exps)
+    y = ops.mx_linear(x, w, F32, bias)
+    _near(y, xv, wv, bias)
+    assert torch.equal(ops.mx_linear(x, w, bias=bias), y.to(BF16)) and torch.equal(ops.mx_linear(ops.mx_quantize(x), w, F32, bias), y)
+    ops.check_tc_status()
+
+
+@pytest.mark.parametrize("limit", [0.0, 1.5])
+def test_glu_of_many_rows(limit):
+    from hi_b200.kernels import ops
+
+    i, k, n = 8224, 5152, 2221
+    assert ops.lib().hb_mx_gemm_form(n, 1, 2 * i, k) == 0
+    g = _gen(i)
+    x, gate, up = _rows(g, n, k), _weight(g, i, k), _weight(g, i, k)
+    w = ops.mx_pack_weight(*(ops.mx_interleave(a, b) for a, b in zip(gate, up)), glu=True)
+    act = ops.mx_glu(x, w, limit)
+    values = ops.mx_values(act, F32).double()
+    _check_unit(values, plain_mx.held(x), plain_mx.values(*gate), plain_mx.values(*up), limit)
+    down = _weight(g, 100, i)
+    _near(ops.mx_linear(act, ops.mx_pack_weight(*down), F32), values, plain_mx.values(*down))       # blocks past its end are zeros
+    ops.check_tc_status()
+
+
 def test_linear_scales():
     """Powers of two over their whole range, and blocks that are not numbers: rows and columns that read them, no others."""
     from hi_b200.kernels import ops
@@ -173,7 +226,7 @@ def test_glu_and_down(i, k, n, limit):
 
 
 @pytest.mark.parametrize("n,experts,top_k,h,i", [(1, 4, 1, 64, 32), (8, 16, 1, 512, 96), (64, 64, 6, 256, 160), (300, 3, 2, 288, 256),
-                                                (700, 5, 1, 1056, 64), (40, 128, 4, 96, 64), (130, 1, 1, 128, 128)])
+                                                (700, 5, 1, 1056, 64), (40, 128, 4, 96, 64), (130, 1, 1, 128, 128), (70, 2, 2, 2080, 64), (900, 3, 1, 544, 96), (12000, 4, 1, 5152, 4128)])
 @pytest.mark.parametrize("scale", ["input", "output"])
 def test_experts(n, experts, top_k, h, i, scale):
     """A token through its experts and back: experts without rows, with less than a tile and with several, the score before or after."""
@@ -229,6 +282,65 @@ def test_edges():
     wide[:, 513: 1025] = x                                             # rows that start at an odd place
     assert torch.equal(y, ops.mx_linear(wide[:, 513: 1025], w, F32)) and torch.equal(y, ops.mx_linear(x.t().contiguous().t(), w, F32))
     ops.check_tc_status()
+
+
+def test_captured():
+    """Calls in a graph, replayed with other inputs; two graphs in turn and side by side on two streams; the same results as eager ones."""
+    from hi_b200.kernels import ops
+
+    g = _gen(6)
+    w = ops.mx_pack_weight(*_weight(g, 640, 1024))
+    gate, up, down = _weight(g, 8, 128, 1024), _weight(g, 8, 128, 1024), _weight(g, 8, 1024, 128)
+    wg, wd = ops.mx_pack_weight(*(ops.mx_interleave(a, b) for a, b in zip(gate, up)), glu=True), ops.mx_pack_weight(*down)
+
+    def step(x, ids, scores):
+        plan = ops.moe_plan(ids, 8)
+        y = ops.mx_experts_linear(ops.mx_experts_glu(x, plan, 2, wg, scores), wd, plan)
+        return ops.mx_linear(x, w), ops.moe_combine(y, plan.slot_of_entry, None, x.shape[0], 2)
+
+    def inputs(n, seed):
+        h = _gen(seed)
+        return _rows(h, n, 1024), torch.randn(n, 8, device=DEV, generator=h).topk(2, 1).indices.int().contiguous(), torch.rand(n, 2, device=DEV, generator=h)
+
+    graphs = []
+    for n in (3, 150):
+        static = inputs(n, 1)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*static)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*static)
+        graphs.append((n, static, graph, out, torch.cuda.Stream()))
+    for seed in (2, 3, 4):
+        for n, static, graph, out, stream in graphs:
+            for a, b in zip(static, inputs(n, seed)):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        for n, static, graph, out, stream in graphs:
+            with torch.cuda.stream(stream):
+                for _ in range(3):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for n, static, graph, out, stream in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, step(*inputs(n, seed))))
+    ops.check_tc_status()
+
+
+def test_a_row_depends_on_itself():
+    """A token's results are the same whichever tokens stand beside it: the same bits where the form is, else to the float32 sums (2^-16 of all
+    magnitudes each; a weight is 0.08 at most)."""
+    from hi_b200.kernels import ops
+
+    g = _gen(8)
+    x, w = _rows(g, 2100, 5120), ops.mx_pack_weight(*_weight(g, 16384, 5120))
+    whole = ops.mx_linear(x, w, F32)
+    size = plain_mx.held(x[:3]).abs() @ plain_mx.values(*plain_mx.quantise(torch.full((1, 5120), 0.08, device=DEV))).abs().t()
+    for n in (1, 40, 100, 300):
+        assert ((ops.mx_linear(x[:n], w, F32)[:1].double() - whole[:1].double()).abs() <= 2.0 ** -15 * size[:1]).all()
+    assert torch.equal(ops.mx_linear(x[1: 2100], w, F32)[:900], whole[1: 901])
 
 
 def test_refusals():
