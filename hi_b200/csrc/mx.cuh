@@ -5,6 +5,7 @@
 //           (r % 32) 16 + r / 32 * 4 + b: lanes of tensor memory are r % 32, columns r / 32 (tcgen05.cp 32x128b.warpx4). Chunks are an
 //           even number, those past K are zeros. Rows of several experts begin a tile each, so tile numbers follow from the plan's offsets.
 #pragma once
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
 
@@ -55,6 +56,67 @@ __device__ __forceinline__ void values8(uint32_t codes, float scale, float (&v)[
     v[2 * i] = f.x * scale;
     v[2 * i + 1] = f.y * scale;
   }
+}
+
+// Eight values as they are read, their largest magnitude's bits as a float's, and themselves as floats.
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = reinterpret_cast<const float4*>(p)[0];
+    b = reinterpret_cast<const float4*>(p)[1];
+  }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void floats(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  __device__ __forceinline__ uint32_t top() const {
+    float v[8];
+    floats(v);
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t = max(t, __float_as_uint(v[i]) & 0x7fffffffu);
+    return t;
+  }
+};
+template <> struct Eight<__nv_bfloat16> {
+  uint4 w;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { w = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void floats(float (&v)[8]) const {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(u[i] << 16);
+      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ uint32_t top() const {       // two 16-bit halves at a time: bits of magnitudes are in the order of the magnitudes
+    constexpr uint32_t M = 0x7fff7fffu;
+    const uint32_t t = __vmaxu2(__vmaxu2(w.x & M, w.y & M), __vmaxu2(w.z & M, w.w & M));
+    return max(t & 0xffff0000u, t << 16);
+  }
+};
+
+// A warp's span of 256 values, eight a lane: the lane's codes, and its block's scale (four lanes have a block).
+template <typename T> __device__ __forceinline__ uint32_t quantize(const Eight<T>& x, uint32_t& scale) {
+  uint32_t top = x.top();
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  scale = scale_of(top);
+  const float by = inverse(scale);                // (what is multiplied by the scale 255 does not matter)
+  float v[8];
+  x.floats(v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] *= by;
+  return codes8(v);
+}
+// The scales of the four blocks of this half of the warp as a word.
+__device__ __forceinline__ uint32_t four_scales(uint32_t scale, int lane) {
+  uint32_t word = scale << (lane / 4 % 4 * 8);
+  word |= __shfl_xor_sync(0xffffffffu, word, 4);
+  return word | __shfl_xor_sync(0xffffffffu, word, 8);
 }
 
 // The tile of a row of expert-sorted rows and its place there, by a whole warp; `offsets` null: one run of rows.

@@ -37,7 +37,11 @@ struct Params {
   int out_f32, rows, experts, n_out, chunks, w_tiles;   // chunks of K; tiles of 128 weight rows an expert
   float limit;
   int behind;                    // right behind the launch that quantises x, which weights do not wait for
+  const void* raw;               // up to FEWEST rows that the blocks quantise themselves (raw_ld apart, of K values), or null
+  long long raw_ld;
+  int raw_f32, K;
 };
+constexpr int FEWEST = 16, FEWEST_K = 10240;      // rows and values of a row that a block can quantise itself: what its shared memory holds beside the weights
 
 struct Call {
   const void *x, *x_scales, *w, *w_scales;

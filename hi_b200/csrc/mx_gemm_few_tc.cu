@@ -25,15 +25,16 @@ using mx::SCALES;
 
 constexpr int BF = 128, A_BYTES = BF * KB / 2;    // weight rows of a tile
 constexpr int EPILOGUE = 16, THREADS = 64 + 32 * EPILOGUE;
+constexpr int X_STAGE = mx::FEWEST * KB / 2;       // RAW: a stage's rows
 constexpr int TRADE = EPILOGUE * 8 * 32 * 4;      // GLU: room for what warps trade
 
 struct Maps {
   CUtensorMap x[4];              // boxes of 16, 32, 64 and 128 rows
   CUtensorMap w;
 };
-struct Tile { int expert, row0, rows, scale_tile, f0; };
+struct Tile { int expert, row0, rows, scale_tile, off, f0; };      // its first row is row `off` of the tile of scales
 
-template <int BT> constexpr int stage_bytes() { return A_BYTES + BT * KB / 2 + SCALES + (BT + 127) / 128 * SCALES; }
+template <bool RAW, int BT> constexpr int stage_bytes() { return A_BYTES + SCALES + (RAW ? 0 : BT * KB / 2 + (BT + 127) / 128 * SCALES); }
 
 // Eight lanes' words of eight codes, one a row: lane i has the row's i % 8 then, eight neighbouring features.
 __device__ __forceinline__ uint32_t transpose(uint32_t x, int lane) {
@@ -45,19 +46,52 @@ __device__ __forceinline__ uint32_t transpose(uint32_t x, int lane) {
   return lane & 1 ? ((y >> 4) & 0x0f0f0f0fu) | (x & 0xf0f0f0f0u) : (x & 0x0f0f0f0fu) | ((y & 0x0f0f0f0fu) << 4);
 }
 
-template <bool GLU, bool SPLIT, int BT, int STAGES>
+// The rows of the stages kb0 .. kb1 - 1, quantised by the warps behind the first two to where the products read them: `x` a stage's 16 rows of 128
+// bytes, swizzled, `scales` its atoms, of which 16 rows are written.
+template <typename T>
+__device__ __forceinline__ void quantize_rows(const Params& p, uint8_t* x, uint8_t* scales, int kb0, int kb1, int warp, int lane) {
+  constexpr int MANY = 8;                         // loads of a lane on their way
+  const int each = EPILOGUE / p.rows, row = (warp - 2) % p.rows, first = (warp - 2) / p.rows;       // warps of a row
+  if (first >= each) return;
+  const T* const from = reinterpret_cast<const T*>(p.raw) + (size_t)row * p.raw_ld + lane * 8;
+  x += row * 128 + ((lane / 4 ^ (row & 7)) << 4) + lane % 4 * 4;
+  scales += lane / 16 * mx::ATOM + row * 16;
+  for (int s0 = first; s0 < kb1 - kb0; s0 += each * MANY) {
+    mx::Eight<T> v[MANY];
+#pragma unroll
+    for (int m = 0; m < MANY; ++m) {
+      const int k = (kb0 + s0 + m * each) * KB;
+      if (s0 + m * each < kb1 - kb0 && k + lane * 8 < p.K) v[m].load(from + k);
+      else v[m].zero();
+    }
+#pragma unroll
+    for (int m = 0; m < MANY; ++m) {
+      const int s = s0 + m * each;
+      if (s >= kb1 - kb0) break;
+      uint32_t scale;
+      const uint32_t codes = mx::quantize(v[m], scale), word = mx::four_scales(scale, lane);
+      *reinterpret_cast<uint32_t*>(x + s * X_STAGE) = codes;
+      if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(scales + s * SCALES) = word;
+    }
+  }
+}
+
+// RAW: up to 16 rows come as they are.
+template <bool GLU, bool SPLIT, bool RAW, int BT, int STAGES>
 __global__ void __launch_bounds__(THREADS, 1)
 mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
-  constexpr int STAGE = stage_bytes<BT>(), X_TILES = (BT + 127) / 128;
-  constexpr int X_AT = A_BYTES, SA_AT = X_AT + BT * KB / 2, SX_AT = SA_AT + SCALES;
+  constexpr int STAGE = stage_bytes<RAW, BT>(), X_TILES = (BT + 127) / 128;
+  constexpr int X_AT = A_BYTES, SA_AT = RAW ? A_BYTES : X_AT + BT * KB / 2, SX_AT = SA_AT + SCALES;
   // Tensor memory: two tiles' sums, which share 64 columns where 512 are not enough, then two stages' scales.
   constexpr bool SHARED = BT == 256;
   constexpr int TMEM_COLS = 512, SLOT1 = SHARED ? 192 : BT, SCALE_AT = SLOT1 + BT, SA_COLS = 8, CHUNK_COLS = X_TILES * 4, SET_COLS = SA_COLS + 2 * CHUNK_COLS;
   static_assert(SCALE_AT + 2 * SET_COLS <= TMEM_COLS && STAGE % 1024 == 0 && BT % 64 == 0 && BT <= 256, "all within tensor memory");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  float* trade = reinterpret_cast<float*>(smem + STAGES * STAGE);          // GLU: [EPILOGUE][8][32]
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE + (GLU && !SPLIT ? TRADE : 0));
+  const int resident = RAW ? p.chunks / 2 : 0;    // RAW: stages of rows that there is room for
+  uint8_t *x_rows = smem + STAGES * STAGE, *x_scales = x_rows + resident * X_STAGE, *behind_ring = x_scales + resident * SCALES;
+  float* trade = reinterpret_cast<float*>(behind_ring);          // GLU: [EPILOGUE][8][32]
+  uint64_t* full = reinterpret_cast<uint64_t*>(behind_ring + (GLU && !SPLIT ? TRADE : 0));
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;            // [2]
   uint64_t* acc_empty = acc_full + 2;             // [2]
@@ -81,34 +115,34 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
     if (!p.offsets) {                             // one run of rows: no table (the first copies leave 0.4 us earlier)
       const int units = (p.rows + BT - 1) / BT, f = units == 1 ? at : at / units, m = at - f * units;
       if (f >= f_tiles) return false;
-      t = {0, m * BT, min(BT, p.rows - m * BT), m * BT / mx::TILE, f * BF};
+      t = {0, m * BT, min(BT, p.rows - m * BT), m * BT / mx::TILE, m * BT % mx::TILE, f * BF};
       return true;
     }
     if (at >= first_unit[p.experts] * f_tiles) return false;
     const int e = mx::expert_of(p, first_unit, f_tiles, at), row = first_row[e];
     const int units = first_unit[e + 1] - first_unit[e], here = at - first_unit[e] * f_tiles, f = here / units, m = here - f * units;
-    t = {e, row + m * BT, min(BT, first_row[e + 1] - row - m * BT), first_tile[e] + m * BT / mx::TILE, f * BF};
+    t = {e, row + m * BT, min(BT, first_row[e + 1] - row - m * BT), first_tile[e] + m * BT / mx::TILE, m * BT % mx::TILE, f * BF};
     return true;
   };
   const uint32_t mine = tc::elect_one(), ring = tc::smem_u32(smem), bars = tc::smem_u32(full);
   auto weights = [&](const Tile& t, int at, int kb) {      // and what the stage waits for
     const uint32_t st = ring + at * STAGE, bar = bars + at * 8;
     const int box = t.rows <= 16 ? 0 : t.rows <= 32 ? 1 : t.rows <= 64 ? 2 : 3;
-    const int two = BT > 128 && t.rows > 128;
-    if (mine) tc::mbar_expect_tx(&full[at], A_BYTES + ((16u << box) * (KB / 2) << two) + SCALES + (SCALES << two));
+    const int more = BT > 128 && t.rows > 128 ? (BT - 128) * (KB / 2) : 0, two = BT > 128 && t.off + t.rows > 128;
+    if (mine) tc::mbar_expect_tx(&full[at], RAW ? A_BYTES + SCALES : A_BYTES + (16u << box) * (KB / 2) + more + SCALES + (SCALES << two));
     tc::tma_load_2d_if(mine, st, &maps.w, kb * (KB / 2), t.expert * p.n_out + t.f0, bar);
     tc::bulk_load_if(mine, st + SA_AT, p.w_scales + ((size_t)(t.expert * p.w_tiles + t.f0 / 128) * p.chunks + kb * 2) * mx::ATOM, SCALES, bar);
   };
   auto rows = [&](const Tile& t, int at, int kb) {
+    if constexpr (RAW) return;
     const uint32_t st = ring + at * STAGE, bar = bars + at * 8;
     const int box = t.rows <= 16 ? 0 : t.rows <= 32 ? 1 : t.rows <= 64 ? 2 : 3;
     const uint8_t* from = p.x_scales + ((size_t)t.scale_tile * p.chunks + kb * 2) * mx::ATOM;
     tc::tma_load_2d_if(mine, st + X_AT, &maps.x[box], kb * (KB / 2), t.row0, bar);
     tc::bulk_load_if(mine, st + SX_AT, from, SCALES, bar);
-    if (BT > 128 && t.rows > 128) {
-      tc::tma_load_2d_if(mine, st + X_AT + 128 * KB / 2, &maps.x[3], kb * (KB / 2), t.row0 + 128, bar);
-      tc::bulk_load_if(mine, st + SX_AT + SCALES, from + (size_t)p.chunks * mx::ATOM, SCALES, bar);
-    }
+    if (BT > 128 && t.rows > 128)
+      tc::tma_load_2d_if(mine, st + X_AT + 128 * KB / 2, &maps.x[BT == 192 ? 2 : 3], kb * (KB / 2), t.row0 + 128, bar);
+    if (BT > 128 && t.off + t.rows > 128) tc::bulk_load_if(mine, st + SX_AT + SCALES, from + (size_t)p.chunks * mx::ATOM, SCALES, bar);
   };
 
   Tile t;
@@ -141,12 +175,18 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
     tc::mbar_init(acc_shared, EPILOGUE);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if constexpr (RAW) {                            // while the first weights are on their way
+    if (warp >= 2) {
+      if (p.raw_f32) quantize_rows<float>(p, x_rows, x_scales, kb0, kb1, warp, lane);
+      else quantize_rows<__nv_bfloat16>(p, x_rows, x_scales, kb0, kb1, warp, lane);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+  }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
-
   if (warp == 0) {                                // ---- what a stage needs
     int s = ahead == STAGES ? 0 : ahead, turn = ahead == STAGES ? 0 : 1, issued = ahead;
     for (int i = 0; ok && tile_at(i, t); ++i)
@@ -171,6 +211,7 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
   } else if (warp == 1) {                         // ---- products
     const uint64_t operands = tc::desc_kmajor(ring), atoms = tc::desc_scales(ring);
     int s = 0, turn = 0, set = 0;
+    const uint64_t resident_x = tc::desc_kmajor(tc::smem_u32(x_rows)), resident_atoms = tc::desc_scales(tc::smem_u32(x_scales));
     for (int i = 0; ok && tile_at(i, t); ++i) {
       const int b = i & 1;
       if ((SHARED && i >= 1 && !tc::mbar_wait_warp(acc_shared, (i - 1) & 1)) || (i >= 2 && !tc::mbar_wait_warp(&acc_empty[b], (i / 2 - 1) & 1))) {
@@ -179,7 +220,8 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
       }
       tc::fence_after();
       const uint32_t acc = tmem + b * SLOT1, idesc = tc::idesc_mxf4(BF, tc::uniform((t.rows + 15) & ~15), 0);
-      const bool two = BT > 128 && tc::uniform(t.rows) > 128;
+      const bool two = BT > 128 && tc::uniform(t.off + t.rows) > 128;
+      const uint32_t off = tc::uniform(t.off / 32);        // columns of the scales before the tile's
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!tc::mbar_wait_warp(&full[s], turn)) {
           if (lane == 0) atomicExch(p.status, 92);
@@ -188,16 +230,18 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
         }
         tc::fence_after();
         const uint32_t sa = tmem + SCALE_AT + set * SET_COLS, sx = sa + SA_COLS;
-        const uint64_t a = operands + (s * STAGE >> 4), x = a + (X_AT >> 4), from = atoms + (s * STAGE >> 4);
+        const uint64_t a = operands + (s * STAGE >> 4), from = atoms + (s * STAGE >> 4);
+        const uint64_t x = RAW ? resident_x + ((kb - kb0) * X_STAGE >> 4) : a + (X_AT >> 4);
+        const uint64_t from_x = RAW ? resident_atoms + ((kb - kb0) * SCALES >> 4) : from + (SX_AT >> 4);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           tc::copy_scales_if(mine, sa + c * 4, from + ((SA_AT + c * mx::ATOM) >> 4));
-          tc::copy_scales_if(mine, sx + c * CHUNK_COLS, from + ((SX_AT + c * mx::ATOM) >> 4));
+          tc::copy_scales_if(mine, sx + c * CHUNK_COLS, from_x + (c * mx::ATOM >> 4));
           if (two) tc::copy_scales_if(mine, sx + c * CHUNK_COLS + 4, from + ((SX_AT + SCALES + c * mx::ATOM) >> 4));
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          tc::mma_mx_if(mine, acc, a + (k * 32 >> 4), x + (k * 32 >> 4), idesc | tc::idesc_mxf4(0, 0, k % 2 * 2), sa + k / 2 * 4, sx + k / 2 * CHUNK_COLS,
+          tc::mma_mx_if(mine, acc, a + (k * 32 >> 4), x + (k * 32 >> 4), idesc | tc::idesc_mxf4(0, 0, k % 2 * 2), sa + k / 2 * 4, sx + k / 2 * CHUNK_COLS + off,
                         (kb - kb0) | k);
         tc::commit_if(mine, &empty[s]);
         if (++s == STAGES) { s = 0; turn ^= 1; }
@@ -282,7 +326,7 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
           if (r >= t.rows) continue;
           *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + (size_t)(t.row0 + r) * (p.n_out / 4) + block * 16 + lane / 8 * 4) = word;
           if (lane < 8) {
-            uint8_t* const to = p.out_scales + (size_t)(t.scale_tile + r / mx::TILE) * out_chunks * mx::ATOM + mx::row_at(r % mx::TILE);
+            uint8_t* const to = p.out_scales + (size_t)(t.scale_tile + (t.off + r) / mx::TILE) * out_chunks * mx::ATOM + mx::row_at((t.off + r) % mx::TILE);
             to[block / 4 * mx::ATOM + block % 4] = (uint8_t)scale;
             if (block == blocks - 1)
               for (int q = blocks; q < out_chunks * 4; ++q) to[q / 4 * mx::ATOM + q % 4] = 0;
@@ -388,28 +432,32 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
   }
 }
 
-template <bool GLU, bool SPLIT, int BT, int STAGES>
+template <bool GLU, bool SPLIT, bool RAW, int BT, int STAGES>
 int launch(const Call& c, const Params& p, int blocks, int cluster) {
   Maps maps;
-  // A map costs the host 0.3 us: those that tiles of these rows ask for, in the others' places the last of them.
-  auto box_of = [](int rows) { return rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3; };
-  const int rest = p.rows % BT ? p.rows % BT : BT;         // rows of one run's last tile
-  int made = -1;
-  for (int b = 3; b >= 0; --b) {
-    const bool asked = p.offsets ? b <= box_of(p.rows < BT ? p.rows : BT) : b == box_of(rest) || (p.rows >= BT && b == box_of(BT));
-    if (asked && !tc::make_map_bytes(&maps.x[b], c.x, (uint64_t)p.rows, (uint64_t)c.K / 2, BT < (16 << b) ? BT : 16 << b)) return HB_ERR_UNSUPPORTED;
-    if (asked) made = b;
-  }
-  for (int b = 0; b < 4; ++b) {
-    const bool asked = p.offsets ? b <= box_of(p.rows < BT ? p.rows : BT) : b == box_of(rest) || (p.rows >= BT && b == box_of(BT));
-    if (!asked) maps.x[b] = maps.x[made];
+  if constexpr (!RAW) {
+    // A map costs the host 0.3 us: those that tiles of these rows ask for, in the others' places the last of them.
+    auto box_of = [](int rows) { return rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3; };
+    const int rest = p.rows % BT ? p.rows % BT : BT;         // rows of one run's last tile; a tile of 192 has 64 of them as a second box
+    int made = -1;
+    for (int b = 3; b >= 0; --b) {
+      const bool asked = p.offsets ? b <= box_of(p.rows < BT ? p.rows : BT) : b == box_of(rest) || (p.rows >= BT && b == box_of(BT)) || (BT == 192 && b == 2);
+      if (asked && !tc::make_map_bytes(&maps.x[b], c.x, (uint64_t)p.rows, (uint64_t)c.K / 2, BT < (16 << b) ? BT : 16 << b)) return HB_ERR_UNSUPPORTED;
+      if (asked) made = b;
+    }
+    for (int b = 0; b < 4; ++b) {
+      const bool asked = p.offsets ? b <= box_of(p.rows < BT ? p.rows : BT) : b == box_of(rest) || (p.rows >= BT && b == box_of(BT)) || (BT == 192 && b == 2);
+      if (!asked) maps.x[b] = maps.x[made];
+    }
   }
   if (!tc::make_map_bytes(&maps.w, c.w, (uint64_t)p.experts * p.n_out, (uint64_t)c.K / 2, BF)) return HB_ERR_UNSUPPORTED;
   constexpr int TRADED = GLU && !SPLIT ? TRADE : 0;
-  static_assert((2 * STAGES + 5) * 8 + 8 <= 256 && STAGES * stage_bytes<BT>() + TRADED + 1280 + 12 * 129 <= 227 * 1024, "with 128 experts at least");
-  const size_t smem = (size_t)STAGES * stage_bytes<BT>() + TRADED + 1024 + 256 + 12 * ((size_t)p.experts + 1);
+  constexpr int RESIDENT = RAW ? mx::FEWEST_K / KB * (X_STAGE + SCALES) : 0;
+  static_assert((2 * STAGES + 5) * 8 + 8 <= 256 && STAGES * stage_bytes<RAW, BT>() + RESIDENT + TRADED + 1280 + 12 * (RAW ? 2 : 129) <= 227 * 1024,
+                "with 128 experts at least");
+  const size_t smem = (size_t)STAGES * stage_bytes<RAW, BT>() + (RAW ? p.chunks / 2 * (X_STAGE + SCALES) : 0) + TRADED + 1024 + 256 + 12 * ((size_t)p.experts + 1);
   if (smem > 227 * 1024) return HB_ERR_UNSUPPORTED;
-  auto* kernel = mx_gemm_few_kernel<GLU, SPLIT, BT, STAGES>;
+  auto* kernel = mx_gemm_few_kernel<GLU, SPLIT, RAW, BT, STAGES>;
   static std::atomic<unsigned long long> allowed{0};
   cudaError_t e = hb::allow_smem(kernel, 227 * 1024, allowed);
   if (e != cudaSuccess) return (int)e;
@@ -423,10 +471,12 @@ int few(const Call& c, const Params& p, int splits, int most) {
     return units * ((p.n_out + BF - 1) / BF);
   };
   auto blocks = [&](int bt) { return (int)(grid(bt) < 148 ? grid(bt) : 148); };
-  if (splits > 1) return launch<GLU, true, 128, 6>(c, p, (int)grid(128) * splits, splits);
-  if (most <= 64) return launch<GLU, false, 64, 7>(c, p, blocks(64), 1);
-  if (most <= 128) return launch<GLU, false, 128, 6>(c, p, blocks(128), 1);
-  return launch<GLU, false, 256, 4>(c, p, blocks(256), 1);
+  if (p.raw) return splits > 1 ? launch<GLU, true, true, 64, 5>(c, p, (int)grid(64) * splits, splits) : launch<GLU, false, true, 64, 5>(c, p, blocks(64), 1);
+  if (splits > 1) return launch<GLU, true, false, 128, 6>(c, p, (int)grid(128) * splits, splits);
+  if (most <= 64) return launch<GLU, false, false, 64, 7>(c, p, blocks(64), 1);
+  if (most <= 128) return launch<GLU, false, false, 128, 6>(c, p, blocks(128), 1);
+  if (most <= 192) return launch<GLU, false, false, 192, GLU ? 4 : 5>(c, p, blocks(192), 1);
+  return launch<GLU, false, false, 256, 4>(c, p, blocks(256), 1);
 }
 
 }  // namespace
@@ -438,8 +488,8 @@ int hb_mx_clusters(int size) {
   if (cudaGetDevice(&device) != cudaSuccess || device > 63 || size > 15) return 148 / size;
   int n = known[device][size].load(std::memory_order_relaxed);
   if (n > 0) return n;
-  auto* kernel = mx_gemm_few_kernel<false, true, 128, 6>;
-  constexpr size_t smem = 6 * stage_bytes<128>() + 1280 + 24;
+  auto* kernel = mx_gemm_few_kernel<false, true, false, 128, 6>;
+  constexpr size_t smem = 6 * stage_bytes<false, 128>() + 1280 + 24;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return 148 / size;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(size * 148);
@@ -456,7 +506,7 @@ int hb_mx_clusters(int size) {
   return n;
 }
 
-// splits: blocks that share K (1: none do); most: rows of a tile, 64 (where there are no more in all), 128 or 256.
+// splits: blocks that share K (1: none do); most: rows of a tile, 64 (where there are no more in all), 128, 192 or 256.
 int hb_mx_gemm_few(const Call& c, const Params& p, bool glu, int splits, int most) {
   return glu ? few<true>(c, p, splits, most) : few<false>(c, p, splits, most);
 }

@@ -349,20 +349,25 @@ int pairs(const Call& c, const Params& p, int pairs) {
 // Measured, as pairs / single blocks: 512 x 16,384 x 5,120 24.1 / 24.2, 700 x 5,120 x 8,192 18.8 / 18.4, 2,048 x 16,384 x 5,120 67.5 / 72.7, units of 2,047 x 8,192
 // x 5,120 64.4 / 75.0, 99 x 5,120 x 8,192 17.7 / 11.5; 4,096 rows of 16 experts of 5,120 x 8,192: up 209 / 218, down 118 / 110, 2,048: 157 / 147 and 87 / 75; in one, two, four and
 // eight parts 1 x 256 x 8,192 7.9 / 6.7 / 5.9 / 5.5, 16 x 2,048 x 8,192 9.0 / 8.7 / 7.5 / 12.4 (more clusters than live at a time), 60 x 2,048 x 4,096 6.8 / 9.1 /
-// 7.9 / 13.3, in three 1 x 5,120 x 8,192 9.5 -> 8.6, 60 rows 10.2 -> 10.8. Tiles of up to 64, 128 and 256 rows: 8 x 7,168 x 5,120 7.5 / 7.8 / 9.4, 2,048 x 16,384 x 5,120
-// - / 84.6 / 72.7.
+// 7.9 / 13.3, in three 1 x 5,120 x 8,192 9.5 -> 8.6, 60 rows 10.2 -> 10.8. Tiles of up to 64, 128 and 256 rows: 8 x 7,168 x 5,120 7.5 / 7.8 / 9.4; of
+// 128, 192 and 256: 256 x 5,120 x 8,192 12.4 / 15.3 / 17.9, 512 x 5,120 x 8,192 19.6 / 15.5 / 18.4, 160 x 16,384 x 5,120 15.1 / 13.4 / 14.6, 700 x 16,384 x
+// 5,120 33.6 / 32.7 / 31.2; experts' up and down of 64 rows 116, 63 / 123, 69 / 124, 74, of 128 165, 79 / 166, 79 / 148, 82, of 256 261, 117 / 235, 128 / 216, 124.
 // `runs`: experts that may have rows. splits 0: pairs of blocks; else single ones, so many of them on a tile, with up to `most_rows` rows of it.
 struct Form { int splits, most_rows; };
-Form form(int rows, int experts, int n_out, int chunks) {
+Form form(int rows, int experts, int n_out, int chunks, bool glu) {
   const int runs = experts < rows ? experts : rows, each = (rows + runs - 1) / runs, stages = chunks / 2;
-  const int most_rows = rows <= 64 ? 64 : each <= 128 ? 128 : 256;
   const long long f_tiles = (n_out + 127) / 128, f_pairs = (n_out + BN - 1) / BN;
-  float single, pair;
+  int most_rows = 64;
+  float single = 3.4e38f, pair;
   if (runs == 1) {
-    const int tiles = (rows + most_rows - 1) / most_rows, n = (rows + tiles - 1) / tiles;
-    single = 3.4f + (f_tiles * tiles + 147) / 148 * stages * fmaxf(0.2f, 0.12f + 0.0014f * n);
+    for (int t = rows <= 64 ? 64 : 128; t <= (rows <= 64 ? 64 : 256); t += 64) {
+      const int tiles = (rows + t - 1) / t;
+      const float us = 3.4f + (f_tiles * tiles + 147) / 148 * stages * fmaxf(0.2f, 0.12f + 0.0014f * ((rows + tiles - 1) / tiles));
+      if (us < single) { single = us; most_rows = t; }
+    }
     pair = 6.5f + ((rows + 2 * BM - 1) / (2 * BM) * f_pairs + 73) / 74 * fmaxf(6.f, stages * 0.44f) - stages * 0.1f;
   } else {
+    if (rows > 64) most_rows = each <= (glu ? 96 : 128) ? 128 : 256;
     const float tiles = runs * (each > most_rows ? (float)each / most_rows + 0.5f : 1.f), pairs = runs * ((float)each / (2 * BM) + 0.5f);
     single = 3.4f + f_tiles / 148.f * stages * fmaxf(0.2f * tiles, 0.12f * tiles + 0.0014f * rows);
     pair = 6.5f + f_pairs / 74.f * pairs * fmaxf(6.f, stages * 0.44f);
@@ -378,8 +383,8 @@ Form form(int rows, int experts, int n_out, int chunks) {
 }
 
 int gemm(const Call& c, const Params& p, bool glu) {
-  const Form f = form(p.rows, p.experts, p.n_out, p.chunks);
-  if (f.splits) return hb_mx_gemm_few(c, p, glu, f.splits, f.most_rows);
+  const Form f = form(p.rows, p.experts, p.n_out, p.chunks, glu);
+  if (f.splits || p.raw) return hb_mx_gemm_few(c, p, glu, f.splits ? f.splits : 1, f.most_rows);
   const int runs = p.experts < p.rows ? p.experts : p.rows;
   const long long most = ((p.rows + 2 * BM - 1) / (2 * BM) + runs - 1LL) * ((p.n_out + BN - 1) / BN);      // tiles that there may be
   const int n = (int)(most < 74 ? most : 74);
@@ -389,13 +394,16 @@ int gemm(const Call& c, const Params& p, bool glu) {
 }  // namespace
 
 // Rows (codes, scales; `offsets` the plan's, or null with experts 1) by weights [experts, n_out, K]. raw not null: they are quantised first, as
-// hb_mx_quantize does (raw_dtype, raw_ld; with offsets in the order of sorted_entry, entries / top_k). glu 0: out [rows, n_out] in out_dtype, bias
+// hb_mx_quantize does (raw_dtype, raw_ld; with offsets in the order of sorted_entry, entries / top_k), or with x null, up to 16 rows of up to 10,240
+// values of one run, by the product's own blocks. glu 0: out [rows, n_out] in out_dtype, bias
 // bfloat16 [n_out] or null. glu 1: n_out is twice the features, gate and up in turn by 32; out codes and out_scales of the features; scores
 // (with sorted_entry: by entry, else by row) or null, limit > 0 for the clamped unit. status: one int on the device, nonzero after a wait that ran out.
 extern "C" int hb_mx_gemm(const void* raw, int raw_dtype, long long raw_ld, int top_k, void* x, void* x_scales, int rows, const int* offsets,
                           int experts, const void* w, const void* w_scales, int n_out, int K, const void* bias, const int* sorted_entry,
                           const float* scores, int glu, float limit, void* out, int out_dtype, void* out_scales, int* status, cudaStream_t stream) {
-  if (!x || !x_scales || !w || !w_scales || !out || !status || rows < 0 || n_out < 0 || K <= 0 || experts < 1 || (!offsets && experts != 1) ||
+  const bool direct = raw && !x;
+  if (direct && (offsets || rows > mx::FEWEST || K > mx::FEWEST_K)) return HB_ERR_BAD_ARG;
+  if ((!direct && (!x || !x_scales)) || !w || !w_scales || !out || !status || rows < 0 || n_out < 0 || K <= 0 || experts < 1 || (!offsets && experts != 1) ||
       (glu ? !out_scales || bias : out_dtype != HB_DTYPE_F32 && out_dtype != HB_DTYPE_BF16))
     return HB_ERR_BAD_ARG;
   if (K % mx::BLOCK || experts > MOST_EXPERTS || (glu && n_out % 64) || (long long)experts * n_out > 0x7fffffffll ||
@@ -406,19 +414,22 @@ extern "C" int hb_mx_gemm(const void* raw, int raw_dtype, long long raw_ld, int 
         reinterpret_cast<uintptr_t>(out)) & 15))
     return HB_ERR_UNSUPPORTED;
   if (rows == 0 || n_out == 0) return HB_OK;
-  if (raw) {
+  if (direct && (K % mx::BLOCK || (reinterpret_cast<uintptr_t>(raw) & 15) || raw_ld * (raw_dtype == HB_DTYPE_F32 ? 4 : 2) % 16 ||
+                 (raw_dtype != HB_DTYPE_F32 && raw_dtype != HB_DTYPE_BF16)))
+    return HB_ERR_UNSUPPORTED;
+  if (raw && !direct) {
     const int e = hb_mx_quantize(raw, raw_dtype, raw_ld, rows, K, offsets ? sorted_entry : nullptr, top_k, offsets, experts, x, x_scales, stream);
     if (e != HB_OK) return e;
   }
   const Params p{(const uint8_t*)x_scales, (const uint8_t*)w_scales, offsets, sorted_entry, scores, (const __nv_bfloat16*)bias, out, (uint8_t*)out_scales, status, out_dtype == HB_DTYPE_F32, rows,
-                 experts, n_out, mx::chunks(K), (n_out + 127) / 128, limit, raw != nullptr};
+                 experts, n_out, mx::chunks(K), (n_out + 127) / 128, limit, raw && !direct, direct ? raw : nullptr, raw_ld, raw_dtype == HB_DTYPE_F32, K};
   const Call c{x, x_scales, w, w_scales, K, (rows + BM - 1) / BM + (experts < rows ? experts : rows) - 1, stream};
   return gemm(c, p, glu != 0);
 }
 
 // The form that hb_mx_gemm takes: 0 pairs of blocks, else 1000 times the blocks that share a tile's K and the rows of a tile.
-extern "C" int hb_mx_gemm_form(int rows, int experts, int n_out, int K) {
+extern "C" int hb_mx_gemm_form(int rows, int experts, int n_out, int K, int glu) {
   if (rows < 1 || experts < 1 || n_out < 1 || K < 1) return -1;
-  const Form f = form(rows, experts, n_out, mx::chunks(K));
+  const Form f = form(rows, experts, n_out, mx::chunks(K), glu != 0);
   return f.splits ? f.splits * 1000 + f.most_rows : 0;
 }

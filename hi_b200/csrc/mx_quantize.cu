@@ -19,47 +19,6 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Eight values as they are read, their largest magnitude's bits as a float's, and themselves as floats.
-template <typename T> struct Eight;
-template <> struct Eight<float> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = reinterpret_cast<const float4*>(p)[0];
-    b = reinterpret_cast<const float4*>(p)[1];
-  }
-  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
-  __device__ __forceinline__ void floats(float (&v)[8]) const {
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  }
-  __device__ __forceinline__ uint32_t top() const {
-    float v[8];
-    floats(v);
-    uint32_t t = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t = max(t, __float_as_uint(v[i]) & 0x7fffffffu);
-    return t;
-  }
-};
-template <> struct Eight<__nv_bfloat16> {
-  uint4 w;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void zero() { w = make_uint4(0u, 0u, 0u, 0u); }
-  __device__ __forceinline__ void floats(float (&v)[8]) const {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(u[i] << 16);
-      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
-  }
-  __device__ __forceinline__ uint32_t top() const {       // two 16-bit halves at a time: bits of magnitudes are in the order of the magnitudes
-    constexpr uint32_t M = 0x7fff7fffu;
-    const uint32_t t = __vmaxu2(__vmaxu2(w.x & M, w.y & M), __vmaxu2(w.z & M, w.w & M));
-    return max(t & 0xffff0000u, t << 16);
-  }
-};
-
 constexpr int SPAN = 256;          // values a warp takes at a time, eight a lane
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 
@@ -75,7 +34,7 @@ mx_quantize_kernel(const T* __restrict__ x, long long x_ld, int rows, int k, con
   if (row >= rows) return;
   const size_t from = sorted_entry ? sorted_entry[row] / top_k : row;
   const T* const in = x + from * x_ld + lane * 8;
-  Eight<T> x8[MANY];
+  mx::Eight<T> x8[MANY];
 #pragma unroll
   for (int m = 0; m < MANY; ++m) {
     const int k0 = (first + m) * SPAN + lane * 8;
@@ -90,20 +49,10 @@ mx_quantize_kernel(const T* __restrict__ x, long long x_ld, int rows, int k, con
   for (int m = 0; m < MANY; ++m) {
     const int span = first + m, k0 = span * SPAN + lane * 8;
     if (span * 2 >= all) break;
-    uint32_t top = x8[m].top();
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t scale = mx::scale_of(top);
-    const float by = mx::inverse(scale);          // (what is multiplied by the scale 255 does not matter)
-    float v[8];
-    x8[m].floats(v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= by;
-    if (k0 < k) *reinterpret_cast<uint32_t*>(to + span * (SPAN / 2)) = mx::codes8(v);
-    // the four blocks of 16 lanes: a word of scales
-    uint32_t word = scale << (lane / 4 % 4 * 8);
-    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    uint32_t scale;
+    const uint32_t eight = mx::quantize(x8[m], scale);
+    if (k0 < k) *reinterpret_cast<uint32_t*>(to + span * (SPAN / 2)) = eight;
+    const uint32_t word = mx::four_scales(scale, lane);
     if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(scale_to + (size_t)(span * 2 + lane / 16) * mx::ATOM) = word;
   }
 }

@@ -126,7 +126,7 @@ def test_linear_of_blocks_that_share_k(m, k, n):
     """Shares of unlike length, the last one short; every block finishes some rows, or has none to finish."""
     from hi_b200.kernels import ops
 
-    assert ops.lib().hb_mx_gemm_form(n, 1, m, k) >= 2000
+    assert ops.lib().hb_mx_gemm_form(n, 1, m, k, 0) >= 2000
     g = _gen(m + k + n)
     x, (codes, exps) = _rows(g, n, k), _weight(g, m, k)
     bias = torch.randn(m, device=DEV, generator=g).to(BF16)
@@ -141,12 +141,36 @@ def test_linear_of_blocks_that_share_k(m, k, n):
     ops.check_tc_status()
 
 
+@pytest.mark.parametrize("m,k,n,rows", [(8200, 1056, 257, 192), (8192, 1056, 384, 192), (5120, 2080, 513, 192), (12032, 544, 190, 192), (12000, 544, 150, 192),
+                                         (12032, 544, 193, 256), (8256, 1056, 500, 256), (8200, 1056, 460, 256)])
+def test_linear_of_large_tiles(m, k, n, rows):
+    """Tiles of up to 192 and 256 rows: second tiles that begin in the middle of a tile of scales, last ones of a few rows, sums that share columns."""
+    from hi_b200.kernels import ops
+
+    g = _gen(m + k + n)
+    x, (codes, exps) = _rows(g, n, k), _weight(g, m, k)
+    bias = torch.randn(m, device=DEV, generator=g).to(BF16)
+    w, xv, wv = ops.mx_pack_weight(codes, exps), plain_mx.held(x), plain_mx.values(codes, exps)
+    assert ops.lib().hb_mx_gemm_form(n, 1, m, k, 0) == 1000 + rows
+    y = ops.mx_linear(x, w, F32, bias)
+    _near(y, xv, wv, bias)
+    assert torch.equal(ops.mx_linear(x, w, bias=bias), y.to(BF16))
+    if m % 64 == 0:
+        act = ops.mx_glu(x, ops.mx_pack_weight(codes, exps, glu=True), 1.5)
+        gate, up = (wv.view(-1, 2, 32, k)[:, i].flatten(0, 1) for i in (0, 1))
+        values = ops.mx_values(act, F32).double()
+        _check_unit(values, xv, gate, up, 1.5)
+        down = _weight(g, 40, m // 2)
+        _near(ops.mx_linear(act, ops.mx_pack_weight(*down), F32), values, plain_mx.values(*down))
+    ops.check_tc_status()
+
+
 @pytest.mark.parametrize("m,k,n", [(16400, 5152, 2221), (16385, 4800, 2147), (24576, 5120, 1500)])
 def test_linear_of_many_rows(m, k, n):
     """Pairs of blocks: several tiles a pair, tiles that are not full in rows, features and k, an odd number of features."""
     from hi_b200.kernels import ops
 
-    assert ops.lib().hb_mx_gemm_form(n, 1, m, k) == 0
+    assert ops.lib().hb_mx_gemm_form(n, 1, m, k, 0) == 0
     g = _gen(m + k + n)
     x, (codes, exps) = _rows(g, n, k), _weight(g, m, k)
     bias = torch.randn(m, device=DEV, generator=g).to(BF16)
@@ -162,7 +186,7 @@ def test_glu_of_many_rows(limit):
     from hi_b200.kernels import ops
 
     i, k, n = 8224, 5152, 2221
-    assert ops.lib().hb_mx_gemm_form(n, 1, 2 * i, k) == 0
+    assert ops.lib().hb_mx_gemm_form(n, 1, 2 * i, k, 1) == 0
     g = _gen(i)
     x, gate, up = _rows(g, n, k), _weight(g, i, k), _weight(g, i, k)
     w = ops.mx_pack_weight(*(ops.mx_interleave(a, b) for a, b in zip(gate, up)), glu=True)
@@ -365,3 +389,28 @@ def test_refusals():
                  lambda: ops.mx_values(rows, torch.float16), lambda: ops.mx_quantize(x, plan, 3)):
         with pytest.raises(ops.KernelError):
             call()
+
+
+@pytest.mark.parametrize("m,k", [(1, 32), (100, 288), (640, 1024), (7168, 5120), (300, 10240), (20000, 544), (128, 10272), (2048, 8192)])
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 9, 15, 16])
+def test_rows_quantised_on_the_way(m, k, n):
+    """Up to 16 rows, which the product's blocks quantise themselves: the same bits as rows that are quantised first; several tiles a block, shares of K,
+    rows that lie apart, values on borders and such that are not finite."""
+    from hi_b200.kernels import ops
+
+    g = _gen(m + k + n + 3)
+    for dtype in (BF16, F32):
+        x = _rows(g, n, k + 24, dtype)[:, 8: 8 + k]
+        x[0, :8] = torch.tensor([0.25, -0.75, 1.25, 1.75, 2.5, -3.5, 5.0, 7.0], device=DEV, dtype=dtype)
+        if n > 2:
+            x[1, 5], x[2, :32] = float("inf"), 0
+        w = ops.mx_pack_weight(*_weight(g, m, k))
+        bias = torch.randn(m, device=DEV, generator=g).to(BF16)
+        bits = lambda t: t.view(torch.int16 if t.dtype == BF16 else torch.int32)
+        for kind in (BF16, F32):
+            assert torch.equal(bits(ops.mx_linear(x, w, kind, bias)), bits(ops.mx_linear(ops.mx_quantize(x), w, kind, bias)))
+        if m % 64 == 0:
+            w = ops.mx_pack_weight(*_weight(g, m, k), glu=True)
+            a, b = (ops.mx_values(ops.mx_glu(v, w, 1.5), F32) for v in (x, ops.mx_quantize(x)))
+            assert torch.equal(a.nan_to_num(99), b.nan_to_num(99))
+    ops.check_tc_status()
