@@ -354,7 +354,7 @@ int pairs(const Call& c, const Params& p, int pairs) {
 // 5,120 33.6 / 32.7 / 31.2; experts' up and down of 64 rows 116, 63 / 123, 69 / 124, 74, of 128 165, 79 / 166, 79 / 148, 82, of 256 261, 117 / 235, 128 / 216, 124.
 // `runs`: experts that may have rows. splits 0: pairs of blocks; else single ones, so many of them on a tile, with up to `most_rows` rows of it.
 struct Form { int splits, most_rows; };
-Form form(int rows, int experts, int n_out, int chunks, bool glu) {
+Form form(int rows, int experts, int n_out, int chunks) {
   const int runs = experts < rows ? experts : rows, each = (rows + runs - 1) / runs, stages = chunks / 2;
   const long long f_tiles = (n_out + 127) / 128, f_pairs = (n_out + BN - 1) / BN;
   int most_rows = 64;
@@ -367,7 +367,7 @@ Form form(int rows, int experts, int n_out, int chunks, bool glu) {
     }
     pair = 6.5f + ((rows + 2 * BM - 1) / (2 * BM) * f_pairs + 73) / 74 * fmaxf(6.f, stages * 0.44f) - stages * 0.1f;
   } else {
-    if (rows > 64) most_rows = each <= (glu ? 96 : 128) ? 128 : 256;
+    if (rows > 64) most_rows = each <= 128 ? 128 : 256;
     const float tiles = runs * (each > most_rows ? (float)each / most_rows + 0.5f : 1.f), pairs = runs * ((float)each / (2 * BM) + 0.5f);
     single = 3.4f + f_tiles / 148.f * stages * fmaxf(0.2f * tiles, 0.12f * tiles + 0.0014f * rows);
     pair = 6.5f + f_pairs / 74.f * pairs * fmaxf(6.f, stages * 0.44f);
@@ -383,7 +383,7 @@ Form form(int rows, int experts, int n_out, int chunks, bool glu) {
 }
 
 int gemm(const Call& c, const Params& p, bool glu) {
-  const Form f = form(p.rows, p.experts, p.n_out, p.chunks, glu);
+  const Form f = form(p.rows, p.experts, p.n_out, p.chunks);
   if (f.splits || p.raw) return hb_mx_gemm_few(c, p, glu, f.splits ? f.splits : 1, f.most_rows);
   const int runs = p.experts < p.rows ? p.experts : p.rows;
   const long long most = ((p.rows + 2 * BM - 1) / (2 * BM) + runs - 1LL) * ((p.n_out + BN - 1) / BN);      // tiles that there may be
@@ -428,8 +428,8 @@ extern "C" int hb_mx_gemm(const void* raw, int raw_dtype, long long raw_ld, int 
 }
 
 // The form that hb_mx_gemm takes: 0 pairs of blocks, else 1000 times the blocks that share a tile's K and the rows of a tile.
-extern "C" int hb_mx_gemm_form(int rows, int experts, int n_out, int K, int glu) {
+extern "C" int hb_mx_gemm_form(int rows, int experts, int n_out, int K) {
   if (rows < 1 || experts < 1 || n_out < 1 || K < 1) return -1;
-  const Form f = form(rows, experts, n_out, mx::chunks(K), glu != 0);
+  const Form f = form(rows, experts, n_out, mx::chunks(K));
   return f.splits ? f.splits * 1000 + f.most_rows : 0;
 }

@@ -45,7 +45,7 @@ _SIGNATURES = {
     "hb_four_bit_linear_tc": [P, c_longlong, P, P, P, I, I, I, I, I, P, P],
     "hb_mx_quantize": [P, I, c_longlong, I, I, P, I, P, I, P, P, P],
     "hb_mx_values": [P, P, I, I, P, I, P, I, P],
-    "hb_mx_gemm_form": [I, I, I, I, I],
+    "hb_mx_gemm_form": [I, I, I, I],
     "hb_mx_gemm": [P, I, c_longlong, I, P, P, I, P, I, P, P, I, I, P, P, P, I, F, P, I, P, P, P],
     "hb_paged_attention": [P, I, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, F, P, P, I, I, P, P, P],
     "hb_attention_portions": [P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, F, I, F, P, P, I, P, P, P],
