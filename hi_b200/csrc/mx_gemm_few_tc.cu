@@ -453,8 +453,8 @@ int launch(const Call& c, const Params& p, int blocks, int cluster) {
   if (!tc::make_map_bytes(&maps.w, c.w, (uint64_t)p.experts * p.n_out, (uint64_t)c.K / 2, BF)) return HB_ERR_UNSUPPORTED;
   constexpr int TRADED = GLU && !SPLIT ? TRADE : 0;
   constexpr int RESIDENT = RAW ? mx::FEWEST_K / KB * (X_STAGE + SCALES) : 0;
-  static_assert((2 * STAGES + 5) * 8 + 8 <= 256 && STAGES * stage_bytes<RAW, BT>() + RESIDENT + TRADED + 1280 + 12 * (RAW ? 2 : 129) <= 227 * 1024,
-                "with 128 experts at least");
+  static_assert((2 * STAGES + 5) * 8 + 8 <= 256 && STAGES * stage_bytes<RAW, BT>() + RESIDENT + TRADED + 1280 + 12 * (RAW ? 2 : 385) <= 227 * 1024,
+                "with 384 experts");
   const size_t smem = (size_t)STAGES * stage_bytes<RAW, BT>() + (RAW ? p.chunks / 2 * (X_STAGE + SCALES) : 0) + TRADED + 1024 + 256 + 12 * ((size_t)p.experts + 1);
   if (smem > 227 * 1024) return HB_ERR_UNSUPPORTED;
   auto* kernel = mx_gemm_few_kernel<GLU, SPLIT, RAW, BT, STAGES>;

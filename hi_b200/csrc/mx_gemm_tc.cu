@@ -27,7 +27,7 @@ using mx::unit;
 constexpr int BM = 128, BN = 256, STAGES = 6;     // rows of a block's tile, features of a pair's
 constexpr int A_BYTES = BM * KB / 2, B_BYTES = BN / 2 * KB / 2, STAGE = A_BYTES + B_BYTES + SCALES + BN / 128 * SCALES;
 constexpr int EPILOGUE = 8, THREADS = 64 + 32 * EPILOGUE;
-constexpr int MOST_EXPERTS = 1024, MOST_SPLITS = 8;
+constexpr int MOST_EXPERTS = 384, MOST_SPLITS = 8;       // experts: whose tables shared memory holds beside the stages
 
 struct Maps { CUtensorMap x, w, x_scales, w_scales; };
 struct Tile { int expert, row0, rows, scale_tile, f0; };      // rows: this block's, none or less perhaps

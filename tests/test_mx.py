@@ -250,7 +250,7 @@ def test_glu_and_down(i, k, n, limit):
 
 
 @pytest.mark.parametrize("n,experts,top_k,h,i", [(1, 4, 1, 64, 32), (8, 16, 1, 512, 96), (64, 64, 6, 256, 160), (300, 3, 2, 288, 256),
-                                                (700, 5, 1, 1056, 64), (40, 128, 4, 96, 64), (130, 1, 1, 128, 128), (70, 2, 2, 2080, 64), (900, 3, 1, 544, 96), (12000, 4, 1, 5152, 4128)])
+                                                (700, 5, 1, 1056, 64), (40, 128, 4, 96, 64), (500, 384, 2, 64, 32), (130, 1, 1, 128, 128), (70, 2, 2, 2080, 64), (900, 3, 1, 544, 96), (12000, 4, 1, 5152, 4128)])
 @pytest.mark.parametrize("scale", ["input", "output"])
 def test_experts(n, experts, top_k, h, i, scale):
     """A token through its experts and back: experts without rows, with less than a tile and with several, the score before or after."""
@@ -378,7 +378,9 @@ def test_refusals():
     other = _plan(g, 10, 3, 2)[1]
     rows = ops.mx_quantize(x, plan, 2)
     scores = torch.rand(10, 2, device=DEV)
-    for call in (lambda: ops.mx_linear(x, wg), lambda: ops.mx_glu(x, w), lambda: ops.mx_linear(x, we), lambda: ops.mx_linear(rows, w),
+    many = ops.mx_pack_weight(*_weight(g, 385, 64, 256), glu=True)
+    ids_many, plan_many = _plan(g, 10, 385, 2)
+    for call in (lambda: ops.mx_experts_glu(x, plan_many, 2, many), lambda: ops.mx_linear(x, wg), lambda: ops.mx_glu(x, w), lambda: ops.mx_linear(x, we), lambda: ops.mx_linear(rows, w),
                  lambda: ops.mx_linear(x[:, :224], w), lambda: ops.mx_linear(x.half(), w), lambda: ops.mx_quantize(x[:, :40]),
                  lambda: ops.mx_linear(x, w, torch.float16), lambda: ops.mx_linear(x, w, bias=torch.zeros(127, dtype=BF16, device=DEV)),
                  lambda: ops.mx_linear(x, w, bias=torch.zeros(128, device=DEV)), lambda: ops.mx_linear(x[0], w),
