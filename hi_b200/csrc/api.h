@@ -99,7 +99,7 @@ int hb_mx_values(const void* codes, const void* scales, int rows, int K, const i
 int hb_mx_gemm(const void* raw, int raw_dtype, long long raw_ld, int top_k, void* x, void* x_scales, int rows, const int* offsets,
                int experts, const void* w, const void* w_scales, int n_out, int K, const void* bias, const int* sorted_entry, const float* scores, int glu, float limit, void* out, int out_dtype,
                void* out_scales, int* status, cudaStream_t stream);
-int hb_mx_gemm_form(int rows, int experts, int n_out, int K);      // 0: pairs of blocks; else 1000 x the blocks that share K + a tile's rows
+int hb_mx_gemm_form(int rows, int experts, int n_out, int K, int glu);      // 0: pairs of blocks; else 1000 x the blocks that share K + a tile's rows
 
 // sink != 0 (every attention entry point): the softmax's denominator has one more term of score 0,
 // p_j = e^{s_j} / (1 + sum e^{s_j}); the term has no value. The general kernel and the merge also take

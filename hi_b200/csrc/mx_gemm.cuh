@@ -12,8 +12,8 @@ namespace mx {
 constexpr int KB = 256;                           // k of a stage
 constexpr int SCALES = KB / CHUNK * ATOM;         // of 128 rows, a stage
 
-// The unit in float32, by the fast exponential and division (2^-21 of the result, and where the gate is far below zero as much of it; denominators
-// past 2^126 give 0).
+// The unit in float32, by the fast exponential and division: off by 2^-21 of the result, by more where the gate is far below zero and the result as good as
+// none (2^-17 of it at -80); denominators past 2^126 give 0.
 template <bool CLAMPED> __device__ __forceinline__ float unit(float gate, float up, float limit) {
   if constexpr (CLAMPED) {
     const float g = fminf(gate, limit), u = fminf(fmaxf(up, -limit), limit);

@@ -1,7 +1,9 @@
 // Products of microscaled 4-bit floats for few rows, and for experts, of which each has its own few (mx_gemm.cuh; many rows: mx_gemm_tc.cu):
 //     C[r, f] = sum_k X[r, k] W[e(r), f, k]      for rows in the order of their experts (one run of rows: one expert)
 // The product is taken transposed: 128 weight rows are the MMA's M, an expert's rows, up to BT of them, its N, rounded up to 16, so that what an
-// expert costs goes by the rows it has and its weights come once for all of them. What bounds it is HBM, which brings the weights.
+// expert costs goes by the rows it has and its weights come once for all of them. What bounds it is HBM, which brings the weights (units of 64 tokens, 1 of
+// 16 experts of 5,120 x 8,192: 97 us, 1.05 of the copy rate), and where a launch does not fill the SMs the issue of copies and products, 0.2 us a stage, behind
+// 1.7 to 2 us until the first weights are there (8 x 2,048 x 2,048 5.0 us, 8 x 5,120 x 8,192 8.5, where HBM alone would take 0.3 and 3.4).
 // Blocks walk the tiles (expert, 128 features, BT rows; rows fastest: neighbours share weights):
 //   warp 0       brings a stage of 256 k: weights and rows by TMA (128-byte rows, swizzled), the scales' atoms as bulk copies; the first stages before
 //                the block's warps meet, and their weights before the launch that quantises the rows has ended;

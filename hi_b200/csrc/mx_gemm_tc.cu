@@ -12,6 +12,8 @@
 //                252 us), and issues the products, four of 64 k;
 //   warps 2 .. 9 read sums back (two warps a quarter of the rows, 64 columns in turn) and write results, while the next tile's sums go to the other slot
 //                of tensor memory. The slots share 64 columns, which are read first.
+// What bounds it: 2,048 x 16,384 x 5,120 takes 66 us, 5.2 PFLOP/s, 90,100 cycles, of which products are 75,000; for a second or more the card's power limit
+// lowers the clock and it takes 78. A stage is 530 cycles (products 512); between two tiles the products wait 1,000 to 1,200 for the sums' first 64 columns.
 // Rows of a tile past its expert's last and weight rows past n_out are computed from whatever is there, and not stored.
 // Every wait is bounded; a block that gave up says where in `status` and leaves by the common exit.
 #include "mx_gemm.cuh"
@@ -343,18 +345,24 @@ int pairs(const Call& c, const Params& p, int pairs) {
   return mx::start(kernel, maps, p, THREADS, 2 * pairs, 2, smem, c.stream);
 }
 
-// The form by a model of the time in us. Few rows (mx_gemm_few_tc.cu): a stage of 128 weight rows by n rows takes a block 0.12 + 0.0014 n, 0.2 at least, and
-// the first stage's way and the last results 3.4; n blocks that share K 4.3, 0.07 a tile, 0.17 a stage and 0.02 + 0.05 / n a row. Pairs: a stage 0.34 in the first round and 0.44 in
-// others (the card is at its power limit then), a tile 6 at least (its results), 6.5 besides. An expert's last tile is taken to be half full.
-// Measured, as pairs / single blocks: 512 x 16,384 x 5,120 24.1 / 24.2, 700 x 5,120 x 8,192 18.8 / 18.4, 2,048 x 16,384 x 5,120 67.5 / 72.7, units of 2,047 x 8,192
-// x 5,120 64.4 / 75.0, 99 x 5,120 x 8,192 17.7 / 11.5; 4,096 rows of 16 experts of 5,120 x 8,192: up 209 / 218, down 118 / 110, 2,048: 157 / 147 and 87 / 75; in one, two, four and
-// eight parts 1 x 256 x 8,192 7.9 / 6.7 / 5.9 / 5.5, 16 x 2,048 x 8,192 9.0 / 8.7 / 7.5 / 12.4 (more clusters than live at a time), 60 x 2,048 x 4,096 6.8 / 9.1 /
-// 7.9 / 13.3, in three 1 x 5,120 x 8,192 9.5 -> 8.6, 60 rows 10.2 -> 10.8. Tiles of up to 64, 128 and 256 rows: 8 x 7,168 x 5,120 7.5 / 7.8 / 9.4; of
-// 128, 192 and 256: 256 x 5,120 x 8,192 12.4 / 15.3 / 17.9, 512 x 5,120 x 8,192 19.6 / 15.5 / 18.4, 160 x 16,384 x 5,120 15.1 / 13.4 / 14.6, 700 x 16,384 x
-// 5,120 33.6 / 32.7 / 31.2; experts' up and down of 64 rows 116, 63 / 123, 69 / 124, 74, of 128 165, 79 / 166, 79 / 148, 82, of 256 261, 117 / 235, 128 / 216, 124.
+// The form by a model of the time in us. Few rows (mx_gemm_few_tc.cu): a stage of 128 weight rows by n rows takes a block 0.12 + 0.0014 n, 0.2 at least,
+// and the first stage's way and the last results 3.4; n blocks that share K 4.3, 0.07 a tile, 0.17 a stage and 0.02 + 0.05 / n a row. Pairs: a stage 0.34
+// in the first round and 0.44 in others (the card is at its power limit then), 6.5 besides. A tile takes what its results take at least: 0.4 + 0.022 n, of a
+// gated unit 0.5 + 0.035 n, a pair 5. An expert's last tile is taken to be half full. Measured (us):
+//   pairs / single blocks: 512 x 16,384 x 5,120 22.3 / 24.0, 700 x 5,120 x 8,192 17.9 / 18.1, 2,048 x 16,384 x 5,120 66 / 73, units of 700 x 8,192 x 5,120
+//   28.8 / 34.0, 99 x 5,120 x 8,192 17.0 / 11.8; 16 experts of 5,120 x 8,192, 4,096 rows: up 210 / 216, down 121 / 117, 2,048 rows: 155 / 148, 83 / 79; 12,288 rows of 64
+//   experts of 2,048 x 1,024: 49 / 57, 45 / 36;
+//   one, two, four and eight parts: 1 x 256 x 8,192 7.9 / 6.7 / 5.9 / 5.5, 16 x 2,048 x 8,192 9.0 / 8.7 / 7.5 / 12.4 (more clusters than live at a
+//   time), 60 x 2,048 x 4,096 6.8 / 9.1 / 7.9 / 13.3; one and three: 1 x 5,120 x 8,192 9.5 / 8.6, 60 x 5,120 x 8,192 10.2 / 10.8;
+//   tiles of up to 64, 128 and 256 rows: 8 x 7,168 x 5,120 7.5 / 7.8 / 9.4; of 128, 192 and 256: 256 x 5,120 x 8,192 12.4 / 15.3 / 17.9, 512 x 5,120 x
+//   8,192 19.6 / 15.5 / 18.4, 160 x 16,384 x 5,120 15.1 / 13.4 / 14.6, 700 x 16,384 x 5,120 33.6 / 32.7 / 31.2; experts' up and down with 64 rows each 116,
+//   63 / 123, 69 / 124, 74, with 128 each 165, 79 / 166, 79 / 148, 82 (for a second or more 307 / 318 / 313 the two together), with 256 each 261, 117 / 235,
+//   128 / 216, 124.
+// A single block's tile of n rows: its stages, or its results where those take longer.
+float tile_us(int stages, float n, bool glu) { return fmaxf(stages * fmaxf(0.2f, 0.12f + 0.0014f * n), glu ? 0.5f + 0.035f * n : 0.4f + 0.022f * n); }
 // `runs`: experts that may have rows. splits 0: pairs of blocks; else single ones, so many of them on a tile, with up to `most_rows` rows of it.
 struct Form { int splits, most_rows; };
-Form form(int rows, int experts, int n_out, int chunks) {
+Form form(int rows, int experts, int n_out, int chunks, bool glu) {
   const int runs = experts < rows ? experts : rows, each = (rows + runs - 1) / runs, stages = chunks / 2;
   const long long f_tiles = (n_out + 127) / 128, f_pairs = (n_out + BN - 1) / BN;
   int most_rows = 64;
@@ -362,15 +370,15 @@ Form form(int rows, int experts, int n_out, int chunks) {
   if (runs == 1) {
     for (int t = rows <= 64 ? 64 : 128; t <= (rows <= 64 ? 64 : 256); t += 64) {
       const int tiles = (rows + t - 1) / t;
-      const float us = 3.4f + (f_tiles * tiles + 147) / 148 * stages * fmaxf(0.2f, 0.12f + 0.0014f * ((rows + tiles - 1) / tiles));
+      const float us = 3.4f + (f_tiles * tiles + 147) / 148 * tile_us(stages, (float)rows / tiles, glu);
       if (us < single) { single = us; most_rows = t; }
     }
-    pair = 6.5f + ((rows + 2 * BM - 1) / (2 * BM) * f_pairs + 73) / 74 * fmaxf(6.f, stages * 0.44f) - stages * 0.1f;
+    pair = 6.5f + ((rows + 2 * BM - 1) / (2 * BM) * f_pairs + 73) / 74 * fmaxf(5.f, stages * 0.44f) - stages * 0.1f;
   } else {
     if (rows > 64) most_rows = each <= 128 ? 128 : 256;
     const float tiles = runs * (each > most_rows ? (float)each / most_rows + 0.5f : 1.f), pairs = runs * ((float)each / (2 * BM) + 0.5f);
-    single = 3.4f + f_tiles / 148.f * stages * fmaxf(0.2f * tiles, 0.12f * tiles + 0.0014f * rows);
-    pair = 6.5f + f_pairs / 74.f * pairs * fmaxf(6.f, stages * 0.44f);
+    single = 3.4f + f_tiles / 148.f * tiles * tile_us(stages, rows / tiles, glu);
+    pair = 6.5f + f_pairs / 74.f * pairs * fmaxf(5.f, stages * 0.44f);
   }
   Form best{single <= pair ? 1 : 0, most_rows};
   float least = fminf(single, pair);
@@ -383,7 +391,7 @@ Form form(int rows, int experts, int n_out, int chunks) {
 }
 
 int gemm(const Call& c, const Params& p, bool glu) {
-  const Form f = form(p.rows, p.experts, p.n_out, p.chunks);
+  const Form f = form(p.rows, p.experts, p.n_out, p.chunks, glu);
   if (f.splits || p.raw) return hb_mx_gemm_few(c, p, glu, f.splits ? f.splits : 1, f.most_rows);
   const int runs = p.experts < p.rows ? p.experts : p.rows;
   const long long most = ((p.rows + 2 * BM - 1) / (2 * BM) + runs - 1LL) * ((p.n_out + BN - 1) / BN);      // tiles that there may be
@@ -428,8 +436,8 @@ extern "C" int hb_mx_gemm(const void* raw, int raw_dtype, long long raw_ld, int 
 }
 
 // The form that hb_mx_gemm takes: 0 pairs of blocks, else 1000 times the blocks that share a tile's K and the rows of a tile.
-extern "C" int hb_mx_gemm_form(int rows, int experts, int n_out, int K) {
+extern "C" int hb_mx_gemm_form(int rows, int experts, int n_out, int K, int glu) {
   if (rows < 1 || experts < 1 || n_out < 1 || K < 1) return -1;
-  const Form f = form(rows, experts, n_out, mx::chunks(K));
+  const Form f = form(rows, experts, n_out, mx::chunks(K), glu != 0);
   return f.splits ? f.splits * 1000 + f.most_rows : 0;
 }

@@ -45,7 +45,7 @@ _SIGNATURES = {
     "hb_four_bit_linear_tc": [P, c_longlong, P, P, P, I, I, I, I, I, P, P],
     "hb_mx_quantize": [P, I, c_longlong, I, I, P, I, P, I, P, P, P],
     "hb_mx_values": [P, P, I, I, P, I, P, I, P],
-    "hb_mx_gemm_form": [I, I, I, I],
+    "hb_mx_gemm_form": [I, I, I, I, I],
     "hb_mx_gemm": [P, I, c_longlong, I, P, P, I, P, I, P, P, I, I, P, P, P, I, F, P, I, P, P, P],
     "hb_paged_attention": [P, I, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, F, P, P, I, I, P, P, P],
     "hb_attention_portions": [P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, F, I, F, P, P, I, P, P, P],
@@ -2165,11 +2165,9 @@ class MoePlan:
         return iter((self.offsets, self.sorted_entry, self.slot_of_entry))
 
 
-def _empty_plan(n: int, experts: int, dev) -> MoePlan:
-    return MoePlan(torch.empty(experts + 1, dtype=torch.int32, device=dev),
-                   torch.empty(max(n, 1), dtype=torch.int32, device=dev),
-                   torch.empty(max(n, 1), dtype=torch.int32, device=dev),
-                   torch.empty(experts + 1, dtype=torch.int32, device=dev))
+def _empty_plan(n: int, experts: int, like: torch.Tensor) -> MoePlan:
+    new = like.new_empty                 # of int32 (1 us less each than torch.empty with a type and a device)
+    return MoePlan(new(experts + 1), new(max(n, 1)), new(max(n, 1)), new(experts + 1))
 
 
 _block_counters: dict = {}     # device -> one int32 that kernels leave at zero; launches that share it must
@@ -2203,7 +2201,7 @@ def router_plan(x: torch.Tensor, w: torch.Tensor, top_k: int, mode: int = 0, sco
     ids = torch.empty((n, top_k), dtype=torch.int32, device=x.device)
     scores = torch.empty((n, top_k), dtype=torch.float32, device=x.device)
     logits = torch.empty((n, experts), dtype=torch.float32, device=x.device)   # the blocks' meeting place
-    plan = _empty_plan(n * top_k, experts, x.device)
+    plan = _empty_plan(n * top_k, experts, ids)
     _check(lib().hb_router_plan(_ptr(x), _dt(x), _ptr(w), _dt(w), _router_bias(bias, experts), n, hidden, experts, top_k, int(mode), float(score_scale),
                                 _ptr(logits), _ptr(ids), _ptr(scores), _ptr(plan.offsets), _ptr(plan.sorted_entry),
                                 _ptr(plan.slot_of_entry), _ptr(plan.active), _ptr(_block_counter(x.device)),
@@ -2215,7 +2213,7 @@ def moe_plan(ids: torch.Tensor, experts: int) -> MoePlan:
     """Group the routing entries by expert, on the device."""
     _need(ids, "ids", torch.int32)
     n = ids.numel()
-    plan = _empty_plan(n, experts, ids.device)
+    plan = _empty_plan(n, experts, ids)
     _check(lib().hb_moe_plan(_ptr(ids), n, experts, _ptr(plan.offsets), _ptr(plan.sorted_entry),
                              _ptr(plan.slot_of_entry), _ptr(plan.active), _stream()), "moe_plan")
     return plan
@@ -2619,6 +2617,7 @@ MX_BLOCK, MX_TILE, MX_CHUNK = 32, 128, 128     # values that share a power of tw
 # 5 us less host work a call (11.5 instead of 16.8). On the device (so / quantised first, us): 1 x 2,048 x 2,048 5.1 / 6.0, 4 rows 5.7 / 6.0, 8 rows 6.2 / 6.0;
 # 1 x 7,168 x 5,120 9.0 / 8.7, 2 rows 9.2 / 8.7, 8 rows 11.5 / 8.9; units of 1 x 8,192 x 5,120 11.6 / 11.7.
 MX_DIRECT_ROWS, MX_DIRECT_VALUES = 16, 10240
+MX_MOST_EXPERTS = 384                          # of a stack: whose tables a block's shared memory holds beside its stages
 
 
 def _mx_chunks(k: int) -> int:
@@ -2829,8 +2828,8 @@ def _mx_both(x, weight: MxWeight):
 
 
 def _mx_rows_for(x, weight: MxWeight, name: str, glu: bool, stack: bool = False) -> None:
-    if not isinstance(weight, MxWeight) or weight.glu != glu or (len(weight.shape) == 3) != stack:
-        raise KernelError(f"{name} takes {'experts' if stack else 'a weight'} in microscaled 4-bit floats" + (" with gate and up rows in turn" if glu else ""))
+    if not isinstance(weight, MxWeight) or weight.glu != glu or (len(weight.shape) == 3) != stack or weight.experts > MX_MOST_EXPERTS:
+        raise KernelError(f"{name} takes {f'up to {MX_MOST_EXPERTS} experts' if stack else 'a weight'} in microscaled 4-bit floats" + (" with gate and up rows in turn" if glu else ""))
 
 
 def mx_linear(x, weight: MxWeight, out_dtype: torch.dtype = torch.bfloat16, bias: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -49,7 +49,7 @@ class _SwiGLU:
             rows += [sg, torch.zeros((-(2 * self.inter + 1) % 8, self.hidden), dtype=sg.dtype, device=sg.device)]
         if len({t.dtype for t in rows}) > 1:
             rows = [t.float() for t in rows]
-        if not self.token_gate and self.inter % ops.MX_BLOCK == 0 and microscaled(rows[0], self.env):
+        if not self.token_gate and (self.limit is None or self.limit > 0) and self.inter % ops.MX_BLOCK == 0 and microscaled(rows[0], self.env):
             self.w_gate_up = ops.mx_quantize_weight(ops.mx_interleave(*rows), glu=True)
         else:
             self.w_gate_up = packed(torch.cat(rows, dim=0).contiguous(), self.env)
@@ -254,7 +254,7 @@ class SigmoidRoutedExperts(Part):
             self.w_gate = expert_tensor(f"{p}.experts.gate_proj.weight") if gated else None
             self.w_up = expert_tensor(f"{p}.experts.up_proj.weight")
             self.w_down = expert_tensor(f"{p}.experts.down_proj.weight")
-        if gated and self.inter % ops.MX_BLOCK == 0 and microscaled(self.w_up, self.env):
+        if gated and self.inter % ops.MX_BLOCK == 0 and self.experts <= ops.MX_MOST_EXPERTS and microscaled(self.w_up, self.env):
             self.w_gate_up = microscaled_stack((ops.mx_interleave(g, u) for g, u in zip(self.w_gate, self.w_up)), glu=True)
             self.w_gate = self.w_up = None
             self.w_down = microscaled_stack(self.w_down)

@@ -126,7 +126,7 @@ def test_linear_of_blocks_that_share_k(m, k, n):
     """Shares of unlike length, the last one short; every block finishes some rows, or has none to finish."""
     from hi_b200.kernels import ops
 
-    assert ops.lib().hb_mx_gemm_form(n, 1, m, k) >= 2000
+    assert ops.lib().hb_mx_gemm_form(n, 1, m, k, 0) >= 2000
     g = _gen(m + k + n)
     x, (codes, exps) = _rows(g, n, k), _weight(g, m, k)
     bias = torch.randn(m, device=DEV, generator=g).to(BF16)
@@ -151,7 +151,7 @@ def test_linear_of_large_tiles(m, k, n, rows):
     x, (codes, exps) = _rows(g, n, k), _weight(g, m, k)
     bias = torch.randn(m, device=DEV, generator=g).to(BF16)
     w, xv, wv = ops.mx_pack_weight(codes, exps), plain_mx.held(x), plain_mx.values(codes, exps)
-    assert ops.lib().hb_mx_gemm_form(n, 1, m, k) == 1000 + rows
+    assert ops.lib().hb_mx_gemm_form(n, 1, m, k, 0) == 1000 + rows
     y = ops.mx_linear(x, w, F32, bias)
     _near(y, xv, wv, bias)
     assert torch.equal(ops.mx_linear(x, w, bias=bias), y.to(BF16))
@@ -170,7 +170,7 @@ def test_linear_of_many_rows(m, k, n):
     """Pairs of blocks: several tiles a pair, tiles that are not full in rows, features and k, an odd number of features."""
     from hi_b200.kernels import ops
 
-    assert ops.lib().hb_mx_gemm_form(n, 1, m, k) == 0
+    assert ops.lib().hb_mx_gemm_form(n, 1, m, k, 0) == 0
     g = _gen(m + k + n)
     x, (codes, exps) = _rows(g, n, k), _weight(g, m, k)
     bias = torch.randn(m, device=DEV, generator=g).to(BF16)
@@ -186,7 +186,7 @@ def test_glu_of_many_rows(limit):
     from hi_b200.kernels import ops
 
     i, k, n = 8224, 5152, 2221
-    assert ops.lib().hb_mx_gemm_form(n, 1, 2 * i, k) == 0
+    assert ops.lib().hb_mx_gemm_form(n, 1, 2 * i, k, 1) == 0
     g = _gen(i)
     x, gate, up = _rows(g, n, k), _weight(g, i, k), _weight(g, i, k)
     w = ops.mx_pack_weight(*(ops.mx_interleave(a, b) for a, b in zip(gate, up)), glu=True)

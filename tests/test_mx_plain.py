@@ -69,13 +69,13 @@ def test_refusals():
 def test_forms():
     """Which kernel a product takes, by sizes alone: clusters that share K where a weight has few tiles, single blocks for few rows and experts, pairs of
     blocks for many rows."""
-    form = ops.lib().hb_mx_gemm_form
+    form = lambda rows, experts, n_out, k, glu=0: ops.lib().hb_mx_gemm_form(rows, experts, n_out, k, glu)
     assert form(1, 1, 5120, 8192) // 1000 in (2, 3) and form(8, 1, 7168, 5120) == 1064 and form(1, 1, 64, 32) == 1064
     assert form(64, 1, 16384, 5120) == 1064 and form(100, 1, 16384, 5120) == 1128 and form(160, 1, 16384, 5120) == 1192
     assert form(256, 1, 5120, 8192) == 1128 and form(512, 1, 5120, 8192) == 1192 and form(256, 1, 16384, 5120) == 1256
     assert form(2048, 1, 16384, 5120) == 0 and form(8192, 1, 5120, 5120) == 0
-    assert form(64, 16, 16384, 5120) == 1064 and form(2048, 16, 16384, 5120) == 1128 and form(2100, 16, 5120, 8192) == 1256
-    assert form(4096, 16, 5120, 8192) == 1256 and form(12000, 4, 8256, 5152) == 0
+    assert form(64, 16, 16384, 5120, 1) == 1064 and form(2048, 16, 16384, 5120, 1) == 1128 and form(2100, 16, 5120, 8192) == 1256
+    assert form(4096, 16, 5120, 8192) == 1256 and form(12000, 4, 8256, 5152, 1) == 0 and form(12288, 64, 2048, 2048, 1) == 0 and form(12288, 64, 2048, 1024) == 1256
     for rows in (1, 2, 7, 64, 65, 128, 129, 500, 3000, 100000):
         for experts in (1, 2, 64, 1024):
             for n_out in (1, 64, 5120, 200000):
