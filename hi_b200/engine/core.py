@@ -146,7 +146,7 @@ class Engine:
         projections, dense feed-forwards and shared experts are quantised to four bits as they are loaded, ``weight_group`` inputs
         to a scale (routed experts, embeddings, the head and other mixers stay as they are, and weights stored in 32 bits or with inputs that are
         not a multiple of 32); with ``weight_format="mxfp4"`` they become microscaled 4-bit floats, routed experts with a gate branch too, and what
-        they multiply is quantised alike, block by block. ``kv_cache_bits=4``: keys and values are
+        they multiply is quantised alike, in blocks of 32 (``weight_group`` says nothing then). ``kv_cache_bits=4``: keys and values are
         cached in four bits (models whose mixers with a paged cache are plain softmax attention, heads of up to 128; where their scores are
         capped or biased by distance, steps are not captured)."""
         arch, cfg, _raw = load_architecture(model_dir)

@@ -59,6 +59,8 @@ class Model:
                              f"{ops.FOUR_BIT_GROUPS} are built")
         if weight_format not in WEIGHT_FORMATS:
             raise ValueError(f"weight format {weight_format!r} is not known: {WEIGHT_FORMATS}")
+        if weight_format != WEIGHT_FORMATS[0] and weight_bits != 4:
+            raise ValueError(f"weight format {weight_format!r} is one of weights in four bits, not in {weight_bits}")
         if dtype != torch.bfloat16 and (weight_bits != 16 or cache_bits != 16):
             raise ValueError("weights and a cache in four bits are built for bfloat16; the float32 path is 32-bit throughout")
         self.spec, self.dtype, self.device = spec, dtype, torch.device(device)

@@ -21,7 +21,8 @@ def test_options_that_are_refused():
         return Model(arch.build_spec(arch.parse_config(TINY_A, None)), kw.pop("dtype", BF16), "cpu", **kw)
 
     assert build(weight_bits=4, weight_format="mxfp4").env.weight_format == "mxfp4"
-    for kw in (dict(weight_bits=4, weight_format="fp4"), dict(weight_format=None), dict(weight_bits=4, weight_format="mxfp4", dtype=torch.float32)):
+    for kw in (dict(weight_bits=4, weight_format="fp4"), dict(weight_format=None), dict(weight_format="mxfp4"),
+               dict(weight_bits=4, weight_format="mxfp4", dtype=torch.float32)):
         with pytest.raises(ValueError):
             build(**kw)
 
