@@ -24,6 +24,8 @@ __device__ __forceinline__ uint32_t scale_of(uint32_t top_bits) {
 }
 // 2^-e of a scale's byte (255: anything): exact as a float, and so is its product with a value that does not become zero as a code
 __device__ __forceinline__ float inverse(uint32_t scale) { return __uint_as_float((254u - scale) << 23); }
+// 2^-e from the bits of the block's largest magnitude: inverse(scale_of(top_bits)), but for what is not finite, where anything will do
+__device__ __forceinline__ float inverse_of(uint32_t top_bits) { return __uint_as_float(min(0x80000000u - (top_bits & 0x7f800000u), 0x7f000000u)); }
 __device__ __forceinline__ float value_of(uint32_t scale) {
   return __uint_as_float(scale == 0 ? 0x00400000u : scale == 255 ? 0x7fffffffu : scale << 23);
 }
@@ -105,7 +107,7 @@ template <typename T> __device__ __forceinline__ uint32_t quantize(const Eight<T
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   scale = scale_of(top);
-  const float by = inverse(scale);                // (what is multiplied by the scale 255 does not matter)
+  const float by = inverse_of(top);
   float v[8];
   x.floats(v);
 #pragma unroll

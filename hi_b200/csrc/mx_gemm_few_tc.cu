@@ -16,6 +16,8 @@
 // blocks' order.
 // Rows past an expert's last and weight rows past n_out are computed from whatever is there, and not stored.
 // Every wait is bounded; a block that gave up says where in `status` and leaves by the common exit.
+#include <type_traits>
+
 #include "mx_gemm.cuh"
 
 namespace {
@@ -279,57 +281,63 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
       for (int j = 0; j < TURNS; ++j) {
         const int c = run_at(j);
         const bool some = there && c < t.rows;
+        // GLU: gate's warp keeps the run's first 8 rows and gives the others to up's, which keeps those
+        const bool up = GLU && (quarter & 1);
         uint32_t v[16];
         if (some) {
-          tc::ld16_nowait(from + c, v);
+          if constexpr (GLU) {
+            tc::ld8_nowait(from + c + (up ? 8 : 0), reinterpret_cast<uint32_t(&)[8]>(v[0]));
+            tc::ld8_nowait(from + c + (up ? 0 : 8), reinterpret_cast<uint32_t(&)[8]>(v[8]));
+          } else {
+            tc::ld16_nowait(from + c, v);
+          }
           tc::wait_ld();
         }
         if (SHARED && j == 0) arrive(acc_shared);
         if (j == TURNS - 1) arrive(&acc_empty[b]);
         if (!some) continue;
         if constexpr (GLU) {
-          const bool up = quarter & 1;
           float* const give = trade + (warp - 2) * 256 + lane;
           const float* const take = trade + ((warp ^ 1) - 2) * 256 + lane;
-          const int first = c + (up ? 8 : 0), r = first + lane % 8;        // gate's warp has the run's first 8 rows, up's the others
-          float own[8];
+          const int r = c + (up ? 8 : 0) + lane % 8;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            give[q * 32] = __uint_as_float(up ? v[q] : v[8 + q]);
-            own[q] = __uint_as_float(up ? v[8 + q] : v[q]);
-          }
+          for (int q = 0; q < 8; ++q) give[q * 32] = __uint_as_float(v[8 + q]);
           asm volatile("bar.sync %0, 64;" ::"r"(1 + part * 2 + quarter / 2) : "memory");
           float act[8];
-          if (p.limit > 0.f) {
+          auto units = [&](auto clamped) {
+            constexpr bool CLAMPED = decltype(clamped)::value;
+            if (up) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const float s = __shfl_sync(0xffffffffu, score, j * 8 + q), a = s * own[q], o = s * take[q * 32];
-              act[q] = mx::unit<true>(up ? o : a, up ? a : o, p.limit);
-            }
-          } else {
+              for (int q = 0; q < 8; ++q) {
+                const float s = __shfl_sync(0xffffffffu, score, j * 8 + q);
+                act[q] = mx::unit<CLAMPED>(s * take[q * 32], s * __uint_as_float(v[q]), p.limit);
+              }
+            } else {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const float s = __shfl_sync(0xffffffffu, score, j * 8 + q), a = s * own[q], o = s * take[q * 32];
-              act[q] = mx::unit<false>(up ? o : a, up ? a : o, 0.f);
+              for (int q = 0; q < 8; ++q) {
+                const float s = __shfl_sync(0xffffffffu, score, j * 8 + q);
+                act[q] = mx::unit<CLAMPED>(s * __uint_as_float(v[q]), s * take[q * 32], p.limit);
+              }
             }
-          }
+          };
+          if (p.limit > 0.f) units(std::true_type{});
+          else units(std::false_type{});
           asm volatile("bar.sync %0, 64;" ::"r"(1 + part * 2 + quarter / 2) : "memory");
           const int block = t.f0 / 64 + quarter / 2, blocks = p.n_out / 64, out_chunks = mx::chunks(p.n_out / 2);
-          uint32_t top[8], scale = 0;
+          uint32_t top[8], mine_top = 0;
 #pragma unroll
           for (int q = 0; q < 8; ++q) top[q] = __reduce_max_sync(0xffffffffu, __float_as_uint(act[q]) & 0x7fffffffu);
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
-            top[q] = mx::scale_of(top[q]);
-            act[q] *= mx::inverse(top[q]);
-            if (lane % 8 == q) scale = top[q];
+            act[q] *= mx::inverse_of(top[q]);
+            if (lane % 8 == q) mine_top = top[q];
           }
           const uint32_t word = transpose(mx::codes8(act), lane);
           if (r >= t.rows) continue;
           *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + (size_t)(t.row0 + r) * (p.n_out / 4) + block * 16 + lane / 8 * 4) = word;
           if (lane < 8) {
             uint8_t* const to = p.out_scales + (size_t)(t.scale_tile + (t.off + r) / mx::TILE) * out_chunks * mx::ATOM + mx::row_at((t.off + r) % mx::TILE);
-            to[block / 4 * mx::ATOM + block % 4] = (uint8_t)scale;
+            to[block / 4 * mx::ATOM + block % 4] = (uint8_t)mx::scale_of(mine_top);
             if (block == blocks - 1)
               for (int q = blocks; q < out_chunks * 4; ++q) to[q / 4 * mx::ATOM + q % 4] = 0;
           }

@@ -90,7 +90,7 @@ __device__ __forceinline__ void store_block(const Params& p, const Tile& t, int 
 #pragma unroll
   for (int j = 0; j < 32; ++j) top = max(top, __float_as_uint(act[j]) & 0x7fffffffu);
   const uint32_t scale = mx::scale_of(top);
-  const float by = mx::inverse(scale);            // (what is multiplied by the scale 255 does not matter)
+  const float by = mx::inverse_of(top);
   uint32_t word[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
