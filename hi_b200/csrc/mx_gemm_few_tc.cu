@@ -284,6 +284,7 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
         // GLU: gate's warp keeps the run's first 8 rows and gives the others to up's, which keeps those
         const bool up = GLU && (quarter & 1);
         uint32_t v[16];
+        __syncwarp();                             // (lanes part where rows or features end; the loads want the warp together)
         if (some) {
           if constexpr (GLU) {
             tc::ld8_nowait(from + c + (up ? 8 : 0), reinterpret_cast<uint32_t(&)[8]>(v[0]));
@@ -333,9 +334,8 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
             if (lane % 8 == q) mine_top = top[q];
           }
           const uint32_t word = transpose(mx::codes8(act), lane);
-          if (r >= t.rows) continue;
-          *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + (size_t)(t.row0 + r) * (p.n_out / 4) + block * 16 + lane / 8 * 4) = word;
-          if (lane < 8) {
+          if (r < t.rows) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + (size_t)(t.row0 + r) * (p.n_out / 4) + block * 16 + lane / 8 * 4) = word;
+          if (r < t.rows && lane < 8) {
             uint8_t* const to = p.out_scales + (size_t)(t.scale_tile + (t.off + r) / mx::TILE) * out_chunks * mx::ATOM + mx::row_at((t.off + r) % mx::TILE);
             to[block / 4 * mx::ATOM + block % 4] = (uint8_t)mx::scale_of(mine_top);
             if (block == blocks - 1)

@@ -286,6 +286,7 @@ mx_gemm_kernel(const __grid_constant__ Maps maps, const Params p) {
         const int g = b == 0 ? 3 - half - 2 * j : half + 2 * j, f = t.f0 + g * 64;
         const bool some = live && f < p.n_out;
         uint32_t lo[32], hi[32];
+        __syncwarp();                             // (lanes part where rows or features end; the loads want the warp together)
         if (some) {
           tc::ld32_nowait(from + g * 64, lo);
           tc::ld32_nowait(from + g * 64 + 32, hi);
