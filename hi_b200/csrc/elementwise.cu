@@ -318,14 +318,17 @@ __global__ void swiglu_kernel(const void* in, void* out, int dtype, size_t rows,
 }
 
 // out[t, :] = shared[t, :] + sum_j y[slot_of_entry[t*k + j], :]   in rank order, no atomics
+// (entries without a slot add nothing)
 // (crates/hi-cuda/src/kernels.cu:10661-10680; models.rs:6099 adds the shared expert).
 __global__ void moe_combine_kernel(const float* y, const int* slot_of_entry, const float* routed_weight,
                                    const void* shared, int shared_dtype, float* out, int hidden, int top_k) {
   const int t = blockIdx.y;
   for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < hidden; j += gridDim.x * blockDim.x) {
     float s = shared ? load_any(shared, shared_dtype, (size_t)t * hidden + j) : 0.f;
-    for (int r = 0; r < top_k; ++r)
-      s += y[(size_t)slot_of_entry[t * top_k + r] * hidden + j] * (routed_weight ? routed_weight[t * top_k + r] : 1.f);
+    for (int r = 0; r < top_k; ++r) {
+      const int slot = slot_of_entry[t * top_k + r];
+      if (slot >= 0) s += y[(size_t)slot * hidden + j] * (routed_weight ? routed_weight[t * top_k + r] : 1.f);
+    }
     out[(size_t)t * hidden + j] = s;
   }
 }
@@ -343,15 +346,18 @@ __global__ void __launch_bounds__(256) moe_combine_vec_kernel(const float* __res
   for (int r0 = 0; r0 < top_k; r0 += 4) {
     float4 v[4];
     float f[4];
+    bool there[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (r0 + i < top_k) {
-        v[i] = *reinterpret_cast<const float4*>(y + (size_t)slot_of_entry[t * top_k + r0 + i] * hidden + j);
+        const int slot = slot_of_entry[t * top_k + r0 + i];
+        there[i] = slot >= 0;
+        if (there[i]) v[i] = *reinterpret_cast<const float4*>(y + (size_t)slot * hidden + j);
         f[i] = routed_weight ? routed_weight[t * top_k + r0 + i] : 1.f;
       }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (r0 + i < top_k) { s.x += v[i].x * f[i]; s.y += v[i].y * f[i]; s.z += v[i].z * f[i]; s.w += v[i].w * f[i]; }
+      if (r0 + i < top_k && there[i]) { s.x += v[i].x * f[i]; s.y += v[i].y * f[i]; s.z += v[i].z * f[i]; s.w += v[i].w * f[i]; }
   }
   *reinterpret_cast<float4*>(out + (size_t)t * hidden + j) = s;
 }

@@ -17,6 +17,8 @@ namespace {
 // Stable counting sort of the n = tokens*top_k routing entries by expert:
 // offsets[e]..offsets[e+1] are the sorted slots of expert e, in entry order.
 // active[0] = number of experts with at least one row, active[1..] = their ids in order.
+// An id outside 0 .. experts - 1 (a padded token's) has no slot: slot_of_entry is -1 there, and the slots that are left over at the end
+// name entry 0, so that a kernel which gathers all n rows reads one that exists.
 // `ids` is read past L1 (other blocks may have written it), or lies in shared memory (IDS_SHARED).
 // `sm` holds 2 * experts ints.
 template <bool IDS_SHARED = false>
@@ -46,6 +48,7 @@ __device__ __forceinline__ void plan_block(const int* ids, int n, int experts, i
   __syncthreads();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
+    int placed = 0;
     for (int start = 0; start < n; start += 32) {
       const int i = start + lane;
       int e = i < n ? (IDS_SHARED ? ids[i] : __ldcg(ids + i)) : -1;
@@ -56,11 +59,15 @@ __device__ __forceinline__ void plan_block(const int* ids, int n, int experts, i
         const int slot = base[e] + rank;
         sorted_entry[slot] = i;
         slot_of_entry[i] = slot;
+      } else if (i < n) {
+        slot_of_entry[i] = -1;
       }
+      placed += __popc(__ballot_sync(0xffffffffu, e >= 0));
       __syncwarp();
       if (e >= 0 && rank == 0) base[e] += __popc(peers);
       __syncwarp();
     }
+    for (int i = placed + lane; i < n; i += 32) sorted_entry[i] = 0;
   }
 }
 
@@ -99,6 +106,8 @@ __device__ __forceinline__ void plan_block_wide(const int* __restrict__ ids, int
           const int slot = mine[e] + rank;
           sorted_entry[slot] = i;
           slot_of_entry[i] = slot;
+        } else if (place && i < end) {
+          slot_of_entry[i] = -1;
         }
         __syncwarp();
         if (e >= 0 && rank == 0) mine[e] += __popc(peers);
@@ -136,6 +145,7 @@ __device__ __forceinline__ void plan_block_wide(const int* __restrict__ ids, int
   }
   __syncthreads();
   walk(true);
+  for (int i = first[experts - 1] + total[experts - 1] + threadIdx.x; i < n; i += blockDim.x) sorted_entry[i] = 0;
 }
 
 // ------------------------------------------------------------------ router

@@ -170,6 +170,8 @@ mx_gemm_few_kernel(const __grid_constant__ Maps maps, const Params p) {
           rows(t, q, kb0 + q);
         }
       }
+    } else if (p.behind) {                        // (where no block has a tile, the launch still ends behind the other one)
+      asm volatile("griddepcontrol.wait;" ::: "memory");
     }
   }
   if (warp == 1) tc::alloc(tmem_slot, TMEM_COLS);

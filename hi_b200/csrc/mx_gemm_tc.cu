@@ -164,6 +164,7 @@ mx_gemm_kernel(const __grid_constant__ Maps maps, const Params p) {
     int s = 0, turn = 1, issued = 0;
     bool ok = true;
     const uint32_t mine = tc::elect_one(), ring = tc::smem_u32(smem), bars = tc::even_block(full);
+    if (p.behind && pair_id >= all) asm volatile("griddepcontrol.wait;" ::: "memory");      // (where no block has a tile, the launch still ends behind the other one)
     for (int i = 0; ok && tile_at(i, t); ++i) {
       const int row = tc::uniform(t.row0), w_row = tc::uniform(t.expert * p.n_out + t.f0 + rank * (BN / 2));
       const int xs = tc::uniform(t.scale_tile * p.chunks), ws = tc::uniform((t.expert * p.w_tiles + t.f0 / 128) * p.chunks);

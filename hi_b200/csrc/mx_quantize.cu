@@ -34,7 +34,9 @@ mx_quantize_kernel(const T* __restrict__ x, long long x_ld, int rows, int k, con
   const long long item = (long long)blockIdx.x * WARPS + warp;
   const int row = (int)(item / groups), first = (int)(item % groups) * MANY;
   if (row >= rows) return;
-  const size_t from = sorted_entry ? sorted_entry[row] / top_k : row;
+  const int last = offsets ? offsets[experts] : rows, entry = sorted_entry ? sorted_entry[row] : 0;
+  if (row >= last) return;                                 // entries without an expert have no row
+  const size_t from = sorted_entry ? entry / top_k : row;
   const T* const in = x + from * x_ld + lane * 8;
   mx::Eight<T> x8[MANY];
 #pragma unroll
@@ -66,7 +68,7 @@ mx_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, all = mx::chunks(k), groups = (all / 2 + MANY - 1) / MANY;
   const long long item = (long long)blockIdx.x * WARPS + warp;
   const int row = (int)(item / groups), first = (int)(item % groups) * MANY;
-  if (row >= rows) return;
+  if (row >= rows || (offsets && row >= offsets[experts])) return;
   int tile, at;
   mx::place_of(offsets, experts, row, tile, at);
   const uint8_t* const from = codes + (size_t)row * (k / 2) + lane * 4;
@@ -109,7 +111,7 @@ void values(const void* codes, const void* scales, int rows, int k, const int* o
 }  // namespace
 
 // x [*, K] (rows x_ld elements apart, 16-byte aligned) -> codes, scales of `rows` rows: row i of x, or with sorted_entry (and the plan's offsets
-// of its experts) row sorted_entry[i] / top_k. K a multiple of 32.
+// of its experts) row sorted_entry[i] / top_k; with offsets, rows from offsets[experts] on are left as they are. K a multiple of 32.
 extern "C" int hb_mx_quantize(const void* x, int dtype, long long x_ld, int rows, int K, const int* sorted_entry, int top_k, const int* offsets,
                               int experts, void* codes, void* scales, cudaStream_t stream) {
   if (!x || !codes || !scales || rows < 0 || K <= 0 || (sorted_entry && (!offsets || top_k < 1 || experts < 1)) ||
@@ -126,7 +128,7 @@ extern "C" int hb_mx_quantize(const void* x, int dtype, long long x_ld, int rows
   return HB_OK;
 }
 
-// The values that rows stand for, [rows, K] in out_dtype.
+// The values that rows stand for, [rows, K] in out_dtype; with offsets, rows from offsets[experts] on are left as they are.
 extern "C" int hb_mx_values(const void* codes, const void* scales, int rows, int K, const int* offsets, int experts, void* out, int out_dtype,
                             cudaStream_t stream) {
   if (!codes || !scales || !out || rows < 0 || K <= 0 || (offsets && experts < 1) || (out_dtype != HB_DTYPE_F32 && out_dtype != HB_DTYPE_BF16))

@@ -999,7 +999,7 @@ def mlstm_out_norm(o: torch.Tensor, nq: torch.Tensor, floor: torch.Tensor, proj:
 def moe_combine(y: torch.Tensor, slot_of_entry: torch.Tensor, shared: Optional[torch.Tensor], n: int,
                 top_k: int, routed_weight: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[t] = shared[t] + sum_j w[t*k + j] * y[slot_of_entry[t*k + j]]  -> float32 [n, H] (w = 1 without
-    ``routed_weight``)."""
+    ``routed_weight``; a slot of -1 adds nothing)."""
     _need(y, "y", torch.float32); _need(slot_of_entry, "slot_of_entry", torch.int32)
     hidden = y.shape[1]
     if shared is not None:
@@ -2154,7 +2154,9 @@ def router_topk(x: torch.Tensor, w: torch.Tensor, top_k: int, want_logits: bool 
 
 class MoePlan:
     """Rows grouped by expert: ``offsets`` [E+1], ``sorted_entry`` [n] (entry of each sorted slot),
-    ``slot_of_entry`` [n], ``active`` [E+1] (count, then the ids of the experts that have rows)."""
+    ``slot_of_entry`` [n], ``active`` [E+1] (count, then the ids of the experts that have rows). An entry whose id is none of
+    0 .. E - 1 (a padded token's) has slot -1 and no row: ``offsets[E]`` rows are there, the products by expert leave those behind as they
+    are, and ``moe_combine`` adds nothing for it (the sums inside a norm want a slot for every entry)."""
 
     __slots__ = ("offsets", "sorted_entry", "slot_of_entry", "active")
 
@@ -2739,7 +2741,8 @@ def _mx_plan(plan: MoePlan, rows: int) -> None:
 
 def mx_quantize(x: torch.Tensor, plan: Optional[MoePlan] = None, top_k: int = 1) -> MxRows:
     """The rows of ``x`` [N, K] (bfloat16 or float32, K a multiple of 32; its rows may be a column slice of a wider matrix) in microscaled 4-bit
-    floats. With ``plan``: the N * top_k rows of its experts, sorted, row i from token sorted_entry[i] // top_k."""
+    floats. With ``plan``: the rows of its experts, sorted, row i from token sorted_entry[i] // top_k; of N * top_k rows those from ``offsets[E]``
+    on (entries without an expert) stay unwritten, here and in what is computed from them."""
     x = _mx_input(x)
     if plan is None:
         _on_current_device(x)

@@ -52,3 +52,50 @@ def test_units_of_tiles_that_end_anywhere(counts, i, k, form):
     for _ in range(5):
         assert torch.equal(ops.mx_values(ops.mx_experts_glu(x, plan, 1, w), F32).double(), values)
     ops.check_tc_status()
+
+
+# ---------------------------------------------------------------- entries without an expert
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,experts,top_k", [(1, 4, 2), (9, 3, 1), (40, 16, 4), (200, 5, 2), (700, 64, 3), (33, 2, 1)])
+@pytest.mark.parametrize("some", [True, False])
+def test_entries_without_an_expert(n, experts, top_k, some):
+    """Ids that name no expert (a padded batch's): the plan's slots, rows and results of the others; or no entry has one."""
+    from hi_b200.kernels import ops
+
+    g, h, i = _gen(n + experts), 416, 160
+    ids = torch.randn(n, experts, device=DEV, generator=g).topk(top_k, 1).indices.to(torch.int32)
+    none = torch.rand(n, top_k, device=DEV, generator=g) < (0.4 if some else 2.0)
+    none[-1] = True
+    ids[none] = torch.tensor([-1, experts, 2 ** 31 - 1, -(2 ** 31)], dtype=torch.int32, device=DEV)[torch.arange(int(none.sum()), device=DEV) % 4]
+    plan = ops.moe_plan(ids.contiguous(), experts)
+    flat = ids.view(-1).long()
+    real = (flat >= 0) & (flat < experts)
+    count = int(real.sum())
+    order = torch.argsort(torch.where(real, flat, torch.full_like(flat, experts)), stable=True)[:count]
+    assert int(plan.offsets[-1]) == count and torch.equal(plan.sorted_entry[:count].long(), order)
+    assert (plan.sorted_entry[count:] == 0).all() and (plan.slot_of_entry[~real] == -1).all()
+    assert torch.equal(plan.slot_of_entry[order].long(), torch.arange(count, device=DEV))
+    x, scores = _rows(g, n, h), torch.rand(n, top_k, device=DEV, generator=g)
+    held = plain_mx.held(x)
+    assert torch.equal(ops.mx_values(ops.mx_quantize(x, plan, top_k), F32)[:count].double(), held[order // top_k])
+    gate, up, down = _weight(g, experts, i, h), _weight(g, experts, i, h), _weight(g, experts, h, i)
+    act = ops.mx_experts_glu(x, plan, top_k, ops.mx_pack_weight(*(ops.mx_interleave(a, b) for a, b in zip(gate, up)), glu=True), scores)
+    y = ops.mx_experts_linear(act, ops.mx_pack_weight(*down), plan)
+    values, offsets = ops.mx_values(act, F32).double(), plan.offsets.tolist()
+    for e in range(experts):
+        rows = slice(offsets[e], offsets[e + 1])
+        if rows.start < rows.stop:
+            entries = order[rows]
+            _check_unit(values[rows], held[entries // top_k], plain_mx.values(gate[0][e], gate[1][e]), plain_mx.values(up[0][e], up[1][e]), 0.0,
+                        scores.view(-1)[entries])
+            _near(y[rows], values[rows], plain_mx.values(down[0][e], down[1][e]))
+    terms = torch.zeros(n * top_k, h, dtype=torch.float64, device=DEV)
+    terms[order] = y[:count].double() * scores.view(-1)[order].double().unsqueeze(1)
+    terms = terms.view(n, top_k, h)
+    out = ops.moe_combine(y, plan.slot_of_entry, None, n, top_k, scores.view(-1))
+    odd = ops.moe_combine(y[:, : h - 1].contiguous(), plan.slot_of_entry, None, n, top_k, scores.view(-1))
+    # a term's rounding and each of k sums, 2^-24 of all magnitudes each
+    for got in (out, odd):
+        want = terms[..., : got.shape[1]]
+        assert ((got.double() - want.sum(1)).abs() <= (top_k + 1) * 2.0 ** -24 * want.abs().sum(1)).all() and not got[-1].any()
+    ops.check_tc_status()
