@@ -12,11 +12,23 @@ namespace mx {
 constexpr int KB = 256;                           // k of a stage
 constexpr int SCALES = KB / CHUNK * ATOM;         // of 128 rows, a stage
 
+// What is not a number stays so (fminf and fmaxf take the other one): the sums of a row or a weight with a block that is none.
+__device__ __forceinline__ float least(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float most(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // The unit in float32, by the fast exponential and division: off by 2^-21 of the result, by more where the gate is far below zero and the result as good as
 // none (2^-17 of it at -80); denominators past 2^126 give 0.
 template <bool CLAMPED> __device__ __forceinline__ float unit(float gate, float up, float limit) {
   if constexpr (CLAMPED) {
-    const float g = fminf(gate, limit), u = fminf(fmaxf(up, -limit), limit);
+    const float g = least(gate, limit), u = least(most(up, -limit), limit);
     return __fdividef(g, 1.f + __expf(-1.702f * g)) * (u + 1.f);
   }
   return __fdividef(gate, 1.f + __expf(-gate)) * up;

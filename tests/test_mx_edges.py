@@ -99,3 +99,62 @@ def test_entries_without_an_expert(n, experts, top_k, some):
         want = terms[..., : got.shape[1]]
         assert ((got.double() - want.sum(1)).abs() <= (top_k + 1) * 2.0 ** -24 * want.abs().sum(1)).all() and not got[-1].any()
     ops.check_tc_status()
+
+
+# ---------------------------------------------------------------- what is not a number
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,i,k,form", [(3, 64, 288, 1064), (33, 64, 288, 1064), (100, 96, 512, 1128), (384, 4096, 1056, 1192), (195, 6016, 288, 1256),
+                                        (500, 4128, 1056, 0), (1, 1024, 9248, 2000), (17, 1024, 9248, 2000)])
+@pytest.mark.parametrize("limit", [0.0, 1.5])
+def test_units_of_what_is_not_a_number(n, i, k, form, limit):
+    """A row with an infinity or with what is not a number leaves as one that is none, whichever the unit, and so does a block of features whose
+    weights have one; all others are what they are without."""
+    from hi_b200.kernels import ops
+
+    taken = ops.lib().hb_mx_gemm_form(n, 1, 2 * i, k, 1)
+    assert taken >= 2000 if form == 2000 else taken == form           # 2000: some blocks share K, how many goes by the device
+    g = _gen(n + i + k)
+    x, gate, up = _rows(g, n, k), _weight(g, i, k), _weight(g, i, k)
+    pack = lambda a, b: ops.mx_pack_weight(*(ops.mx_interleave(c, d) for c, d in zip(a, b)), glu=True)
+    before = ops.mx_values(ops.mx_glu(x, pack(gate, up), limit), F32)
+    assert before.isfinite().all()
+    bad = torch.zeros(n, i, dtype=torch.bool, device=DEV)
+    x[n // 2, 5], x[n - 1, k - 1] = float("inf"), float("nan")
+    bad[n // 2], bad[n - 1] = True, True
+    for rows in (x, ops.mx_quantize(x)):
+        got = ops.mx_values(ops.mx_glu(rows, pack(gate, up), limit), F32)
+        assert torch.equal(got.isnan(), bad) and torch.equal(got[~bad], before[~bad])
+    gate[1][3, 0], up[1][i - 1, k // 32 - 1] = 255, 255
+    bad[:, :32], bad[:, i - 32:] = True, True
+    got = ops.mx_values(ops.mx_glu(x, pack(gate, up), limit), F32)
+    assert torch.equal(got.isnan(), bad) and torch.equal(got[~bad], before[~bad])
+    ops.check_tc_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("limit", [0.0, 1.5])
+@pytest.mark.parametrize("scale", [None, "input"])
+def test_experts_of_what_is_not_a_number(limit, scale):
+    """The same for tokens among their experts, and for a score that is not a number."""
+    from hi_b200.kernels import ops
+
+    g, counts, h, i = _gen(11), [40, 0, 7, 200], 288, 96
+    n, plan = sum(counts), _plan_of(counts)
+    x, gate, up, down = _rows(g, n, h), _weight(g, 4, i, h), _weight(g, 4, i, h), _weight(g, 4, 64, i)
+    scores = torch.rand(n, 1, device=DEV, generator=g) if scale else None
+    w, wd = ops.mx_pack_weight(*(ops.mx_interleave(a, b) for a, b in zip(gate, up)), glu=True), ops.mx_pack_weight(*down)
+
+    def run():
+        act = ops.mx_experts_glu(x, plan, 1, w, scores, limit)
+        return ops.moe_combine(ops.mx_experts_linear(act, wd, plan), plan.slot_of_entry, None, n, 1)
+
+    before = run()
+    bad = torch.zeros(n, dtype=torch.bool, device=DEV)
+    x[3, 7], x[100, 287] = -float("inf"), float("nan")
+    bad[3], bad[100] = True, True
+    if scale:
+        scores[50] = float("nan")
+        bad[50] = True
+    got = run()
+    assert before.isfinite().all() and got[bad].isnan().all() and torch.equal(got[~bad], before[~bad])
+    ops.check_tc_status()
