@@ -2859,6 +2859,8 @@ def mx_experts_glu(x: torch.Tensor, plan: MoePlan, top_k: int, weight: MxWeight,
     (float32 [N, top_k], or None) before the unit."""
     _mx_rows_for(x, weight, "mx_experts_glu", True, True)
     if scores is not None:
+        if torch.is_grad_enabled() and scores.requires_grad:
+            raise KernelError("mx_experts_glu: units of microscaled weights have no gradients, their scores neither")
         _need(scores, "scores", torch.float32)
         if scores.numel() != x.shape[0] * top_k:
             raise KernelError(f"mx_experts_glu: {scores.numel()} scores for {x.shape[0]} tokens of {top_k} experts")

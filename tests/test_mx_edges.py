@@ -158,3 +158,28 @@ def test_experts_of_what_is_not_a_number(limit, scale):
     got = run()
     assert before.isfinite().all() and got[bad].isnan().all() and torch.equal(got[~bad], before[~bad])
     ops.check_tc_status()
+
+
+# ---------------------------------------------------------------- refusals
+def _packed(*shape, glu=False):
+    """A weight on the host."""
+    from hi_b200.kernels import ops
+
+    return ops.mx_pack_weight(*plain_mx.quantise(torch.randn(*shape, generator=torch.Generator().manual_seed(sum(shape)))), glu=glu)
+
+
+def _host_plan(n, experts):
+    from hi_b200.kernels import ops
+
+    z = lambda m: torch.zeros(m, dtype=torch.int32)
+    return ops.MoePlan(z(experts + 1), z(n), z(n), z(experts + 1))
+
+
+def test_scores_that_want_gradients_are_refused():
+    from hi_b200.kernels import ops
+
+    x, w, scores = torch.zeros(4, 64, dtype=BF16), _packed(3, 128, 64, glu=True), torch.rand(4, 2, requires_grad=True)
+    with pytest.raises(ops.KernelError, match="no gradients"):
+        ops.mx_experts_glu(x, _host_plan(8, 3), 2, w, scores)
+    with torch.no_grad(), pytest.raises(ops.KernelError, match="CUDA"):            # what is refused then is the host's tensor
+        ops.mx_experts_glu(x, _host_plan(8, 3), 2, w, scores)
