@@ -2619,6 +2619,7 @@ MX_BLOCK, MX_TILE, MX_CHUNK = 32, 128, 128     # values that share a power of tw
 # 5 us less host work a call (11.5 instead of 16.8). On the device (so / quantised first, us): 1 x 2,048 x 2,048 5.1 / 6.0, 4 rows 5.7 / 6.0, 8 rows 6.2 / 6.0;
 # 1 x 7,168 x 5,120 9.0 / 8.7, 2 rows 9.2 / 8.7, 8 rows 11.5 / 8.9; units of 1 x 8,192 x 5,120 11.6 / 11.7.
 MX_DIRECT_ROWS, MX_DIRECT_VALUES = 16, 10240
+MX_MOST = 2 ** 31 - 1                          # rows, and values of a row: what an int of the entry points holds
 MX_MOST_EXPERTS = 384                          # of a stack: whose tables a block's shared memory holds beside its stages
 
 
@@ -2638,6 +2639,8 @@ class MxRows:
 
     def __init__(self, like: torch.Tensor, n: int, k: int, offsets=None):
         """Room for ``n`` rows of ``k`` values beside ``like``, nothing written."""
+        if max(n, k) > MX_MOST:
+            raise KernelError(f"{n} rows of {k} values: up to {MX_MOST} of each")
         runs = 1 if offsets is None else min(offsets.numel() - 1, n or 1)
         self.shape, self.offsets, self.scales_at = (n, k), offsets, -(-n * k // 1024) * 512
         tiles = -(-n // MX_TILE) + runs - 1                 # as many as runs of these rows can begin
@@ -2670,7 +2673,7 @@ class MxWeight:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, glu: bool = False):
         e, m, k = (1, *shape) if len(shape) == 2 else tuple(shape)
-        if min(e, m, k) < 1 or k % MX_BLOCK or (glu and m % (2 * MX_BLOCK)) or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or \
+        if min(e, m, k) < 1 or max(e * m, k) > MX_MOST or k % MX_BLOCK or (glu and m % (2 * MX_BLOCK)) or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or \
                 codes.shape != (e, m, k // 2) or scales.shape != (e, -(-m // MX_TILE), _mx_chunks(k), 512) or \
                 not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device:
             raise KernelError(f"codes {codes.dtype} {tuple(codes.shape)} and scales {scales.dtype} {tuple(scales.shape)} are not those of a "
@@ -2709,6 +2712,8 @@ def mx_pack_weight(codes: torch.Tensor, exponents: torch.Tensor, glu: bool = Fal
 
 
 def _mx_input(x: torch.Tensor, k: Optional[int] = None) -> torch.Tensor:
+    if isinstance(x, MxRows):
+        raise KernelError("x is quantised already, or in another order")
     if not x.is_cuda:
         raise KernelError("x must be a CUDA tensor; this engine has no CPU path")
     shape, dtype = x.shape, x.dtype
@@ -2732,7 +2737,9 @@ def _mx_quantize(x: torch.Tensor, rows: int, sorted_entry, top_k: int, offsets) 
     return out
 
 
-def _mx_plan(plan: MoePlan, rows: int) -> None:
+def _mx_plan(plan: MoePlan, rows: int, top_k: int) -> None:
+    if top_k < 1:
+        raise KernelError(f"a plan of {top_k} experts a token")
     for t, name in ((plan.offsets, "plan.offsets"), (plan.sorted_entry, "plan.sorted_entry")):
         _need(t, name, torch.int32)
     if plan.offsets.numel() < 2 or plan.sorted_entry.numel() != max(rows, 1):
@@ -2748,13 +2755,15 @@ def mx_quantize(x: torch.Tensor, plan: Optional[MoePlan] = None, top_k: int = 1)
         _on_current_device(x)
         return _mx_quantize(x, x.shape[0], None, 1, None)
     rows = x.shape[0] * top_k
-    _mx_plan(plan, rows)
+    _mx_plan(plan, rows, top_k)
     _on_current_device(x, plan.offsets, plan.sorted_entry)
     return _mx_quantize(x, rows, plan.sorted_entry, top_k, plan.offsets)
 
 
 def mx_values(rows: MxRows, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that quantised rows stand for, [N, K] in bfloat16 or float32 (both hold them exactly)."""
+    if not isinstance(rows, MxRows):
+        raise KernelError(f"mx_values takes rows that mx_quantize or a gated unit returned, not {type(rows).__name__}")
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise KernelError(f"values are bfloat16 or float32, not {out_dtype}")
     data = rows.data
@@ -2865,13 +2874,15 @@ def mx_experts_glu(x: torch.Tensor, plan: MoePlan, top_k: int, weight: MxWeight,
         if scores.numel() != x.shape[0] * top_k:
             raise KernelError(f"mx_experts_glu: {scores.numel()} scores for {x.shape[0]} tokens of {top_k} experts")
     raw, rows = _mx_input(x, weight.shape[-1]), x.shape[0] * top_k
-    _mx_plan(plan, rows)
+    _mx_plan(plan, rows, top_k)
     return _mx_gemm(MxRows(raw, rows, raw.shape[1], plan.offsets), weight, "mx_experts_glu", plan=plan, scores=scores, limit=limit, raw=raw, top_k=top_k)
 
 
 def mx_experts_linear(rows: MxRows, weight: MxWeight, plan: MoePlan) -> torch.Tensor:
     """y[slot] = rows[slot] W[e]^T, float32 [N*k, M], for rows in the plan's order (:func:`mx_experts_glu`); ``moe_combine`` sums a token's."""
     _mx_rows_for(rows, weight, "mx_experts_linear", False, True)
+    if not isinstance(rows, MxRows):
+        raise KernelError(f"mx_experts_linear takes the rows that mx_experts_glu returned, not {type(rows).__name__}")
     if rows.offsets is not plan.offsets:
         raise KernelError("mx_experts_linear: the rows are in another plan's order")
     return _mx_gemm(rows, weight, "mx_experts_linear", torch.float32)

@@ -183,3 +183,30 @@ def test_scores_that_want_gradients_are_refused():
         ops.mx_experts_glu(x, _host_plan(8, 3), 2, w, scores)
     with torch.no_grad(), pytest.raises(ops.KernelError, match="CUDA"):            # what is refused then is the host's tensor
         ops.mx_experts_glu(x, _host_plan(8, 3), 2, w, scores)
+
+
+def test_what_is_not_rows_is_refused():
+    """Rows that are not quantised, or are already, where the others are asked for; plans of no expert a token; sizes that an int does not hold."""
+    from hi_b200.kernels import ops
+
+    x, w, wg = torch.zeros(4, 64, dtype=BF16), _packed(3, 128, 64), _packed(3, 128, 64, glu=True)
+    rows, plan = ops.MxRows(x, 4, 64), _host_plan(4, 3)
+    for call in (lambda: ops.mx_values(x), lambda: ops.mx_experts_linear(x, w, plan), lambda: ops.mx_quantize(rows), lambda: ops.mx_quantize(rows, plan, 1),
+                 lambda: ops.mx_experts_glu(rows, plan, 1, wg), lambda: ops.MxRows(torch.empty(0, device="meta"), 2 ** 31, 32),
+                 lambda: ops.MxRows(torch.empty(0, device="meta"), 1, 2 ** 31),
+                 lambda: ops.MxWeight(torch.empty(2, 2 ** 30, 16, dtype=torch.uint8, device="meta"),
+                                      torch.empty(2, 2 ** 23, 2, 512, dtype=torch.uint8, device="meta"), (2, 2 ** 30, 32))):
+        with pytest.raises(ops.KernelError):
+            call()
+
+
+@pytest.mark.gpu
+def test_plans_of_no_expert_a_token_are_refused():
+    from hi_b200.kernels import ops
+
+    x, plan, w = torch.zeros(1, 64, dtype=BF16, device=DEV), _plan_of([1, 0, 0]), ops.mx_pack_weight(*_weight(_gen(1), 3, 128, 64), glu=True)
+    for top_k in (0, -1):
+        with pytest.raises(ops.KernelError):
+            ops.mx_quantize(x, plan, top_k)
+        with pytest.raises(ops.KernelError):
+            ops.mx_experts_glu(x, plan, top_k, w)
