@@ -54,6 +54,43 @@ def test_units_of_tiles_that_end_anywhere(counts, i, k, form):
     ops.check_tc_status()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("at", [0, 1, 2])
+@pytest.mark.parametrize("h,i", [(8192, 96), (8192, 1024), (640, 8192), (5120, 8192)])
+@pytest.mark.parametrize("limit", [0.0, 1.5])
+def test_one_routed_row(at, h, i, limit):
+    """One token through its expert, whose products' K a cluster of blocks shares: the unit's, the down product's, or both."""
+    from hi_b200.kernels import ops
+
+    forms = [ops.lib().hb_mx_gemm_form(1, 3, 2 * i, h, 1), ops.lib().hb_mx_gemm_form(1, 3, h, i, 0)]
+    assert max(forms) >= 2000
+    g, counts = _gen(h + i + at), [int(e == at) for e in range(3)]
+    x, plan, gate, up, down = _rows(g, 1, h), _plan_of(counts), _weight(g, 3, i, h), _weight(g, 3, i, h), _weight(g, 3, h, i)
+    scores = torch.rand(1, 1, device=DEV, generator=g) + 0.5
+    for s in (None, scores):
+        w, act, values = _units(x, counts, plan, gate, up, limit, s)
+        y = ops.mx_experts_linear(act, ops.mx_pack_weight(*down), plan)
+        _near(y, values, plain_mx.values(down[0][at], down[1][at]))
+        out = ops.moe_combine(y, plan.slot_of_entry, None, 1, 1, scores.view(-1))
+        assert ((out.double() - y.double() * scores.double()).abs() <= 2 * 2.0 ** -24 * y.double().abs() * scores.double()).all()
+    ops.check_tc_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,i,h,form", [([3, 0, 20, 9], 96, 288, 1064), ([100, 17, 1, 128, 33], 160, 288, 1128), ([250, 3, 131, 193], 4128, 288, 1256),
+                                             ([700, 129, 1450], 8224, 2080, 0)])
+def test_clamped_experts(counts, i, h, form):
+    """The clamped unit by expert in every form, gates and ups on both sides of the limit, with the score on what an expert reads and without."""
+    from hi_b200.kernels import ops
+
+    assert ops.lib().hb_mx_gemm_form(sum(counts), len(counts), 2 * i, h, 1) == form
+    g = _gen(i + h + len(counts))
+    x, plan, gate, up = _rows(g, sum(counts), h), _plan_of(counts), _weight(g, len(counts), i, h), _weight(g, len(counts), i, h)
+    for scores in (None, torch.rand(sum(counts), 1, device=DEV, generator=g) + 0.5):
+        _units(x, counts, plan, gate, up, 1.0, scores)
+    ops.check_tc_status()
+
+
 # ---------------------------------------------------------------- entries without an expert
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,experts,top_k", [(1, 4, 2), (9, 3, 1), (40, 16, 4), (200, 5, 2), (700, 64, 3), (33, 2, 1)])
