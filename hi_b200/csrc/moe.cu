@@ -34,8 +34,9 @@ __device__ __forceinline__ void plan_block(const int* ids, int n, int experts, i
     if (e >= 0 && e < experts) atomicAdd(&cnt[e], 1);
   }
   __syncthreads();
+  int run = 0;
   if (threadIdx.x == 0) {
-    int run = 0, n_active = 0;
+    int n_active = 0;
     for (int e = 0; e < experts; ++e) {
       offsets[e] = run;
       base[e] = run;
@@ -48,7 +49,6 @@ __device__ __forceinline__ void plan_block(const int* ids, int n, int experts, i
   __syncthreads();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    int placed = 0;
     for (int start = 0; start < n; start += 32) {
       const int i = start + lane;
       int e = i < n ? (IDS_SHARED ? ids[i] : __ldcg(ids + i)) : -1;
@@ -62,12 +62,11 @@ __device__ __forceinline__ void plan_block(const int* ids, int n, int experts, i
       } else if (i < n) {
         slot_of_entry[i] = -1;
       }
-      placed += __popc(__ballot_sync(0xffffffffu, e >= 0));
       __syncwarp();
       if (e >= 0 && rank == 0) base[e] += __popc(peers);
       __syncwarp();
     }
-    for (int i = placed + lane; i < n; i += 32) sorted_entry[i] = 0;
+    for (int i = __shfl_sync(0xffffffffu, run, 0) + lane; i < n; i += 32) sorted_entry[i] = 0;
   }
 }
 
@@ -144,8 +143,8 @@ __device__ __forceinline__ void plan_block_wide(const int* __restrict__ ids, int
     }
   }
   __syncthreads();
-  walk(true);
   for (int i = first[experts - 1] + total[experts - 1] + threadIdx.x; i < n; i += blockDim.x) sorted_entry[i] = 0;
+  walk(true);
 }
 
 // ------------------------------------------------------------------ router

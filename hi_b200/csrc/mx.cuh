@@ -121,12 +121,12 @@ __device__ __forceinline__ uint32_t four_scales(uint32_t scale, int lane) {
   return word | __shfl_xor_sync(0xffffffffu, word, 8);
 }
 
-// The tile of a row of expert-sorted rows and its place there, by a whole warp; `offsets` null: one run of rows.
-__device__ __forceinline__ void place_of(const int* offsets, int experts, int row, int& tile, int& at) {
+// The tile of a row of expert-sorted rows and its place there, by a whole warp; `offsets` null: one run of rows. False: behind the last expert's rows.
+__device__ __forceinline__ bool place_of(const int* offsets, int experts, int row, int& tile, int& at) {
   if (!offsets) {
     tile = row / TILE;
     at = row_at(row % TILE);
-    return;
+    return true;
   }
   const int lane = threadIdx.x & 31;
   int tiles = 0, first = 0;
@@ -136,9 +136,11 @@ __device__ __forceinline__ void place_of(const int* offsets, int experts, int ro
     else if (a <= row) first = a + 1;
   }
   tiles = __reduce_add_sync(0xffffffffu, tiles);
-  first = row - (int)__reduce_max_sync(0xffffffffu, first) + 1;
+  const int found = (int)__reduce_max_sync(0xffffffffu, first);
+  first = row - found + 1;
   tile = tiles + first / TILE;
   at = row_at(first % TILE);
+  return found > 0;
 }
 
 }  // namespace mx

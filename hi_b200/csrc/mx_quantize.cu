@@ -34,9 +34,8 @@ mx_quantize_kernel(const T* __restrict__ x, long long x_ld, int rows, int k, con
   const long long item = (long long)blockIdx.x * WARPS + warp;
   const int row = (int)(item / groups), first = (int)(item % groups) * MANY;
   if (row >= rows) return;
-  const int last = offsets ? offsets[experts] : rows, entry = sorted_entry ? sorted_entry[row] : 0;
-  if (row >= last) return;                                 // entries without an expert have no row
-  const size_t from = sorted_entry ? entry / top_k : row;
+  // (behind the last expert's rows stands anything; x is asked for all the same, before the offsets are there)
+  const size_t from = sorted_entry ? min((unsigned)sorted_entry[row], (unsigned)(rows - 1)) / (unsigned)top_k : row;
   const T* const in = x + from * x_ld + lane * 8;
   mx::Eight<T> x8[MANY];
 #pragma unroll
@@ -46,7 +45,7 @@ mx_quantize_kernel(const T* __restrict__ x, long long x_ld, int rows, int k, con
     else x8[m].zero();
   }
   int tile, at;
-  mx::place_of(offsets, experts, row, tile, at);
+  if (!mx::place_of(offsets, experts, row, tile, at)) return;
   uint8_t* const to = codes + (size_t)row * (k / 2) + lane * 4;
   uint8_t* const scale_to = scales + (size_t)tile * all * mx::ATOM + at;
 #pragma unroll
@@ -68,9 +67,9 @@ mx_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, all = mx::chunks(k), groups = (all / 2 + MANY - 1) / MANY;
   const long long item = (long long)blockIdx.x * WARPS + warp;
   const int row = (int)(item / groups), first = (int)(item % groups) * MANY;
-  if (row >= rows || (offsets && row >= offsets[experts])) return;
+  if (row >= rows) return;
   int tile, at;
-  mx::place_of(offsets, experts, row, tile, at);
+  if (!mx::place_of(offsets, experts, row, tile, at)) return;
   const uint8_t* const from = codes + (size_t)row * (k / 2) + lane * 4;
   const uint8_t* const scale_from = scales + (size_t)tile * all * mx::ATOM + at + lane / 4 % 4;
   uint32_t word[MANY], scale[MANY];
