@@ -24,8 +24,10 @@ __device__ __forceinline__ float most(float a, float b) {
   return r;
 }
 
-// The unit in float32, by the fast exponential and division: off by 2^-21 of the result, by more where the gate is far below zero and the result as good as
-// none (2^-17 of it at -80); denominators past 2^126 give 0.
+// The unit in float32, by the fast exponential and division. By their documented errors it is off by at most (5 + 1.2 |gate|) 2^-23 of the result
+// (of which the gate's part goes away above zero), the clamped unit, whose 1.702 gate is rounded too, by (6 + 3.7 |gate|) 2^-23. The most that was
+// found, over 2^24 gates a range, in units of 2^-23: 1.8 above -1, 4.7 from there to -8, 8.5 to -16, 33 to -80; clamped 2.4, 10.8, 20.4, 55.
+// Denominators past 2^126 give 0.
 template <bool CLAMPED> __device__ __forceinline__ float unit(float gate, float up, float limit) {
   if constexpr (CLAMPED) {
     const float g = least(gate, limit), u = least(most(up, -limit), limit);

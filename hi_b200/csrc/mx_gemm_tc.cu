@@ -350,7 +350,9 @@ int pairs(const Call& c, const Params& p, int pairs) {
 // The form by a model of the time in us. Few rows (mx_gemm_few_tc.cu): a stage of 128 weight rows by n rows takes a block 0.12 + 0.0014 n, 0.2 at least,
 // and the first stage's way and the last results 3.4; n blocks that share K 4.3, 0.07 a tile, 0.17 a stage and 0.02 + 0.05 / n a row. Pairs: a stage 0.34
 // in the first round and 0.44 in others (the card is at its power limit then), 6.5 besides. A tile takes what its results take at least: 0.4 + 0.022 n, of a
-// gated unit 0.5 + 0.035 n, a pair 5. An expert's last tile is taken to be half full. Measured (us):
+// gated unit 0.5 + 0.035 n, a pair 5. An expert's last tile is taken to be half full. For several experts' rows fractions of a round count, which is right for
+// many tiles and too little for fewer than there are SMs: clusters share K for one run of rows and for a single routed row only (two rows of 16
+// experts of 2,048 x 8,192 would take 9.8 by these constants, 4.8 by the rule, 7.9 in four parts). Measured (us):
 //   pairs / single blocks: 512 x 16,384 x 5,120 22.3 / 24.0, 700 x 5,120 x 8,192 17.9 / 18.1, 2,048 x 16,384 x 5,120 66 / 73, units of 700 x 8,192 x 5,120
 //   28.8 / 34.0, 99 x 5,120 x 8,192 17.0 / 11.8; 16 experts of 5,120 x 8,192, 4,096 rows: up 210 / 216, down 121 / 117, 2,048 rows: 155 / 148, 83 / 79; 12,288 rows of 64
 //   experts of 2,048 x 1,024: 49 / 57, 45 / 36;

@@ -2617,7 +2617,8 @@ def four_bit_linear(x: torch.Tensor, weight: FourBitWeight, out_dtype: torch.dty
 MX_BLOCK, MX_TILE, MX_CHUNK = 32, 128, 128     # values that share a power of two; rows and values of 512 bytes of scales (csrc/mx.cuh)
 # Up to 16 rows of up to 10,240 values in all are quantised by the product's own blocks, each of which needs all of them: one launch instead of two,
 # 5 us less host work a call (11.5 instead of 16.8). On the device (so / quantised first, us): 1 x 2,048 x 2,048 5.1 / 6.0, 4 rows 5.7 / 6.0, 8 rows 6.2 / 6.0;
-# 1 x 7,168 x 5,120 9.0 / 8.7, 2 rows 9.2 / 8.7, 8 rows 11.5 / 8.9; units of 1 x 8,192 x 5,120 11.6 / 11.7.
+# 1 x 7,168 x 5,120 9.0 / 8.7, 2 rows 9.2 / 8.7, 8 rows 11.5 / 8.9; units of 1 x 8,192 x 5,120 11.6 / 11.7. The rule is that of eager calls: captured
+# ones, which have no host work, take it too, 0.3 to 0.5 us the slower where a row has 5,120 values.
 MX_DIRECT_ROWS, MX_DIRECT_VALUES = 16, 10240
 MX_MOST = 2 ** 31 - 1                          # rows, and values of a row: what an int of the entry points holds
 MX_MOST_EXPERTS = 384                          # of a stack: whose tables a block's shared memory holds beside its stages
@@ -2639,7 +2640,7 @@ class MxRows:
 
     def __init__(self, like: torch.Tensor, n: int, k: int, offsets=None):
         """Room for ``n`` rows of ``k`` values beside ``like``, nothing written."""
-        if max(n, k) > MX_MOST:
+        if n > MX_MOST or k > MX_MOST:
             raise KernelError(f"{n} rows of {k} values: up to {MX_MOST} of each")
         runs = 1 if offsets is None else min(offsets.numel() - 1, n or 1)
         self.shape, self.offsets, self.scales_at = (n, k), offsets, -(-n * k // 1024) * 512
@@ -2695,7 +2696,8 @@ def mx_interleave(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 def mx_pack_weight(codes: torch.Tensor, exponents: torch.Tensor, glu: bool = False) -> MxWeight:
     """``codes`` uint8 [M, K] or [E, M, K] of 0 .. 15 (e2m1, 8 is the sign) and ``exponents`` uint8 [..., K / 32] (127 + e; 255: not a number) as
-    an :class:`MxWeight`. Once, when a model is loaded; works on any device."""
+    an :class:`MxWeight`, for a caller who has them so (models' loaders quantise 16-bit weights: :func:`mx_quantize_weight`). Once, when weights
+    are loaded; works on any device."""
     if codes.dim() not in (2, 3) or codes.dtype != torch.uint8 or exponents.dtype != torch.uint8 or codes.device != exponents.device or \
             codes.numel() == 0 or codes.shape[-1] % MX_BLOCK or exponents.shape != (*codes.shape[:-1], codes.shape[-1] // MX_BLOCK):
         raise KernelError(f"a microscaled weight is uint8 codes [M, K] or [E, M, K] and exponents [..., K / {MX_BLOCK}] on one device, not "

@@ -52,7 +52,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor | ops.FourBitWeight | ops.MxWei
     A weight kept in float32 while activations are bfloat16 (a tensor stored in 32-bit stays
     so) is multiplied in float32. ``out_dtype=torch.float32`` asks for a float32 result from
     bfloat16 operands (the logits). A weight held in four bits is multiplied by ``ops.four_bit_linear``, one in microscaled
-    4-bit floats, with ``x`` quantised alike, by ``ops.mx_linear``.
+    4-bit floats, with ``x`` quantised alike, by ``ops.mx_linear`` (a bias of either is rounded to bfloat16, as the bfloat16 path takes it).
     """
     if isinstance(weight, ops.FourBitWeight):
         return ops.four_bit_linear(x, weight, out_dtype or x.dtype, None if bias is None else bias.to(x.dtype))

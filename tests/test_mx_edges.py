@@ -3,7 +3,20 @@ import pytest
 import torch
 
 import plain_mx
-from test_mx import BF16, DEV, F32, _check_unit, _gen, _near, _rows, _weight
+from test_mx import BF16, DEV, F32, _gen, _near, _rows, _weight
+
+
+def _check_unit(act, x, gate, up, limit, score=None):
+    """Values of a unit against 64 bits. Sums as in _near; the unit's slope in the gate is at most 1.2. Then, in units of 2^-23 of the result: the
+    exponential 2 + 1.173 of its argument's magnitude and the division 2, as CUDA documents them, the clamped unit's 1.702 g, rounded twice, another
+    1.702 |g| in the exponent, and half a unit each for 1 + e, u + 1 and the product: at most 6 + 3.7 |g|."""
+    s = 1.0 if score is None else score.double().unsqueeze(1)
+    g, u = s * (x @ gate.t()), s * (x @ up.t())
+    tg, tu = (2.0 ** -16 * s * (x.abs() @ w.abs().t()) for w in (gate, up))
+    want = plain_mx.unit(g, u, limit)
+    wide = (u.abs() if limit == 0 else u.clamp(-limit, limit).abs() + 1) + tu
+    tol = 1.2 * tg * wide + (g.abs() + tg) * tu + (6 + 3.7 * g.abs()) * 2.0 ** -23 * want.abs()
+    assert plain_mx.is_quantised(act, want, tol)
 
 
 def _plan_of(counts):
